@@ -295,6 +295,61 @@ int j4b_attention_prefill(j4b_buf q, j4b_buf k_cache, j4b_buf v_cache, int64_t b
 /* out [rows, width] = gate * sigmoid(gate) * up, gate_up [rows, 2 * width] = gate | up. */
 int j4b_swiglu(j4b_buf gate_up, int64_t rows, int64_t width, j4b_buf out, j4b_stream s);
 
+/* ---- 8-bit paged KV cache (no reference counterpart). Keys and values are e4m3 codes in pages of
+ * `page` tokens; every block of 16 tokens and head has one f32 scale, a power of two, for its keys
+ * and one for its values: value = code * scale. The scale of a block is the smallest power of two
+ * (at least 2^-120) of which no finite |value| exceeds 448 times; a block that gets more tokens
+ * keeps its scale or takes a larger one (its codes are then rescaled). Sequences name their pages
+ * in token order through rows of an int32 page table on the device ([batch, table_width], rows
+ * table_stride apart); an entry outside [0, pages) is unmapped: its tokens are neither written nor
+ * seen. Lengths, starts and offsets are int32 arrays on the device, so a call can be captured in a
+ * graph and replayed while they change. heads is a multiple of kv_heads (grouped heads: query head
+ * h reads kv head h / (heads / kv_heads)). Activation types: J4B_F32, J4B_BF16. ---- */
+#define J4B_F32 0
+#define J4B_BF16 1
+typedef struct j4b_kv8_cache {
+  j4b_buf k, v;             /* codes [layers, pages, kv_heads, page, head_dim], 16-byte aligned */
+  j4b_buf k_scale, v_scale; /* f32 [layers, pages, kv_heads, page / 16] */
+  int64_t layers, pages;
+  int32_t kv_heads, page, head_dim; /* page: a multiple of 16; head_dim: 64 or 128 */
+} j4b_kv8_cache;
+/* Writes new tokens: qkv [tokens, (heads + 2 kv_heads) * head_dim] f32 (q | k | v, rows qkv_stride
+ * floats apart). Sequence b has the rows [offsets[b], offsets[b + 1]) (offsets 0: row b alone), its
+ * first at position starts[b]. RoPE as j4b_rope_kv's, by the angles of rope [rope_positions,
+ * head_dim / 2] (cos, sin) f32. Writes q_out [tokens, heads, head_dim] and the codes and scales of
+ * k (rotated) and v. Tokens at or past rope_positions are not written. Two sequences of a call must
+ * not write to the same page. */
+int j4b_kv8_append(const j4b_kv8_cache* cache, int64_t layer, j4b_buf qkv, int64_t qkv_stride, int64_t tokens,
+                   int64_t heads, j4b_buf rope, int64_t rope_positions, j4b_buf table, int64_t table_stride,
+                   int64_t table_width, j4b_buf starts, j4b_buf offsets, int64_t batch, j4b_buf q_out, int q_type,
+                   j4b_stream s);
+/* Attention of one query per sequence, q [batch, heads, head_dim] (sequences q_stride elements
+ * apart), at position lengths[b] - 1 over the sequence's lengths[b] cached tokens; out [batch,
+ * heads, head_dim] dense. window > 0 limits a query at position p to the keys j > p - window and
+ * the first `sinks` tokens; window 0: all. A query that sees no key (length 0, unmapped pages) gives
+ * zeros. f32-accurate (queries and probabilities enter the tensor cores as two f16 terms).
+ * workspace: j4b_kv8_decode_workspace bytes of device memory, 16-byte aligned, used by this call
+ * alone until it has run. */
+int j4b_kv8_decode_workspace(const j4b_kv8_cache* cache, int64_t heads, int64_t batch, int64_t* bytes);
+int j4b_kv8_attention_decode(const j4b_kv8_cache* cache, int64_t layer, j4b_buf q, int q_type, int64_t q_stride,
+                             int64_t heads, j4b_buf table, int64_t table_stride, int64_t table_width, j4b_buf lengths,
+                             int64_t batch, int64_t window, int64_t sinks, double scale, j4b_buf out, int out_type,
+                             j4b_buf workspace, int64_t workspace_bytes, j4b_stream s);
+/* Causal attention of ragged chunks: sequence b's queries are the rows [offsets[b], offsets[b + 1])
+ * of q [tokens, heads, head_dim] (rows q_stride elements apart), its last tokens: query i of n is
+ * at position lengths[b] - n + i. Window, sinks and empty rows as above. Tensor-core products of
+ * f16 operands with f32 softmax and accumulation (the rel 1e-2 tensor-core bar). */
+int j4b_kv8_attention_prefill(const j4b_kv8_cache* cache, int64_t layer, j4b_buf q, int q_type, int64_t q_stride,
+                              int64_t tokens, int64_t heads, j4b_buf offsets, j4b_buf table, int64_t table_stride,
+                              int64_t table_width, j4b_buf lengths, int64_t batch, int64_t window, int64_t sinks,
+                              double scale, j4b_buf out, int out_type, j4b_stream s);
+/* Copies pages within every layer: move i takes the blocks that hold the first tokens[i] tokens
+ * (tokens NULL: all) of page src[i] to page dst[i], codes and scales. The lists are host arrays,
+ * read before the call returns. The moves run at the same time: J4B_EINVAL if a page is written
+ * twice, or both read and written. */
+int j4b_kv8_copy_pages(const j4b_kv8_cache* cache, int64_t moves, const int32_t* src, const int32_t* dst,
+                       const int32_t* tokens, j4b_stream s);
+
 /* ---- JIT tapes: ExecutionPlan.capture / execute (core/tensor/ExecutionPlan.java:49-132) ----
  *
  * A tape is the SPI call list a compiled function records once per input signature

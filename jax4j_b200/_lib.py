@@ -20,6 +20,8 @@ Q4_0, Q8_0, Q4_K, Q6_K, Q2_0 = 2, 8, 12, 14, 42
 QUANT_NAMES = {Q4_0: "Q4_0", Q8_0: "Q8_0", Q4_K: "Q4_K", Q6_K: "Q6_K", Q2_0: "Q2_0"}
 QUANT_BLOCK = {Q4_0: (32, 18), Q8_0: (32, 34), Q4_K: (256, 144), Q6_K: (256, 210), Q2_0: (128, 34)}
 
+F32, BF16 = 0, 1  # activation types of the 8-bit KV cache's operators
+
 OPS = ["ADD", "SUB", "MUL", "DIV", "MAX", "MIN", "NEG", "EXP", "LOG", "SQRT", "RSQRT", "TANH",
        "SIGMOID", "RELU", "ABS", "SIGN"]
 OP = {name: i for i, name in enumerate(OPS)}
@@ -37,6 +39,12 @@ class TapeStats(ctypes.Structure):
                 ("launches", ctypes.c_int), ("arena_bytes", ctypes.c_int64)]
 
 
+class Kv8CacheDesc(ctypes.Structure):
+    _fields_ = [("k", ctypes.c_uint64), ("v", ctypes.c_uint64), ("k_scale", ctypes.c_uint64),
+                ("v_scale", ctypes.c_uint64), ("layers", ctypes.c_int64), ("pages", ctypes.c_int64),
+                ("kv_heads", ctypes.c_int32), ("page", ctypes.c_int32), ("head_dim", ctypes.c_int32)]
+
+
 _u64 = ctypes.c_uint64
 _i64 = ctypes.c_int64
 _int = ctypes.c_int
@@ -44,6 +52,7 @@ _vp = ctypes.c_void_p
 _i64p = ctypes.POINTER(ctypes.c_int64)
 _i32p = ctypes.POINTER(ctypes.c_int32)
 _f64p = ctypes.POINTER(ctypes.c_double)
+_kv8 = ctypes.POINTER(Kv8CacheDesc)
 
 # name -> argtypes (every function returns int status)
 SIGNATURES = {
@@ -99,6 +108,13 @@ SIGNATURES = {
     "j4b_attention_decode": [_u64, _u64, _u64, _i64, _i64, _i64, _i64, _i64, _u64, _vp],
     "j4b_attention_prefill": [_u64, _u64, _u64, _i64, _i64, _i64, _i64, _i64, _u64, _vp],
     "j4b_swiglu": [_u64, _i64, _i64, _u64, _vp],
+    "j4b_kv8_append": [_kv8, _i64, _u64, _i64, _i64, _i64, _u64, _i64, _u64, _i64, _i64, _u64, _u64, _i64, _u64, _int, _vp],
+    "j4b_kv8_decode_workspace": [_kv8, _i64, _i64, _i64p],
+    "j4b_kv8_attention_decode": [_kv8, _i64, _u64, _int, _i64, _i64, _u64, _i64, _i64, _u64, _i64, _i64, _i64,
+                                 ctypes.c_double, _u64, _int, _u64, _i64, _vp],
+    "j4b_kv8_attention_prefill": [_kv8, _i64, _u64, _int, _i64, _i64, _i64, _u64, _u64, _i64, _i64, _u64, _i64, _i64, _i64,
+                                  ctypes.c_double, _u64, _int, _vp],
+    "j4b_kv8_copy_pages": [_kv8, _i64, _i32p, _i32p, _i32p, _vp],
     "j4b_peer_alloc": [_int, ctypes.c_size_t, ctypes.POINTER(_u64), ctypes.c_char_p],
     "j4b_peer_open": [_int, ctypes.c_char_p, ctypes.POINTER(_u64)],
     "j4b_peer_close": [_u64],

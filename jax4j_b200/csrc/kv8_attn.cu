@@ -1,0 +1,745 @@
+// Attention over the 8-bit paged KV cache (format: kv8_common.cuh): one query per sequence
+// (decode) and ragged causal chunks (prefill), grouped heads, sliding window with sinks.
+//
+// A warp takes a 16-token block of one kv head at a time straight from the pages into mma.sync
+// m16n8k16 operands: 8 tokens are the n columns of S = Q K^T, and since a contraction may run over
+// its index in any order, a thread takes 16 consecutive dims of its token (one 16-byte load) as
+// the k indices of four MMAs. For O = P V the 16 tokens are the k index and 8 dims the columns; a
+// thread loads the 4 tokens whose probabilities it holds, whole 16-byte pieces, and pairs their
+// bytes by byte permutes. e4m3 to f16 is exact, so the only roundings are those of Q and P.
+// Scales are powers of two: a block's key scale multiplies its scores, and its value scale, over
+// the largest seen so far, its probabilities.
+#include <algorithm>
+#include <cmath>
+
+#include "kv8_common.cuh"
+
+namespace j4b {
+
+int kv8_check(const j4b_kv8_cache* c, int64_t layer, Kv8View* view, int* dev);
+
+namespace {
+
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t h2(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+// what h2 rounded away, as f16x2
+__device__ __forceinline__ uint32_t h2_rest(float a, float b, uint32_t hi) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+  return h2(a - f.x, b - f.y);
+}
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp8(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ float quad_max(float v) {
+  v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
+  return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
+}
+__device__ __forceinline__ float quad_sum(float v) {
+  v += __shfl_xor_sync(0xffffffffu, v, 1);
+  return v + __shfl_xor_sync(0xffffffffu, v, 2);
+}
+
+// The blocks that queries at positions first .. last of a sequence of `len` tokens see: the first
+// `sink_blocks` ones, then those from `from` on to `end` (exclusive). count() of them in order.
+struct Span {
+  int sink_blocks, from, end;
+  __device__ __forceinline__ int count() const { return sink_blocks + end - from; }
+  __device__ __forceinline__ int block(int i) const { return i < sink_blocks ? i : from + i - sink_blocks; }
+};
+__device__ __forceinline__ Span span_of(int first, int last, int window, int sinks) {
+  const int lo = window > 0 ? max(0, first - window + 1) : 0;  // first position in the window of `first`
+  Span s;
+  s.from = lo / kKvBlock;
+  s.end = last < 0 ? s.from : last / kKvBlock + 1;
+  s.sink_blocks = min((sinks + kKvBlock - 1) / kKvBlock, s.from);
+  return s;
+}
+
+// Per-lane pieces of a block: keys of tokens g and 8 + g (dims 16 (t + 4 i) .. + 15), values of
+// tokens 2t, 2t + 1, 2t + 8, 2t + 9 (dims (D / 8) g .. + D / 8 - 1), g = lane / 4, t = lane % 4.
+template <int D>
+struct Piece {
+  static constexpr int kK = D / 64;   // 16-byte key pieces of a token
+  static constexpr int kW = D / 32;   // 4-byte words of a value piece
+  static constexpr int kStage = 32 * D;  // bytes of a block, keys and values, in a warp's ring
+};
+
+// Starts the copy of block `id` into a warp's stage. A lane reads back only what it copied itself,
+// so its own wait_group is all the synchronisation the ring needs.
+template <int D>
+__device__ __forceinline__ void fetch(const Kv8View& c, int id, uint32_t stage, int lane) {
+  const int g = lane >> 2, t = lane & 3;
+  const uint8_t* kb = c.k + (int64_t)id * (kKvBlock * D);
+  const uint8_t* vb = c.v + (int64_t)id * (kKvBlock * D);
+#pragma unroll
+  for (int n = 0; n < 2; ++n)
+#pragma unroll
+    for (int i = 0; i < Piece<D>::kK; ++i)
+      cp16(stage + (n * Piece<D>::kK + i) * 512 + lane * 16, kb + (8 * n + g) * D + 16 * (t + 4 * i));
+  const uint32_t vs = stage + kKvBlock * D;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint8_t* src = vb + (2 * t + (j & 1) + 8 * (j >> 1)) * D + (D / 8) * g;
+    if (D == 128)
+      cp16(vs + j * 512 + lane * 16, src);
+    else
+      cp8(vs + j * 256 + lane * 8, src);
+  }
+}
+
+// A warp's online softmax over the blocks it visits. SPLIT: the 16 rows of the MMAs are 8 queries,
+// rows 0-7 the f16 values of Q (and P), rows 8-15 what the rounding left, so that every product is
+// f32-accurate at no extra MMA (a group of up to 8 heads leaves those rows idle otherwise); a
+// thread's query is row g alone. Otherwise 16 queries; a thread's are g and g + 8.
+template <int D, bool SPLIT>
+struct Warp {
+  static constexpr int kRows = SPLIT ? 1 : 2;
+  uint32_t q[D / 16][4];
+  float o[D / 8][4];
+  float factor[kRows];  // scores in log2 units per unit of the MMA's result and of key scale
+  float m[kRows], l[kRows];
+  float ref;  // value scale that the accumulators are in units of (times 2^-kPShift)
+
+  // probabilities enter the second product as p 2^kPShift <= 4096: f16 keeps p's bits down to
+  // 2^-24 / 4096, below f32's for a row of a million tokens
+  static constexpr int kPShift = 12;
+
+  __device__ __forceinline__ void reset() {
+#pragma unroll
+    for (int j = 0; j < D / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) m[r] = -INFINITY, l[r] = 0.f;
+    ref = 0.f;
+  }
+
+  // Loads the query rows (null: a row of zeros). Each row is first brought to a largest element in
+  // [2^11, 2^12) by a power of two, so f16's range does not limit queries.
+  __device__ __forceinline__ void load_q(const void* base, int type, const int64_t (&row)[kRows], float scale_log2, int t) {
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      float4 x[D / 16];
+      float most = 0.f;
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) {
+        x[i] = row[r] >= 0 ? load4(base, type, row[r] + 16 * (t + 4 * (i >> 2)) + 4 * (i & 3)) : make_float4(0.f, 0.f, 0.f, 0.f);
+        most = fmaxf(most, fmaxf(fmaxf(fabsf(x[i].x), fabsf(x[i].y)), fmaxf(fabsf(x[i].z), fabsf(x[i].w))));
+      }
+      most = quad_max(most);
+      // the power of two below `most`, biased; queries of tiny, infinite or no magnitude stay as they are
+      const int e = (int)(__float_as_uint(most) >> 23);
+      const float down = e < 24 || e > 240 ? 1.f : __uint_as_float((uint32_t)(e - 11) << 23);
+      const float up = e < 24 || e > 240 ? 1.f : __uint_as_float((uint32_t)(254 - (e - 11)) << 23);
+      factor[r] = scale_log2 * down;
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) {
+        const float4 y = make_float4(x[i].x * up, x[i].y * up, x[i].z * up, x[i].w * up);
+        q[i][r] = h2(y.x, y.y);
+        q[i][2 + r] = h2(y.z, y.w);
+        if (SPLIT) {
+          q[i][1] = h2_rest(y.x, y.y, q[i][0]);
+          q[i][3] = h2_rest(y.z, y.w, q[i][2]);
+        }
+      }
+    }
+  }
+
+  // One block: its codes in the lane's ring stage, its scales, and which of its tokens row r sees:
+  // tokens j with (first[r] <= j or j < sink) and j <= last[r], counted from the block's start.
+  // `all`: every row sees every token. A masked token's value codes are replaced by zeros: they may
+  // hold anything, NaN too, in a page that is not full.
+  __device__ __forceinline__ void block(const uint8_t* stage, float ks, float vs, bool all, const int (&first)[kRows],
+                                        const int (&last)[kRows], int sink, int lane) {
+    const int t = lane & 3;
+    float s[2][4];
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+#pragma unroll
+      for (int i = 0; i < Piece<D>::kK; ++i) {
+        const uint4 kw = *reinterpret_cast<const uint4*>(stage + (n * Piece<D>::kK + i) * 512 + lane * 16);
+        const uint32_t w[4] = {kw.x, kw.y, kw.z, kw.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          uint32_t b0, b1;
+          e4m3x4_f16(w[j], b0, b1);
+          mma16816(s[n], q[4 * i + j], b0, b1);
+        }
+      }
+    }
+    float x[kRows][4];  // scores of tokens 2t, 2t + 1, 2t + 8, 2t + 9
+    bool seen_by_any[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int tok = 2 * t + (j & 1) + 8 * (j >> 1);
+      seen_by_any[j] = all;
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) {
+        const float raw = SPLIT ? s[j >> 1][j & 1] + s[j >> 1][2 + (j & 1)] : s[j >> 1][2 * r + (j & 1)];
+        x[r][j] = raw * (factor[r] * ks);
+        if (!all) {
+          const bool see = (tok >= first[r] || tok < sink) && tok <= last[r];
+          if (!see) x[r][j] = -INFINITY;
+          seen_by_any[j] |= see;
+        }
+      }
+    }
+    bool grown = vs > ref;
+    float mn[kRows];
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      mn[r] = fmaxf(m[r], quad_max(fmaxf(fmaxf(x[r][0], x[r][1]), fmaxf(x[r][2], x[r][3]))));
+      grown |= mn[r] > m[r];
+    }
+    if (__any_sync(0xffffffffu, grown)) {
+      const float now = fmaxf(ref, vs);
+      const float down = ref * kv8_inverse(now);  // 0 at the first block
+      ref = now;
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) {
+        const float c = mn[r] == -INFINITY ? 1.f : exp2f(m[r] - mn[r]);
+        l[r] *= c;
+        m[r] = mn[r];
+#pragma unroll
+        for (int j = 0; j < D / 8; ++j) {
+          o[j][2 * r] *= c * down;
+          o[j][2 * r + 1] *= c * down;
+          if (SPLIT) {
+            o[j][2] *= c * down;
+            o[j][3] *= c * down;
+          }
+        }
+      }
+    }
+    const float weight = (float)(1 << kPShift) * vs * kv8_inverse(ref);
+    uint32_t p[4];
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      const float base = m[r] == -INFINITY ? 0.f : m[r];
+      float e[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        e[j] = exp2f(x[r][j] - base);
+        l[r] += e[j];
+        e[j] *= weight;
+      }
+      p[r] = h2(e[0], e[1]);
+      p[2 + r] = h2(e[2], e[3]);
+      if (SPLIT) {
+        p[1] = h2_rest(e[0], e[1], p[0]);
+        p[3] = h2_rest(e[2], e[3], p[2]);
+      }
+    }
+    const uint8_t* vb = stage + kKvBlock * D;
+    uint32_t v[4][Piece<D>::kW];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (D == 128)
+        *reinterpret_cast<uint4*>(v[j]) = *reinterpret_cast<const uint4*>(vb + j * 512 + lane * 16);
+      else
+        *reinterpret_cast<uint2*>(v[j]) = *reinterpret_cast<const uint2*>(vb + j * 256 + lane * 8);
+      if (!all && !seen_by_any_quad(seen_by_any[j]))
+#pragma unroll
+        for (int w = 0; w < Piece<D>::kW; ++w) v[j][w] = 0;
+    }
+#pragma unroll
+    for (int w = 0; w < Piece<D>::kW; ++w) {
+      const uint32_t a0 = __byte_perm(v[0][w], v[1][w], 0x5140), a1 = __byte_perm(v[0][w], v[1][w], 0x7362);
+      const uint32_t c0 = __byte_perm(v[2][w], v[3][w], 0x5140), c1 = __byte_perm(v[2][w], v[3][w], 0x7362);
+      uint32_t b00, b01, b10, b11;
+      e4m3x4_f16(a0, b00, b10);
+      e4m3x4_f16(c0, b01, b11);
+      mma16816(o[4 * w], p, b00, b01);
+      mma16816(o[4 * w + 1], p, b10, b11);
+      e4m3x4_f16(a1, b00, b10);
+      e4m3x4_f16(c1, b01, b11);
+      mma16816(o[4 * w + 2], p, b00, b01);
+      mma16816(o[4 * w + 3], p, b10, b11);
+    }
+  }
+  // Whether any row of the warp sees the token: the lanes of the same t hold the other rows.
+  __device__ __forceinline__ bool seen_by_any_quad(bool mine) const {
+    uint32_t v = mine;
+    v |= __shfl_xor_sync(0xffffffffu, v, 4);
+    v |= __shfl_xor_sync(0xffffffffu, v, 8);
+    v |= __shfl_xor_sync(0xffffffffu, v, 16);
+    return v != 0;
+  }
+  // the accumulators' unit
+  __device__ __forceinline__ float unit() const { return ref * (1.f / (1 << kPShift)); }
+};
+
+struct AttnArgs {
+  Kv8View c;
+  Kv8Table t;
+  const void* q;
+  int64_t q_stride;
+  int q_type;
+  const int* lengths;
+  const int* offsets;  // prefill
+  int64_t tokens;      // rows of q
+  int batch, heads, group;
+  int window, sinks;
+  float scale_log2;
+  void* out;
+  int out_type;
+};
+
+// ---------------------------------------------------------------------------------------------
+// Decode. Rows are (sequence, kv head, run of up to 8 of its query heads); a row's units are its
+// visible blocks. All units of the call, in order, are cut into equal shares, one a CTA (a CTA's
+// warps take every fourth block of its share of a row), so a batch of any mix of lengths fills the
+// GPU evenly. A row that lies in one share is finished there; one cut by a share's end leaves an
+// unnormalised part (running maximum, sum, 8 x D) in the workspace for kv8_join_kernel.
+constexpr int kDecWarps = 4;
+constexpr int kDecStages = 4;
+constexpr int kDecHeads = 8;
+
+struct DecArgs {
+  AttnArgs a;
+  int chunks;   // runs of 8 heads of a kv head
+  float* part;  // [2 * CTAs][kDecHeads][D + 2]
+  int64_t* cum; // [batch + 1] units of a row of the sequences before b
+};
+
+__device__ __forceinline__ int decode_blocks(const AttnArgs& a, int b) {
+  return span_of(__ldg(a.lengths + b) - 1, __ldg(a.lengths + b) - 1, a.window, a.sinks).count();
+}
+__device__ __forceinline__ int64_t share_of(int64_t units, int cta, int ctas) {
+  // shares are whole numbers of kDecWarps units, one for each warp
+  const int64_t quads = (units + kDecWarps - 1) / kDecWarps;
+  return min(units, quads * cta / ctas * kDecWarps);
+}
+
+template <int D>
+__global__ void __launch_bounds__(kDecWarps * 32, 3) kv8_decode_kernel(const DecArgs d) {
+  const AttnArgs& a = d.a;
+  extern __shared__ __align__(128) uint8_t smem[];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+  const int rows = a.c.kv_heads * d.chunks;
+  const Kv8Place at = kv8_find<kDecWarps * 32>(
+      a.batch, [&](int b) -> int64_t { return (int64_t)decode_blocks(a, b) * rows; },
+      [&](int64_t units) -> int64_t { return share_of(units, blockIdx.x, gridDim.x); });
+  int64_t left = at.seq < 0 ? 0 : share_of(at.total, blockIdx.x + 1, gridDim.x) - share_of(at.total, blockIdx.x, gridDim.x);
+  if (blockIdx.x == 0 && tid == 0) {  // for the join
+    int64_t sum = 0;
+    for (int b = 0; b < a.batch; ++b) {
+      d.cum[b] = sum;
+      sum += decode_blocks(a, b);
+    }
+    d.cum[a.batch] = sum;
+  }
+  uint8_t* ring = smem + warp * (kDecStages * Piece<D>::kStage);
+  const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
+  // the merge of the warps' states reuses the rings (drained by then): per warp m, l, then 8 x D
+  float* merge = reinterpret_cast<float*>(ring);
+  constexpr int kMergeStride = kDecStages * Piece<D>::kStage / 4;
+  static_assert(kMergeStride >= kDecHeads * (D + 2), "a warp's state must fit its ring");
+  int b = at.seq;
+  int64_t in_seq = at.at;
+  int segment = 0;
+  Warp<D, true> w;
+  while (left > 0) {
+    const int len = __ldg(a.lengths + b);
+    const Span span = span_of(len - 1, len - 1, a.window, a.sinks);
+    const int nb = span.count();
+    if (in_seq >= (int64_t)nb * rows) {
+      ++b;
+      in_seq = 0;
+      continue;
+    }
+    const int row = (int)(in_seq / nb), begin = (int)(in_seq % nb);
+    const int end = (int)min((int64_t)nb, begin + left);
+    const int head = row / d.chunks, h0 = head * a.group + row % d.chunks * kDecHeads;
+    const int nh = min(kDecHeads, (head + 1) * a.group - h0);
+    const int lo = a.window > 0 ? max(0, len - a.window) : 0;
+    w.reset();
+    {
+      const int64_t qrow[1] = {g < nh ? (int64_t)b * a.q_stride + (int64_t)(h0 + g) * D : -1};
+      w.load_q(a.q, a.q_type, qrow, a.scale_log2, t);
+    }
+    // Blocks begin + warp + 4 i; lane i of 32 looks up the page, scales of the i-th
+    const int mine = max(0, (end - begin - warp + kDecWarps - 1) / kDecWarps);
+    for (int base = 0; base < mine; base += 32) {
+      const int n = min(32, mine - base);
+      int id = -1;
+      float ks = 0.f, vs = 0.f;
+      int blk = 0;
+      if (lane < n) {
+        blk = span.block(begin + warp + kDecWarps * (base + lane));
+        id = kv8_block_id(a.c, a.t, b, head, blk);
+        if (id >= 0) {
+          ks = __ldg(a.c.ks + id);
+          vs = __ldg(a.c.vs + id);
+        }
+      }
+#pragma unroll
+      for (int s = 0; s < kDecStages - 1; ++s) {
+        const int nid = __shfl_sync(0xffffffffu, id, s);
+        if (s < n && nid >= 0) fetch<D>(a.c, nid, ring_at + s * Piece<D>::kStage, lane);
+        cp_commit();
+      }
+      for (int i = 0; i < n; ++i) {
+        {
+          const int next = i + kDecStages - 1;
+          const int nid = __shfl_sync(0xffffffffu, id, next & 31);
+          if (next < n && nid >= 0) fetch<D>(a.c, nid, ring_at + next % kDecStages * Piece<D>::kStage, lane);
+          cp_commit();
+        }
+        cp_wait<kDecStages - 1>();
+        if (__shfl_sync(0xffffffffu, id, i) < 0) continue;
+        const int p0 = __shfl_sync(0xffffffffu, blk, i) * kKvBlock;
+        const float kss = __shfl_sync(0xffffffffu, ks, i), vss = __shfl_sync(0xffffffffu, vs, i);
+        const bool all = p0 + kKvBlock <= len && (p0 >= lo || p0 + kKvBlock <= a.sinks);
+        const int first[1] = {lo - p0}, last[1] = {len - 1 - p0};
+        w.block(ring + i % kDecStages * Piece<D>::kStage, kss, vss, all, first, last, a.sinks - p0, lane);
+      }
+      cp_wait<0>();
+    }
+    // merge the warps
+    __syncwarp();
+    {
+      const float l = quad_sum(w.l[0]), unit = w.unit();
+      float* mm = merge + g * (D + 2);
+      if (t == 0) {
+        mm[0] = w.m[0];
+        mm[1] = l;
+      }
+      // columns of tile j are dims (D / 8) n + j: this thread's n are 2t and 2t + 1
+#pragma unroll
+      for (int j = 0; j < D / 8; ++j) {
+        mm[2 + (D / 8) * (2 * t) + j] = (w.o[j][0] + w.o[j][2]) * unit;
+        mm[2 + (D / 8) * (2 * t + 1) + j] = (w.o[j][1] + w.o[j][3]) * unit;
+      }
+    }
+    __syncthreads();
+    const bool whole = begin == 0 && end == nb;
+    const float* all = reinterpret_cast<const float*>(smem);
+    for (int e = tid; e < nh * (D / 4); e += kDecWarps * 32) {
+      const int h = e / (D / 4), c = e % (D / 4) * 4;
+      float mt = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < kDecWarps; ++i) mt = fmaxf(mt, all[i * kMergeStride + h * (D + 2)]);
+      float lt = 0.f;
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int i = 0; i < kDecWarps; ++i) {
+        const float* src = all + i * kMergeStride + h * (D + 2);
+        const float f = src[0] == -INFINITY ? 0.f : exp2f(src[0] - mt);
+        lt = fmaf(src[1], f, lt);
+        v.x = fmaf(src[2 + c], f, v.x);
+        v.y = fmaf(src[3 + c], f, v.y);
+        v.z = fmaf(src[4 + c], f, v.z);
+        v.w = fmaf(src[5 + c], f, v.w);
+      }
+      if (whole) {
+        const float inv = mt == -INFINITY ? 0.f : 1.f / lt;
+        if (mt == -INFINITY) v = make_float4(0.f, 0.f, 0.f, 0.f);
+        store4(a.out, a.out_type, ((int64_t)b * a.heads + h0 + h) * D + c, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
+      } else {
+        float* dst = d.part + (((int64_t)blockIdx.x * 2 + (segment > 0)) * kDecHeads + h) * (D + 2);
+        if (c == 0) {
+          dst[0] = mt;
+          dst[1] = lt;
+        }
+        *reinterpret_cast<float2*>(dst + 2 + c) = make_float2(v.x, v.y);
+        *reinterpret_cast<float2*>(dst + 4 + c) = make_float2(v.z, v.w);
+      }
+    }
+    __syncthreads();
+    left -= end - begin;
+    in_seq += end - begin;
+    ++segment;
+  }
+}
+
+// Rows without a block give zeros; rows cut into parts are joined in the order of the parts. One
+// warp per (sequence, query head).
+template <int D>
+__global__ void __launch_bounds__(128) kv8_join_kernel(const DecArgs d, int ctas) {
+  const AttnArgs& a = d.a;
+  const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (i >= (int64_t)a.batch * a.heads) return;
+  const int b = (int)(i / a.heads), qh = (int)(i % a.heads);
+  const int head = qh / a.group, chunk = qh % a.group / kDecHeads, h = qh % a.group % kDecHeads;
+  const int rows = a.c.kv_heads * d.chunks;
+  const int64_t before = d.cum[b], units = d.cum[a.batch] * rows;
+  const int nb = (int)(d.cum[b + 1] - before);
+  constexpr int kPer = D / 32;
+  float acc[kPer];
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) acc[e] = 0.f;
+  float lt = 0.f;
+  if (nb > 0) {
+    const int64_t u0 = before * rows + (int64_t)(head * d.chunks + chunk) * nb, u1 = u0 + nb;
+    // the share that holds u0: shares are close to even, so start from the estimate
+    int cta = (int)(u0 / (double)units * ctas);
+    cta = max(0, min(ctas - 1, cta));
+    while (cta > 0 && share_of(units, cta, ctas) > u0) --cta;
+    while (share_of(units, cta + 1, ctas) <= u0) ++cta;
+    if (share_of(units, cta + 1, ctas) >= u1) return;  // finished by its CTA
+    float mt = -INFINITY;
+    for (int c = cta; share_of(units, c, ctas) < u1; ++c) {
+      const int64_t s0 = share_of(units, c, ctas);
+      if (share_of(units, c + 1, ctas) == s0) continue;
+      const int slot = 2 * c + (s0 < u0);  // a share's first segment, or a later one
+      const float* src = d.part + ((int64_t)slot * kDecHeads + h) * (D + 2);
+      const float ms = src[0];
+      if (ms == -INFINITY) continue;
+      const float mn = fmaxf(mt, ms), f0 = mt == -INFINITY ? 0.f : exp2f(mt - mn), f1 = exp2f(ms - mn);
+      mt = mn;
+      lt = lt * f0 + src[1] * f1;
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) acc[e] = acc[e] * f0 + src[2 + lane + 32 * e] * f1;
+    }
+  }
+  const float inv = nb > 0 && lt != 0.f ? 1.f / lt : 0.f;
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) {
+    const int64_t o = ((int64_t)b * a.heads + qh) * D + lane + 32 * e;
+    if (a.out_type == J4B_F32)
+      static_cast<float*>(a.out)[o] = acc[e] * inv;
+    else
+      static_cast<__nv_bfloat16*>(a.out)[o] = __float2bfloat16_rn(acc[e] * inv);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// Prefill. A CTA of 4 warps takes 64 consecutive rows of one (sequence, kv head): row r is query
+// r / group, head r % group of the group; a warp 16 of them. The warps walk the same blocks, each
+// through its own ring (the others' copies come from L1/L2).
+constexpr int kPreWarps = 4;
+constexpr int kPreRows = 16 * kPreWarps;
+
+template <int D>
+__global__ void __launch_bounds__(kPreWarps * 32, 3) kv8_prefill_kernel(const AttnArgs a) {
+  extern __shared__ __align__(128) uint8_t smem[];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+  const int head = blockIdx.y;
+  const Kv8Place at = kv8_find<kPreWarps * 32>(
+      a.batch, [&](int b) -> int64_t { return ((int64_t)max(0, a.offsets[b + 1] - a.offsets[b]) * a.group + kPreRows - 1) / kPreRows; },
+      [&](int64_t total) -> int64_t { return total - 1 - (int64_t)blockIdx.x < 0 ? total : total - 1 - (int64_t)blockIdx.x; });
+  if (at.seq < 0) return;
+  const int b = at.seq, row0 = a.offsets[b], n = a.offsets[b + 1] - row0, len = __ldg(a.lengths + b);
+  const int total_rows = n * a.group, r0 = (int)at.at * kPreRows;
+  const int first_q = r0 / a.group, last_q = (min(total_rows, r0 + kPreRows) - 1) / a.group;
+  const int pos0 = len - n;  // position of query 0 (negative: the first queries are before the cache and see nothing)
+  const Span span = span_of(max(0, pos0 + first_q), min(len - 1, pos0 + last_q), a.window, a.sinks);
+  const int nb = max(0, span.count());
+  Warp<D, false> w;
+  w.reset();
+  int qp[2], lo[2];
+  int64_t qrow[2], orow[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int r = r0 + warp * 16 + g + 8 * i;
+    const int tok = r / a.group;
+    const int64_t row = row0 + tok;
+    const bool ok = r < total_rows && row >= 0 && row < a.tokens;
+    qrow[i] = ok ? row * a.q_stride + (int64_t)(head * a.group + r % a.group) * D : -1;
+    orow[i] = ok ? (row * a.heads + head * a.group + r % a.group) * D : -1;
+    qp[i] = ok ? pos0 + tok : -1;
+    lo[i] = a.window > 0 ? max(0, qp[i] - a.window + 1) : 0;
+  }
+  w.load_q(a.q, a.q_type, qrow, a.scale_log2, t);
+  const int least = __reduce_min_sync(0xffffffffu, min(qp[0], qp[1])), most_lo = __reduce_max_sync(0xffffffffu, max(lo[0], lo[1]));
+  uint8_t* ring = smem + warp * (kDecStages * Piece<D>::kStage);
+  const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
+  for (int base = 0; base < nb; base += 32) {
+    const int m = min(32, nb - base);
+    int id = -1;
+    float ks = 0.f, vs = 0.f;
+    const int blk = span.block(base + lane);
+    if (lane < m) {
+      id = kv8_block_id(a.c, a.t, b, head, blk);
+      if (id >= 0) {
+        ks = __ldg(a.c.ks + id);
+        vs = __ldg(a.c.vs + id);
+      }
+    }
+#pragma unroll
+    for (int s = 0; s < kDecStages - 1; ++s) {
+      const int nid = __shfl_sync(0xffffffffu, id, s);
+      if (s < m && nid >= 0) fetch<D>(a.c, nid, ring_at + s * Piece<D>::kStage, lane);
+      cp_commit();
+    }
+    for (int i = 0; i < m; ++i) {
+      {
+        const int next = i + kDecStages - 1;
+        const int nid = __shfl_sync(0xffffffffu, id, next & 31);
+        if (next < m && nid >= 0) fetch<D>(a.c, nid, ring_at + next % kDecStages * Piece<D>::kStage, lane);
+        cp_commit();
+      }
+      cp_wait<kDecStages - 1>();
+      if (__shfl_sync(0xffffffffu, id, i) < 0) continue;
+      const int p0 = __shfl_sync(0xffffffffu, blk, i) * kKvBlock;
+      const float kss = __shfl_sync(0xffffffffu, ks, i), vss = __shfl_sync(0xffffffffu, vs, i);
+      const bool all = p0 + kKvBlock - 1 <= least && (p0 >= most_lo || p0 + kKvBlock <= a.sinks);
+      const int first[2] = {lo[0] - p0, lo[1] - p0}, last[2] = {qp[0] - p0, qp[1] - p0};
+      w.block(ring + i % kDecStages * Piece<D>::kStage, kss, vss, all, first, last, a.sinks - p0, lane);
+    }
+    cp_wait<0>();
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const float l = quad_sum(w.l[i]);
+    const float inv = w.m[i] == -INFINITY ? 0.f : w.unit() / l;
+    if (orow[i] < 0) continue;
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int j = 0; j < D / 8; j += 4) {
+        const float4 v = make_float4(w.o[j][2 * i + c] * inv, w.o[j + 1][2 * i + c] * inv, w.o[j + 2][2 * i + c] * inv, w.o[j + 3][2 * i + c] * inv);
+        store4(a.out, a.out_type, orow[i] + (D / 8) * (2 * t + c) + j, w.m[i] == -INFINITY ? make_float4(0.f, 0.f, 0.f, 0.f) : v);
+      }
+  }
+}
+
+int check_attention(const j4b_kv8_cache* cache, int64_t layer, j4b_buf q, int q_type, int64_t q_stride, int64_t tokens, int64_t heads,
+                    j4b_buf table, int64_t table_stride, int64_t table_width, j4b_buf lengths, int64_t batch, int64_t window, int64_t sinks,
+                    double scale, j4b_buf out, int out_type, AttnArgs* a, int* dev) {
+  Kv8View view;
+  if (const int st = kv8_check(cache, layer, &view, dev)) return st;
+  J4B_REQUIRE(heads > 0 && heads <= 65536 && heads % cache->kv_heads == 0, "kv8 attention: heads (%lld) must be a multiple of kv_heads (%d)",
+              (long long)heads, cache->kv_heads);
+  J4B_REQUIRE(batch >= 0 && batch <= 0xffffff && tokens >= 0 && tokens <= 0x7fffffff, "kv8 attention: bad batch or token count");
+  J4B_REQUIRE((q_type == J4B_F32 || q_type == J4B_BF16) && (out_type == J4B_F32 || out_type == J4B_BF16),
+              "kv8 attention: q and out types must be f32 or bf16, got %d and %d", q_type, out_type);
+  J4B_REQUIRE(q_stride >= heads * cache->head_dim && q_stride % 8 == 0, "kv8 attention: rows of q must be at least heads * head_dim elements and a multiple of 8 apart");
+  J4B_REQUIRE(table_width > 0 && table_width <= 0x7ffffff && table_stride >= table_width, "kv8 attention: bad page table shape");
+  J4B_REQUIRE(window >= 0 && sinks >= 0, "kv8 attention: window and sinks must not be negative");
+  J4B_REQUIRE(std::isfinite(scale), "kv8 attention: scale must be finite");
+  if (batch > 0 && tokens > 0)
+    J4B_REQUIRE(q && table && lengths && out && ((q | out) & 15) == 0 && ((table | lengths) & 3) == 0, "kv8 attention: misaligned or null buffers");
+  const int64_t far = 0x3fffffff;
+  *a = {view,
+        {(const int*)(uintptr_t)table, table_stride, (int)table_width},
+        (const void*)(uintptr_t)q,
+        q_stride,
+        q_type,
+        (const int*)(uintptr_t)lengths,
+        nullptr,
+        tokens,
+        (int)batch,
+        (int)heads,
+        (int)(heads / cache->kv_heads),
+        (int)std::min(window, far),
+        window > 0 ? (int)std::min(sinks, far) : 0,
+        (float)(scale * 1.4426950408889634),
+        (void*)(uintptr_t)out,
+        out_type};
+  return J4B_OK;
+}
+
+int decode_ctas(int dev) {
+  const DeviceCtx* ctx = device_ctx(dev);
+  return 3 * (ctx && ctx->sm_count > 0 ? ctx->sm_count : 148);
+}
+
+int64_t decode_bytes(int dim, int64_t batch, int ctas) {
+  const int64_t part = (int64_t)2 * ctas * kDecHeads * (dim + 2) * 4;
+  return (part + 15) / 16 * 16 + (batch + 1) * 8;
+}
+
+template <class Kernel>
+int allow_smem(Kernel kernel, int bytes, int dev, bool (&done)[kMaxDevices]) {
+  if (!done[dev]) {
+    J4B_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), "cudaFuncSetAttribute");
+    done[dev] = true;
+  }
+  return J4B_OK;
+}
+
+template <int D>
+int launch_decode(const DecArgs& d, int dev, int ctas, cudaStream_t stream) {
+  static bool done[kMaxDevices] = {};
+  const int smem = kDecWarps * kDecStages * Piece<D>::kStage;
+  if (const int st = allow_smem(kv8_decode_kernel<D>, smem, dev, done)) return st;
+  kv8_decode_kernel<D><<<ctas, kDecWarps * 32, smem, stream>>>(d);
+  J4B_CHECK_LAUNCH("kv8_decode_kernel");
+  const int64_t rows = (int64_t)d.a.batch * d.a.heads;
+  kv8_join_kernel<D><<<(unsigned)((rows + 3) / 4), 128, 0, stream>>>(d, ctas);
+  J4B_CHECK_LAUNCH("kv8_join_kernel");
+  return J4B_OK;
+}
+
+template <int D>
+int launch_prefill(const AttnArgs& a, int dev, cudaStream_t stream) {
+  static bool done[kMaxDevices] = {};
+  const int smem = kPreWarps * kDecStages * Piece<D>::kStage;
+  if (const int st = allow_smem(kv8_prefill_kernel<D>, smem, dev, done)) return st;
+  const int64_t tiles = std::min(a.tokens * a.group, a.tokens * a.group / kPreRows + a.batch);
+  J4B_REQUIRE(tiles <= 0x7fffffffLL, "kv8 prefill: too many rows");
+  kv8_prefill_kernel<D><<<dim3((unsigned)tiles, (unsigned)a.c.kv_heads), kPreWarps * 32, smem, stream>>>(a);
+  J4B_CHECK_LAUNCH("kv8_prefill_kernel");
+  return J4B_OK;
+}
+
+}  // namespace
+}  // namespace j4b
+
+using namespace j4b;
+
+extern "C" int j4b_kv8_decode_workspace(const j4b_kv8_cache* cache, int64_t heads, int64_t batch, int64_t* bytes) {
+  J4B_REQUIRE(bytes, "kv8 decode: bytes is null");
+  Kv8View view;
+  int dev = 0;
+  if (const int st = kv8_check(cache, 0, &view, &dev)) return st;
+  J4B_REQUIRE(heads > 0 && batch >= 0 && batch <= 0xffffff, "kv8 decode: bad heads or batch");
+  *bytes = decode_bytes(cache->head_dim, batch, decode_ctas(dev));
+  return J4B_OK;
+}
+
+extern "C" int j4b_kv8_attention_decode(const j4b_kv8_cache* cache, int64_t layer, j4b_buf q, int q_type, int64_t q_stride, int64_t heads,
+                                        j4b_buf table, int64_t table_stride, int64_t table_width, j4b_buf lengths, int64_t batch,
+                                        int64_t window, int64_t sinks, double scale, j4b_buf out, int out_type, j4b_buf workspace,
+                                        int64_t workspace_bytes, j4b_stream s) {
+  DecArgs d;
+  int dev = 0;
+  if (const int st = check_attention(cache, layer, q, q_type, q_stride, batch, heads, table, table_stride, table_width, lengths, batch,
+                                     window, sinks, scale, out, out_type, &d.a, &dev))
+    return st;
+  if (batch == 0) return J4B_OK;
+  const int ctas = decode_ctas(dev);
+  J4B_REQUIRE(workspace && (workspace & 15) == 0 && workspace_bytes >= decode_bytes(cache->head_dim, batch, ctas),
+              "kv8 decode: workspace must be 16-byte aligned and hold %lld bytes", (long long)decode_bytes(cache->head_dim, batch, ctas));
+  DeviceGuard guard(dev);
+  cudaStream_t stream = resolve_stream(dev, s);
+  d.chunks = (d.a.group + kDecHeads - 1) / kDecHeads;
+  d.part = (float*)(uintptr_t)workspace;
+  d.cum = (int64_t*)((uintptr_t)workspace + ((int64_t)2 * ctas * kDecHeads * (cache->head_dim + 2) * 4 + 15) / 16 * 16);
+  return cache->head_dim == 128 ? launch_decode<128>(d, dev, ctas, stream) : launch_decode<64>(d, dev, ctas, stream);
+}
+
+extern "C" int j4b_kv8_attention_prefill(const j4b_kv8_cache* cache, int64_t layer, j4b_buf q, int q_type, int64_t q_stride, int64_t tokens,
+                                         int64_t heads, j4b_buf offsets, j4b_buf table, int64_t table_stride, int64_t table_width,
+                                         j4b_buf lengths, int64_t batch, int64_t window, int64_t sinks, double scale, j4b_buf out,
+                                         int out_type, j4b_stream s) {
+  AttnArgs a;
+  int dev = 0;
+  if (const int st = check_attention(cache, layer, q, q_type, q_stride, tokens, heads, table, table_stride, table_width, lengths, batch,
+                                     window, sinks, scale, out, out_type, &a, &dev))
+    return st;
+  if (batch == 0 || tokens == 0) return J4B_OK;
+  J4B_REQUIRE(offsets && (offsets & 3) == 0, "kv8 prefill: misaligned or null offsets");
+  a.offsets = (const int*)(uintptr_t)offsets;
+  DeviceGuard guard(dev);
+  cudaStream_t stream = resolve_stream(dev, s);
+  return cache->head_dim == 128 ? launch_prefill<128>(a, dev, stream) : launch_prefill<64>(a, dev, stream);
+}

@@ -1,0 +1,148 @@
+// The 8-bit paged KV cache: what its kernels share (kv8_cache.cu, kv8_attn.cu).
+//
+// Codes are e4m3 [layers, pages, kv_heads, page, head_dim], for keys and for values. The 16-token
+// block is the unit everywhere: page is a multiple of 16, a block of one head is 16 * head_dim
+// contiguous bytes and has one f32 scale, a power of two, in [layers, pages, kv_heads, page / 16].
+// A value is code * scale. So a block's number, (page * kv_heads + head) * (page / 16) + block in
+// page, indexes the scales directly and the codes times 16 * head_dim.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "j4b_internal.h"
+
+namespace j4b {
+
+constexpr int kKvBlock = 16;       // tokens that share a scale
+constexpr float kE4m3Max = 448.f;  // 1.75 * 2^8
+
+// One layer's cache as the kernels take it.
+struct Kv8View {
+  uint8_t* k;
+  uint8_t* v;
+  float* ks;
+  float* vs;
+  int pages, kv_heads, bpp;  // bpp: blocks of a page
+};
+
+// The sequences' pages: row b of the table names them in token order (-1 or any number outside
+// [0, pages): unmapped).
+struct Kv8Table {
+  const int* pages;
+  int64_t stride;
+  int width;
+};
+
+__device__ __forceinline__ int kv8_block_id(const Kv8View& c, const Kv8Table& t, int b, int head, int blk) {
+  const int pg = blk / c.bpp;
+  if (pg >= t.width) return -1;
+  const int id = __ldg(t.pages + b * t.stride + pg);
+  if ((unsigned)id >= (unsigned)c.pages) return -1;
+  return (id * c.kv_heads + head) * c.bpp + (blk - pg * c.bpp);
+}
+
+// The smallest power of two s >= 2^-120 with amax <= 448 s, from amax's exponent and mantissa
+// (amax = m 2^E, 1 <= m < 2: s = 2^(E - 8) if m <= 1.75, else 2^(E - 7)). A power of two costs no
+// accuracy (the codes are floating point) and a block's scale can grow without rounding its codes
+// again. amax is finite and not negative.
+__device__ __forceinline__ float kv8_scale(float amax) {
+  const uint32_t u = __float_as_uint(amax);
+  int e = (int)(u >> 23) - 8 + ((u & 0x7fffffu) > 0x600000u);
+  e = e < 7 ? 7 : e;  // biased: 2^-120 and above
+  return __uint_as_float((uint32_t)e << 23);
+}
+// 1 / s of a power of two in [2^-120, 2^120]
+__device__ __forceinline__ float kv8_inverse(float s) { return __uint_as_float((254u << 23) - __float_as_uint(s)); }
+
+// two f32 -> two e4m3 (round to nearest even, saturating; lo in the low byte)
+__device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %2, %1;" : "=h"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) { return e4m3x2(a, b) | (e4m3x2(c, d) << 16); }
+// two e4m3 -> f16x2, exact
+__device__ __forceinline__ uint32_t e4m3_f16x2(uint16_t v) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(v));
+  return r;
+}
+__device__ __forceinline__ void e4m3x4_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  uint16_t a, b;
+  asm("mov.b32 {%0, %1}, %2;" : "=h"(a), "=h"(b) : "r"(w));
+  lo = e4m3_f16x2(a);
+  hi = e4m3_f16x2(b);
+}
+
+// Activation element types of the entry points (J4B_F32, J4B_BF16).
+__device__ __forceinline__ float4 load4(const void* p, int type, int64_t i) {
+  if (type == J4B_F32) return *reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
+  const uint2 u = *reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(p) + i);
+  return make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16),
+                     __uint_as_float(u.y & 0xffff0000u));
+}
+__device__ __forceinline__ void store4(void* p, int type, int64_t i, float4 v) {
+  if (type == J4B_F32) {
+    *reinterpret_cast<float4*>(static_cast<float*>(p) + i) = v;
+  } else {
+    const __nv_bfloat162 a = __floats2bfloat162_rn(v.x, v.y), b = __floats2bfloat162_rn(v.z, v.w);
+    uint2 u;
+    u.x = *reinterpret_cast<const uint32_t*>(&a);
+    u.y = *reinterpret_cast<const uint32_t*>(&b);
+    *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p) + i) = u;
+  }
+}
+
+// Where a unit of work lies when sequence b has count(b) consecutive units.
+struct Kv8Place {
+  int seq;        // -1: past the last unit
+  int64_t at;     // its number among the sequence's
+  int64_t total;  // units of all sequences
+};
+
+// Finds unit unit(total) for a CTA of THREADS threads (all of them call it): every thread sums a
+// contiguous share of the sequences, the shares are scanned, and the thread whose share holds the
+// unit walks it.
+template <int THREADS, class Count, class Unit>
+__device__ __forceinline__ Kv8Place kv8_find(int batch, Count count, Unit unit) {
+  __shared__ int64_t warp_sum[THREADS / 32];
+  __shared__ int64_t found_at;
+  __shared__ int found_seq;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int per = (batch + THREADS - 1) / THREADS;
+  const int b0 = min(batch, tid * per), b1 = min(batch, b0 + per);
+  int64_t mine = 0;
+  for (int b = b0; b < b1; ++b) mine += count(b);
+  int64_t incl = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t up = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += up;
+  }
+  if (lane == 31) warp_sum[warp] = incl;
+  __syncthreads();
+  int64_t before = incl - mine, total = 0;
+#pragma unroll
+  for (int w = 0; w < THREADS / 32; ++w) {
+    if (w < warp) before += warp_sum[w];
+    total += warp_sum[w];
+  }
+  int64_t left = unit(total) - before;
+  if (left >= 0 && left < mine) {
+    int b = b0;
+    for (int64_t n; left >= (n = count(b)); ++b) left -= n;
+    found_seq = b;
+    found_at = left;
+  } else if (tid == 0 && unit(total) >= total) {
+    found_seq = -1;
+    found_at = 0;
+  }
+  __syncthreads();
+  return {found_seq, found_at, total};
+}
+
+}  // namespace j4b

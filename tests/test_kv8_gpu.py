@@ -1,0 +1,429 @@
+"""GPU parity of the 8-bit paged KV cache's operators against the float64 oracle (oracle/kv8.py).
+
+Bars, derived from the arithmetic:
+  - append: rotations are two products and one sum, each rounded in f32, as numpy's float32 does
+    them; everything after is exact or rounded by the format, so codes, scales and f32 queries are
+    equal bit for bit.
+  - decode: scores carry f32 rounding (|s| up to ~16 here: 16 * 2^-20 in the exponent), the second
+    product f32 rounding: normwise 3e-5. A bf16 output adds half a unit, 2^-9 of the value.
+  - prefill: f16 probabilities (2^-11 each) and f16 queries where they come as f32 (2^-11 of a
+    score): the engine's tensor-core bar, normwise 1e-2.
+  - copies: equal.
+"""
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+DECODE_BAR, PREFILL_BAR = 3e-5, 1e-2
+
+
+def normwise(got, ref):
+    return float(np.abs(np.asarray(got, np.float64) - ref).max() / max(np.abs(ref).max(), 1e-30))
+
+
+def to_f8(values):
+    return torch.from_numpy(np.ascontiguousarray(values, dtype=np.float32)).cuda().to(torch.float8_e4m3fn)
+
+
+def ints(x):
+    return torch.tensor(np.asarray(x), dtype=torch.int32, device="cuda")
+
+
+def make_pool(rng, pages, kv, page, dim):
+    """Random (codes, scales) of one layer, blocks of different scales."""
+    from oracle.kv8 import BLOCK, e4m3, scale_of
+    x = rng.standard_normal((pages, kv, page // BLOCK, BLOCK, dim)) * 10.0 ** rng.uniform(-1, 1, (pages, kv, page // BLOCK, 1, 1))
+    s = np.vectorize(scale_of)(np.abs(x).max((-1, -2)))
+    return e4m3(x / s[..., None, None]).reshape(pages, kv, page, dim), s
+
+
+class Pool:
+    """A layer's cache on the host and the device, and sequences of given lengths on random pages.
+    Everything that no sequence holds is NaN: unused pages, slots past a length, their scales."""
+
+    def __init__(self, rng, lengths, kv, page, dim, spare=2, layers=1, layer=0, room=0):
+        from jax4j_b200.kv8 import Kv8Cache
+        mapped = [-(-(n + room) // page) for n in lengths]
+        pages = sum(mapped) + spare
+        self.k, self.ks = make_pool(rng, pages, kv, page, dim)
+        self.v, self.vs = make_pool(rng, pages, kv, page, dim)
+        order = rng.permutation(pages)
+        self.table = np.full((len(lengths), max(1, max(mapped))), -1)
+        at = 0
+        for b, m in enumerate(mapped):
+            self.table[b, :m] = order[at:at + m]
+            at += m
+        self.lengths = list(lengths)
+        self.kv, self.page, self.dim = kv, page, dim
+        codes = [np.full(self.k.shape, np.nan) for _ in range(2)]
+        for b, n in enumerate(lengths):
+            for j0 in range(0, n, page):
+                pg, m = self.table[b, j0 // page], min(page, n - j0)
+                for dst, src in zip(codes, (self.k, self.v)):
+                    dst[pg, :, :m] = src[pg, :, :m]
+        self.codes = codes
+        self.cache = Kv8Cache(pages, kv, page, dim, layers)
+        self.layer = layer
+        for t, c in ((self.cache.k, codes[0]), (self.cache.v, codes[1])):
+            t[layer].view(torch.uint8).copy_(to_f8(c).view(torch.uint8))
+        self.cache.k_scale[layer] = torch.from_numpy(self.ks).float()
+        self.cache.v_scale[layer] = torch.from_numpy(self.vs).float()
+
+    def unmap(self, b, pages):
+        self.table[b, pages] = -1
+
+    def reference(self, q, b, first_pos, window, sinks, scale=None):
+        from oracle.kv8 import attention, values
+        return attention(np.asarray(q, np.float64), values(self.k, self.ks), values(self.v, self.vs), self.table[b], self.lengths[b], first_pos,
+                         window, sinks, scale)
+
+
+DECODE = [
+    # lengths, heads, kv_heads, dim, page, window, sinks
+    ([0, 1, 2, 15, 16, 17, 100, 0], 4, 4, 128, 32, 0, 0),
+    ([1], 1, 1, 64, 16, 0, 0),
+    ([33, 200, 7], 8, 2, 128, 64, 0, 0),
+    ([33, 200, 7], 16, 2, 64, 48, 0, 0),
+    ([129, 64], 15, 3, 128, 16, 0, 0),       # 5 heads a group
+    ([300, 77, 1], 24, 2, 128, 128, 0, 0),   # 12 heads a group: two runs
+    ([3001], 8, 1, 64, 64, 0, 0),            # one row on many CTAs
+    ([5000, 3, 0, 1234], 2, 1, 128, 32, 0, 0),
+    ([100, 400, 31, 0], 6, 2, 128, 32, 40, 0),
+    ([100, 400, 31, 50], 6, 2, 64, 16, 40, 5),
+    ([257, 90], 4, 1, 128, 64, 1, 1),
+    ([1000, 999], 4, 4, 128, 32, 100, 37),
+    ([500], 4, 4, 128, 32, 600, 4),          # a window longer than the sequence
+    ([70, 90], 4, 2, 128, 32, 20, 60),       # sinks that reach the window
+]
+
+
+@pytest.mark.parametrize("lengths,heads,kv,dim,page,window,sinks", DECODE)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_decode_matches_float64(lengths, heads, kv, dim, page, window, sinks, dtype):
+    rng = np.random.default_rng(len(lengths) + heads + dim + window)
+    pool = Pool(rng, lengths, kv, page, dim)
+    q = torch.from_numpy(rng.standard_normal((len(lengths), heads, dim)).astype(np.float32)).cuda().to(dtype)
+    out = pool.cache.attention_decode(q, ints(pool.table), ints(lengths), window=window, sinks=sinks)
+    assert out.dtype == dtype
+    full = pool.cache.attention_decode(q, ints(pool.table), ints(lengths), window=window, sinks=sinks, out_dtype=torch.float32)
+    assert torch.equal(out, full.to(dtype))
+    qh, got = q.double().cpu().numpy(), full.cpu().numpy()
+    ref = np.stack([pool.reference(qh[b:b + 1], b, n - 1, window, sinks)[0] for b, n in enumerate(lengths)])
+    assert np.all(np.isfinite(got))
+    assert not got[np.array(lengths) == 0].any()
+    assert normwise(got, ref) <= DECODE_BAR
+
+
+def test_decode_takes_strided_queries_tables_and_other_output_types():
+    rng = np.random.default_rng(5)
+    lengths, heads, kv, dim = [40, 9, 120], 4, 2, 128
+    pool = Pool(rng, lengths, kv, 32, dim, layers=3, layer=2)
+    wide = torch.from_numpy(rng.standard_normal((3, (heads + 2 * kv) * dim)).astype(np.float32)).cuda()
+    q = wide[:, :heads * dim].unflatten(1, (heads, dim))  # rows further apart than heads * dim
+    table = torch.full((3, pool.table.shape[1] + 5), 10 ** 6, dtype=torch.int32, device="cuda")
+    table[:, :pool.table.shape[1]] = ints(pool.table)
+    ref = np.stack([pool.reference(q.double().cpu().numpy()[b:b + 1], b, n - 1, 0, 0, 0.2)[0] for b, n in enumerate(lengths)])
+    out = torch.full((3, heads, dim), 7.0, dtype=torch.bfloat16, device="cuda")
+    got = pool.cache.attention_decode(q, table[:, :pool.table.shape[1]], ints(lengths), scale=0.2, layer=2, out=out)
+    assert got is out
+    full = pool.cache.attention_decode(q, table, ints(lengths), scale=0.2, layer=2)  # entries past the pages are not pages
+    assert normwise(full.cpu().numpy(), ref) <= DECODE_BAR
+    assert torch.equal(out, full.to(torch.bfloat16))
+
+
+def test_decode_skips_unmapped_pages_and_gives_zeros_where_nothing_is_seen():
+    rng = np.random.default_rng(6)
+    lengths, heads, kv, dim, page = [300, 100, 64], 4, 2, 64, 32
+    pool = Pool(rng, lengths, kv, page, dim)
+    pool.unmap(0, [1, 4, 9])
+    pool.unmap(1, slice(None))
+    q = torch.from_numpy(rng.standard_normal((3, heads, dim)).astype(np.float32)).cuda()
+    got = pool.cache.attention_decode(q, ints(pool.table), ints(lengths)).double().cpu().numpy()
+    ref = np.stack([pool.reference(q.double().cpu().numpy()[b:b + 1], b, n - 1, 0, 0)[0] for b, n in enumerate(lengths)])
+    assert not got[1].any()
+    assert normwise(got, ref) <= DECODE_BAR
+    # a length past the mapped pages sees what is mapped
+    short = pool.cache.attention_decode(q, ints(pool.table[:, :2]), ints(lengths)).double().cpu().numpy()
+    pool.table = pool.table[:, :2]
+    ref = np.stack([pool.reference(q.double().cpu().numpy()[b:b + 1], b, n - 1, 0, 0)[0] for b, n in enumerate(lengths)])
+    assert normwise(short, ref) <= DECODE_BAR
+
+
+def test_decode_queries_and_values_of_extreme_magnitudes():
+    """Large and tiny queries (against tiny and large keys) and value blocks whose scales differ by
+    2^30: the f16 operands must not overflow or lose them."""
+    rng = np.random.default_rng(7)
+    lengths, heads, dim = [90], 2, 128
+    for big in (1e20, 1e-20):
+        pool = Pool(rng, lengths, 2, 32, dim)
+        up = 2.0 ** np.round(-np.log2(big))
+        pool.ks *= up
+        pool.vs[:, :, 0] *= 2.0 ** 30
+        pool.cache.k_scale[0] = torch.from_numpy(pool.ks).float()
+        pool.cache.v_scale[0] = torch.from_numpy(pool.vs).float()
+        q = (rng.standard_normal((1, heads, dim)) * big).astype(np.float32)
+        got = pool.cache.attention_decode(torch.from_numpy(q).cuda(), ints(pool.table), ints(lengths)).double().cpu().numpy()
+        assert normwise(got, pool.reference(q, 0, 89, 0, 0)[None, 0]) <= DECODE_BAR
+
+
+def test_decode_carries_nan_of_what_it_sees():
+    rng = np.random.default_rng(8)
+    pool = Pool(rng, [40, 40], 1, 32, 64)
+    pool.cache.v.view(torch.uint8)[0, int(pool.table[1, 0]), 0, 3] = 0x7f  # a NaN value among the seen
+    q = torch.randn(2, 2, 64, device="cuda")
+    got = pool.cache.attention_decode(q, ints(pool.table), ints([40, 40]))
+    assert torch.isfinite(got[0]).all() and torch.isnan(got[1]).all()
+
+
+def test_decode_on_another_stream_and_in_a_graph():
+    rng = np.random.default_rng(9)
+    lengths = [200, 30]
+    pool = Pool(rng, lengths, 2, 32, 128)
+    q = torch.from_numpy(rng.standard_normal((2, 4, 128)).astype(np.float32)).cuda()
+    table, n = ints(pool.table), ints(lengths)
+    want = pool.cache.attention_decode(q, table, n)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = pool.cache.attention_decode(q, table, n)
+    side.synchronize()
+    assert torch.equal(want, got)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = pool.cache.attention_decode(q, table, n)
+    for m in ([200, 30], [0, 1], [33, 16]):  # the captured call follows the device's lengths
+        n.copy_(ints(m))
+        graph.replay()
+        assert torch.equal(out, pool.cache.attention_decode(q, table, n)), m
+
+
+def test_decode_is_deterministic():
+    rng = np.random.default_rng(10)
+    pool = Pool(rng, [4000, 17, 900], 2, 64, 128)
+    q = torch.from_numpy(rng.standard_normal((3, 8, 128)).astype(np.float32)).cuda()
+    a = pool.cache.attention_decode(q, ints(pool.table), ints(pool.lengths))
+    for _ in range(5):
+        assert torch.equal(a, pool.cache.attention_decode(q, ints(pool.table), ints(pool.lengths)))
+
+
+PREFILL = [
+    # (past, new) of each sequence, heads, kv_heads, dim, page, window, sinks
+    ([(0, 1), (0, 64), (5, 3)], 2, 2, 128, 32, 0, 0),
+    ([(0, 130)], 1, 1, 64, 16, 0, 0),
+    ([(100, 0), (33, 70), (0, 0), (1, 1)], 8, 2, 128, 64, 0, 0),
+    ([(200, 45), (16, 129)], 10, 2, 128, 48, 0, 0),
+    ([(0, 300)], 12, 1, 64, 128, 0, 0),
+    ([(130, 150), (0, 40)], 4, 2, 128, 32, 50, 0),
+    ([(130, 150), (0, 40)], 4, 2, 64, 32, 50, 7),
+    ([(0, 400)], 2, 1, 128, 16, 33, 130),
+    ([(7, 260)], 4, 4, 128, 64, 1, 0),
+]
+
+
+def prefill_inputs(rng, spans, heads, kv, dim, page, dtype):
+    pool = Pool(rng, [m + n for m, n in spans], kv, page, dim)
+    offsets = np.cumsum([0] + [n for _, n in spans])
+    q = torch.from_numpy(rng.standard_normal((offsets[-1], heads, dim)).astype(np.float32)).cuda().to(dtype)
+    return pool, offsets, q
+
+
+@pytest.mark.parametrize("spans,heads,kv,dim,page,window,sinks", PREFILL)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_prefill_matches_float64(spans, heads, kv, dim, page, window, sinks, dtype):
+    rng = np.random.default_rng(sum(n for _, n in spans) + heads + dim + window)
+    pool, offsets, q = prefill_inputs(rng, spans, heads, kv, dim, page, dtype)
+    out = pool.cache.attention_prefill(q, ints(offsets), ints(pool.table), ints(pool.lengths), window=window, sinks=sinks)
+    got, qh = out.double().cpu().numpy(), q.double().cpu().numpy()
+    assert np.all(np.isfinite(got))
+    for b, (past, n) in enumerate(spans):
+        if n:
+            rows = slice(offsets[b], offsets[b + 1])
+            assert normwise(got[rows], pool.reference(qh[rows], b, past, window, sinks)) <= PREFILL_BAR, b
+
+
+def test_prefill_unmapped_pages_strides_types_and_empty_rows():
+    rng = np.random.default_rng(21)
+    spans, heads, kv, dim, page = [(96, 100), (40, 30)], 6, 2, 128, 32
+    pool, offsets, q = prefill_inputs(rng, spans, heads, kv, dim, page, torch.float32)
+    pool.unmap(0, [0, 2, 4])
+    pool.unmap(1, slice(None))
+    wide = torch.zeros(q.shape[0], heads + 3, dim, device="cuda")
+    wide[:, :heads] = q
+    got = pool.cache.attention_prefill(wide[:, :heads], ints(offsets), ints(pool.table), ints(pool.lengths), window=40, sinks=3,
+                                       out_dtype=torch.bfloat16)
+    assert got.dtype == torch.bfloat16
+    got = got.double().cpu().numpy()
+    qh = q.double().cpu().numpy()
+    assert normwise(got[:100], pool.reference(qh[:100], 0, 96, 40, 3)) <= PREFILL_BAR
+    assert not got[100:].any()
+
+
+def test_prefill_agrees_with_decode_on_the_last_token():
+    rng = np.random.default_rng(22)
+    spans = [(0, 77), (300, 20), (10, 1)]
+    pool, offsets, q = prefill_inputs(rng, spans, 8, 2, 128, 32, torch.float32)
+    full = pool.cache.attention_prefill(q, ints(offsets), ints(pool.table), ints(pool.lengths))
+    last = torch.tensor(offsets[1:] - 1, device="cuda")
+    one = pool.cache.attention_decode(q[last], ints(pool.table), ints(pool.lengths))
+    assert normwise(full[last].cpu().numpy(), one.double().cpu().numpy()) <= PREFILL_BAR
+
+
+APPEND = [
+    # (start, new) of each sequence, heads, kv_heads, dim, page
+    ([(0, 1)], 1, 1, 64, 16),
+    ([(0, 16), (16, 16), (5, 11)], 2, 2, 128, 32),
+    ([(3, 1), (15, 1), (16, 1), (40, 1), (0, 1)], 8, 2, 128, 32),
+    ([(7, 50), (0, 0), (64, 3), (31, 33)], 6, 3, 64, 48),
+    ([(0, 200), (190, 7)], 4, 4, 128, 64),
+]
+
+
+@pytest.mark.parametrize("spans,heads,kv,dim,page", APPEND)
+@pytest.mark.parametrize("louder", [False, True])
+def test_append_matches_the_oracle_exactly(spans, heads, kv, dim, page, louder):
+    """`louder`: the new tokens outgrow the scale of the block that they join, so its old codes are
+    rescaled; otherwise they are quieter and the scale stays."""
+    from jax4j_b200.kv8 import rope_table
+    from oracle import kv8 as O
+    rng = np.random.default_rng(sum(n for _, n in spans) + heads + dim)
+    pool = Pool(rng, [m for m, _ in spans], kv, page, dim, room=max(n for _, n in spans))
+    offsets = np.cumsum([0] + [n for _, n in spans])
+    tokens = int(offsets[-1])
+    qkv = (rng.standard_normal((tokens, (heads + 2 * kv) * dim)) * (300.0 if louder else 0.01)).astype(np.float32)
+    rope = rope_table(max(m + n for m, n in spans), dim, device="cuda")
+    q = pool.cache.append(torch.from_numpy(qkv).cuda(), rope, ints(pool.table), ints([m for m, _ in spans]), heads,
+                          offsets=None if all(n == 1 for _, n in spans) else ints(offsets))
+    cs = rope.cpu().numpy()
+    x = qkv.reshape(tokens, heads + 2 * kv, dim)
+    k, ks, v, vs = pool.codes[0].copy(), pool.ks.copy(), pool.codes[1].copy(), pool.vs.copy()
+    want_q = np.empty((tokens, heads, dim), np.float32)
+    for b, (start, n) in enumerate(spans):
+        rot = np.empty((n, heads + kv, dim), np.float32)
+        for i in range(n):
+            rot[i] = O.rope(x[offsets[b] + i, :heads + kv], cs[start + i])
+        want_q[offsets[b]:offsets[b + 1]] = rot[:, :heads]
+        O.append(k, ks, rot[:, heads:].astype(np.float64), pool.table[b], start)
+        O.append(v, vs, x[offsets[b]:offsets[b + 1], heads + kv:].astype(np.float64), pool.table[b], start)
+    assert np.array_equal(q.cpu().numpy(), want_q)
+    assert np.array_equal(pool.cache.k_scale[0].double().cpu().numpy(), ks)
+    assert np.array_equal(pool.cache.v_scale[0].double().cpu().numpy(), vs)
+    assert np.array_equal(pool.cache.k[0].double().cpu().numpy(), k, equal_nan=True)
+    assert np.array_equal(pool.cache.v[0].double().cpu().numpy(), v, equal_nan=True)
+
+
+def test_append_token_by_token_equals_its_own_rule_and_rounds_q_to_bf16():
+    from jax4j_b200.kv8 import Kv8Cache, rope_table
+    from oracle import kv8 as O
+    rng = np.random.default_rng(31)
+    heads, kv, dim, page, n = 4, 2, 128, 32, 40
+    cache = Kv8Cache(3, kv, page, dim)
+    table = np.array([[2, 0]])
+    rope = rope_table(n, dim, device="cuda")
+    k, v = np.zeros((3, kv, page, dim)), np.zeros((3, kv, page, dim))
+    ks, vs = np.zeros((3, kv, 2)), np.zeros((3, kv, 2))
+    for pos in range(n):
+        qkv = (rng.standard_normal((1, (heads + 2 * kv) * dim)) * 2.0 ** rng.integers(-6, 6)).astype(np.float32)
+        q = cache.append(torch.from_numpy(qkv).cuda(), rope, ints(table), ints([pos]), heads, q_dtype=torch.bfloat16)
+        x = qkv.reshape(heads + 2 * kv, dim)
+        rot = O.rope(x[:heads + kv], rope[pos].cpu().numpy())
+        assert torch.equal(q[0].cpu(), torch.from_numpy(rot[:heads]).to(torch.bfloat16))
+        O.append(k, ks, rot[None, heads:].astype(np.float64), table[0], pos)
+        O.append(v, vs, x[None, heads + kv:].astype(np.float64), table[0], pos)
+    assert np.array_equal(cache.k[0].double().cpu().numpy(), k) and np.array_equal(cache.k_scale[0].double().cpu().numpy(), ks)
+    assert np.array_equal(cache.v[0].double().cpu().numpy(), v) and np.array_equal(cache.v_scale[0].double().cpu().numpy(), vs)
+
+
+def test_append_special_values_unmapped_pages_and_positions_past_the_table():
+    from jax4j_b200.kv8 import Kv8Cache, rope_table
+    from oracle import kv8 as O
+    dim, page = 64, 16
+    cache = Kv8Cache(4, 1, page, dim)
+    rope = rope_table(40, dim, device="cuda")
+    qkv = torch.zeros(48, 3 * dim, device="cuda")
+    qkv[:, 2 * dim:] = torch.randn(48, dim, device="cuda")
+    qkv[0, 2 * dim] = float("inf")
+    qkv[1, 2 * dim + 1] = -float("inf")
+    qkv[2, 2 * dim + 2] = float("nan")
+    table = np.array([[3, -1, 1]])
+    cache.append(qkv, rope, ints(table), ints([0]), 1, offsets=ints([0, 48]))
+    v, vs = np.zeros((4, 1, page, dim)), np.zeros((4, 1, 1))
+    O.append(v, vs, qkv[:40, 2 * dim:].double().cpu().numpy()[:, None], table[0], 0)  # positions 40 .. 47 are past the rope table
+    got = cache.v[0].double().cpu().numpy()
+    assert np.array_equal(got, v, equal_nan=True)
+    assert np.array_equal(cache.v_scale[0].double().cpu().numpy(), vs)
+    assert np.isnan(got[3, 0, 2, 2]) and got[3, 0, 0, 0] == 448 and got[3, 0, 1, 1] == -448
+    assert not cache.k[0].float().any()  # all-zero keys: zeros (some of them -0), the smallest scale
+    assert cache.k_scale[0, 3, 0, 0] == 2.0 ** -120
+
+
+@pytest.mark.parametrize("layers,kv,page,dim,moves", [(1, 1, 16, 64, 1), (3, 2, 48, 128, 5), (2, 8, 64, 128, 300), (5, 3, 32, 64, 40)])
+@pytest.mark.parametrize("partial", [False, True])
+def test_copy_pages_moves_blocks_and_scales(layers, kv, page, dim, moves, partial):
+    from jax4j_b200.kv8 import Kv8Cache
+    rng = np.random.default_rng(moves)
+    pages = 2 * moves + 1
+    cache = Kv8Cache(pages, kv, page, dim, layers)
+    for t in (cache.k, cache.v):
+        t.view(torch.uint8).copy_(torch.randint(0, 256, t.shape, dtype=torch.uint8, device="cuda"))
+    for t in (cache.k_scale, cache.v_scale):
+        t.copy_(torch.randn(t.shape, device="cuda"))
+    order = rng.permutation(pages)
+    src, dst = [int(x) for x in order[:moves]], [int(x) for x in order[moves:2 * moves]]
+    tokens = [int(x) for x in rng.integers(0, page + 1, moves)] if partial else None
+    want = [t.clone() for t in (cache.k.view(torch.uint8), cache.v.view(torch.uint8), cache.k_scale, cache.v_scale)]
+    for i in range(moves):
+        nb = -(-(tokens[i] if partial else page) // 16)
+        for t in want[:2]:
+            t[:, dst[i], :, :16 * nb] = t[:, src[i], :, :16 * nb]
+        for t in want[2:]:
+            t[:, dst[i], :, :nb] = t[:, src[i], :, :nb]
+    cache.copy_pages(src, dst, tokens)
+    for got, t in zip((cache.k.view(torch.uint8), cache.v.view(torch.uint8), cache.k_scale, cache.v_scale), want):
+        assert torch.equal(got, t)
+
+
+def test_refusals():
+    from jax4j_b200.kv8 import Kv8Cache, rope_table
+    cache = Kv8Cache(4, 2, 32, 128, layers=2)
+    table, n = ints([[0, 1]]), ints([5])
+    q = torch.zeros(1, 4, 128, device="cuda")
+    with pytest.raises(ValueError, match="multiple of kv_heads"):
+        cache.attention_decode(torch.zeros(1, 3, 128, device="cuda"), table, n)
+    with pytest.raises(ValueError, match="layer 2 outside"):
+        cache.attention_decode(q, table, n, layer=2)
+    with pytest.raises(ValueError, match="window and sinks"):
+        cache.attention_decode(q, table, n, window=-1)
+    with pytest.raises(ValueError, match="finite"):
+        cache.attention_decode(q, table, n, scale=float("inf"))
+    with pytest.raises(ValueError, match="float32 or bfloat16"):
+        cache.attention_decode(q.half(), table, n)
+    with pytest.raises(ValueError, match="int32"):
+        cache.attention_decode(q, table.long(), n)
+    with pytest.raises(ValueError, match="int32"):
+        cache.attention_decode(q, table, n.cpu())
+    with pytest.raises(ValueError, match="rows for"):
+        cache.attention_decode(torch.zeros(2, 4, 128, device="cuda"), table, n)
+    with pytest.raises(ValueError, match="dense within a row"):
+        cache.attention_decode(torch.zeros(1, 4, 256, device="cuda")[..., ::2], table, n)
+    with pytest.raises(ValueError, match="offsets"):
+        cache.attention_prefill(q, n, table, n)
+    rope = rope_table(8, 128, device="cuda")
+    with pytest.raises(ValueError, match="qkv must be"):
+        cache.append(torch.zeros(1, 7 * 128, device="cuda"), rope, table, n, 4)
+    with pytest.raises(ValueError, match="one token for each sequence"):
+        cache.append(torch.zeros(2, 8 * 128, device="cuda"), rope, table, n, 4)
+    with pytest.raises(ValueError, match="rope must be"):
+        cache.append(torch.zeros(1, 8 * 128, device="cuda"), rope[:, :32], table, n, 4)
+    with pytest.raises(ValueError, match="written twice"):
+        cache.copy_pages([0, 1], [2, 2])
+    with pytest.raises(ValueError, match="both read and written"):
+        cache.copy_pages([0, 1], [1, 2])
+    with pytest.raises(ValueError, match="outside"):
+        cache.copy_pages([0], [4])
+    with pytest.raises(ValueError, match="tokens of a page"):
+        cache.copy_pages([0], [1], [33])
+    empty = cache.attention_decode(torch.zeros(0, 4, 128, device="cuda"), table[:0], n[:0])
+    assert empty.shape == (0, 4, 128)
+    cache.copy_pages([], [])
