@@ -13,6 +13,7 @@
 #include <cmath>
 
 #include "kv8_common.cuh"
+#include "tc_common.cuh"
 
 namespace j4b {
 
@@ -21,7 +22,7 @@ int kv8_check(const j4b_kv8_cache* c, int64_t layer, Kv8View* view, int* dev);
 namespace {
 
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -35,16 +36,10 @@ __device__ __forceinline__ uint32_t h2_rest(float a, float b, uint32_t hi) {
   const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi));
   return h2(a - f.x, b - f.y);
 }
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp8(uint32_t dst, const void* src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+__device__ __forceinline__ float exp2_ftz(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 __device__ __forceinline__ float quad_max(float v) {
   v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
@@ -71,37 +66,25 @@ __device__ __forceinline__ Span span_of(int first, int last, int window, int sin
   return s;
 }
 
-// Per-lane pieces of a block: keys of tokens g and 8 + g (dims 16 (t + 4 i) .. + 15), values of
-// tokens 2t, 2t + 1, 2t + 8, 2t + 9 (dims (D / 8) g .. + D / 8 - 1), g = lane / 4, t = lane % 4.
+// A block in shared memory: 16 rows of D bytes as TMA writes them with its 128-byte (D = 128) or
+// 64-byte (D = 64) swizzle, so that the reads below touch every bank once (16-byte pieces whose
+// rows are 128 bytes apart would meet in the same banks). A lane's pieces, g = lane / 4, t = lane % 4:
+// keys of tokens g and 8 + g, dims kK 16 t .. + kK 16 - 1; values of tokens 2t, 2t + 1, 2t + 8,
+// 2t + 9, dims (D / 8) g .. + D / 8 - 1.
 template <int D>
 struct Piece {
-  static constexpr int kK = D / 64;   // 16-byte key pieces of a token
-  static constexpr int kW = D / 32;   // 4-byte words of a value piece
-  static constexpr int kStage = 32 * D;  // bytes of a block, keys and values, in a warp's ring
-};
-
-// Starts the copy of block `id` into a warp's stage. A lane reads back only what it copied itself,
-// so its own wait_group is all the synchronisation the ring needs.
-template <int D>
-__device__ __forceinline__ void fetch(const Kv8View& c, int id, uint32_t stage, int lane) {
-  const int g = lane >> 2, t = lane & 3;
-  const uint8_t* kb = c.k + (int64_t)id * (kKvBlock * D);
-  const uint8_t* vb = c.v + (int64_t)id * (kKvBlock * D);
-#pragma unroll
-  for (int n = 0; n < 2; ++n)
-#pragma unroll
-    for (int i = 0; i < Piece<D>::kK; ++i)
-      cp16(stage + (n * Piece<D>::kK + i) * 512 + lane * 16, kb + (8 * n + g) * D + 16 * (t + 4 * i));
-  const uint32_t vs = stage + kKvBlock * D;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const uint8_t* src = vb + (2 * t + (j & 1) + 8 * (j >> 1)) * D + (D / 8) * g;
-    if (D == 128)
-      cp16(vs + j * 512 + lane * 16, src);
-    else
-      cp8(vs + j * 256 + lane * 8, src);
+  static constexpr int kK = D / 64;            // 16-byte key pieces of a token
+  static constexpr int kW = D / 32;            // 4-byte words of a value piece
+  static constexpr int kBytes = kKvBlock * D;  // of a block's keys, and of its values
+  static constexpr int kBuffer = 4 * kBytes;   // a warp's: keys of two blocks, then values of two blocks
+  // 16-byte chunk `c` of row r
+  static __device__ __forceinline__ int at(int r, int c) { return r * D + ((c ^ (D == 128 ? r & 7 : r >> 1 & 3)) << 4); }
+  static __device__ __forceinline__ int key(int lane, int i) { return at(lane >> 2, kK * (lane & 3) + i); }
+  static __device__ __forceinline__ int value(int lane, int j) {
+    const int g = lane >> 2, r = 2 * (lane & 3) + j;
+    return D == 128 ? at(r, g) : at(r, g >> 1) + (g & 1) * 8;
   }
-}
+};
 
 // A warp's online softmax over the blocks it visits. SPLIT: the 16 rows of the MMAs are 8 queries,
 // rows 0-7 the f16 values of Q (and P), rows 8-15 what the rounding left, so that every product is
@@ -110,7 +93,7 @@ __device__ __forceinline__ void fetch(const Kv8View& c, int id, uint32_t stage, 
 template <int D, bool SPLIT>
 struct Warp {
   static constexpr int kRows = SPLIT ? 1 : 2;
-  uint32_t q[D / 16][4];
+  const uint4* q;  // the A operands of the D / 16 k steps, [step][lane], in shared memory
   float o[D / 8][4];
   float factor[kRows];  // scores in log2 units per unit of the MMA's result and of key scale
   float m[kRows], l[kRows];
@@ -128,16 +111,19 @@ struct Warp {
     ref = 0.f;
   }
 
-  // Loads the query rows (null: a row of zeros). Each row is first brought to a largest element in
-  // [2^11, 2^12) by a power of two, so f16's range does not limit queries.
-  __device__ __forceinline__ void load_q(const void* base, int type, const int64_t (&row)[kRows], float scale_log2, int t) {
+  // Writes the operands of the query rows (row < 0: zeros) to `dst`, and keeps it. Each row is first
+  // brought to a largest element in [2^11, 2^12) by a power of two, so f16's range does not limit
+  // queries. Every lane writes what it reads back; a warp whose rows are another's writes the same.
+  __device__ __forceinline__ void load_q(uint4* dst, const void* base, int type, const int64_t (&row)[kRows], float scale_log2, int lane) {
+    const int t = lane & 3;
+    uint32_t frag[D / 16][4];
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
       float4 x[D / 16];
       float most = 0.f;
 #pragma unroll
       for (int i = 0; i < D / 16; ++i) {
-        x[i] = row[r] >= 0 ? load4(base, type, row[r] + 16 * (t + 4 * (i >> 2)) + 4 * (i & 3)) : make_float4(0.f, 0.f, 0.f, 0.f);
+        x[i] = row[r] >= 0 ? load4(base, type, row[r] + 16 * (Piece<D>::kK * t + (i >> 2)) + 4 * (i & 3)) : make_float4(0.f, 0.f, 0.f, 0.f);
         most = fmaxf(most, fmaxf(fmaxf(fabsf(x[i].x), fabsf(x[i].y)), fmaxf(fabsf(x[i].z), fabsf(x[i].w))));
       }
       most = quad_max(most);
@@ -149,65 +135,100 @@ struct Warp {
 #pragma unroll
       for (int i = 0; i < D / 16; ++i) {
         const float4 y = make_float4(x[i].x * up, x[i].y * up, x[i].z * up, x[i].w * up);
-        q[i][r] = h2(y.x, y.y);
-        q[i][2 + r] = h2(y.z, y.w);
+        frag[i][r] = h2(y.x, y.y);
+        frag[i][2 + r] = h2(y.z, y.w);
         if (SPLIT) {
-          q[i][1] = h2_rest(y.x, y.y, q[i][0]);
-          q[i][3] = h2_rest(y.z, y.w, q[i][2]);
+          frag[i][1] = h2_rest(y.x, y.y, frag[i][0]);
+          frag[i][3] = h2_rest(y.z, y.w, frag[i][2]);
         }
       }
     }
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) dst[i * 32 + lane] = make_uint4(frag[i][0], frag[i][1], frag[i][2], frag[i][3]);
+    q = dst + lane;
   }
 
-  // One block: its codes in the lane's ring stage, its scales, and which of its tokens row r sees:
-  // tokens j with (first[r] <= j or j < sink) and j <= last[r], counted from the block's start.
-  // `all`: every row sees every token. A masked token's value codes are replaced by zeros: they may
+  // Two blocks, first half: their key codes in the lane's buffer, their scales, and which of their
+  // tokens row r sees: tokens j with (first[r] <= j or j < sinks) and j <= last[r] (a block that is
+  // not there has p0 far past every row). `all`: every row sees every token of both. Two at a time:
+  // their MMA chains are independent, and one maximum, one vote on rescaling serve both.
+  // Leaves the probabilities in p, and in `seen` (bit 4 u + j) which of the lane's tokens any row
+  // sees: a masked token's value codes are replaced by zeros in the second half, since they may
   // hold anything, NaN too, in a page that is not full.
-  __device__ __forceinline__ void block(const uint8_t* stage, float ks, float vs, bool all, const int (&first)[kRows],
-                                        const int (&last)[kRows], int sink, int lane) {
+  __device__ __forceinline__ void scores(const uint8_t* stage, const float (&ks)[2], const float (&vs)[2], bool all, const int (&first)[kRows],
+                                         const int (&last)[kRows], int sinks, const int (&p0)[2], int lane, uint32_t (&p)[2][4], uint32_t& seen) {
     const int t = lane & 3;
-    float s[2][4];
+    float s[2][2][4];
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {
-      s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+    for (int u = 0; u < 2; ++u)
 #pragma unroll
-      for (int i = 0; i < Piece<D>::kK; ++i) {
-        const uint4 kw = *reinterpret_cast<const uint4*>(stage + (n * Piece<D>::kK + i) * 512 + lane * 16);
-        const uint32_t w[4] = {kw.x, kw.y, kw.z, kw.w};
+      for (int n = 0; n < 2; ++n) s[u][n][0] = s[u][n][1] = s[u][n][2] = s[u][n][3] = 0.f;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          uint32_t b0, b1;
-          e4m3x4_f16(w[j], b0, b1);
-          mma16816(s[n], q[4 * i + j], b0, b1);
-        }
+    for (int i = 0; i < Piece<D>::kK; ++i) {
+      uint32_t w[2][2][4];
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+          *reinterpret_cast<uint4*>(w[u][n]) =
+              *reinterpret_cast<const uint4*>(stage + u * Piece<D>::kBytes + n * (8 * D) + Piece<D>::key(lane, i));
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {  // the four chains in turn: an MMA never waits for the one before it
+        const uint4 qf = q[(4 * i + j) * 32];
+        const uint32_t a[4] = {qf.x, qf.y, qf.z, qf.w};
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int n = 0; n < 2; ++n) {
+            uint32_t b0, b1;
+            e4m3x4_f16(w[u][n][j], b0, b1);
+            mma16816(s[u][n], a, b0, b1);
+          }
       }
     }
-    float x[kRows][4];  // scores of tokens 2t, 2t + 1, 2t + 8, 2t + 9
-    bool seen_by_any[4];
+    float x[kRows][2][4];  // scores of tokens 2t, 2t + 1, 2t + 8, 2t + 9 of each block
+    seen = all ? 0xffu : 0u;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int tok = 2 * t + (j & 1) + 8 * (j >> 1);
-      seen_by_any[j] = all;
+    for (int u = 0; u < 2; ++u)
 #pragma unroll
       for (int r = 0; r < kRows; ++r) {
-        const float raw = SPLIT ? s[j >> 1][j & 1] + s[j >> 1][2 + (j & 1)] : s[j >> 1][2 * r + (j & 1)];
-        x[r][j] = raw * (factor[r] * ks);
-        if (!all) {
-          const bool see = (tok >= first[r] || tok < sink) && tok <= last[r];
-          if (!see) x[r][j] = -INFINITY;
-          seen_by_any[j] |= see;
+        const float f = factor[r] * ks[u];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float raw = SPLIT ? s[u][j >> 1][j & 1] + s[u][j >> 1][2 + (j & 1)] : s[u][j >> 1][2 * r + (j & 1)];
+          x[r][u][j] = raw * f;
         }
       }
+    if (!all) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int tok = p0[u] + 2 * t + (j & 1) + 8 * (j >> 1);
+#pragma unroll
+          for (int r = 0; r < kRows; ++r) {
+            const bool see = (tok >= first[r] || tok < sinks) && tok <= last[r];
+            if (!see) x[r][u][j] = -INFINITY;
+            seen |= (uint32_t)see << (4 * u + j);
+          }
+        }
+      // the lanes of the same t hold the other rows
+      seen |= __shfl_xor_sync(0xffffffffu, seen, 4);
+      seen |= __shfl_xor_sync(0xffffffffu, seen, 8);
+      seen |= __shfl_xor_sync(0xffffffffu, seen, 16);
     }
-    bool grown = vs > ref;
+    const float vmax = fmaxf(vs[0], vs[1]);
+    bool grown = vmax > ref;
     float mn[kRows];
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
-      mn[r] = fmaxf(m[r], quad_max(fmaxf(fmaxf(x[r][0], x[r][1]), fmaxf(x[r][2], x[r][3]))));
+      float v = fmaxf(fmaxf(fmaxf(x[r][0][0], x[r][0][1]), fmaxf(x[r][0][2], x[r][0][3])),
+                      fmaxf(fmaxf(x[r][1][0], x[r][1][1]), fmaxf(x[r][1][2], x[r][1][3])));
+      mn[r] = fmaxf(m[r], quad_max(v));
       grown |= mn[r] > m[r];
     }
     if (__any_sync(0xffffffffu, grown)) {
-      const float now = fmaxf(ref, vs);
+      const float now = fmaxf(ref, vmax);
       const float down = ref * kv8_inverse(now);  // 0 at the first block
       ref = now;
 #pragma unroll
@@ -226,62 +247,154 @@ struct Warp {
         }
       }
     }
-    const float weight = (float)(1 << kPShift) * vs * kv8_inverse(ref);
-    uint32_t p[4];
 #pragma unroll
-    for (int r = 0; r < kRows; ++r) {
-      const float base = m[r] == -INFINITY ? 0.f : m[r];
-      float e[4];
+    for (int u = 0; u < 2; ++u) {
+      const float weight = (float)(1 << kPShift) * vs[u] * kv8_inverse(ref);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        e[j] = exp2f(x[r][j] - base);
-        l[r] += e[j];
-        e[j] *= weight;
+      for (int r = 0; r < kRows; ++r) {
+        const float base = m[r] == -INFINITY ? 0.f : m[r];
+        float e[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          e[j] = exp2_ftz(x[r][u][j] - base);
+          l[r] += e[j];
+          e[j] *= weight;
+        }
+        p[u][r] = h2(e[0], e[1]);
+        p[u][2 + r] = h2(e[2], e[3]);
+        if (SPLIT) {
+          p[u][1] = h2_rest(e[0], e[1], p[u][0]);
+          p[u][3] = h2_rest(e[2], e[3], p[u][2]);
+        }
       }
-      p[r] = h2(e[0], e[1]);
-      p[2 + r] = h2(e[2], e[3]);
-      if (SPLIT) {
-        p[1] = h2_rest(e[0], e[1], p[0]);
-        p[3] = h2_rest(e[2], e[3], p[2]);
-      }
-    }
-    const uint8_t* vb = stage + kKvBlock * D;
-    uint32_t v[4][Piece<D>::kW];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (D == 128)
-        *reinterpret_cast<uint4*>(v[j]) = *reinterpret_cast<const uint4*>(vb + j * 512 + lane * 16);
-      else
-        *reinterpret_cast<uint2*>(v[j]) = *reinterpret_cast<const uint2*>(vb + j * 256 + lane * 8);
-      if (!all && !seen_by_any_quad(seen_by_any[j]))
-#pragma unroll
-        for (int w = 0; w < Piece<D>::kW; ++w) v[j][w] = 0;
-    }
-#pragma unroll
-    for (int w = 0; w < Piece<D>::kW; ++w) {
-      const uint32_t a0 = __byte_perm(v[0][w], v[1][w], 0x5140), a1 = __byte_perm(v[0][w], v[1][w], 0x7362);
-      const uint32_t c0 = __byte_perm(v[2][w], v[3][w], 0x5140), c1 = __byte_perm(v[2][w], v[3][w], 0x7362);
-      uint32_t b00, b01, b10, b11;
-      e4m3x4_f16(a0, b00, b10);
-      e4m3x4_f16(c0, b01, b11);
-      mma16816(o[4 * w], p, b00, b01);
-      mma16816(o[4 * w + 1], p, b10, b11);
-      e4m3x4_f16(a1, b00, b10);
-      e4m3x4_f16(c1, b01, b11);
-      mma16816(o[4 * w + 2], p, b00, b01);
-      mma16816(o[4 * w + 3], p, b10, b11);
     }
   }
-  // Whether any row of the warp sees the token: the lanes of the same t hold the other rows.
-  __device__ __forceinline__ bool seen_by_any_quad(bool mine) const {
-    uint32_t v = mine;
-    v |= __shfl_xor_sync(0xffffffffu, v, 4);
-    v |= __shfl_xor_sync(0xffffffffu, v, 8);
-    v |= __shfl_xor_sync(0xffffffffu, v, 16);
-    return v != 0;
+
+  // Second half: the accumulators take the two blocks' values, their codes in the lane's buffer.
+  __device__ __forceinline__ void values(const uint8_t* stage, const uint32_t (&p)[2][4], uint32_t seen, int lane) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const uint8_t* vb = stage + u * Piece<D>::kBytes;
+      uint32_t v[4][Piece<D>::kW];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (D == 128)
+          *reinterpret_cast<uint4*>(v[j]) = *reinterpret_cast<const uint4*>(vb + (j >> 1) * (8 * D) + Piece<D>::value(lane, j & 1));
+        else
+          *reinterpret_cast<uint2*>(v[j]) = *reinterpret_cast<const uint2*>(vb + (j >> 1) * (8 * D) + Piece<D>::value(lane, j & 1));
+        if (!(seen >> (4 * u + j) & 1))
+#pragma unroll
+          for (int w = 0; w < Piece<D>::kW; ++w) v[j][w] = 0;
+      }
+#pragma unroll
+      for (int w = 0; w < Piece<D>::kW; ++w) {
+        const uint32_t a0 = __byte_perm(v[0][w], v[1][w], 0x5140), a1 = __byte_perm(v[0][w], v[1][w], 0x7362);
+        const uint32_t c0 = __byte_perm(v[2][w], v[3][w], 0x5140), c1 = __byte_perm(v[2][w], v[3][w], 0x7362);
+        uint32_t b00, b01, b10, b11;
+        e4m3x4_f16(a0, b00, b10);
+        e4m3x4_f16(c0, b01, b11);
+        mma16816(o[4 * w], p[u], b00, b01);
+        mma16816(o[4 * w + 1], p[u], b10, b11);
+        e4m3x4_f16(a1, b00, b10);
+        e4m3x4_f16(c1, b01, b11);
+        mma16816(o[4 * w + 2], p[u], b00, b01);
+        mma16816(o[4 * w + 3], p[u], b10, b11);
+      }
+    }
   }
   // the accumulators' unit
   __device__ __forceinline__ float unit() const { return ref * (1.f / (1 << kPShift)); }
+};
+
+// A warp's way through its blocks. Lane 0 has TMA bring a pair of blocks' keys and values to the
+// warp's buffer, each on an mbarrier of its own; a pair's keys are replaced by the next pair's once
+// its scores are done, its values once they are accumulated, so either copy has the other half's
+// work (and the SM's other warps) to arrive in. TMA for the copies because they are 2 KB rows of
+// memory in one instruction: the same loop with 16-byte cp.async straight from the lanes' own places
+// (64-byte pieces of rows) reached 4.7 TB/s with the arithmetic taken out, with TMA 6.4.
+template <int D>
+struct Walker {
+  const CUtensorMap *mk, *mv;
+  uint8_t* buffer;
+  uint64_t* bars;  // keys, values
+  uint32_t phase;  // of both: they are used in turn
+  bool ok;
+
+  __device__ __forceinline__ void init(const CUtensorMap* k, const CUtensorMap* v, uint8_t* buf, uint64_t* b, int lane) {
+    mk = k;
+    mv = v;
+    buffer = buf;
+    bars = b;
+    phase = 0;
+    ok = true;
+    if (lane == 0) {
+      bar_init(&bars[0], 1);
+      bar_init(&bars[1], 1);
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncwarp();
+  }
+  // the pair's blocks that are there (number >= 0), keys (which = 0) or values (1)
+  __device__ __forceinline__ void fetch(int which, int id0, int id1, int lane) {
+    if (lane == 0 && ok) {
+      uint8_t* dst = buffer + which * 2 * Piece<D>::kBytes;
+      bar_expect_tx(&bars[which], ((id0 >= 0) + (id1 >= 0)) * Piece<D>::kBytes);
+      if (id0 >= 0) tma_tile(dst, which ? mv : mk, 0, id0 * kKvBlock, &bars[which]);
+      if (id1 >= 0) tma_tile(dst + Piece<D>::kBytes, which ? mv : mk, 0, id1 * kKvBlock, &bars[which]);
+    }
+  }
+  __device__ __forceinline__ void wait(int which) { ok = ok && bar_wait(&bars[which], phase); }
+  // At the kernel's end. After a wait that gave up nothing more is copied or waited for, but for
+  // one last bounded wait for what was in flight then.
+  __device__ __forceinline__ void finish(int* timeout) {
+    if (ok) return;
+    bar_wait(&bars[0], phase);
+    bar_wait(&bars[1], phase);
+    *timeout = 1;
+  }
+
+  // look(i, pos) gives block i's number (-1: unmapped, its tokens are skipped) and first position;
+  // all_seen(p0) says whether every row sees all of a pair. Lane i looks up the i-th of 32 blocks.
+  template <bool SPLIT, class Look, class All>
+  __device__ __forceinline__ void run(const Kv8View& c, Warp<D, SPLIT>& w, int mine, int lane, Look look, All all_seen,
+                                      const int (&first)[Warp<D, SPLIT>::kRows], const int (&last)[Warp<D, SPLIT>::kRows], int sinks) {
+    constexpr int kNowhere = 0x3fffffff;
+    for (int base = 0; base < mine; base += 32) {
+      const int n = min(32, mine - base);
+      int id = -1, at = kNowhere;
+      float ks = 0.f, vs = 0.f;
+      if (lane < n) {
+        int pos;
+        id = look(base + lane, pos);
+        if (id >= 0) {
+          at = pos;
+          ks = __ldg(c.ks + id);
+          vs = __ldg(c.vs + id);
+        }
+      }
+      int id0 = __shfl_sync(0xffffffffu, id, 0), id1 = __shfl_sync(0xffffffffu, id, 1);
+      fetch(0, id0, id1, lane);
+      fetch(1, id0, id1, lane);
+      for (int i = 0; i < n; i += 2) {
+        const int p0[2] = {__shfl_sync(0xffffffffu, at, i), __shfl_sync(0xffffffffu, at, i + 1)};
+        const float kk[2] = {__shfl_sync(0xffffffffu, ks, i), __shfl_sync(0xffffffffu, ks, i + 1)};
+        const float vv[2] = {__shfl_sync(0xffffffffu, vs, i), __shfl_sync(0xffffffffu, vs, i + 1)};
+        const bool more = i + 2 < n, any = p0[0] != kNowhere || p0[1] != kNowhere;
+        id0 = __shfl_sync(0xffffffffu, id, (i + 2) & 31);
+        id1 = __shfl_sync(0xffffffffu, id, (i + 3) & 31);
+        uint32_t p[2][4], seen;
+        wait(0);
+        if (any) w.scores(buffer, kk, vv, all_seen(p0), first, last, sinks, p0, lane, p, seen);
+        __syncwarp();
+        if (more) fetch(0, id0, id1, lane);
+        wait(1);
+        if (any) w.values(buffer + 2 * Piece<D>::kBytes, p, seen, lane);
+        __syncwarp();
+        if (more) fetch(1, id0, id1, lane);
+        phase ^= 1;
+      }
+    }
+  }
 };
 
 struct AttnArgs {
@@ -298,7 +411,12 @@ struct AttnArgs {
   float scale_log2;
   void* out;
   int out_type;
+  int* timeout;  // host memory; set when a wait gave up
 };
+
+__device__ __forceinline__ uint8_t* aligned_smem(uint8_t* raw) {  // the swizzle goes by address bits
+  return raw + ((1024u - (saddr(raw) & 1023u)) & 1023u);
+}
 
 // ---------------------------------------------------------------------------------------------
 // Decode. Rows are (sequence, kv head, run of up to 8 of its query heads); a row's units are its
@@ -307,7 +425,7 @@ struct AttnArgs {
 // GPU evenly. A row that lies in one share is finished there; one cut by a share's end leaves an
 // unnormalised part (running maximum, sum, 8 x D) in the workspace for kv8_join_kernel.
 constexpr int kDecWarps = 4;
-constexpr int kDecStages = 4;
+constexpr int kDecCtas = 4;  // of an SM
 constexpr int kDecHeads = 8;
 
 struct DecArgs {
@@ -320,36 +438,42 @@ struct DecArgs {
 __device__ __forceinline__ int decode_blocks(const AttnArgs& a, int b) {
   return span_of(__ldg(a.lengths + b) - 1, __ldg(a.lengths + b) - 1, a.window, a.sinks).count();
 }
-__device__ __forceinline__ int64_t share_of(int64_t units, int cta, int ctas) {
-  // shares are whole numbers of kDecWarps units, one for each warp
-  const int64_t quads = (units + kDecWarps - 1) / kDecWarps;
-  return min(units, quads * cta / ctas * kDecWarps);
+// Units of a CTA: a whole number for each of its warps, the same for all CTAs (the last ones may get none).
+__device__ __forceinline__ int64_t share_of(int64_t units, int ctas) {
+  const int64_t each = (int64_t)ctas * kDecWarps;
+  return (units + each - 1) / each * kDecWarps;
 }
 
 template <int D>
-__global__ void __launch_bounds__(kDecWarps * 32, 3) kv8_decode_kernel(const DecArgs d) {
+__global__ void __launch_bounds__(kDecWarps * 32, kDecCtas) kv8_decode_kernel(const DecArgs d, const __grid_constant__ CUtensorMap mk,
+                                                                           const __grid_constant__ CUtensorMap mv) {
   const AttnArgs& a = d.a;
-  extern __shared__ __align__(128) uint8_t smem[];
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = aligned_smem(smem_raw);
+  __shared__ uint64_t bars[kDecWarps][2];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   const int rows = a.c.kv_heads * d.chunks;
+  const bool record = blockIdx.x == 0;  // the sequences' first units, for the join
   const Kv8Place at = kv8_find<kDecWarps * 32>(
       a.batch, [&](int b) -> int64_t { return (int64_t)decode_blocks(a, b) * rows; },
-      [&](int64_t units) -> int64_t { return share_of(units, blockIdx.x, gridDim.x); });
-  int64_t left = at.seq < 0 ? 0 : share_of(at.total, blockIdx.x + 1, gridDim.x) - share_of(at.total, blockIdx.x, gridDim.x);
-  if (blockIdx.x == 0 && tid == 0) {  // for the join
-    int64_t sum = 0;
-    for (int b = 0; b < a.batch; ++b) {
-      d.cum[b] = sum;
-      sum += decode_blocks(a, b);
-    }
-    d.cum[a.batch] = sum;
-  }
-  uint8_t* ring = smem + warp * (kDecStages * Piece<D>::kStage);
-  const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
-  // the merge of the warps' states reuses the rings (drained by then): per warp m, l, then 8 x D
-  float* merge = reinterpret_cast<float*>(ring);
-  constexpr int kMergeStride = kDecStages * Piece<D>::kStage / 4;
-  static_assert(kMergeStride >= kDecHeads * (D + 2), "a warp's state must fit its ring");
+      [&](int64_t units) -> int64_t { return share_of(units, gridDim.x) * blockIdx.x; },
+      [&](int b0, int b1, int64_t before) {
+        if (!record) return;
+        for (int b = b0; b < b1; ++b) {
+          d.cum[b] = before;
+          before += (int64_t)decode_blocks(a, b) * rows;
+        }
+        if (b1 == a.batch) d.cum[a.batch] = before;  // the threads past the last sequence write the same total
+      });
+  int64_t left = at.seq < 0 ? 0 : min(share_of(at.total, gridDim.x), at.total - share_of(at.total, gridDim.x) * blockIdx.x);
+  uint8_t* buffer = smem + warp * Piece<D>::kBuffer;
+  uint4* queries = reinterpret_cast<uint4*>(smem + kDecWarps * Piece<D>::kBuffer) + warp * (2 * D);
+  // the merge of the warps' states reuses the buffers (drained by then): per warp 8 x (m, l, D)
+  float* merge = reinterpret_cast<float*>(buffer);
+  constexpr int kMergeStride = Piece<D>::kBuffer / 4;
+  static_assert(kMergeStride >= kDecHeads * (D + 2), "a warp's state must fit its buffer");
+  Walker<D> walker;
+  walker.init(&mk, &mv, buffer, bars[warp], lane);
   int b = at.seq;
   int64_t in_seq = at.at;
   int segment = 0;
@@ -371,51 +495,28 @@ __global__ void __launch_bounds__(kDecWarps * 32, 3) kv8_decode_kernel(const Dec
     w.reset();
     {
       const int64_t qrow[1] = {g < nh ? (int64_t)b * a.q_stride + (int64_t)(h0 + g) * D : -1};
-      w.load_q(a.q, a.q_type, qrow, a.scale_log2, t);
+      w.load_q(queries, a.q, a.q_type, qrow, a.scale_log2, lane);
     }
-    // Blocks begin + warp + 4 i; lane i of 32 looks up the page, scales of the i-th
-    const int mine = max(0, (end - begin - warp + kDecWarps - 1) / kDecWarps);
-    for (int base = 0; base < mine; base += 32) {
-      const int n = min(32, mine - base);
-      int id = -1;
-      float ks = 0.f, vs = 0.f;
-      int blk = 0;
-      if (lane < n) {
-        blk = span.block(begin + warp + kDecWarps * (base + lane));
-        id = kv8_block_id(a.c, a.t, b, head, blk);
-        if (id >= 0) {
-          ks = __ldg(a.c.ks + id);
-          vs = __ldg(a.c.vs + id);
-        }
-      }
-#pragma unroll
-      for (int s = 0; s < kDecStages - 1; ++s) {
-        const int nid = __shfl_sync(0xffffffffu, id, s);
-        if (s < n && nid >= 0) fetch<D>(a.c, nid, ring_at + s * Piece<D>::kStage, lane);
-        cp_commit();
-      }
-      for (int i = 0; i < n; ++i) {
-        {
-          const int next = i + kDecStages - 1;
-          const int nid = __shfl_sync(0xffffffffu, id, next & 31);
-          if (next < n && nid >= 0) fetch<D>(a.c, nid, ring_at + next % kDecStages * Piece<D>::kStage, lane);
-          cp_commit();
-        }
-        cp_wait<kDecStages - 1>();
-        if (__shfl_sync(0xffffffffu, id, i) < 0) continue;
-        const int p0 = __shfl_sync(0xffffffffu, blk, i) * kKvBlock;
-        const float kss = __shfl_sync(0xffffffffu, ks, i), vss = __shfl_sync(0xffffffffu, vs, i);
-        const bool all = p0 + kKvBlock <= len && (p0 >= lo || p0 + kKvBlock <= a.sinks);
-        const int first[1] = {lo - p0}, last[1] = {len - 1 - p0};
-        w.block(ring + i % kDecStages * Piece<D>::kStage, kss, vss, all, first, last, a.sinks - p0, lane);
-      }
-      cp_wait<0>();
-    }
+    // the warp's blocks are begin + warp + 4 i
+    const int first[1] = {lo}, last[1] = {len - 1};
+    walker.run(
+        a.c, w, max(0, (end - begin - warp + kDecWarps - 1) / kDecWarps), lane,
+        [&](int i, int& pos) {
+          const int blk = span.block(begin + warp + kDecWarps * i);
+          pos = blk * kKvBlock;
+          return kv8_block_id(a.c, a.t, b, head, blk);
+        },
+        [&](const int (&p0)[2]) {
+          const int far = max(p0[0], p0[1]) + kKvBlock, near = min(p0[0], p0[1]);
+          return far <= len && (near >= lo || far <= a.sinks);
+        },
+        first, last, a.sinks);
     // merge the warps
     __syncwarp();
     {
       const float l = quad_sum(w.l[0]), unit = w.unit();
       float* mm = merge + g * (D + 2);
+      if (g < nh) {
       if (t == 0) {
         mm[0] = w.m[0];
         mm[1] = l;
@@ -425,6 +526,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, 3) kv8_decode_kernel(const Dec
       for (int j = 0; j < D / 8; ++j) {
         mm[2 + (D / 8) * (2 * t) + j] = (w.o[j][0] + w.o[j][2]) * unit;
         mm[2 + (D / 8) * (2 * t + 1) + j] = (w.o[j][1] + w.o[j][3]) * unit;
+      }
       }
     }
     __syncthreads();
@@ -461,15 +563,17 @@ __global__ void __launch_bounds__(kDecWarps * 32, 3) kv8_decode_kernel(const Dec
         *reinterpret_cast<float2*>(dst + 4 + c) = make_float2(v.z, v.w);
       }
     }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the buffers go back to TMA
     __syncthreads();
     left -= end - begin;
     in_seq += end - begin;
     ++segment;
   }
+  walker.finish(a.timeout);
 }
 
-// Rows without a block give zeros; rows cut into parts are joined in the order of the parts. One
-// warp per (sequence, query head).
+// Rows without a block give zeros; rows cut into parts are joined, in the parts' order whatever
+// CTA wrote them first. One warp per (sequence, query head).
 template <int D>
 __global__ void __launch_bounds__(128) kv8_join_kernel(const DecArgs d, int ctas) {
   const AttnArgs& a = d.a;
@@ -478,38 +582,51 @@ __global__ void __launch_bounds__(128) kv8_join_kernel(const DecArgs d, int ctas
   if (i >= (int64_t)a.batch * a.heads) return;
   const int b = (int)(i / a.heads), qh = (int)(i % a.heads);
   const int head = qh / a.group, chunk = qh % a.group / kDecHeads, h = qh % a.group % kDecHeads;
-  const int rows = a.c.kv_heads * d.chunks;
-  const int64_t before = d.cum[b], units = d.cum[a.batch] * rows;
-  const int nb = (int)(d.cum[b + 1] - before);
+  const int64_t before = d.cum[b], units = d.cum[a.batch];
+  const int64_t nb = (d.cum[b + 1] - before) / (a.c.kv_heads * d.chunks);
   constexpr int kPer = D / 32;
   float acc[kPer];
 #pragma unroll
   for (int e = 0; e < kPer; ++e) acc[e] = 0.f;
   float lt = 0.f;
   if (nb > 0) {
-    const int64_t u0 = before * rows + (int64_t)(head * d.chunks + chunk) * nb, u1 = u0 + nb;
-    // the share that holds u0: shares are close to even, so start from the estimate
-    int cta = (int)(u0 / (double)units * ctas);
-    cta = max(0, min(ctas - 1, cta));
-    while (cta > 0 && share_of(units, cta, ctas) > u0) --cta;
-    while (share_of(units, cta + 1, ctas) <= u0) ++cta;
-    if (share_of(units, cta + 1, ctas) >= u1) return;  // finished by its CTA
+    const int64_t share = share_of(units, ctas), u0 = before + (head * d.chunks + chunk) * nb;
+    const int c0 = (int)(u0 / share), c1 = (int)((u0 + nb - 1) / share);
+    if (c0 == c1) return;  // finished by its CTA
+    // part i of the row is the first segment of CTA c0 + i, but for part 0 when c0 starts before the row
+    const float* first = d.part + ((int64_t)(2 * c0 + (share * c0 < u0)) * kDecHeads + h) * (D + 2);
+    const float* rest = d.part + ((int64_t)2 * (c0 + 1) * kDecHeads + h) * (D + 2);
+    constexpr int64_t kNext = (int64_t)2 * kDecHeads * (D + 2);
+    const int parts = c1 - c0 + 1;
     float mt = -INFINITY;
-    for (int c = cta; share_of(units, c, ctas) < u1; ++c) {
-      const int64_t s0 = share_of(units, c, ctas);
-      if (share_of(units, c + 1, ctas) == s0) continue;
-      const int slot = 2 * c + (s0 < u0);  // a share's first segment, or a later one
-      const float* src = d.part + ((int64_t)slot * kDecHeads + h) * (D + 2);
-      const float ms = src[0];
-      if (ms == -INFINITY) continue;
-      const float mn = fmaxf(mt, ms), f0 = mt == -INFINITY ? 0.f : exp2f(mt - mn), f1 = exp2f(ms - mn);
-      mt = mn;
-      lt = lt * f0 + src[1] * f1;
+    for (int base = 0; base < parts; base += 32) {
+      const int n = min(32, parts - base);
+      const float* mine = base + lane == 0 ? first : rest + (base + lane - 1) * kNext;
+      float2 ml = make_float2(-INFINITY, 0.f);
+      if (lane < n) ml = *reinterpret_cast<const float2*>(mine);
+      float mn = ml.x;
 #pragma unroll
-      for (int e = 0; e < kPer; ++e) acc[e] = acc[e] * f0 + src[2 + lane + 32 * e] * f1;
+      for (int o = 16; o > 0; o >>= 1) mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
+      mn = fmaxf(mn, mt);
+      if (mn == -INFINITY) continue;
+      const float old = exp2f(mt - mn), w = exp2f(ml.x - mn);  // 0 for parts that saw nothing
+      mt = mn;
+      float sum = w * ml.y;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      lt = lt * old + sum;
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) acc[e] *= old;
+#pragma unroll 8
+      for (int p = 0; p < n; ++p) {
+        const float f = __shfl_sync(0xffffffffu, w, p);
+        const float* src = (base + p == 0 ? first : rest + (base + p - 1) * kNext) + 2 + lane;
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) acc[e] = fmaf(f, src[32 * e], acc[e]);
+      }
     }
   }
-  const float inv = nb > 0 && lt != 0.f ? 1.f / lt : 0.f;
+  const float inv = lt != 0.f ? 1.f / lt : 0.f;
 #pragma unroll
   for (int e = 0; e < kPer; ++e) {
     const int64_t o = ((int64_t)b * a.heads + qh) * D + lane + 32 * e;
@@ -528,8 +645,11 @@ constexpr int kPreWarps = 4;
 constexpr int kPreRows = 16 * kPreWarps;
 
 template <int D>
-__global__ void __launch_bounds__(kPreWarps * 32, 3) kv8_prefill_kernel(const AttnArgs a) {
-  extern __shared__ __align__(128) uint8_t smem[];
+__global__ void __launch_bounds__(kPreWarps * 32, 3) kv8_prefill_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap mk,
+                                                                         const __grid_constant__ CUtensorMap mv) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = aligned_smem(smem_raw);
+  __shared__ uint64_t bars[kPreWarps][2];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   const int head = blockIdx.y;
   const Kv8Place at = kv8_find<kPreWarps * 32>(
@@ -557,45 +677,24 @@ __global__ void __launch_bounds__(kPreWarps * 32, 3) kv8_prefill_kernel(const At
     qp[i] = ok ? pos0 + tok : -1;
     lo[i] = a.window > 0 ? max(0, qp[i] - a.window + 1) : 0;
   }
-  w.load_q(a.q, a.q_type, qrow, a.scale_log2, t);
+  uint8_t* buffer = smem + warp * Piece<D>::kBuffer;
+  w.load_q(reinterpret_cast<uint4*>(smem + kPreWarps * Piece<D>::kBuffer) + warp * (2 * D), a.q, a.q_type, qrow, a.scale_log2, lane);
   const int least = __reduce_min_sync(0xffffffffu, min(qp[0], qp[1])), most_lo = __reduce_max_sync(0xffffffffu, max(lo[0], lo[1]));
-  uint8_t* ring = smem + warp * (kDecStages * Piece<D>::kStage);
-  const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
-  for (int base = 0; base < nb; base += 32) {
-    const int m = min(32, nb - base);
-    int id = -1;
-    float ks = 0.f, vs = 0.f;
-    const int blk = span.block(base + lane);
-    if (lane < m) {
-      id = kv8_block_id(a.c, a.t, b, head, blk);
-      if (id >= 0) {
-        ks = __ldg(a.c.ks + id);
-        vs = __ldg(a.c.vs + id);
-      }
-    }
-#pragma unroll
-    for (int s = 0; s < kDecStages - 1; ++s) {
-      const int nid = __shfl_sync(0xffffffffu, id, s);
-      if (s < m && nid >= 0) fetch<D>(a.c, nid, ring_at + s * Piece<D>::kStage, lane);
-      cp_commit();
-    }
-    for (int i = 0; i < m; ++i) {
-      {
-        const int next = i + kDecStages - 1;
-        const int nid = __shfl_sync(0xffffffffu, id, next & 31);
-        if (next < m && nid >= 0) fetch<D>(a.c, nid, ring_at + next % kDecStages * Piece<D>::kStage, lane);
-        cp_commit();
-      }
-      cp_wait<kDecStages - 1>();
-      if (__shfl_sync(0xffffffffu, id, i) < 0) continue;
-      const int p0 = __shfl_sync(0xffffffffu, blk, i) * kKvBlock;
-      const float kss = __shfl_sync(0xffffffffu, ks, i), vss = __shfl_sync(0xffffffffu, vs, i);
-      const bool all = p0 + kKvBlock - 1 <= least && (p0 >= most_lo || p0 + kKvBlock <= a.sinks);
-      const int first[2] = {lo[0] - p0, lo[1] - p0}, last[2] = {qp[0] - p0, qp[1] - p0};
-      w.block(ring + i % kDecStages * Piece<D>::kStage, kss, vss, all, first, last, a.sinks - p0, lane);
-    }
-    cp_wait<0>();
-  }
+  Walker<D> walker;
+  walker.init(&mk, &mv, buffer, bars[warp], lane);
+  walker.run(
+      a.c, w, nb, lane,
+      [&](int i, int& pos) {
+        const int blk = span.block(i);
+        pos = blk * kKvBlock;
+        return kv8_block_id(a.c, a.t, b, head, blk);
+      },
+      [&](const int (&p0)[2]) {
+        const int far = max(p0[0], p0[1]) + kKvBlock, near = min(p0[0], p0[1]);
+        return far - 1 <= least && (near >= most_lo || far <= a.sinks);
+      },
+      lo, qp, a.sinks);
+  walker.finish(a.timeout);
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const float l = quad_sum(w.l[i]);
@@ -609,6 +708,18 @@ __global__ void __launch_bounds__(kPreWarps * 32, 3) kv8_prefill_kernel(const At
         store4(a.out, a.out_type, orow[i] + (D / 8) * (2 * t + c) + j, w.m[i] == -INFINITY ? make_float4(0.f, 0.f, 0.f, 0.f) : v);
       }
   }
+}
+
+// One word of page-locked host memory, which kernels of any device can write and the host reads
+// without waiting: set when a bounded wait gave up, reported (and cleared) by the next call.
+int* timeout_word() {
+  static int* word = [] {
+    void* p = nullptr;
+    if (cudaHostAlloc(&p, sizeof(int), cudaHostAllocPortable | cudaHostAllocMapped) != cudaSuccess) return (int*)nullptr;
+    *(int*)p = 0;
+    return (int*)p;
+  }();
+  return word;
 }
 
 int check_attention(const j4b_kv8_cache* cache, int64_t layer, j4b_buf q, int q_type, int64_t q_stride, int64_t tokens, int64_t heads,
@@ -643,13 +754,31 @@ int check_attention(const j4b_kv8_cache* cache, int64_t layer, j4b_buf q, int q_
         window > 0 ? (int)std::min(sinks, far) : 0,
         (float)(scale * 1.4426950408889634),
         (void*)(uintptr_t)out,
-        out_type};
+        out_type,
+        timeout_word()};
+  if (!a->timeout) return set_error(J4B_ENOMEM, "kv8 attention: no host memory for the status word");
+  if (*(volatile int*)a->timeout) {
+    *(volatile int*)a->timeout = 0;
+    return set_error(J4B_ETIMEOUT, "kv8 attention: a wait of an earlier call gave up; its output is not valid");
+  }
   return J4B_OK;
+}
+
+// Rows of one block of 16 tokens of D codes, swizzled as Piece<D>::at.
+bool code_map(CUtensorMap* map, const uint8_t* codes, const Kv8View& v, int dim) {
+  const auto fn = encode_fn();
+  if (!fn) return false;
+  const cuuint64_t dims[2] = {(cuuint64_t)dim, (cuuint64_t)v.pages * v.kv_heads * v.bpp * kKvBlock};
+  const cuuint64_t strides[1] = {(cuuint64_t)dim};
+  const cuuint32_t box[2] = {(cuuint32_t)dim, kKvBlock}, ones[2] = {1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(codes), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            dim == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 int decode_ctas(int dev) {
   const DeviceCtx* ctx = device_ctx(dev);
-  return 3 * (ctx && ctx->sm_count > 0 ? ctx->sm_count : 148);
+  return kDecCtas * (ctx && ctx->sm_count > 0 ? ctx->sm_count : 148);
 }
 
 int64_t decode_bytes(int dim, int64_t batch, int ctas) {
@@ -669,9 +798,11 @@ int allow_smem(Kernel kernel, int bytes, int dev, bool (&done)[kMaxDevices]) {
 template <int D>
 int launch_decode(const DecArgs& d, int dev, int ctas, cudaStream_t stream) {
   static bool done[kMaxDevices] = {};
-  const int smem = kDecWarps * kDecStages * Piece<D>::kStage;
+  const int smem = kDecWarps * (Piece<D>::kBuffer + 32 * D) + 1024;
+  CUtensorMap mk, mv;
+  if (!code_map(&mk, d.a.c.k, d.a.c, D) || !code_map(&mv, d.a.c.v, d.a.c, D)) return set_error(J4B_ECUDA, "cuTensorMapEncodeTiled failed for the cache");
   if (const int st = allow_smem(kv8_decode_kernel<D>, smem, dev, done)) return st;
-  kv8_decode_kernel<D><<<ctas, kDecWarps * 32, smem, stream>>>(d);
+  kv8_decode_kernel<D><<<ctas, kDecWarps * 32, smem, stream>>>(d, mk, mv);
   J4B_CHECK_LAUNCH("kv8_decode_kernel");
   const int64_t rows = (int64_t)d.a.batch * d.a.heads;
   kv8_join_kernel<D><<<(unsigned)((rows + 3) / 4), 128, 0, stream>>>(d, ctas);
@@ -682,11 +813,13 @@ int launch_decode(const DecArgs& d, int dev, int ctas, cudaStream_t stream) {
 template <int D>
 int launch_prefill(const AttnArgs& a, int dev, cudaStream_t stream) {
   static bool done[kMaxDevices] = {};
-  const int smem = kPreWarps * kDecStages * Piece<D>::kStage;
+  const int smem = kPreWarps * (Piece<D>::kBuffer + 32 * D) + 1024;
+  CUtensorMap mk, mv;
+  if (!code_map(&mk, a.c.k, a.c, D) || !code_map(&mv, a.c.v, a.c, D)) return set_error(J4B_ECUDA, "cuTensorMapEncodeTiled failed for the cache");
   if (const int st = allow_smem(kv8_prefill_kernel<D>, smem, dev, done)) return st;
   const int64_t tiles = std::min(a.tokens * a.group, a.tokens * a.group / kPreRows + a.batch);
   J4B_REQUIRE(tiles <= 0x7fffffffLL, "kv8 prefill: too many rows");
-  kv8_prefill_kernel<D><<<dim3((unsigned)tiles, (unsigned)a.c.kv_heads), kPreWarps * 32, smem, stream>>>(a);
+  kv8_prefill_kernel<D><<<dim3((unsigned)tiles, (unsigned)a.c.kv_heads), kPreWarps * 32, smem, stream>>>(a, mk, mv);
   J4B_CHECK_LAUNCH("kv8_prefill_kernel");
   return J4B_OK;
 }

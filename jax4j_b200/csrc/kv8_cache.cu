@@ -189,8 +189,9 @@ int kv8_check(const j4b_kv8_cache* c, int64_t layer, Kv8View* view, int* dev) {
   J4B_REQUIRE(c->kv_heads > 0 && c->kv_heads <= 4096, "kv8: kv_heads must lie in [1, 4096], got %d", c->kv_heads);
   J4B_REQUIRE(c->layers > 0 && c->pages > 0, "kv8: layers and pages must be positive");
   const int bpp = c->page / kKvBlock;
-  const int64_t blocks = c->pages <= 0x7fffffffLL / ((int64_t)c->kv_heads * bpp) ? c->pages * c->kv_heads * bpp : -1;
-  J4B_REQUIRE(blocks > 0, "kv8: a layer holds at most 2^31 - 1 blocks of 16 tokens and head");
+  // rows of head_dim codes are numbered in 32 bits (coordinates of the copies)
+  const int64_t blocks = c->pages <= 0x7ffffffLL / ((int64_t)c->kv_heads * bpp) ? c->pages * c->kv_heads * bpp : -1;
+  J4B_REQUIRE(blocks > 0, "kv8: a layer must hold fewer than 2^31 rows (token and head)");
   J4B_REQUIRE(layer >= 0 && layer < c->layers, "kv8: layer %lld outside [0, %lld)", (long long)layer, (long long)c->layers);
   J4B_REQUIRE(c->k && c->v && c->k_scale && c->v_scale && ((c->k | c->v) & 15) == 0 && ((c->k_scale | c->v_scale) & 3) == 0,
               "kv8: codes must be 16-byte aligned, scales 4-byte");

@@ -106,9 +106,9 @@ struct Kv8Place {
 
 // Finds unit unit(total) for a CTA of THREADS threads (all of them call it): every thread sums a
 // contiguous share of the sequences, the shares are scanned, and the thread whose share holds the
-// unit walks it.
-template <int THREADS, class Count, class Unit>
-__device__ __forceinline__ Kv8Place kv8_find(int batch, Count count, Unit unit) {
+// unit walks it. each(b0, b1, before) sees every thread's share and the units before it.
+template <int THREADS, class Count, class Unit, class Each>
+__device__ __forceinline__ Kv8Place kv8_find(int batch, Count count, Unit unit, Each each) {
   __shared__ int64_t warp_sum[THREADS / 32];
   __shared__ int64_t found_at;
   __shared__ int found_seq;
@@ -131,6 +131,7 @@ __device__ __forceinline__ Kv8Place kv8_find(int batch, Count count, Unit unit) 
     if (w < warp) before += warp_sum[w];
     total += warp_sum[w];
   }
+  each(b0, b1, before);
   int64_t left = unit(total) - before;
   if (left >= 0 && left < mine) {
     int b = b0;
@@ -143,6 +144,10 @@ __device__ __forceinline__ Kv8Place kv8_find(int batch, Count count, Unit unit) 
   }
   __syncthreads();
   return {found_seq, found_at, total};
+}
+template <int THREADS, class Count, class Unit>
+__device__ __forceinline__ Kv8Place kv8_find(int batch, Count count, Unit unit) {
+  return kv8_find<THREADS>(batch, count, unit, [](int, int, int64_t) {});
 }
 
 }  // namespace j4b
