@@ -113,8 +113,9 @@ struct Warp {
 
   // Writes the operands of the query rows (row < 0: zeros) to `dst`, and keeps it. Each row is first
   // brought to a largest element in [2^11, 2^12) by a power of two, so f16's range does not limit
-  // queries. Every lane writes what it reads back; a warp whose rows are another's writes the same.
-  __device__ __forceinline__ void load_q(uint4* dst, const void* base, int type, const int64_t (&row)[kRows], float scale_log2, int lane) {
+  // queries. `warps` warps with the same rows share the operands, each writes every warps-th step.
+  __device__ __forceinline__ void load_q(uint4* dst, const void* base, int type, const int64_t (&row)[kRows], float scale_log2, int lane,
+                                         int warp = 0, int warps = 1) {
     const int t = lane & 3;
     uint32_t frag[D / 16][4];
 #pragma unroll
@@ -144,7 +145,8 @@ struct Warp {
       }
     }
 #pragma unroll
-    for (int i = 0; i < D / 16; ++i) dst[i * 32 + lane] = make_uint4(frag[i][0], frag[i][1], frag[i][2], frag[i][3]);
+    for (int i = 0; i < D / 16; ++i)
+      if (i % warps == warp) dst[i * 32 + lane] = make_uint4(frag[i][0], frag[i][1], frag[i][2], frag[i][3]);
     q = dst + lane;
   }
 
@@ -306,14 +308,23 @@ struct Warp {
   __device__ __forceinline__ float unit() const { return ref * (1.f / (1 << kPShift)); }
 };
 
-// A warp's way through its blocks. Lane 0 has TMA bring a pair of blocks' keys and values to the
-// warp's buffer, each on an mbarrier of its own; a pair's keys are replaced by the next pair's once
-// its scores are done, its values once they are accumulated, so either copy has the other half's
-// work (and the SM's other warps) to arrive in. TMA for the copies because they are 2 KB rows of
-// memory in one instruction: the same loop with 16-byte cp.async straight from the lanes' own places
-// (64-byte pieces of rows) reached 4.7 TB/s with the arithmetic taken out, with TMA 6.4.
+// What a warp knows of a block: its number in the cache (-1: unmapped, or past the end), the position
+// of its first token (then far past every row) and its scales.
+struct __align__(16) Block {
+  int id, pos;
+  float ks, vs;
+};
+constexpr int kNowhere = 0x3fffffff;
+constexpr int kBatch = 32;  // blocks that a warp looks up at once, one a lane
+
+// A warp's copies. Lane 0 has TMA bring a pair of blocks' keys and values to the warp's buffer, each
+// on an mbarrier of its own; a pair's keys are replaced by the next pair's once its scores are done,
+// its values once they are accumulated, so either copy has the other half's work (and the SM's other
+// warps) to arrive in. TMA for the copies because they are 2 KB rows of memory in one instruction:
+// the same loop with 16-byte cp.async straight from the lanes' own places (64-byte pieces of rows)
+// reached 4.7 TB/s with the arithmetic taken out, with TMA 6.4.
 template <int D>
-struct Walker {
+struct Copies {
   const CUtensorMap *mk, *mv;
   uint8_t* buffer;
   uint64_t* bars;  // keys, values
@@ -334,9 +345,10 @@ struct Walker {
     }
     __syncwarp();
   }
-  // the pair's blocks that are there (number >= 0), keys (which = 0) or values (1)
-  __device__ __forceinline__ void fetch(int which, int id0, int id1, int lane) {
+  // keys (which = 0) or values (1) of the pair's blocks that are there
+  __device__ __forceinline__ void fetch(int which, const Block* pair, int lane) {
     if (lane == 0 && ok) {
+      const int id0 = pair[0].id, id1 = pair[1].id;
       uint8_t* dst = buffer + which * 2 * Piece<D>::kBytes;
       bar_expect_tx(&bars[which], ((id0 >= 0) + (id1 >= 0)) * Piece<D>::kBytes);
       if (id0 >= 0) tma_tile(dst, which ? mv : mk, 0, id0 * kKvBlock, &bars[which]);
@@ -351,49 +363,6 @@ struct Walker {
     bar_wait(&bars[0], phase);
     bar_wait(&bars[1], phase);
     *timeout = 1;
-  }
-
-  // look(i, pos) gives block i's number (-1: unmapped, its tokens are skipped) and first position;
-  // all_seen(p0) says whether every row sees all of a pair. Lane i looks up the i-th of 32 blocks.
-  template <bool SPLIT, class Look, class All>
-  __device__ __forceinline__ void run(const Kv8View& c, Warp<D, SPLIT>& w, int mine, int lane, Look look, All all_seen,
-                                      const int (&first)[Warp<D, SPLIT>::kRows], const int (&last)[Warp<D, SPLIT>::kRows], int sinks) {
-    constexpr int kNowhere = 0x3fffffff;
-    for (int base = 0; base < mine; base += 32) {
-      const int n = min(32, mine - base);
-      int id = -1, at = kNowhere;
-      float ks = 0.f, vs = 0.f;
-      if (lane < n) {
-        int pos;
-        id = look(base + lane, pos);
-        if (id >= 0) {
-          at = pos;
-          ks = __ldg(c.ks + id);
-          vs = __ldg(c.vs + id);
-        }
-      }
-      int id0 = __shfl_sync(0xffffffffu, id, 0), id1 = __shfl_sync(0xffffffffu, id, 1);
-      fetch(0, id0, id1, lane);
-      fetch(1, id0, id1, lane);
-      for (int i = 0; i < n; i += 2) {
-        const int p0[2] = {__shfl_sync(0xffffffffu, at, i), __shfl_sync(0xffffffffu, at, i + 1)};
-        const float kk[2] = {__shfl_sync(0xffffffffu, ks, i), __shfl_sync(0xffffffffu, ks, i + 1)};
-        const float vv[2] = {__shfl_sync(0xffffffffu, vs, i), __shfl_sync(0xffffffffu, vs, i + 1)};
-        const bool more = i + 2 < n, any = p0[0] != kNowhere || p0[1] != kNowhere;
-        id0 = __shfl_sync(0xffffffffu, id, (i + 2) & 31);
-        id1 = __shfl_sync(0xffffffffu, id, (i + 3) & 31);
-        uint32_t p[2][4], seen;
-        wait(0);
-        if (any) w.scores(buffer, kk, vv, all_seen(p0), first, last, sinks, p0, lane, p, seen);
-        __syncwarp();
-        if (more) fetch(0, id0, id1, lane);
-        wait(1);
-        if (any) w.values(buffer + 2 * Piece<D>::kBytes, p, seen, lane);
-        __syncwarp();
-        if (more) fetch(1, id0, id1, lane);
-        phase ^= 1;
-      }
-    }
   }
 };
 
@@ -420,23 +389,31 @@ __device__ __forceinline__ uint8_t* aligned_smem(uint8_t* raw) {  // the swizzle
 
 // ---------------------------------------------------------------------------------------------
 // Decode. Rows are (sequence, kv head, run of up to 8 of its query heads); a row's units are its
-// visible blocks. All units of the call, in order, are cut into equal shares, one a CTA (a CTA's
-// warps take every fourth block of its share of a row), so a batch of any mix of lengths fills the
-// GPU evenly. A row that lies in one share is finished there; one cut by a share's end leaves an
-// unnormalised part (running maximum, sum, 8 x D) in the workspace for kv8_join_kernel.
+// visible blocks, and kRowUnits more in front of them for what a row costs by itself. All units of
+// the call, in order, are cut into equal shares, one a CTA (a CTA's warps take every fourth block of
+// its segment of a row), so a batch of any mix of lengths fills the GPU evenly. A row whose blocks lie
+// in one share is finished there; one cut by a share's end leaves an unnormalised part (running
+// maximum, sum, 8 x D) in the workspace for kv8_join_kernel.
+//
+// Bound by HBM once the rows are long: 2 x 16 D bytes a block against ~430 warp instructions at 12
+// warps an SM. What the short ones cost is latency, so a warp never lets its copies run dry: it looks
+// up the next 32 blocks, of its next segment too, while it works on these, and fetches the first
+// pair's keys of the next segment before it merges.
 constexpr int kDecWarps = 4;
-constexpr int kDecCtas = 4;  // of an SM
+constexpr int kDecCtas = 3;  // of an SM
 constexpr int kDecHeads = 8;
+constexpr int kRowUnits = 20;  // 4: ragged batch (48 x up to 8191 tokens) 78.9 us, 12: 67.8, 20: 61.6, 28: 61.7, 40: 63.5
 
 struct DecArgs {
   AttnArgs a;
-  int chunks;   // runs of 8 heads of a kv head
-  float* part;  // [2 * CTAs][kDecHeads][D + 2]
-  int64_t* cum; // [batch + 1] units of a row of the sequences before b
+  int chunks;    // runs of 8 heads of a kv head
+  float* part;   // [2 * CTAs][kDecHeads][D + 2]
+  int64_t* cum;  // [batch + 1] units of the sequences before b
 };
 
-__device__ __forceinline__ int decode_blocks(const AttnArgs& a, int b) {
-  return span_of(__ldg(a.lengths + b) - 1, __ldg(a.lengths + b) - 1, a.window, a.sinks).count();
+__device__ __forceinline__ int64_t row_units(const AttnArgs& a, int b) {
+  const int len = __ldg(a.lengths + b), n = span_of(len - 1, len - 1, a.window, a.sinks).count();
+  return n > 0 ? n + kRowUnits : 0;
 }
 // Units of a CTA: a whole number for each of its warps, the same for all CTAs (the last ones may get none).
 __device__ __forceinline__ int64_t share_of(int64_t units, int ctas) {
@@ -444,174 +421,258 @@ __device__ __forceinline__ int64_t share_of(int64_t units, int ctas) {
   return (units + each - 1) / each * kDecWarps;
 }
 
+// A CTA's part of a row: its blocks begin .. end - 1 of the row's nb.
+struct Segment {
+  int b, row, begin, end, nb, len;
+  Span span;
+  __device__ __forceinline__ int mine(int warp) const { return max(0, (end - begin - warp + kDecWarps - 1) / kDecWarps); }
+};
+
+// The share's segments one by one; false after the last.
+struct Share {
+  int b;
+  int64_t at, left;  // the next unit among sequence b's, units left
+  __device__ __forceinline__ bool next(const AttnArgs& a, int rows, Segment& s) {
+    while (left > 0) {
+      s.len = __ldg(a.lengths + b);
+      s.span = span_of(s.len - 1, s.len - 1, a.window, a.sinks);
+      s.nb = s.span.count();
+      const int units = s.nb > 0 ? s.nb + kRowUnits : 0;
+      if (at >= (int64_t)units * rows) {
+        ++b;
+        at = 0;
+        continue;
+      }
+      s.b = b;
+      s.row = (int)(at / units);
+      const int from = (int)(at - (int64_t)s.row * units), to = (int)min((int64_t)units, from + left);
+      left -= to - from;
+      at += to - from;
+      s.begin = max(0, from - kRowUnits);
+      s.end = to - kRowUnits;
+      if (s.end > s.begin) return true;
+    }
+    return false;
+  }
+};
+
+// where the merge keeps 4 floats c of head h's D: spread over the banks
+__device__ __forceinline__ int merge_at(int h, int c, int d) { return h * d + 4 * (c ^ (((c >> 3) * 2 + (h & 1)) & 7)); }
+
 template <int D>
 __global__ void __launch_bounds__(kDecWarps * 32, kDecCtas) kv8_decode_kernel(const DecArgs d, const __grid_constant__ CUtensorMap mk,
-                                                                           const __grid_constant__ CUtensorMap mv) {
+                                                                              const __grid_constant__ CUtensorMap mv) {
   const AttnArgs& a = d.a;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = aligned_smem(smem_raw);
   __shared__ uint64_t bars[kDecWarps][2];
+  __shared__ float2 states[kDecWarps][kDecHeads];  // (m, l)
+  asm volatile("griddepcontrol.launch_dependents;");
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   const int rows = a.c.kv_heads * d.chunks;
   const bool record = blockIdx.x == 0;  // the sequences' first units, for the join
   const Kv8Place at = kv8_find<kDecWarps * 32>(
-      a.batch, [&](int b) -> int64_t { return (int64_t)decode_blocks(a, b) * rows; },
+      a.batch, [&](int b) -> int64_t { return row_units(a, b) * rows; },
       [&](int64_t units) -> int64_t { return share_of(units, gridDim.x) * blockIdx.x; },
       [&](int b0, int b1, int64_t before) {
         if (!record) return;
         for (int b = b0; b < b1; ++b) {
           d.cum[b] = before;
-          before += (int64_t)decode_blocks(a, b) * rows;
+          before += row_units(a, b) * rows;
         }
         if (b1 == a.batch) d.cum[a.batch] = before;  // the threads past the last sequence write the same total
       });
-  int64_t left = at.seq < 0 ? 0 : min(share_of(at.total, gridDim.x), at.total - share_of(at.total, gridDim.x) * blockIdx.x);
+  if (at.seq < 0) return;
+  const int64_t share = share_of(at.total, gridDim.x);
+  Share work = {at.seq, at.at, min(share, at.total - share * blockIdx.x)};
+  // per warp: its copies (keys, values of a pair; the values' half holds its state in the merge) and
+  // the blocks of this batch and of the next; per CTA: the row's queries
   uint8_t* buffer = smem + warp * Piece<D>::kBuffer;
-  uint4* queries = reinterpret_cast<uint4*>(smem + kDecWarps * Piece<D>::kBuffer) + warp * (2 * D);
-  // the merge of the warps' states reuses the buffers (drained by then): per warp 8 x (m, l, D)
-  float* merge = reinterpret_cast<float*>(buffer);
-  constexpr int kMergeStride = Piece<D>::kBuffer / 4;
-  static_assert(kMergeStride >= kDecHeads * (D + 2), "a warp's state must fit its buffer");
-  Walker<D> walker;
-  walker.init(&mk, &mv, buffer, bars[warp], lane);
-  int b = at.seq;
-  int64_t in_seq = at.at;
-  int segment = 0;
-  Warp<D, true> w;
-  while (left > 0) {
-    const int len = __ldg(a.lengths + b);
-    const Span span = span_of(len - 1, len - 1, a.window, a.sinks);
-    const int nb = span.count();
-    if (in_seq >= (int64_t)nb * rows) {
-      ++b;
-      in_seq = 0;
-      continue;
+  Block* blocks = reinterpret_cast<Block*>(smem + kDecWarps * Piece<D>::kBuffer) + warp * (2 * kBatch);
+  uint4* queries = reinterpret_cast<uint4*>(smem + kDecWarps * (Piece<D>::kBuffer + 2 * kBatch * (int)sizeof(Block)));
+  float* merge = reinterpret_cast<float*>(buffer + 2 * Piece<D>::kBytes);
+  static_assert(2 * Piece<D>::kBytes >= kDecHeads * D * 4, "a warp's state must fit its values' buffer");
+  Copies<D> copies;
+  copies.init(&mk, &mv, buffer, bars[warp], lane);
+
+  // Block i of this warp in a segment: first its page, then (once that is there) number and scales.
+  auto page_of = [&](const Segment& s, int i, int count) -> int {
+    if (i >= count) return -1;
+    const int pg = s.span.block(s.begin + warp + kDecWarps * i) / a.c.bpp;
+    return pg < a.t.width ? __ldg(a.t.pages + s.b * a.t.stride + pg) : -1;
+  };
+  auto look_up = [&](const Segment& s, int i, int page, Block* dst) {
+    Block k = {-1, kNowhere, 0.f, 0.f};
+    if ((unsigned)page < (unsigned)a.c.pages) {
+      const int blk = s.span.block(s.begin + warp + kDecWarps * i);
+      k.id = (page * a.c.kv_heads + s.row / d.chunks) * a.c.bpp + blk % a.c.bpp;
+      k.pos = blk * kKvBlock;
+      k.ks = __ldg(a.c.ks + k.id);
+      k.vs = __ldg(a.c.vs + k.id);
     }
-    const int row = (int)(in_seq / nb), begin = (int)(in_seq % nb);
-    const int end = (int)min((int64_t)nb, begin + left);
-    const int head = row / d.chunks, h0 = head * a.group + row % d.chunks * kDecHeads;
+    dst[lane] = k;
+  };
+
+  Segment cur, nxt;
+  bool more = work.next(a, rows, cur);
+  int which = 0;  // half of `blocks` in use
+  if (more) {
+    look_up(cur, lane, page_of(cur, lane, cur.mine(warp)), blocks);
+    __syncwarp();
+    if (cur.mine(warp) > 0) {
+      copies.fetch(0, blocks, lane);
+      copies.fetch(1, blocks, lane);
+    }
+  }
+  Warp<D, true> w;
+  for (int done = 0; more; ++done, cur = nxt) {
+    more = work.next(a, rows, nxt);
+    const int head = cur.row / d.chunks, h0 = head * a.group + cur.row % d.chunks * kDecHeads;
     const int nh = min(kDecHeads, (head + 1) * a.group - h0);
-    const int lo = a.window > 0 ? max(0, len - a.window) : 0;
+    const int first[1] = {a.window > 0 ? max(0, cur.len - a.window) : 0}, last[1] = {cur.len - 1};
     w.reset();
     {
-      const int64_t qrow[1] = {g < nh ? (int64_t)b * a.q_stride + (int64_t)(h0 + g) * D : -1};
-      w.load_q(queries, a.q, a.q_type, qrow, a.scale_log2, lane);
-    }
-    // the warp's blocks are begin + warp + 4 i
-    const int first[1] = {lo}, last[1] = {len - 1};
-    walker.run(
-        a.c, w, max(0, (end - begin - warp + kDecWarps - 1) / kDecWarps), lane,
-        [&](int i, int& pos) {
-          const int blk = span.block(begin + warp + kDecWarps * i);
-          pos = blk * kKvBlock;
-          return kv8_block_id(a.c, a.t, b, head, blk);
-        },
-        [&](const int (&p0)[2]) {
-          const int far = max(p0[0], p0[1]) + kKvBlock, near = min(p0[0], p0[1]);
-          return far <= len && (near >= lo || far <= a.sinks);
-        },
-        first, last, a.sinks);
-    // merge the warps
-    __syncwarp();
-    {
-      const float l = quad_sum(w.l[0]), unit = w.unit();
-      float* mm = merge + g * (D + 2);
-      if (g < nh) {
-      if (t == 0) {
-        mm[0] = w.m[0];
-        mm[1] = l;
-      }
-      // columns of tile j are dims (D / 8) n + j: this thread's n are 2t and 2t + 1
-#pragma unroll
-      for (int j = 0; j < D / 8; ++j) {
-        mm[2 + (D / 8) * (2 * t) + j] = (w.o[j][0] + w.o[j][2]) * unit;
-        mm[2 + (D / 8) * (2 * t + 1) + j] = (w.o[j][1] + w.o[j][3]) * unit;
-      }
-      }
+      const int64_t qrow[1] = {g < nh ? (int64_t)cur.b * a.q_stride + (int64_t)(h0 + g) * D : -1};
+      w.load_q(queries, a.q, a.q_type, qrow, a.scale_log2, lane, warp, kDecWarps);
     }
     __syncthreads();
-    const bool whole = begin == 0 && end == nb;
-    const float* all = reinterpret_cast<const float*>(smem);
+    const int mine = cur.mine(warp), next_mine = more ? nxt.mine(warp) : 0;
+    for (int base = 0; base < mine; base += kBatch) {
+      const int n = min(kBatch, mine - base);
+      const bool same = base + kBatch < mine;  // the next batch is of this segment
+      const int next_base = same ? base + kBatch : 0, next_n = same ? mine : next_mine;
+      const int page = same ? page_of(cur, next_base + lane, next_n) : page_of(nxt, lane, next_n);
+      const Block* now = blocks + which * kBatch;
+      Block* then = blocks + (which ^ 1) * kBatch;
+      const int look_at = min(4, (n - 1) & ~1);
+      for (int i = 0; i < n; i += 2) {
+        const Block b0 = now[i], b1 = now[i + 1];  // past n: not there
+        const int p0[2] = {b0.pos, b1.pos};
+        const float kk[2] = {b0.ks, b1.ks}, vv[2] = {b0.vs, b1.vs};
+        const bool any = b0.id >= 0 || b1.id >= 0;
+        const int far = max(p0[0], p0[1]) + kKvBlock, near = min(p0[0], p0[1]);
+        const bool all = far <= cur.len && (near >= first[0] || far <= a.sinks);
+        if (i == look_at) look_up(same ? cur : nxt, next_base + lane, page, then);
+        uint32_t p[2][4], seen;
+        copies.wait(0);
+        if (any) w.scores(buffer, kk, vv, all, first, last, a.sinks, p0, lane, p, seen);
+        __syncwarp();
+        const bool end = i + 2 >= n;
+        if (!end)
+          copies.fetch(0, now + i + 2, lane);
+        else if (next_n > next_base)
+          copies.fetch(0, then, lane);
+        copies.wait(1);
+        if (any) w.values(buffer + 2 * Piece<D>::kBytes, p, seen, lane);
+        __syncwarp();
+        if (!end)
+          copies.fetch(1, now + i + 2, lane);
+        else if (same)
+          copies.fetch(1, then, lane);
+        copies.phase ^= 1;
+      }
+      which ^= 1;
+    }
+    if (mine == 0 && next_mine > 0) {  // a segment of fewer blocks than warps
+      Block* then = blocks + (which ^ 1) * kBatch;
+      look_up(nxt, lane, page_of(nxt, lane, next_mine), then);
+      __syncwarp();
+      copies.fetch(0, then, lane);
+      which ^= 1;
+    }
+    // merge the warps
+    const float l = quad_sum(w.l[0]), unit = w.unit();
+    if (g < nh) {
+      if (t == 0) states[warp][g] = make_float2(w.m[0], l);
+      // columns of tile j are dims (D / 8) n + j: this thread's n are 2t and 2t + 1
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int j = 0; j < D / 8; j += 4)
+          *reinterpret_cast<float4*>(merge + merge_at(g, ((D / 8) * (2 * t + n) + j) / 4, D)) =
+              make_float4((w.o[j][n] + w.o[j][2 + n]) * unit, (w.o[j + 1][n] + w.o[j + 1][2 + n]) * unit,
+                          (w.o[j + 2][n] + w.o[j + 2][2 + n]) * unit, (w.o[j + 3][n] + w.o[j + 3][2 + n]) * unit);
+    }
+    __syncthreads();
+    const bool whole = cur.begin == 0 && cur.end == cur.nb;
     for (int e = tid; e < nh * (D / 4); e += kDecWarps * 32) {
-      const int h = e / (D / 4), c = e % (D / 4) * 4;
+      const int h = e / (D / 4), c = e % (D / 4);
       float mt = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < kDecWarps; ++i) mt = fmaxf(mt, all[i * kMergeStride + h * (D + 2)]);
+      for (int i = 0; i < kDecWarps; ++i) mt = fmaxf(mt, states[i][h].x);
       float lt = 0.f;
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (mt != -INFINITY) {
 #pragma unroll
-      for (int i = 0; i < kDecWarps; ++i) {
-        const float* src = all + i * kMergeStride + h * (D + 2);
-        const float f = src[0] == -INFINITY ? 0.f : exp2f(src[0] - mt);
-        lt = fmaf(src[1], f, lt);
-        v.x = fmaf(src[2 + c], f, v.x);
-        v.y = fmaf(src[3 + c], f, v.y);
-        v.z = fmaf(src[4 + c], f, v.z);
-        v.w = fmaf(src[5 + c], f, v.w);
+        for (int i = 0; i < kDecWarps; ++i) {
+          const float2 st = states[i][h];
+          const float4 x = *reinterpret_cast<const float4*>(smem + i * Piece<D>::kBuffer + 2 * Piece<D>::kBytes + 4 * merge_at(h, c, D));
+          const float f = exp2f(st.x - mt);
+          lt = fmaf(st.y, f, lt);
+          v.x = fmaf(x.x, f, v.x);
+          v.y = fmaf(x.y, f, v.y);
+          v.z = fmaf(x.z, f, v.z);
+          v.w = fmaf(x.w, f, v.w);
+        }
       }
       if (whole) {
         const float inv = mt == -INFINITY ? 0.f : 1.f / lt;
-        if (mt == -INFINITY) v = make_float4(0.f, 0.f, 0.f, 0.f);
-        store4(a.out, a.out_type, ((int64_t)b * a.heads + h0 + h) * D + c, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
+        store4(a.out, a.out_type, ((int64_t)cur.b * a.heads + h0 + h) * D + 4 * c, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
       } else {
-        float* dst = d.part + (((int64_t)blockIdx.x * 2 + (segment > 0)) * kDecHeads + h) * (D + 2);
-        if (c == 0) {
-          dst[0] = mt;
-          dst[1] = lt;
-        }
-        *reinterpret_cast<float2*>(dst + 2 + c) = make_float2(v.x, v.y);
-        *reinterpret_cast<float2*>(dst + 4 + c) = make_float2(v.z, v.w);
+        float* dst = d.part + (((int64_t)blockIdx.x * 2 + (done > 0)) * kDecHeads + h) * (D + 2);
+        if (c == 0) *reinterpret_cast<float2*>(dst) = make_float2(mt, lt);
+        *reinterpret_cast<float2*>(dst + 2 + 4 * c) = make_float2(v.x, v.y);
+        *reinterpret_cast<float2*>(dst + 4 + 4 * c) = make_float2(v.z, v.w);
       }
     }
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the buffers go back to TMA
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the values' half goes back to TMA
     __syncthreads();
-    left -= end - begin;
-    in_seq += end - begin;
-    ++segment;
+    if (next_mine > 0) copies.fetch(1, blocks + which * kBatch, lane);
   }
-  walker.finish(a.timeout);
+  copies.finish(a.timeout);
 }
 
-// Rows without a block give zeros; rows cut into parts are joined, in the parts' order whatever
-// CTA wrote them first. One warp per (sequence, query head).
+// Rows without a block give zeros; rows cut into parts are joined, in an order that only their
+// lengths set. One CTA per (sequence, query head), its warps share the parts.
 template <int D>
 __global__ void __launch_bounds__(128) kv8_join_kernel(const DecArgs d, int ctas) {
   const AttnArgs& a = d.a;
-  const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  if (i >= (int64_t)a.batch * a.heads) return;
+  const int64_t i = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int b = (int)(i / a.heads), qh = (int)(i % a.heads);
   const int head = qh / a.group, chunk = qh % a.group / kDecHeads, h = qh % a.group % kDecHeads;
+  __shared__ float sums[4][D];
+  __shared__ float2 states[4];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int64_t before = d.cum[b], units = d.cum[a.batch];
-  const int64_t nb = (d.cum[b + 1] - before) / (a.c.kv_heads * d.chunks);
+  const int64_t row = (d.cum[b + 1] - before) / (a.c.kv_heads * d.chunks);
   constexpr int kPer = D / 32;
   float acc[kPer];
 #pragma unroll
   for (int e = 0; e < kPer; ++e) acc[e] = 0.f;
-  float lt = 0.f;
-  if (nb > 0) {
-    const int64_t share = share_of(units, ctas), u0 = before + (head * d.chunks + chunk) * nb;
-    const int c0 = (int)(u0 / share), c1 = (int)((u0 + nb - 1) / share);
+  float lt = 0.f, mt = -INFINITY;
+  if (row > 0) {
+    const int64_t share = share_of(units, ctas), u0 = before + (head * d.chunks + chunk) * row;
+    const int c0 = (int)((u0 + kRowUnits) / share), c1 = (int)((u0 + row - 1) / share);
     if (c0 == c1) return;  // finished by its CTA
     // part i of the row is the first segment of CTA c0 + i, but for part 0 when c0 starts before the row
     const float* first = d.part + ((int64_t)(2 * c0 + (share * c0 < u0)) * kDecHeads + h) * (D + 2);
     const float* rest = d.part + ((int64_t)2 * (c0 + 1) * kDecHeads + h) * (D + 2);
     constexpr int64_t kNext = (int64_t)2 * kDecHeads * (D + 2);
     const int parts = c1 - c0 + 1;
-    float mt = -INFINITY;
-    for (int base = 0; base < parts; base += 32) {
-      const int n = min(32, parts - base);
-      const float* mine = base + lane == 0 ? first : rest + (base + lane - 1) * kNext;
+    // warp w takes parts w, w + 4, ..: lane j looks at the j-th of 32
+    for (int base = 0; base * 4 < parts; base += 32) {
+      const int mine = warp + 4 * (base + lane), n = min(32, (parts - warp + 3) / 4 - base);
       float2 ml = make_float2(-INFINITY, 0.f);
-      if (lane < n) ml = *reinterpret_cast<const float2*>(mine);
+      if (mine < parts) ml = *reinterpret_cast<const float2*>(mine == 0 ? first : rest + (mine - 1) * kNext);
       float mn = ml.x;
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
       mn = fmaxf(mn, mt);
       if (mn == -INFINITY) continue;
-      const float old = exp2f(mt - mn), w = exp2f(ml.x - mn);  // 0 for parts that saw nothing
+      const float old = exp2f(mt - mn), f = exp2f(ml.x - mn);  // 0 for parts that saw nothing
       mt = mn;
-      float sum = w * ml.y;
+      float sum = f * ml.y;
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
       lt = lt * old + sum;
@@ -619,22 +680,36 @@ __global__ void __launch_bounds__(128) kv8_join_kernel(const DecArgs d, int ctas
       for (int e = 0; e < kPer; ++e) acc[e] *= old;
 #pragma unroll 8
       for (int p = 0; p < n; ++p) {
-        const float f = __shfl_sync(0xffffffffu, w, p);
-        const float* src = (base + p == 0 ? first : rest + (base + p - 1) * kNext) + 2 + lane;
+        const int at = warp + 4 * (base + p);
+        const float fp = __shfl_sync(0xffffffffu, f, p);
+        const float* src = (at == 0 ? first : rest + (at - 1) * kNext) + 2 + lane;
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) acc[e] = fmaf(f, src[32 * e], acc[e]);
+        for (int e = 0; e < kPer; ++e) acc[e] = fmaf(fp, src[32 * e], acc[e]);
       }
     }
   }
-  const float inv = lt != 0.f ? 1.f / lt : 0.f;
+  if (lane == 0) states[warp] = make_float2(mt, lt);
 #pragma unroll
-  for (int e = 0; e < kPer; ++e) {
-    const int64_t o = ((int64_t)b * a.heads + qh) * D + lane + 32 * e;
-    if (a.out_type == J4B_F32)
-      static_cast<float*>(a.out)[o] = acc[e] * inv;
-    else
-      static_cast<__nv_bfloat16*>(a.out)[o] = __float2bfloat16_rn(acc[e] * inv);
+  for (int e = 0; e < kPer; ++e) sums[warp][lane + 32 * e] = acc[e];
+  __syncthreads();
+  if (tid >= D) return;
+  float m = -INFINITY, l = 0.f, v = 0.f;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) m = fmaxf(m, states[w].x);
+  if (m != -INFINITY) {
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float f = exp2f(states[w].x - m);
+      l = fmaf(states[w].y, f, l);
+      v = fmaf(sums[w][tid], f, v);
+    }
+    v /= l;
   }
+  const int64_t o = i * D + tid;
+  if (a.out_type == J4B_F32)
+    static_cast<float*>(a.out)[o] = v;
+  else
+    static_cast<__nv_bfloat16*>(a.out)[o] = __float2bfloat16_rn(v);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -678,23 +753,44 @@ __global__ void __launch_bounds__(kPreWarps * 32, 3) kv8_prefill_kernel(const At
     lo[i] = a.window > 0 ? max(0, qp[i] - a.window + 1) : 0;
   }
   uint8_t* buffer = smem + warp * Piece<D>::kBuffer;
+  Block* blocks = reinterpret_cast<Block*>(smem + kPreWarps * (Piece<D>::kBuffer + 32 * D)) + warp * kBatch;
   w.load_q(reinterpret_cast<uint4*>(smem + kPreWarps * Piece<D>::kBuffer) + warp * (2 * D), a.q, a.q_type, qrow, a.scale_log2, lane);
   const int least = __reduce_min_sync(0xffffffffu, min(qp[0], qp[1])), most_lo = __reduce_max_sync(0xffffffffu, max(lo[0], lo[1]));
-  Walker<D> walker;
-  walker.init(&mk, &mv, buffer, bars[warp], lane);
-  walker.run(
-      a.c, w, nb, lane,
-      [&](int i, int& pos) {
-        const int blk = span.block(i);
-        pos = blk * kKvBlock;
-        return kv8_block_id(a.c, a.t, b, head, blk);
-      },
-      [&](const int (&p0)[2]) {
-        const int far = max(p0[0], p0[1]) + kKvBlock, near = min(p0[0], p0[1]);
-        return far - 1 <= least && (near >= most_lo || far <= a.sinks);
-      },
-      lo, qp, a.sinks);
-  walker.finish(a.timeout);
+  Copies<D> copies;
+  copies.init(&mk, &mv, buffer, bars[warp], lane);
+  for (int base = 0; base < nb; base += kBatch) {
+    const int m = min(kBatch, nb - base);
+    {
+      Block k = {-1, kNowhere, 0.f, 0.f};
+      const int blk = span.block(base + lane);
+      if (lane < m) k.id = kv8_block_id(a.c, a.t, b, head, blk);
+      if (k.id >= 0) k = {k.id, blk * kKvBlock, __ldg(a.c.ks + k.id), __ldg(a.c.vs + k.id)};
+      __syncwarp();
+      blocks[lane] = k;
+      __syncwarp();
+    }
+    copies.fetch(0, blocks, lane);
+    copies.fetch(1, blocks, lane);
+    for (int i = 0; i < m; i += 2) {
+      const Block b0 = blocks[i], b1 = blocks[i + 1];
+      const int p0[2] = {b0.pos, b1.pos};
+      const float kk[2] = {b0.ks, b1.ks}, vv[2] = {b0.vs, b1.vs};
+      const bool any = b0.id >= 0 || b1.id >= 0;
+      const int far = max(p0[0], p0[1]) + kKvBlock, near = min(p0[0], p0[1]);
+      const bool all = far - 1 <= least && (near >= most_lo || far <= a.sinks);
+      uint32_t p[2][4], seen;
+      copies.wait(0);
+      if (any) w.scores(buffer, kk, vv, all, lo, qp, a.sinks, p0, lane, p, seen);
+      __syncwarp();
+      if (i + 2 < m) copies.fetch(0, blocks + i + 2, lane);
+      copies.wait(1);
+      if (any) w.values(buffer + 2 * Piece<D>::kBytes, p, seen, lane);
+      __syncwarp();
+      if (i + 2 < m) copies.fetch(1, blocks + i + 2, lane);
+      copies.phase ^= 1;
+    }
+  }
+  copies.finish(a.timeout);
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const float l = quad_sum(w.l[i]);
@@ -798,14 +894,23 @@ int allow_smem(Kernel kernel, int bytes, int dev, bool (&done)[kMaxDevices]) {
 template <int D>
 int launch_decode(const DecArgs& d, int dev, int ctas, cudaStream_t stream) {
   static bool done[kMaxDevices] = {};
-  const int smem = kDecWarps * (Piece<D>::kBuffer + 32 * D) + 1024;
+  const int smem = kDecWarps * (Piece<D>::kBuffer + 2 * kBatch * (int)sizeof(Block)) + 32 * D + 1024;
   CUtensorMap mk, mv;
   if (!code_map(&mk, d.a.c.k, d.a.c, D) || !code_map(&mv, d.a.c.v, d.a.c, D)) return set_error(J4B_ECUDA, "cuTensorMapEncodeTiled failed for the cache");
   if (const int st = allow_smem(kv8_decode_kernel<D>, smem, dev, done)) return st;
   kv8_decode_kernel<D><<<ctas, kDecWarps * 32, smem, stream>>>(d, mk, mv);
   J4B_CHECK_LAUNCH("kv8_decode_kernel");
-  const int64_t rows = (int64_t)d.a.batch * d.a.heads;
-  kv8_join_kernel<D><<<(unsigned)((rows + 3) / 4), 128, 0, stream>>>(d, ctas);
+  // launched while the decode kernel runs: its CTAs wait for it on the device
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3((unsigned)((int64_t)d.a.batch * d.a.heads));
+  config.blockDim = dim3(128);
+  config.stream = stream;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = &attr;
+  config.numAttrs = 1;
+  J4B_CUDA(cudaLaunchKernelEx(&config, kv8_join_kernel<D>, d, ctas), "kv8_join_kernel");
   J4B_CHECK_LAUNCH("kv8_join_kernel");
   return J4B_OK;
 }
@@ -813,7 +918,7 @@ int launch_decode(const DecArgs& d, int dev, int ctas, cudaStream_t stream) {
 template <int D>
 int launch_prefill(const AttnArgs& a, int dev, cudaStream_t stream) {
   static bool done[kMaxDevices] = {};
-  const int smem = kPreWarps * (Piece<D>::kBuffer + 32 * D) + 1024;
+  const int smem = kPreWarps * (Piece<D>::kBuffer + 32 * D + kBatch * (int)sizeof(Block)) + 1024;
   CUtensorMap mk, mv;
   if (!code_map(&mk, a.c.k, a.c, D) || !code_map(&mv, a.c.v, a.c, D)) return set_error(J4B_ECUDA, "cuTensorMapEncodeTiled failed for the cache");
   if (const int st = allow_smem(kv8_prefill_kernel<D>, smem, dev, done)) return st;
@@ -848,6 +953,7 @@ extern "C" int j4b_kv8_attention_decode(const j4b_kv8_cache* cache, int64_t laye
   if (const int st = check_attention(cache, layer, q, q_type, q_stride, batch, heads, table, table_stride, table_width, lengths, batch,
                                      window, sinks, scale, out, out_type, &d.a, &dev))
     return st;
+  J4B_REQUIRE(batch * heads <= 0x7fffffffLL, "kv8 decode: too many rows");
   if (batch == 0) return J4B_OK;
   const int ctas = decode_ctas(dev);
   J4B_REQUIRE(workspace && (workspace & 15) == 0 && workspace_bytes >= decode_bytes(cache->head_dim, batch, ctas),
