@@ -1,5 +1,5 @@
-// Attention over the 8-bit paged KV cache (format: kv8_common.cuh): one query per sequence
-// (decode) and ragged causal chunks (prefill), grouped heads, sliding window with sinks.
+// Decode attention over the 8-bit paged KV cache (format: kv8_common.cuh): one query per sequence,
+// grouped heads, sliding window with sinks. Prefill: kv8_prefill.cu.
 //
 // A warp takes a 16-token block of one kv head at a time straight from the pages into mma.sync
 // m16n8k16 operands: 8 tokens are the n columns of S = Q K^T, and since a contraction may run over
@@ -17,8 +17,6 @@
 
 namespace j4b {
 
-int kv8_check(const j4b_kv8_cache* c, int64_t layer, Kv8View* view, int* dev);
-
 namespace {
 
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -27,19 +25,10 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ uint32_t h2(float a, float b) {
-  const __half2 h = __floats2half2_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
 // what h2 rounded away, as f16x2
 __device__ __forceinline__ uint32_t h2_rest(float a, float b, uint32_t hi) {
   const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi));
   return h2(a - f.x, b - f.y);
-}
-__device__ __forceinline__ float exp2_ftz(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
 }
 __device__ __forceinline__ float quad_max(float v) {
   v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
@@ -48,22 +37,6 @@ __device__ __forceinline__ float quad_max(float v) {
 __device__ __forceinline__ float quad_sum(float v) {
   v += __shfl_xor_sync(0xffffffffu, v, 1);
   return v + __shfl_xor_sync(0xffffffffu, v, 2);
-}
-
-// The blocks that queries at positions first .. last of a sequence of `len` tokens see: the first
-// `sink_blocks` ones, then those from `from` on to `end` (exclusive). count() of them in order.
-struct Span {
-  int sink_blocks, from, end;
-  __device__ __forceinline__ int count() const { return sink_blocks + end - from; }
-  __device__ __forceinline__ int block(int i) const { return i < sink_blocks ? i : from + i - sink_blocks; }
-};
-__device__ __forceinline__ Span span_of(int first, int last, int window, int sinks) {
-  const int lo = window > 0 ? max(0, first - window + 1) : 0;  // first position in the window of `first`
-  Span s;
-  s.from = lo / kKvBlock;
-  s.end = last < 0 ? s.from : last / kKvBlock + 1;
-  s.sink_blocks = min((sinks + kKvBlock - 1) / kKvBlock, s.from);
-  return s;
 }
 
 // A block in shared memory: 16 rows of D bytes as TMA writes them with its 128-byte (D = 128) or
@@ -314,7 +287,6 @@ struct __align__(16) Block {
   int id, pos;
   float ks, vs;
 };
-constexpr int kNowhere = 0x3fffffff;
 constexpr int kBatch = 32;  // blocks that a warp looks up at once, one a lane
 
 // A warp's copies. Lane 0 has TMA bring a pair of blocks' keys and values to the warp's buffer, each
@@ -365,27 +337,6 @@ struct Copies {
     *timeout = 1;
   }
 };
-
-struct AttnArgs {
-  Kv8View c;
-  Kv8Table t;
-  const void* q;
-  int64_t q_stride;
-  int q_type;
-  const int* lengths;
-  const int* offsets;  // prefill
-  int64_t tokens;      // rows of q
-  int batch, heads, group;
-  int window, sinks;
-  float scale_log2;
-  void* out;
-  int out_type;
-  int* timeout;  // host memory; set when a wait gave up
-};
-
-__device__ __forceinline__ uint8_t* aligned_smem(uint8_t* raw) {  // the swizzle goes by address bits
-  return raw + ((1024u - (saddr(raw) & 1023u)) & 1023u);
-}
 
 // ---------------------------------------------------------------------------------------------
 // Decode. Rows are (sequence, kv head, run of up to 8 of its query heads); a row's units are its
@@ -712,98 +663,16 @@ __global__ void __launch_bounds__(128) kv8_join_kernel(const DecArgs d, int ctas
     static_cast<__nv_bfloat16*>(a.out)[o] = __float2bfloat16_rn(v);
 }
 
-// ---------------------------------------------------------------------------------------------
-// Prefill. A CTA of 4 warps takes 64 consecutive rows of one (sequence, kv head): row r is query
-// r / group, head r % group of the group; a warp 16 of them. The warps walk the same blocks, each
-// through its own ring (the others' copies come from L1/L2).
-constexpr int kPreWarps = 4;
-constexpr int kPreRows = 16 * kPreWarps;
-
-template <int D>
-__global__ void __launch_bounds__(kPreWarps * 32, 3) kv8_prefill_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap mk,
-                                                                         const __grid_constant__ CUtensorMap mv) {
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = aligned_smem(smem_raw);
-  __shared__ uint64_t bars[kPreWarps][2];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-  const int head = blockIdx.y;
-  const Kv8Place at = kv8_find<kPreWarps * 32>(
-      a.batch, [&](int b) -> int64_t { return ((int64_t)max(0, a.offsets[b + 1] - a.offsets[b]) * a.group + kPreRows - 1) / kPreRows; },
-      [&](int64_t total) -> int64_t { return total - 1 - (int64_t)blockIdx.x < 0 ? total : total - 1 - (int64_t)blockIdx.x; });
-  if (at.seq < 0) return;
-  const int b = at.seq, row0 = a.offsets[b], n = a.offsets[b + 1] - row0, len = __ldg(a.lengths + b);
-  const int total_rows = n * a.group, r0 = (int)at.at * kPreRows;
-  const int first_q = r0 / a.group, last_q = (min(total_rows, r0 + kPreRows) - 1) / a.group;
-  const int pos0 = len - n;  // position of query 0 (negative: the first queries are before the cache and see nothing)
-  const Span span = span_of(max(0, pos0 + first_q), min(len - 1, pos0 + last_q), a.window, a.sinks);
-  const int nb = max(0, span.count());
-  Warp<D, false> w;
-  w.reset();
-  int qp[2], lo[2];
-  int64_t qrow[2], orow[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int r = r0 + warp * 16 + g + 8 * i;
-    const int tok = r / a.group;
-    const int64_t row = row0 + tok;
-    const bool ok = r < total_rows && row >= 0 && row < a.tokens;
-    qrow[i] = ok ? row * a.q_stride + (int64_t)(head * a.group + r % a.group) * D : -1;
-    orow[i] = ok ? (row * a.heads + head * a.group + r % a.group) * D : -1;
-    qp[i] = ok ? pos0 + tok : -1;
-    lo[i] = a.window > 0 ? max(0, qp[i] - a.window + 1) : 0;
-  }
-  uint8_t* buffer = smem + warp * Piece<D>::kBuffer;
-  Block* blocks = reinterpret_cast<Block*>(smem + kPreWarps * (Piece<D>::kBuffer + 32 * D)) + warp * kBatch;
-  w.load_q(reinterpret_cast<uint4*>(smem + kPreWarps * Piece<D>::kBuffer) + warp * (2 * D), a.q, a.q_type, qrow, a.scale_log2, lane);
-  const int least = __reduce_min_sync(0xffffffffu, min(qp[0], qp[1])), most_lo = __reduce_max_sync(0xffffffffu, max(lo[0], lo[1]));
-  Copies<D> copies;
-  copies.init(&mk, &mv, buffer, bars[warp], lane);
-  for (int base = 0; base < nb; base += kBatch) {
-    const int m = min(kBatch, nb - base);
-    {
-      Block k = {-1, kNowhere, 0.f, 0.f};
-      const int blk = span.block(base + lane);
-      if (lane < m) k.id = kv8_block_id(a.c, a.t, b, head, blk);
-      if (k.id >= 0) k = {k.id, blk * kKvBlock, __ldg(a.c.ks + k.id), __ldg(a.c.vs + k.id)};
-      __syncwarp();
-      blocks[lane] = k;
-      __syncwarp();
-    }
-    copies.fetch(0, blocks, lane);
-    copies.fetch(1, blocks, lane);
-    for (int i = 0; i < m; i += 2) {
-      const Block b0 = blocks[i], b1 = blocks[i + 1];
-      const int p0[2] = {b0.pos, b1.pos};
-      const float kk[2] = {b0.ks, b1.ks}, vv[2] = {b0.vs, b1.vs};
-      const bool any = b0.id >= 0 || b1.id >= 0;
-      const int far = max(p0[0], p0[1]) + kKvBlock, near = min(p0[0], p0[1]);
-      const bool all = far - 1 <= least && (near >= most_lo || far <= a.sinks);
-      uint32_t p[2][4], seen;
-      copies.wait(0);
-      if (any) w.scores(buffer, kk, vv, all, lo, qp, a.sinks, p0, lane, p, seen);
-      __syncwarp();
-      if (i + 2 < m) copies.fetch(0, blocks + i + 2, lane);
-      copies.wait(1);
-      if (any) w.values(buffer + 2 * Piece<D>::kBytes, p, seen, lane);
-      __syncwarp();
-      if (i + 2 < m) copies.fetch(1, blocks + i + 2, lane);
-      copies.phase ^= 1;
-    }
-  }
-  copies.finish(a.timeout);
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const float l = quad_sum(w.l[i]);
-    const float inv = w.m[i] == -INFINITY ? 0.f : w.unit() / l;
-    if (orow[i] < 0) continue;
-#pragma unroll
-    for (int c = 0; c < 2; ++c)
-#pragma unroll
-      for (int j = 0; j < D / 8; j += 4) {
-        const float4 v = make_float4(w.o[j][2 * i + c] * inv, w.o[j + 1][2 * i + c] * inv, w.o[j + 2][2 * i + c] * inv, w.o[j + 3][2 * i + c] * inv);
-        store4(a.out, a.out_type, orow[i] + (D / 8) * (2 * t + c) + j, w.m[i] == -INFINITY ? make_float4(0.f, 0.f, 0.f, 0.f) : v);
-      }
-  }
+// Rows of one block of 16 tokens of D codes, swizzled as Piece<D>::at.
+bool code_map(CUtensorMap* map, const uint8_t* codes, const Kv8View& v, int dim) {
+  const auto fn = encode_fn();
+  if (!fn) return false;
+  const cuuint64_t dims[2] = {(cuuint64_t)dim, (cuuint64_t)v.pages * v.kv_heads * v.bpp * kKvBlock};
+  const cuuint64_t strides[1] = {(cuuint64_t)dim};
+  const cuuint32_t box[2] = {(cuuint32_t)dim, kKvBlock}, ones[2] = {1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(codes), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            dim == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 // One word of page-locked host memory, which kernels of any device can write and the host reads
@@ -816,60 +685,6 @@ int* timeout_word() {
     return (int*)p;
   }();
   return word;
-}
-
-int check_attention(const j4b_kv8_cache* cache, int64_t layer, j4b_buf q, int q_type, int64_t q_stride, int64_t tokens, int64_t heads,
-                    j4b_buf table, int64_t table_stride, int64_t table_width, j4b_buf lengths, int64_t batch, int64_t window, int64_t sinks,
-                    double scale, j4b_buf out, int out_type, AttnArgs* a, int* dev) {
-  Kv8View view;
-  if (const int st = kv8_check(cache, layer, &view, dev)) return st;
-  J4B_REQUIRE(heads > 0 && heads <= 65536 && heads % cache->kv_heads == 0, "kv8 attention: heads (%lld) must be a multiple of kv_heads (%d)",
-              (long long)heads, cache->kv_heads);
-  J4B_REQUIRE(batch >= 0 && batch <= 0xffffff && tokens >= 0 && tokens <= 0x7fffffff, "kv8 attention: bad batch or token count");
-  J4B_REQUIRE((q_type == J4B_F32 || q_type == J4B_BF16) && (out_type == J4B_F32 || out_type == J4B_BF16),
-              "kv8 attention: q and out types must be f32 or bf16, got %d and %d", q_type, out_type);
-  J4B_REQUIRE(q_stride >= heads * cache->head_dim && q_stride % 8 == 0, "kv8 attention: rows of q must be at least heads * head_dim elements and a multiple of 8 apart");
-  J4B_REQUIRE(table_width > 0 && table_width <= 0x7ffffff && table_stride >= table_width, "kv8 attention: bad page table shape");
-  J4B_REQUIRE(window >= 0 && sinks >= 0, "kv8 attention: window and sinks must not be negative");
-  J4B_REQUIRE(std::isfinite(scale), "kv8 attention: scale must be finite");
-  if (batch > 0 && tokens > 0)
-    J4B_REQUIRE(q && table && lengths && out && ((q | out) & 15) == 0 && ((table | lengths) & 3) == 0, "kv8 attention: misaligned or null buffers");
-  const int64_t far = 0x3fffffff;
-  *a = {view,
-        {(const int*)(uintptr_t)table, table_stride, (int)table_width},
-        (const void*)(uintptr_t)q,
-        q_stride,
-        q_type,
-        (const int*)(uintptr_t)lengths,
-        nullptr,
-        tokens,
-        (int)batch,
-        (int)heads,
-        (int)(heads / cache->kv_heads),
-        (int)std::min(window, far),
-        window > 0 ? (int)std::min(sinks, far) : 0,
-        (float)(scale * 1.4426950408889634),
-        (void*)(uintptr_t)out,
-        out_type,
-        timeout_word()};
-  if (!a->timeout) return set_error(J4B_ENOMEM, "kv8 attention: no host memory for the status word");
-  if (*(volatile int*)a->timeout) {
-    *(volatile int*)a->timeout = 0;
-    return set_error(J4B_ETIMEOUT, "kv8 attention: a wait of an earlier call gave up; its output is not valid");
-  }
-  return J4B_OK;
-}
-
-// Rows of one block of 16 tokens of D codes, swizzled as Piece<D>::at.
-bool code_map(CUtensorMap* map, const uint8_t* codes, const Kv8View& v, int dim) {
-  const auto fn = encode_fn();
-  if (!fn) return false;
-  const cuuint64_t dims[2] = {(cuuint64_t)dim, (cuuint64_t)v.pages * v.kv_heads * v.bpp * kKvBlock};
-  const cuuint64_t strides[1] = {(cuuint64_t)dim};
-  const cuuint32_t box[2] = {(cuuint32_t)dim, kKvBlock}, ones[2] = {1, 1};
-  return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(codes), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
-            dim == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 int decode_ctas(int dev) {
@@ -915,21 +730,50 @@ int launch_decode(const DecArgs& d, int dev, int ctas, cudaStream_t stream) {
   return J4B_OK;
 }
 
-template <int D>
-int launch_prefill(const AttnArgs& a, int dev, cudaStream_t stream) {
-  static bool done[kMaxDevices] = {};
-  const int smem = kPreWarps * (Piece<D>::kBuffer + 32 * D + kBatch * (int)sizeof(Block)) + 1024;
-  CUtensorMap mk, mv;
-  if (!code_map(&mk, a.c.k, a.c, D) || !code_map(&mv, a.c.v, a.c, D)) return set_error(J4B_ECUDA, "cuTensorMapEncodeTiled failed for the cache");
-  if (const int st = allow_smem(kv8_prefill_kernel<D>, smem, dev, done)) return st;
-  const int64_t tiles = std::min(a.tokens * a.group, a.tokens * a.group / kPreRows + a.batch);
-  J4B_REQUIRE(tiles <= 0x7fffffffLL, "kv8 prefill: too many rows");
-  kv8_prefill_kernel<D><<<dim3((unsigned)tiles, (unsigned)a.c.kv_heads), kPreWarps * 32, smem, stream>>>(a, mk, mv);
-  J4B_CHECK_LAUNCH("kv8_prefill_kernel");
+}  // namespace
+
+int kv8_check_attention(const j4b_kv8_cache* cache, int64_t layer, j4b_buf q, int q_type, int64_t q_stride, int64_t tokens, int64_t heads,
+                    j4b_buf table, int64_t table_stride, int64_t table_width, j4b_buf lengths, int64_t batch, int64_t window, int64_t sinks,
+                    double scale, j4b_buf out, int out_type, AttnArgs* a, int* dev) {
+  Kv8View view;
+  if (const int st = kv8_check(cache, layer, &view, dev)) return st;
+  J4B_REQUIRE(heads > 0 && heads <= 65536 && heads % cache->kv_heads == 0, "kv8 attention: heads (%lld) must be a multiple of kv_heads (%d)",
+              (long long)heads, cache->kv_heads);
+  J4B_REQUIRE(batch >= 0 && batch <= 0xffffff && tokens >= 0 && tokens <= 0x7fffffff, "kv8 attention: bad batch or token count");
+  J4B_REQUIRE((q_type == J4B_F32 || q_type == J4B_BF16) && (out_type == J4B_F32 || out_type == J4B_BF16),
+              "kv8 attention: q and out types must be f32 or bf16, got %d and %d", q_type, out_type);
+  J4B_REQUIRE(q_stride >= heads * cache->head_dim && q_stride % 8 == 0, "kv8 attention: rows of q must be at least heads * head_dim elements and a multiple of 8 apart");
+  J4B_REQUIRE(table_width > 0 && table_width <= 0x7ffffff && table_stride >= table_width, "kv8 attention: bad page table shape");
+  J4B_REQUIRE(window >= 0 && sinks >= 0, "kv8 attention: window and sinks must not be negative");
+  J4B_REQUIRE(std::isfinite(scale), "kv8 attention: scale must be finite");
+  if (batch > 0 && tokens > 0)
+    J4B_REQUIRE(q && table && lengths && out && ((q | out) & 15) == 0 && ((table | lengths) & 3) == 0, "kv8 attention: misaligned or null buffers");
+  const int64_t far = 0x3fffffff;
+  *a = {view,
+        {(const int*)(uintptr_t)table, table_stride, (int)table_width},
+        (const void*)(uintptr_t)q,
+        q_stride,
+        q_type,
+        (const int*)(uintptr_t)lengths,
+        nullptr,
+        tokens,
+        (int)batch,
+        (int)heads,
+        (int)(heads / cache->kv_heads),
+        (int)std::min(window, far),
+        window > 0 ? (int)std::min(sinks, far) : 0,
+        (float)(scale * 1.4426950408889634),
+        (void*)(uintptr_t)out,
+        out_type,
+        timeout_word()};
+  if (!a->timeout) return set_error(J4B_ENOMEM, "kv8 attention: no host memory for the status word");
+  if (*(volatile int*)a->timeout) {
+    *(volatile int*)a->timeout = 0;
+    return set_error(J4B_ETIMEOUT, "kv8 attention: a wait of an earlier call gave up; its output is not valid");
+  }
   return J4B_OK;
 }
 
-}  // namespace
 }  // namespace j4b
 
 using namespace j4b;
@@ -950,7 +794,7 @@ extern "C" int j4b_kv8_attention_decode(const j4b_kv8_cache* cache, int64_t laye
                                         int64_t workspace_bytes, j4b_stream s) {
   DecArgs d;
   int dev = 0;
-  if (const int st = check_attention(cache, layer, q, q_type, q_stride, batch, heads, table, table_stride, table_width, lengths, batch,
+  if (const int st = kv8_check_attention(cache, layer, q, q_type, q_stride, batch, heads, table, table_stride, table_width, lengths, batch,
                                      window, sinks, scale, out, out_type, &d.a, &dev))
     return st;
   J4B_REQUIRE(batch * heads <= 0x7fffffffLL, "kv8 decode: too many rows");
@@ -964,21 +808,4 @@ extern "C" int j4b_kv8_attention_decode(const j4b_kv8_cache* cache, int64_t laye
   d.part = (float*)(uintptr_t)workspace;
   d.cum = (int64_t*)((uintptr_t)workspace + ((int64_t)2 * ctas * kDecHeads * (cache->head_dim + 2) * 4 + 15) / 16 * 16);
   return cache->head_dim == 128 ? launch_decode<128>(d, dev, ctas, stream) : launch_decode<64>(d, dev, ctas, stream);
-}
-
-extern "C" int j4b_kv8_attention_prefill(const j4b_kv8_cache* cache, int64_t layer, j4b_buf q, int q_type, int64_t q_stride, int64_t tokens,
-                                         int64_t heads, j4b_buf offsets, j4b_buf table, int64_t table_stride, int64_t table_width,
-                                         j4b_buf lengths, int64_t batch, int64_t window, int64_t sinks, double scale, j4b_buf out,
-                                         int out_type, j4b_stream s) {
-  AttnArgs a;
-  int dev = 0;
-  if (const int st = check_attention(cache, layer, q, q_type, q_stride, tokens, heads, table, table_stride, table_width, lengths, batch,
-                                     window, sinks, scale, out, out_type, &a, &dev))
-    return st;
-  if (batch == 0 || tokens == 0) return J4B_OK;
-  J4B_REQUIRE(offsets && (offsets & 3) == 0, "kv8 prefill: misaligned or null offsets");
-  a.offsets = (const int*)(uintptr_t)offsets;
-  DeviceGuard guard(dev);
-  cudaStream_t stream = resolve_stream(dev, s);
-  return cache->head_dim == 128 ? launch_prefill<128>(a, dev, stream) : launch_prefill<64>(a, dev, stream);
 }

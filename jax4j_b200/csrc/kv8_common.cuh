@@ -97,6 +97,56 @@ __device__ __forceinline__ void store4(void* p, int type, int64_t i, float4 v) {
   }
 }
 
+// two f32 -> f16x2, a in the low half
+__device__ __forceinline__ uint32_t h2(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float exp2_ftz(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+constexpr int kNowhere = 0x3fffffff;  // the position of what is not there: past every query
+
+// The blocks that queries at positions first .. last of a sequence of `len` tokens see: the first
+// `sink_blocks` ones, then those from `from` on to `end` (exclusive). count() of them in order.
+struct Span {
+  int sink_blocks, from, end;
+  __device__ __forceinline__ int count() const { return sink_blocks + end - from; }
+  __device__ __forceinline__ int block(int i) const { return i < sink_blocks ? i : from + i - sink_blocks; }
+};
+__device__ __forceinline__ Span span_of(int first, int last, int window, int sinks) {
+  const int lo = window > 0 ? max(0, first - window + 1) : 0;  // first position in the window of `first`
+  Span s;
+  s.from = lo / kKvBlock;
+  s.end = last < 0 ? s.from : last / kKvBlock + 1;
+  s.sink_blocks = min((sinks + kKvBlock - 1) / kKvBlock, s.from);
+  return s;
+}
+
+struct AttnArgs {
+  Kv8View c;
+  Kv8Table t;
+  const void* q;
+  int64_t q_stride;
+  int q_type;
+  const int* lengths;
+  const int* offsets;  // prefill
+  int64_t tokens;      // rows of q
+  int batch, heads, group;
+  int window, sinks;
+  float scale_log2;
+  void* out;
+  int out_type;
+  int* timeout;  // host memory; set when a wait gave up
+};
+
+__device__ __forceinline__ uint8_t* aligned_smem(uint8_t* raw) {  // the swizzle goes by address bits
+  return raw + ((1024u - ((uint32_t)__cvta_generic_to_shared(raw) & 1023u)) & 1023u);
+}
+
 // Where a unit of work lies when sequence b has count(b) consecutive units.
 struct Kv8Place {
   int seq;        // -1: past the last unit
@@ -149,5 +199,11 @@ template <int THREADS, class Count, class Unit>
 __device__ __forceinline__ Kv8Place kv8_find(int batch, Count count, Unit unit) {
   return kv8_find<THREADS>(batch, count, unit, [](int, int, int64_t) {});
 }
+
+// Checks an entry point's arguments (kv8_cache.cu, kv8_attn.cu).
+int kv8_check(const j4b_kv8_cache* c, int64_t layer, Kv8View* view, int* dev);
+int kv8_check_attention(const j4b_kv8_cache* cache, int64_t layer, j4b_buf q, int q_type, int64_t q_stride, int64_t tokens, int64_t heads,
+                        j4b_buf table, int64_t table_stride, int64_t table_width, j4b_buf lengths, int64_t batch, int64_t window,
+                        int64_t sinks, double scale, j4b_buf out, int out_type, AttnArgs* a, int* dev);
 
 }  // namespace j4b
