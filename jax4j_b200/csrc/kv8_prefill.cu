@@ -13,10 +13,12 @@
 // moves only when a row outgrows it by 2^kLazy, so O is seldom rescaled.
 //
 // Warps: 0-3 and 4-7 softmax of tile 0 and 1; 8-11 bring pages: each thread loads 16-code pieces of
-// the next tile while it turns this one's into the swizzled f16 operands; 12 issues the MMAs. S of
-// one tile is computed while the other's softmax runs.
+// the next tile while it turns this one's into the swizzled f16 operands; 12 issues the MMAs (13-15
+// only fill up their warpgroup, so that its registers can go to the softmax, which holds a row of
+// 128 scores). S of one tile is computed while the other's softmax runs.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "kv8_common.cuh"
 #include "tc_common.cuh"
@@ -27,8 +29,8 @@ namespace {
 constexpr int kRows = 128;           // of a tile
 constexpr int kKeys = 128;           // of a key tile
 constexpr int kTileBlocks = kKeys / kKvBlock;
-constexpr int kThreads = 13 * 32;
-constexpr int kStages = 2;           // of K and of V
+constexpr int kThreads = 16 * 32;
+constexpr int kStages = 2;           // of K and of V (their parity is counted with & 1)
 constexpr int kInfos = 4;            // of what is known of a key tile: the softmax may be two behind
 constexpr float kLazy = 5.f;         // log2: P <= 2^(kShift + kLazy) = 2^15, inside f16
 constexpr int kShift = 10;           // log2: keeps f16's bits for blocks of small value scale
@@ -97,11 +99,120 @@ __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void to_async_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
+// pairs of f32 in one instruction
+__device__ __forceinline__ uint64_t pair(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ float2 unpair(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// The positions that a row sees: [lo, qp] and [0, sinks) up to qp.
+struct View {
+  int lo, qp, sinks;
+  static __device__ __forceinline__ uint32_t below(int n) { return n <= 0 ? 0u : n >= 16 ? 0xffffu : (1u << n) - 1u; }
+  // bit e: it sees position p + e, e < 16
+  __device__ __forceinline__ uint32_t mask(int p) const { return below(qp + 1 - p) & (~below(lo - p) | below(sinks - p)); }
+};
+
+// A row's scores of a key tile, held in registers from TMEM until its probabilities go back there.
+struct Row {
+  uint32_t v[4][32];
+
+  __device__ __forceinline__ void load(uint32_t s_at) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) tmem_ld32(s_at + 32u * c, v[c]);
+    tmem_ld_wait();
+  }
+  // The largest score (times its factor). ALL: the row sees the whole tile; otherwise the scores of
+  // what it does not see become -inf, and `bad` says whether it sees a token with a NaN value (the
+  // operand holds 0 there).
+  template <bool ALL>
+  __device__ __forceinline__ float most(const TileInfo& info, const View& view, float factor, bool& bad) {
+    float mx = -INFINITY;
+    uint32_t found = 0;
+#pragma unroll
+    for (int k = 0; k < kTileBlocks; ++k) {
+      uint32_t* x = v[k >> 1] + 16 * (k & 1);
+      if (!ALL) {
+        const uint32_t see = view.mask(info.pos[k]);
+        found |= see & (info.nan[k >> 1] >> (16 * (k & 1)));
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (!(see >> e & 1)) x[e] = 0xff800000u;
+      }
+      float t = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
+#pragma unroll
+      for (int e = 2; e < 16; e += 2) t = fmaxf(t, fmaxf(__uint_as_float(x[e]), __uint_as_float(x[e + 1])));
+      const float f = factor * info.ks[k];
+      mx = fmaxf(mx, t == -INFINITY ? t : t * f);
+    }
+    bad = ALL ? (info.nan[0] | info.nan[1] | info.nan[2] | info.nan[3]) != 0 : found != 0;
+    return mx;
+  }
+  // The probabilities, in f16, each block's weighed by its value scale, go over the scores in TMEM;
+  // returns their sum without the weights.
+  template <bool ALL>
+  __device__ __forceinline__ float store(uint32_t s_at, const TileInfo& info, float factor, float base, int eref) {
+    float l = 0.f;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      uint32_t p[16];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int k = 2 * c + h;
+        const uint32_t* x = v[c] + 16 * h;
+        // -inf * 0 would be NaN: with a key scale of 0 the visible scores are 0 whatever the factor
+        const float f = ALL ? factor * info.ks[k] : fmaxf(factor * info.ks[k], 1e-37f);
+        const int w = max(-60, info.ev[k] - eref) + kShift;
+        const uint64_t ff = pair(f, f), add = pair((float)w - base, (float)w - base);
+        uint64_t sum = 0;
+#pragma unroll
+        for (int e = 0; e < 16; e += 2) {
+          float2 y = unpair(fma2(pair(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), ff, add));
+          y.x = exp2_ftz(y.x);
+          y.y = exp2_ftz(y.y);
+          sum = add2(sum, pair(y.x, y.y));
+          p[8 * h + e / 2] = h2(y.x, y.y);
+        }
+        const float2 t = unpair(sum);
+        l = fmaf(t.x + t.y, __uint_as_float((uint32_t)(127 - w) << 23), l);
+      }
+      tmem_st16(s_at + 16u * c, p);
+    }
+    return l;
+  }
+};
+
 // Which key tiles a row tile takes: [begin, end) of the CTA's list.
 struct Range {
   int begin, end;
   __device__ __forceinline__ bool has(int j) const { return j >= begin && j < end; }
 };
+
+// Registers of a thread by warpgroup: the launch's 4 x 128 shared out as 2 x 176 + 104 + 56.
+template <int N>
+__device__ __forceinline__ void more_registers() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void fewer_registers() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
 
 template <int D>
 __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const AttnArgs a) {
@@ -112,6 +223,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const AttnArgs
   TileInfo* infos = reinterpret_cast<TileInfo*>(sk + 2 * kStages * Smem<D>::kOperand);
   __shared__ uint64_t q_ready[2], k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], s_full[2], p_ready[2], o_full[2], info_full[kInfos];
   __shared__ uint32_t tmem_slot;
+  __shared__ float factors[2][kRows];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int head = blockIdx.y;
   // the last rows of a sequence see the most keys: they go first
@@ -138,7 +250,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const AttnArgs
     const int begin = a.sinks > 0 ? 0 : span.sink_blocks + max(0, s.from - span.from);
     return {begin / kTileBlocks, (max(end, span.sink_blocks) + kTileBlocks - 1) / kTileBlocks};
   };
-  const Range range[2] = {range_of(0), range_of(1)};
+  const Range range0 = range_of(0), range1 = range_of(1);
 
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
@@ -167,47 +279,88 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const AttnArgs
   bool ok = true;
 
   if (warp < 8) {
+    more_registers<176>();
     // ---- softmax of tile i, one row a thread ----
     const int i = warp >> 2, r = tid & 127;
-    const Range rg = range[i];
+    const Range rg = i ? range1 : range0;
     const int64_t gr = r0 + i * kRows + r;
     const int tok = (int)(gr / a.group), gh = head * a.group + (int)(gr % a.group);
     const bool valid = gr < total_rows && row0 + tok >= 0 && row0 + tok < a.tokens;
     const int qp = valid ? pos0 + tok : -1;
-    const int lo = a.window > 0 ? max(0, qp - a.window + 1) : 0;
+    const View view = {a.window > 0 ? max(0, qp - a.window + 1) : 0, qp, a.sinks};
     // every valid row of the tile sees the positions [most_lo, least]
     const int least = first_of(i), most_lo = a.window > 0 ? max(0, last_of(i) - a.window + 1) : 0;
-    // Q: each row by a power of two to a largest element in [2^11, 2^12), then f16 (bf16 is exact there)
-    float factor = a.scale_log2;
+    // Q: each row by a power of two to a largest element in [2^11, 2^12), then f16 (bf16 is exact
+    // there); 8 lanes a row, 4 rows at a time
+    float factor = 0.f;
     if (i < tiles) {
-      const int64_t src = valid ? (int64_t)(row0 + tok) * a.q_stride + (int64_t)gh * D : 0;
-      float most = 0.f;
-      if (valid)
-#pragma unroll 4
-        for (int c = 0; c < D; c += 4) {
-          const float4 x = load4(a.q, a.q_type, src + c);
-          most = fmaxf(most, fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))));
-        }
-      const int e = (int)(__float_as_uint(most) >> 23);
-      const bool plain = e < 24 || e > 240;
-      float up = plain ? 1.f : __uint_as_float((uint32_t)(254 - (e - 11)) << 23);
-      factor *= plain ? 1.f : __uint_as_float((uint32_t)(e - 11) << 23);
-      if (factor < 0.f) {  // the maxima below are taken before the factor
-        factor = -factor;
-        up = -up;
-      }
       uint8_t* tile = sq + i * Smem<D>::kQ;
-#pragma unroll 4
-      for (int c = 0; c < D; c += 8) {
-        uint4 h = make_uint4(0, 0, 0, 0);
-        if (valid) {
-          const float4 x = load4(a.q, a.q_type, src + c), y = load4(a.q, a.q_type, src + c + 4);
-          h = make_uint4(h2(x.x * up, x.y * up), h2(x.z * up, x.w * up), h2(y.x * up, y.y * up), h2(y.z * up, y.w * up));
+      const int sub = lane & 7;
+      auto rows = [&](auto type) {
+        constexpr bool kF32 = decltype(type)::value == J4B_F32;
+        constexpr int kWords = kF32 ? D / 32 : D / 64, kStep = kF32 ? 4 : 8;  // 16-byte pieces of a row and lane, rows in flight
+#pragma unroll 1
+        for (int k0 = 0; k0 < 8; k0 += kStep) {
+          uint4 raw[kStep][kWords];
+#pragma unroll
+          for (int k = 0; k < kStep; ++k) {
+            const int64_t g = r0 + i * kRows + (warp & 3) * 32 + 4 * (k0 + k) + (lane >> 3), row = row0 + g / a.group;
+            const bool there = g < total_rows && row >= 0 && row < a.tokens;
+            const int64_t src = row * a.q_stride + (int64_t)(head * a.group + (int)(g % a.group)) * D + 8 * sub;
+#pragma unroll
+            for (int c = 0; c < kWords; ++c)
+              raw[k][c] = !there ? make_uint4(0, 0, 0, 0)
+                          : kF32 ? __ldg(reinterpret_cast<const uint4*>(static_cast<const float*>(a.q) + src + 64 * (c >> 1) + 4 * (c & 1)))
+                                 : __ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.q) + src + 64 * c));
+          }
+#pragma unroll
+          for (int k = 0; k < kStep; ++k) {
+            const int qr = (warp & 3) * 32 + 4 * (k0 + k) + (lane >> 3);
+            float x[D / 8];
+            float most = 0.f;
+#pragma unroll
+            for (int c = 0; c < kWords; ++c) {
+              const uint32_t w[4] = {raw[k][c].x, raw[k][c].y, raw[k][c].z, raw[k][c].w};
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                if (kF32) {
+                  x[4 * c + e] = __uint_as_float(w[e]);
+                } else {
+                  x[8 * c + 2 * e] = __uint_as_float(w[e] << 16);
+                  x[8 * c + 2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
+                }
+              }
+            }
+#pragma unroll
+            for (int e = 0; e < D / 8; ++e) most = fmaxf(most, fabsf(x[e]));
+#pragma unroll
+            for (int o = 1; o < 8; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+            const int e = (int)(__float_as_uint(most) >> 23);
+            const bool plain = e < 24 || e > 240;
+            float up = plain ? 1.f : __uint_as_float((uint32_t)(254 - (e - 11)) << 23);
+            float f = plain ? a.scale_log2 : a.scale_log2 * __uint_as_float((uint32_t)(e - 11) << 23);
+            if (f < 0.f) {  // maxima are taken before the factor
+              f = -f;
+              up = -up;
+            }
+            if (sub == 0) factors[i][qr] = f;
+#pragma unroll
+            for (int c = 0; c < D / 64; ++c) {
+              const float* y = x + 8 * c;
+              *reinterpret_cast<uint4*>(tile + c * (kRows * 128) + sw128_offset(qr, 8 * sub)) =
+                  make_uint4(h2(y[0] * up, y[1] * up), h2(y[2] * up, y[3] * up), h2(y[4] * up, y[5] * up), h2(y[6] * up, y[7] * up));
+            }
+          }
         }
-        *reinterpret_cast<uint4*>(tile + (c >> 6) * (kRows * 128) + sw128_offset(r, c & 63)) = h;
-      }
+      };
+      if (a.q_type == J4B_F32)
+        rows(std::integral_constant<int, J4B_F32>{});
+      else
+        rows(std::integral_constant<int, J4B_BF16>{});
       to_async_proxy();
       bar_arrive(&q_ready[i]);
+      __syncwarp();  // a warp wrote the factors of its own rows
+      factor = factors[i][r];
     }
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const uint32_t s_at = lanes + (uint32_t)(i * 128), o_at = lanes + 256u + (uint32_t)(i * 128);
@@ -226,35 +379,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const AttnArgs
         far = max(far, info.pos[k] + kKvBlock);
       }
       const bool all = far - 1 <= least && (near >= most_lo || far <= a.sinks);
-      uint32_t v[32];
-      // the row's maximum, and whether it sees a token with a NaN value (the operand holds 0 there)
-      float mx = -INFINITY;
       bool bad = false;
-#pragma unroll 1
-      for (int c = 0; c < kKeys; c += 32) {
-        tmem_ld32(s_at + (uint32_t)c, v);
-        tmem_ld_wait();
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int blk = c / kKvBlock + h;
-          float t = -INFINITY;
-          if (all) {
-#pragma unroll
-            for (int e = 0; e < 16; ++e) t = fmaxf(t, __uint_as_float(v[16 * h + e]));
-          } else {
-            const int p = info.pos[blk];
-            const unsigned nan = info.nan[c / 32] >> (16 * h);
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const bool see = (p + e >= lo || p + e < a.sinks) && p + e <= qp;
-              if (see) t = fmaxf(t, __uint_as_float(v[16 * h + e]));
-              bad |= see && (nan >> e & 1);
-            }
-          }
-          mx = fmaxf(mx, t * (factor * info.ks[blk]));
-        }
-      }
-      if (all) bad = (info.nan[0] | info.nan[1] | info.nan[2] | info.nan[3]) != 0;
+      Row row;
+      row.load(s_at);
+      const float mx = all ? row.most<true>(info, view, factor, bad) : row.most<false>(info, view, factor, bad);
       if (bad) l = NAN;
       int ev = info.ev[0];
 #pragma unroll
@@ -269,6 +397,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const AttnArgs
         const float cm = m == -INFINITY ? 0.f : exp2_ftz(m - mnew), co = cm * exp2_ftz((float)(eref - enew));
         l *= m == mnew ? 1.f : cm;
         m = mnew;
+        uint32_t v[32];
 #pragma unroll 1
         for (int c = 0; c < D; c += 32) {
           tmem_ld32(o_at + (uint32_t)c, v);
@@ -280,33 +409,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const AttnArgs
       }
       eref = enew;
       const float base = m == -INFINITY ? 0.f : m;
-#pragma unroll 1
-      for (int c = 0; c < kKeys; c += 32) {
-        tmem_ld32(s_at + (uint32_t)c, v);
-        tmem_ld_wait();
-        uint32_t p[16];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int blk = c / kKvBlock + h;
-          const float f = factor * info.ks[blk];
-          const int w = max(-60, info.ev[blk] - eref) + kShift;
-          const float add = (float)w - base;
-          const int p0 = info.pos[blk];
-          float sum = 0.f;
-#pragma unroll
-          for (int e = 0; e < 16; e += 2) {
-            float x = exp2_ftz(fmaf(__uint_as_float(v[16 * h + e]), f, add)), y = exp2_ftz(fmaf(__uint_as_float(v[16 * h + e + 1]), f, add));
-            if (!all) {
-              if (!((p0 + e >= lo || p0 + e < a.sinks) && p0 + e <= qp)) x = 0.f;
-              if (!((p0 + e + 1 >= lo || p0 + e + 1 < a.sinks) && p0 + e + 1 <= qp)) y = 0.f;
-            }
-            sum += x + y;
-            p[8 * h + e / 2] = h2(x, y);
-          }
-          l = fmaf(sum, __uint_as_float((uint32_t)(127 - w) << 23), l);
-        }
-        tmem_st16(s_at + (uint32_t)(c / 2), p);
-      }
+      l += all ? row.store<true>(s_at, info, factor, base, eref) : row.store<false>(s_at, info, factor, base, eref);
       tmem_st_wait();
       tc_fence_before();
       bar_arrive(&p_ready[i]);
@@ -316,25 +419,58 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const AttnArgs
       ok = ok && bar_wait(&o_full[i], 0);
       tc_fence_after();
     }
+    const int64_t out_row = valid ? ((int64_t)(row0 + tok) * a.heads + gh) * D : -1;
     const float inv = m == -INFINITY ? 0.f : exp2_ftz((float)(eref - kShift)) / l;
-    const int64_t dst = ((int64_t)(row0 + tok) * a.heads + gh) * D;
+    // through the warp's rows of the query tile (its MMAs are done), so that the stores are whole
+    // rows: 256 bytes of a row at a time, 16-byte pieces swizzled by the row
+    uint8_t* stage = sq + i * Smem<D>::kQ + (warp & 3) * (32 * 2 * D);
+    const bool f32 = a.out_type == J4B_F32;
+    const int bytes = min(f32 ? 4 * D : 2 * D, 2 * D), passes = f32 ? 2 : 1;  // of a row and pass
 #pragma unroll 1
-    for (int c = 0; c < D && i < tiles; c += 32) {
-      uint32_t v[32];
-      if (rg.end > rg.begin) {
-        tmem_ld32(o_at + (uint32_t)c, v);
-        tmem_ld_wait();
-      }
-      if (valid) {
-#pragma unroll
-        for (int e = 0; e < 32; e += 4) {
-          const float4 x = m == -INFINITY ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(__uint_as_float(v[e]) * inv, __uint_as_float(v[e + 1]) * inv,
-                                                                                                  __uint_as_float(v[e + 2]) * inv, __uint_as_float(v[e + 3]) * inv);
-          store4(a.out, a.out_type, dst + c + e, x);
+    for (int pass = 0; pass < passes && i < tiles; ++pass) {
+      __syncwarp();
+#pragma unroll 1
+      for (int c = pass * (D / 2); c < (f32 ? (pass + 1) * (D / 2) : D); c += 32) {
+        uint32_t v[32];
+        if (rg.end > rg.begin) {
+          tmem_ld32(o_at + (uint32_t)c, v);
+          tmem_ld_wait();
         }
+        float x[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) x[e] = m == -INFINITY ? 0.f : __uint_as_float(v[e]) * inv;
+        const int first = (f32 ? 4 * (c - pass * (D / 2)) : 2 * c) / 16;  // 16-byte piece of the row
+        if (f32) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            *reinterpret_cast<float4*>(stage + lane * bytes + (((first + e) ^ (lane & 7)) << 4)) = make_float4(x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            uint32_t w[4];
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+              const __nv_bfloat162 t = __floats2bfloat162_rn(x[8 * e + 2 * y], x[8 * e + 2 * y + 1]);
+              w[y] = *reinterpret_cast<const uint32_t*>(&t);
+            }
+            *reinterpret_cast<uint4*>(stage + lane * bytes + (((first + e) ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        }
+      }
+      __syncwarp();
+      constexpr int kLanes = D / 8, kAtOnce = 32 / kLanes;  // lanes of a row, rows of a store
+      uint8_t* out = static_cast<uint8_t*>(a.out) + pass * bytes;
+#pragma unroll 8
+      for (int k = 0; k < 32 / kAtOnce; ++k) {
+        const int qr = kAtOnce * k + lane / kLanes, piece = lane % kLanes;
+        const int64_t dst = __shfl_sync(0xffffffffu, out_row, qr);
+        if (dst >= 0)
+          *reinterpret_cast<uint4*>(out + dst * (f32 ? 4 : 2) + 16 * piece) =
+              *reinterpret_cast<const uint4*>(stage + qr * bytes + ((piece ^ (qr & 7)) << 4));
       }
     }
   } else if (warp < 12) {
+    fewer_registers<104>();
     // ---- pages to operands: this warp the rows 32 w .. + 31 (2 blocks) of each key tile ----
     const int w = warp - 8;
     constexpr int kHalves = D / 64, kPieces = 4 * kHalves;  // 16-code pieces of a thread, K or V
@@ -438,39 +574,53 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const AttnArgs
         nid[0] = id_at(nblk[0]), nid[1] = id_at(nblk[1]);
       }
     }
-  } else if (lane == 0) {
+  } else {
+    fewer_registers<56>();
+    if (warp == 12 && lane == 0) {
     // ---- the MMAs ----
     constexpr uint32_t is = idesc_f16(kRows, kKeys, false), io = idesc_f16(kRows, D, true);
+    // descriptors count in 16-byte units: stepping one is an addition
+    uint64_t qd = kmajor_sw128(saddr(sq)), kd = kmajor_sw128(saddr(sk)), vd = rows_sw128(saddr(sk) + Smem<D>::kOperand, kKeys * 128);
+    constexpr uint32_t kStage = 2 * Smem<D>::kOperand / 16;
     for (int i = 0; i < tiles; ++i) ok = ok && bar_wait(&q_ready[i], 0);
     tc_fence_after();
-    uint32_t uses[2] = {0, 0};
+    uint32_t uses0 = 0, uses1 = 0;
     for (int j = -1; j < nt && ok; ++j) {
       if (j + 1 < nt) ok = ok && bar_wait(&k_full[(j + 1) % kStages], (uint32_t)((j + 1) / kStages & 1));
       if (j >= 0) ok = ok && bar_wait(&v_full[j % kStages], (uint32_t)(j / kStages & 1));
       tc_fence_after();
-      for (int i = 0; i < tiles; ++i) {
+      // opaque, or every step's descriptor is kept across the loop and spilled: the issue then waits for
+      // local memory (8 x 2048: PV's 8 MMAs took 2 us to issue instead of 0.3)
+      asm volatile("" : "+l"(qd), "+l"(kd), "+l"(vd));
+      const uint64_t vt = vd + (uint32_t)(j & 1) * kStage, kt = kd + (uint32_t)((j + 1) & 1) * kStage;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const Range rg = i ? range1 : range0;
+        uint32_t& uses = i ? uses1 : uses0;
         const uint32_t s_at = tmem + (uint32_t)(i * 128), o_at = tmem + 256u + (uint32_t)(i * 128);
-        if (range[i].has(j)) {
-          ok = ok && bar_wait(&p_ready[i], uses[i]++ & 1);
+        if (rg.has(j)) {
+          ok = ok && bar_wait(&p_ready[i], uses & 1);
+          ++uses;
           tc_fence_after();
-          const uint32_t vt = saddr(sk + (j % kStages) * 2 * Smem<D>::kOperand + Smem<D>::kOperand);
+          const uint32_t later = j > rg.begin;
 #pragma unroll
           for (int k = 0; k < kKeys / 16; ++k)  // 16 keys: 8 columns of P, 2 groups of 8 rows of V
-            umma_ts(o_at, s_at + 8u * k, rows_sw128(vt + k * 2048, kKeys * 128), io, (j > range[i].begin || k > 0) ? 1u : 0u);
-          if (j + 1 == range[i].end) umma_commit(&o_full[i]);
+            umma_ts(o_at, s_at + 8u * k, vt + k * (2048 / 16), io, k > 0 ? 1u : later);
+          if (j + 1 == rg.end) umma_commit(&o_full[i]);
         }
-        if (range[i].has(j + 1)) {
-          const uint32_t kt = saddr(sk + ((j + 1) % kStages) * 2 * Smem<D>::kOperand), qt = saddr(sq + i * Smem<D>::kQ);
+        if (rg.has(j + 1)) {
+          const uint64_t qt = qd + (uint32_t)(i * Smem<D>::kQ / 16);
 #pragma unroll
           for (int k = 0; k < D / 16; ++k) {
-            const uint32_t off = (k >> 2) * (kRows * 128) + (k & 3) * 32;  // kRows == kKeys
-            umma_bf16(s_at, kmajor_sw128(qt + off), kmajor_sw128(kt + off), is, k > 0 ? 1u : 0u);
+            const uint32_t off = ((k >> 2) * (kRows * 128) + (k & 3) * 32) / 16;  // kRows == kKeys
+            umma_bf16(s_at, qt + off, kt + off, is, k > 0 ? 1u : 0u);
           }
           umma_commit(&s_full[i]);
         }
       }
       if (j + 1 < nt) umma_commit(&k_empty[(j + 1) % kStages]);
       if (j >= 0) umma_commit(&v_empty[j % kStages]);
+    }
     }
   }
   if (!ok) *a.timeout = 1;
