@@ -327,13 +327,13 @@ struct Copies {
       if (id1 >= 0) tma_tile(dst + Piece<D>::kBytes, which ? mv : mk, 0, id1 * kKvBlock, &bars[which]);
     }
   }
-  __device__ __forceinline__ void wait(int which) { ok = ok && bar_wait(&bars[which], phase); }
+  __device__ __forceinline__ void wait(int which) { ok = ok && kv8_wait(&bars[which], phase); }
   // At the kernel's end. After a wait that gave up nothing more is copied or waited for, but for
   // one last bounded wait for what was in flight then.
   __device__ __forceinline__ void finish(int* timeout) {
     if (ok) return;
-    bar_wait(&bars[0], phase);
-    bar_wait(&bars[1], phase);
+    kv8_wait(&bars[0], phase);
+    kv8_wait(&bars[1], phase);
     *timeout = 1;
   }
 };

@@ -14,6 +14,7 @@
 #include <cstdint>
 
 #include "j4b_internal.h"
+#include "j4b_wait.cuh"
 
 namespace j4b {
 
@@ -145,6 +146,25 @@ struct AttnArgs {
 
 __device__ __forceinline__ uint8_t* aligned_smem(uint8_t* raw) {  // the swizzle goes by address bits
   return raw + ((1024u - ((uint32_t)__cvta_generic_to_shared(raw) & 1023u)) & 1023u);
+}
+
+// Waits for an mbarrier's phase, bounded as mbar_wait_timed's waits are, but the clock is read once
+// in 64 polls: the read takes long enough to make a waiter late where tiles are handed on every
+// microsecond.
+__device__ __forceinline__ bool kv8_wait(uint64_t* bar, uint32_t parity) {
+  const uint32_t at = (uint32_t)__cvta_generic_to_shared(bar);
+  if (mbar_try_wait_parity(at, parity)) return true;
+  uint64_t t0 = 0;
+  for (;;) {
+#pragma unroll 1
+    for (int i = 0; i < 64; ++i)
+      if (mbar_try_wait_parity(at, parity)) return true;
+    const uint64_t now = global_ns();
+    if (t0 == 0)
+      t0 = now;
+    else if (now - t0 > kWaitNs)
+      return false;
+  }
 }
 
 // Where a unit of work lies when sequence b has count(b) consecutive units.

@@ -12,13 +12,16 @@
 // over the largest seen, is the w of its probabilities (both powers of two). The running maximum m
 // moves only when a row outgrows it by 2^kLazy, so O is seldom rescaled.
 //
-// Warps: 0-3 and 4-7 softmax of tile 0 and 1; 8-11 bring pages: each thread loads 16-code pieces of
-// the next tile while it turns this one's into the swizzled f16 operands; 12 issues the MMAs (13-15
-// only fill up their warpgroup, so that its registers can go to the softmax, which holds a row of
-// 128 scores). S of one tile is computed while the other's softmax runs.
+// Warps: 0-3 and 4-7 queries, softmax and output of tile 0 and 1; 8-11 bring pages: each thread loads
+// 16-code pieces of the next tile while it turns this one's into the swizzled f16 operands; 12 issues
+// the MMAs; 13 finds the next item. S of one tile is computed while the other's softmax runs.
+//
+// One CTA an SM stays for the whole call and takes items (256 rows of a sequence and kv head): the
+// pages and queries of the next item come while this one's last tiles are worked on. Items are
+// numbered by how far from their sequence's end they lie, so the longest come first, and dealt out
+// to the CTAs forth and back.
 #include <algorithm>
 #include <cmath>
-#include <type_traits>
 
 #include "kv8_common.cuh"
 #include "tc_common.cuh"
@@ -29,25 +32,27 @@ namespace {
 constexpr int kRows = 128;           // of a tile
 constexpr int kKeys = 128;           // of a key tile
 constexpr int kTileBlocks = kKeys / kKvBlock;
-constexpr int kThreads = 16 * 32;
+constexpr int kThreads = 14 * 32;
 constexpr int kStages = 2;           // of K and of V (their parity is counted with & 1)
 constexpr int kInfos = 4;            // of what is known of a key tile: the softmax may be two behind
 constexpr float kLazy = 5.f;         // log2: P <= 2^(kShift + kLazy) = 2^15, inside f16
 constexpr int kShift = 10;           // log2: keeps f16's bits for blocks of small value scale
 
 // What the softmax needs of a key tile.
-struct TileInfo {
+struct __align__(16) TileInfo {
   int pos[kTileBlocks];    // first position of each block; far past every row where none is there
   float ks[kTileBlocks];
   int ev[kTileBlocks];     // exponent of the value scale
-  unsigned nan[kKeys / 32];  // tokens whose values hold a NaN
+  __align__(16) unsigned nan[kKeys / 32];  // tokens whose values hold a NaN; there with the values, not the keys
 };
 
 template <int D>
 struct Smem {
   static constexpr int kQ = kRows * D * 2;       // bytes of a query tile
   static constexpr int kOperand = kKeys * D * 2; // of K or V
-  static constexpr int kBytes = 2 * kQ + 2 * kStages * kOperand + kInfos * (int)sizeof(TileInfo) + 1024;
+  static constexpr int kOut = 8 * 32 * 64;       // output staging: 64 bytes of each row
+  static constexpr int kRaw = kKeys * D;         // codes of the next tile's keys
+  static constexpr int kBytes = 2 * kQ + 2 * kStages * kOperand + kOut + kRaw + kInfos * (int)sizeof(TileInfo) + 1024;
 };
 
 // kind::f16 with f16 operands; b_rows: B's shared-memory rows run along N (its 16-bit "MN-major" form)
@@ -99,6 +104,13 @@ __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void to_async_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
+// 16 bytes that are read once: past L1, which shared memory leaves little of and the spilled registers need
+__device__ __forceinline__ uint4 load_once(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+
 // pairs of f32 in one instruction
 __device__ __forceinline__ uint64_t pair(float x, float y) {
   uint64_t r;
@@ -129,143 +141,349 @@ struct View {
   __device__ __forceinline__ uint32_t mask(int p) const { return below(qp + 1 - p) & (~below(lo - p) | below(sinks - p)); }
 };
 
-// A row's scores of a key tile, held in registers from TMEM until its probabilities go back there.
-struct Row {
-  uint32_t v[4][32];
+// Whether a row sees a token with a NaN value: the operand holds 0 in its place, since NaN times the
+// probability 0 of a row that does not see it would be NaN too.
+__device__ __forceinline__ bool sees_nan(const TileInfo& info, const View& view) {
+  const uint4 nan = *reinterpret_cast<const uint4*>(info.nan);
+  if ((nan.x | nan.y | nan.z | nan.w) == 0) return false;
+  uint32_t found = 0;
+  for (int k = 0; k < kTileBlocks; ++k) found |= view.mask(info.pos[k]) & (info.nan[k >> 1] >> (16 * (k & 1)));
+  return found != 0;
+}
 
-  __device__ __forceinline__ void load(uint32_t s_at) {
-#pragma unroll
-    for (int c = 0; c < 4; ++c) tmem_ld32(s_at + 32u * c, v[c]);
+// Calls work(c, scores) for the four 32-key chunks of a row of scores in TMEM, the next chunk's load
+// in flight meanwhile. The loop stays rolled and the row in TMEM: a row of 128 scores in registers
+// left the kernel spilling and its code beyond the instruction cache (11 local loads a tile and
+// warp, most of them L2 round trips: 750 us for 8 x 2048).
+template <class Work>
+__device__ __forceinline__ void over_row(uint32_t s_at, Work work) {
+  uint32_t v0[32], v1[32];
+  tmem_ld32(s_at, v0);
+#pragma unroll 1
+  for (int c = 0; c < kKeys / 32; c += 2) {
     tmem_ld_wait();
+    tmem_ld32(s_at + 32u * (c + 1), v1);
+    work(c, v0);
+    tmem_ld_wait();
+    if (c + 2 < kKeys / 32) tmem_ld32(s_at + 32u * (c + 2), v0);
+    work(c + 1, v1);
   }
-  // The largest score (times its factor). ALL: the row sees the whole tile; otherwise the scores of
-  // what it does not see become -inf, and `bad` says whether it sees a token with a NaN value (the
-  // operand holds 0 there).
-  template <bool ALL>
-  __device__ __forceinline__ float most(const TileInfo& info, const View& view, float factor, bool& bad) {
-    float mx = -INFINITY;
-    uint32_t found = 0;
+}
+
+// The largest score of a row, times its factor. ALL: it sees the whole tile.
+template <bool ALL>
+__device__ __forceinline__ float row_max(uint32_t s_at, const TileInfo& info, const View& view, float factor) {
+  float mx = -INFINITY;
+  over_row(s_at, [&](int c, const uint32_t (&v)[32]) {
 #pragma unroll
-    for (int k = 0; k < kTileBlocks; ++k) {
-      uint32_t* x = v[k >> 1] + 16 * (k & 1);
-      if (!ALL) {
-        const uint32_t see = view.mask(info.pos[k]);
-        found |= see & (info.nan[k >> 1] >> (16 * (k & 1)));
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t* x = v + 16 * h;
+      const float f = factor * info.ks[2 * c + h];
+      float t = -INFINITY;
+      if (ALL) {
 #pragma unroll
-        for (int e = 0; e < 16; ++e)
-          if (!(see >> e & 1)) x[e] = 0xff800000u;
+        for (int e = 0; e < 16; e += 2) t = fmaxf(t, fmaxf(__uint_as_float(x[e]), __uint_as_float(x[e + 1])));
+      } else {
+        const uint32_t see = view.mask(info.pos[2 * c + h]);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) t = fmaxf(t, see >> e & 1 ? __uint_as_float(x[e]) : -INFINITY);
       }
-      float t = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
-#pragma unroll
-      for (int e = 2; e < 16; e += 2) t = fmaxf(t, fmaxf(__uint_as_float(x[e]), __uint_as_float(x[e + 1])));
-      const float f = factor * info.ks[k];
       mx = fmaxf(mx, t == -INFINITY ? t : t * f);
     }
-    bad = ALL ? (info.nan[0] | info.nan[1] | info.nan[2] | info.nan[3]) != 0 : found != 0;
-    return mx;
-  }
-  // The probabilities, in f16, each block's weighed by its value scale, go over the scores in TMEM;
-  // returns their sum without the weights.
-  template <bool ALL>
-  __device__ __forceinline__ float store(uint32_t s_at, const TileInfo& info, float factor, float base, int eref) {
-    float l = 0.f;
+  });
+  return mx;
+}
+
+// The probabilities, in f16, each block's weighed by its value scale, go over the scores in TMEM;
+// returns their sum without the weights.
+template <bool ALL>
+__device__ __forceinline__ float row_exp(uint32_t s_at, const TileInfo& info, const View& view, float factor, float base, int eref) {
+  float l = 0.f;
+  over_row(s_at, [&](int c, const uint32_t (&v)[32]) {
+    uint32_t p[16];
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      uint32_t p[16];
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t* x = v + 16 * h;
+      const float f = factor * info.ks[2 * c + h];
+      const int w = max(-60, info.ev[2 * c + h] - eref) + kShift;
+      const uint64_t ff = pair(f, f), add = pair((float)w - base, (float)w - base);
+      const uint32_t see = ALL ? 0 : view.mask(info.pos[2 * c + h]);
+      uint64_t sum = 0;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int k = 2 * c + h;
-        const uint32_t* x = v[c] + 16 * h;
-        // -inf * 0 would be NaN: with a key scale of 0 the visible scores are 0 whatever the factor
-        const float f = ALL ? factor * info.ks[k] : fmaxf(factor * info.ks[k], 1e-37f);
-        const int w = max(-60, info.ev[k] - eref) + kShift;
-        const uint64_t ff = pair(f, f), add = pair((float)w - base, (float)w - base);
-        uint64_t sum = 0;
-#pragma unroll
-        for (int e = 0; e < 16; e += 2) {
-          float2 y = unpair(fma2(pair(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), ff, add));
-          y.x = exp2_ftz(y.x);
-          y.y = exp2_ftz(y.y);
-          sum = add2(sum, pair(y.x, y.y));
-          p[8 * h + e / 2] = h2(y.x, y.y);
+      for (int e = 0; e < 16; e += 2) {
+        float2 y = unpair(fma2(pair(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), ff, add));
+        y.x = exp2_ftz(y.x);
+        y.y = exp2_ftz(y.y);
+        if (!ALL) {
+          y.x = see >> e & 1 ? y.x : 0.f;
+          y.y = see >> (e + 1) & 1 ? y.y : 0.f;
         }
-        const float2 t = unpair(sum);
-        l = fmaf(t.x + t.y, __uint_as_float((uint32_t)(127 - w) << 23), l);
+        sum = add2(sum, pair(y.x, y.y));
+        p[8 * h + e / 2] = h2(y.x, y.y);
       }
-      tmem_st16(s_at + 16u * c, p);
+      const float2 t = unpair(sum);
+      l = fmaf(t.x + t.y, __uint_as_float((uint32_t)(127 - w) << 23), l);
     }
-    return l;
+    tmem_st16(s_at + 16u * c, p);
+  });
+  return l;
+}
+
+// One arrival for a warp: 32 threads' arrivals on one word are 32 operations one after the other,
+// and the waiter's time.
+__device__ __forceinline__ void warp_arrive(uint64_t* bar, int lane) {
+  __syncwarp();
+  if (lane == 0) bar_arrive(bar);
+}
+
+// 256 rows of one (sequence, kv head).
+struct Item {
+  int seq, head;               // seq -1: no more
+  int row0, len, pos0;         // the sequence's first row of q, its length, the position of its query 0
+  int first_row, rows;         // this item's first row, and its number of rows
+  Span span;                   // blocks that any of them sees
+  int begin[2], end[2];        // key tiles of each tile of 128 rows: [begin, end) of the span's list
+  __device__ __forceinline__ bool active(int i) const { return end[i] > begin[i]; }
+  __device__ __forceinline__ int blocks() const { return max(0, span.count()); }
+  __device__ __forceinline__ int tiles() const { return (blocks() + kTileBlocks - 1) / kTileBlocks; }
+};
+
+// Items of a sequence, before its kv heads.
+__device__ __forceinline__ int items_of(const AttnArgs& a, int b) {
+  const int64_t rows = (int64_t)max(0, __ldg(a.offsets + b + 1) - __ldg(a.offsets + b)) * a.group;
+  return (int)((rows + 2 * kRows - 1) / (2 * kRows));
+}
+// Sum over the sequences of min(items, most), by a warp.
+__device__ __forceinline__ int64_t items_up_to(const AttnArgs& a, int most, int lane) {
+  int64_t n = 0;
+  for (int b = lane; b < a.batch; b += 32) n += min(most, items_of(a, b));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+  return n;
+}
+
+// Item number f of the call, for a warp: all last items of the sequences, then all last but one, ...
+__device__ __forceinline__ void find_item(const AttnArgs& a, int64_t f, int lane, Item& it) {
+  it.seq = -1;
+  const int64_t m = f / a.c.kv_heads;
+  if (m >= items_up_to(a, 0x7fffffff, lane)) return;
+  int lo = 0, hi = 1;  // items_up_to(lo) <= m < items_up_to(hi)
+  while (items_up_to(a, hi, lane) <= m) {
+    lo = hi;
+    hi *= 2;
+  }
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) / 2;
+    if (items_up_to(a, mid, lane) <= m)
+      lo = mid;
+    else
+      hi = mid;
+  }
+  int64_t left = m - items_up_to(a, lo, lane);  // this many sequences of more than lo items come before
+  int b = 0;
+  for (int base = 0;; base += 32) {
+    const uint32_t has = __ballot_sync(0xffffffffu, base + lane < a.batch && items_of(a, min(base + lane, a.batch - 1)) > lo);
+    if (left >= __popc(has)) {
+      left -= __popc(has);
+      continue;
+    }
+    b = base + __fns(has, 0, (int)left + 1);
+    break;
+  }
+  it.seq = b;
+  it.head = (int)(f % a.c.kv_heads);
+  it.row0 = __ldg(a.offsets + b);
+  const int n = __ldg(a.offsets + b + 1) - it.row0;
+  it.len = __ldg(a.lengths + b);
+  it.pos0 = it.len - n;  // negative: the first queries are before the cache and see nothing
+  it.first_row = (items_of(a, b) - 1 - lo) * (2 * kRows);
+  it.rows = (int)min((int64_t)2 * kRows, (int64_t)n * a.group - it.first_row);
+  auto span_of_tile = [&](int i, int tiles) {  // of tiles i .. i + tiles - 1
+    const int from = it.first_row + i * kRows, to = it.first_row + min(it.rows, (i + tiles) * kRows) - 1;
+    return span_of(max(0, it.pos0 + from / a.group), min(it.len - 1, it.pos0 + to / a.group), a.window, a.sinks);
+  };
+  it.span = span_of_tile(0, 2);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    it.begin[i] = it.end[i] = 0;
+    if (i * kRows >= it.rows) continue;
+    // a tile leaves out the key tiles past its last row, and without sinks those before its window
+    const Span s = span_of_tile(i, 1);
+    if (s.count() <= 0) continue;
+    const int end = it.span.sink_blocks + max(0, s.end - it.span.from);
+    const int begin = a.sinks > 0 ? 0 : max(0, s.from - it.span.from);
+    it.begin[i] = begin / kTileBlocks;
+    it.end[i] = (max(end, it.span.sink_blocks) + kTileBlocks - 1) / kTileBlocks;
+  }
+}
+
+// O of a warp's rows times a factor of each.
+template <int D>
+__device__ __forceinline__ void rescale(uint32_t o_at, float by) {
+#pragma unroll 1
+  for (int c = 0; c < D; c += 32) {
+    uint32_t v[32];
+    tmem_ld32(o_at + (uint32_t)c, v);
+    tmem_ld_wait();
+#pragma unroll
+    for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * by);
+    tmem_st32(o_at + (uint32_t)c, v);
+  }
+}
+
+// A warp's 32 output rows from TMEM: each lane's times its `inv` (zeros where `none`).
+template <int D, int TYPE>
+__device__ __forceinline__ void put_rows(void* out, uint8_t* stage, uint32_t o_at, bool none, float inv, int64_t out_row, int lane) {
+  constexpr int kItem = TYPE == J4B_F32 ? 4 : 2, kCols = 64 / kItem;  // columns of a pass
+#pragma unroll 1
+  for (int c0 = 0; c0 < D; c0 += 32) {
+    uint32_t v[32];
+    tmem_ld32(o_at + (uint32_t)c0, v);
+    tmem_ld_wait();
+    float x[32];
+#pragma unroll
+    for (int e = 0; e < 32; ++e) x[e] = none ? 0.f : __uint_as_float(v[e]) * inv;
+#pragma unroll
+    for (int c = 0; c < 32; c += kCols) {
+      __syncwarp();
+#pragma unroll
+      for (int e = 0; e < kCols; e += 16 / kItem) {
+        uint32_t w[4];
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          if (TYPE == J4B_F32) {
+            w[y] = __float_as_uint(x[c + e + y]);
+          } else {
+            const __nv_bfloat162 t = __floats2bfloat162_rn(x[c + e + 2 * y], x[c + e + 2 * y + 1]);
+            w[y] = *reinterpret_cast<const uint32_t*>(&t);
+          }
+        }
+        // rows are 64 bytes: two of them cover the banks, so pieces are swizzled by every other row
+        *reinterpret_cast<uint4*>(stage + lane * 64 + (((e * kItem / 16) ^ (lane >> 1 & 3)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+      __syncwarp();
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {  // 8 rows x 4 pieces
+        const int qr = 8 * k + (lane >> 2), piece = lane & 3;
+        const int64_t dst = __shfl_sync(0xffffffffu, out_row, qr);
+        if (dst >= 0)
+          *reinterpret_cast<uint4*>(static_cast<uint8_t*>(out) + (dst + c0 + c) * kItem + 16 * piece) =
+              *reinterpret_cast<const uint4*>(stage + qr * 64 + ((piece ^ (qr >> 1 & 3)) << 4));
+      }
+    }
+  }
+}
+
+// A warp's 32 query rows of a tile, 8 lanes a row, 4 rows at a time: `fetch` has the loads in
+// flight while the last item's output is written, `put` brings each row by a power of two to a
+// largest element in [2^11, 2^12), then to f16 (bf16 is exact there), in the tile's swizzled operand.
+// Returns lane's own row's power of two, by which its scores are to be multiplied.
+template <int D, int TYPE>
+struct Queries {
+  static constexpr int kWords = TYPE == J4B_F32 ? D / 32 : D / 64;  // 16-byte pieces of a row and lane
+  static constexpr int kHeld = 8 / kWords;                         // rows of a lane that fetch holds
+  uint4 raw[kHeld][kWords];
+
+  static __device__ __forceinline__ void get(const AttnArgs& a, const Item& it, int i, int warp, int k, int lane, uint4 (&dst)[kWords]) {
+    const int qr = 32 * warp + 4 * k + (lane >> 3), g = it.first_row + i * kRows + qr, row = it.row0 + g / a.group;
+    const bool there = i * kRows + qr < it.rows && row >= 0 && row < a.tokens;
+    const int64_t src = (int64_t)row * a.q_stride + (int64_t)(it.head * a.group + g % a.group) * D + 8 * (lane & 7);
+#pragma unroll
+    for (int c = 0; c < kWords; ++c)
+      dst[c] = !there ? make_uint4(0, 0, 0, 0)
+               : TYPE == J4B_F32 ? load_once(static_cast<const float*>(a.q) + src + 64 * (c >> 1) + 4 * (c & 1))
+                                 : load_once(static_cast<const __nv_bfloat16*>(a.q) + src + 64 * c);
+  }
+  __device__ __forceinline__ void fetch(const AttnArgs& a, const Item* it, int i, int warp, int lane) {
+#pragma unroll
+    for (int k = 0; k < kHeld; ++k) {
+      if (it) {
+        get(a, *it, i, warp, k, lane, raw[k]);
+      } else {  // all of it set anew, or it would be held through the key tiles
+#pragma unroll
+        for (int c = 0; c < kWords; ++c) raw[k][c] = make_uint4(0, 0, 0, 0);
+      }
+    }
+  }
+  __device__ __forceinline__ float put(const AttnArgs& a, const Item& it, int i, int warp, uint8_t* tile, int lane) {
+    float mine = 1.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      if (k >= kHeld) get(a, it, i, warp, k, lane, raw[k % kHeld]);
+      const int qr = 32 * warp + 4 * k + (lane >> 3);
+      float x[D / 8];
+      float most = 0.f;
+#pragma unroll
+      for (int c = 0; c < kWords; ++c) {
+        const uint32_t w[4] = {raw[k % kHeld][c].x, raw[k % kHeld][c].y, raw[k % kHeld][c].z, raw[k % kHeld][c].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (TYPE == J4B_F32) {
+            x[4 * c + e] = __uint_as_float(w[e]);
+          } else {
+            x[8 * c + 2 * e] = __uint_as_float(w[e] << 16);
+            x[8 * c + 2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
+          }
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < D / 8; ++e) most = fmaxf(most, fabsf(x[e]));
+#pragma unroll
+      for (int o = 1; o < 8; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+      const int e = (int)(__float_as_uint(most) >> 23);
+      const bool plain = e < 24 || e > 240;
+      float up = plain ? 1.f : __uint_as_float((uint32_t)(254 - (e - 11)) << 23);
+      const float down = plain ? 1.f : __uint_as_float((uint32_t)(e - 11) << 23);
+      if (a.scale_log2 < 0.f) up = -up;  // maxima are taken before the factor
+      // row 4 k + x of the warp is handled by lanes 8 x ..: lane 4 k + x takes its factor from there
+      const float theirs = __shfl_sync(0xffffffffu, down, (lane & 3) << 3);
+      if (lane >> 2 == k) mine = theirs;
+#pragma unroll
+      for (int c = 0; c < D / 64; ++c) {
+        const float* y = x + 8 * c;
+        *reinterpret_cast<uint4*>(tile + c * (kRows * 128) + sw128_offset(qr, 8 * (lane & 7))) =
+            make_uint4(h2(y[0] * up, y[1] * up), h2(y[2] * up, y[3] * up), h2(y[4] * up, y[5] * up), h2(y[6] * up, y[7] * up));
+      }
+    }
+    return mine;
   }
 };
 
-// Which key tiles a row tile takes: [begin, end) of the CTA's list.
-struct Range {
-  int begin, end;
-  __device__ __forceinline__ bool has(int j) const { return j >= begin && j < end; }
-};
+constexpr int kItems = 4;         // found ahead
+constexpr int kItemReaders = 13;  // warps
 
-// Registers of a thread by warpgroup: the launch's 4 x 128 shared out as 2 x 176 + 104 + 56.
-template <int N>
-__device__ __forceinline__ void more_registers() {
-  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
-}
-template <int N>
-__device__ __forceinline__ void fewer_registers() {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
-}
-
-template <int D>
+template <int D, int TYPE>
 __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const AttnArgs a) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = aligned_smem(smem_raw);
-  uint8_t* sq = smem;                                       // [2 tiles]
-  uint8_t* sk = smem + 2 * Smem<D>::kQ;                     // [stage][K | V]
-  TileInfo* infos = reinterpret_cast<TileInfo*>(sk + 2 * kStages * Smem<D>::kOperand);
-  __shared__ uint64_t q_ready[2], k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], s_full[2], p_ready[2], o_full[2], info_full[kInfos];
+  uint8_t* sq = smem;                    // [2 tiles]
+  uint8_t* sk = smem + 2 * Smem<D>::kQ;  // [stage][K | V]
+  uint8_t* sout = sk + 2 * kStages * Smem<D>::kOperand;
+  uint8_t* sraw = sout + Smem<D>::kOut;
+  TileInfo* infos = reinterpret_cast<TileInfo*>(sraw + Smem<D>::kRaw);
+  __shared__ uint64_t item_full[kItems], item_empty[kItems], q_ready[2], q_empty[2], k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages],
+      s_full[2], p_ready[2], o_full[2];
   __shared__ uint32_t tmem_slot;
-  __shared__ float factors[2][kRows];
+  __shared__ Item items[kItems];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int head = blockIdx.y;
-  // the last rows of a sequence see the most keys: they go first
-  const Kv8Place at = kv8_find<kThreads>(
-      a.batch, [&](int b) -> int64_t { return ((int64_t)max(0, a.offsets[b + 1] - a.offsets[b]) * a.group + 2 * kRows - 1) / (2 * kRows); },
-      [&](int64_t total) -> int64_t { return total > (int64_t)blockIdx.x ? total - 1 - (int64_t)blockIdx.x : total; });
-  if (at.seq < 0) return;
-  const int b = at.seq, row0 = a.offsets[b], n = a.offsets[b + 1] - row0, len = __ldg(a.lengths + b);
-  const int64_t total_rows = (int64_t)n * a.group, r0 = at.at * (2 * kRows);
-  const int pos0 = len - n;  // position of query 0 (queries before the cache see nothing)
-  // positions of a tile's first and last row
-  auto first_of = [&](int i) { return pos0 + (int)((r0 + i * kRows) / a.group); };
-  auto last_of = [&](int i) { return min(len - 1, pos0 + (int)((min(total_rows, r0 + (i + 1) * kRows) - 1) / a.group)); };
-  const int tiles = total_rows > r0 + kRows ? 2 : 1;
-  const Span span = span_of(max(0, first_of(0)), last_of(tiles - 1), a.window, a.sinks);
-  const int nb = max(0, span.count()), nt = (nb + kTileBlocks - 1) / kTileBlocks;
-  // a tile leaves out key tiles past its last row, and those before its first row's window
-  auto range_of = [&](int i) -> Range {
-    if (i >= tiles) return {0, 0};
-    const Span s = span_of(max(0, first_of(i)), last_of(i), a.window, a.sinks);
-    if (s.count() <= 0) return {0, 0};
-    const int end = span.sink_blocks + max(0, s.end - span.from);  // blocks of the list up to the tile's last
-    // with sinks the tile also takes the list's first blocks, so it starts at 0
-    const int begin = a.sinks > 0 ? 0 : span.sink_blocks + max(0, s.from - span.from);
-    return {begin / kTileBlocks, (max(end, span.sink_blocks) + kTileBlocks - 1) / kTileBlocks};
-  };
-  const Range range0 = range_of(0), range1 = range_of(1);
-
   if (tid == 0) {
+    for (int i = 0; i < kItems; ++i) {
+      bar_init(&item_full[i], 1);
+      bar_init(&item_empty[i], kItemReaders);
+    }
     for (int i = 0; i < 2; ++i) {
-      bar_init(&q_ready[i], kRows);
-      bar_init(&s_full[i], 1);
-      bar_init(&p_ready[i], kRows);
-      bar_init(&o_full[i], 1);
+      bar_init(&q_ready[i], 4);  // warps
+      bar_init(&q_empty[i], 1);
+      bar_init(&s_full[i], 2);  // the MMAs, and the thread that saw keys, info and queries ready
+      bar_init(&p_ready[i], 4);
+      bar_init(&o_full[i], 2);
     }
     for (int s = 0; s < kStages; ++s) {
-      bar_init(&k_full[s], 128);
-      bar_init(&v_full[s], 128);
+      bar_init(&k_full[s], 4);
+      bar_init(&v_full[s], 4);
       bar_init(&k_empty[s], 1);
       bar_init(&v_empty[s], 1);
     }
-    for (int s = 0; s < kInfos; ++s) bar_init(&info_full[s], 128);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 12) {
@@ -277,372 +495,351 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const AttnArgs
   tc_fence_after();
   const uint32_t tmem = tmem_slot;  // S0, S1 at columns 0, 128 (P over them); O0, O1 at 256, 384
   bool ok = true;
+  // The next item, for every warp but the one that finds them (null after the last); the one before
+  // is given back. Read where it is: a copy would cost registers.
+  uint32_t nth = 0;
+  auto next_item = [&](bool alone = false) -> const Item* {
+    if (!alone) __syncwarp();
+    if (nth > 0 && lane == 0) bar_arrive(&item_empty[(nth - 1) % kItems]);
+    ok = ok && kv8_wait(&item_full[nth % kItems], nth / kItems & 1);
+    const Item* it = &items[nth % kItems];
+    ++nth;
+    return ok && it->seq >= 0 ? it : nullptr;
+  };
 
   if (warp < 8) {
-    more_registers<176>();
     // ---- softmax of tile i, one row a thread ----
     const int i = warp >> 2, r = tid & 127;
-    const Range rg = i ? range1 : range0;
-    const int64_t gr = r0 + i * kRows + r;
-    const int tok = (int)(gr / a.group), gh = head * a.group + (int)(gr % a.group);
-    const bool valid = gr < total_rows && row0 + tok >= 0 && row0 + tok < a.tokens;
-    const int qp = valid ? pos0 + tok : -1;
-    const View view = {a.window > 0 ? max(0, qp - a.window + 1) : 0, qp, a.sinks};
-    // every valid row of the tile sees the positions [most_lo, least]
-    const int least = first_of(i), most_lo = a.window > 0 ? max(0, last_of(i) - a.window + 1) : 0;
-    // Q: each row by a power of two to a largest element in [2^11, 2^12), then f16 (bf16 is exact
-    // there); 8 lanes a row, 4 rows at a time
-    float factor = 0.f;
-    if (i < tiles) {
-      uint8_t* tile = sq + i * Smem<D>::kQ;
-      const int sub = lane & 7;
-      auto rows = [&](auto type) {
-        constexpr bool kF32 = decltype(type)::value == J4B_F32;
-        constexpr int kWords = kF32 ? D / 32 : D / 64, kStep = kF32 ? 4 : 8;  // 16-byte pieces of a row and lane, rows in flight
-#pragma unroll 1
-        for (int k0 = 0; k0 < 8; k0 += kStep) {
-          uint4 raw[kStep][kWords];
-#pragma unroll
-          for (int k = 0; k < kStep; ++k) {
-            const int64_t g = r0 + i * kRows + (warp & 3) * 32 + 4 * (k0 + k) + (lane >> 3), row = row0 + g / a.group;
-            const bool there = g < total_rows && row >= 0 && row < a.tokens;
-            const int64_t src = row * a.q_stride + (int64_t)(head * a.group + (int)(g % a.group)) * D + 8 * sub;
-#pragma unroll
-            for (int c = 0; c < kWords; ++c)
-              raw[k][c] = !there ? make_uint4(0, 0, 0, 0)
-                          : kF32 ? __ldg(reinterpret_cast<const uint4*>(static_cast<const float*>(a.q) + src + 64 * (c >> 1) + 4 * (c & 1)))
-                                 : __ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.q) + src + 64 * c));
-          }
-#pragma unroll
-          for (int k = 0; k < kStep; ++k) {
-            const int qr = (warp & 3) * 32 + 4 * (k0 + k) + (lane >> 3);
-            float x[D / 8];
-            float most = 0.f;
-#pragma unroll
-            for (int c = 0; c < kWords; ++c) {
-              const uint32_t w[4] = {raw[k][c].x, raw[k][c].y, raw[k][c].z, raw[k][c].w};
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                if (kF32) {
-                  x[4 * c + e] = __uint_as_float(w[e]);
-                } else {
-                  x[8 * c + 2 * e] = __uint_as_float(w[e] << 16);
-                  x[8 * c + 2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
-                }
-              }
-            }
-#pragma unroll
-            for (int e = 0; e < D / 8; ++e) most = fmaxf(most, fabsf(x[e]));
-#pragma unroll
-            for (int o = 1; o < 8; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-            const int e = (int)(__float_as_uint(most) >> 23);
-            const bool plain = e < 24 || e > 240;
-            float up = plain ? 1.f : __uint_as_float((uint32_t)(254 - (e - 11)) << 23);
-            float f = plain ? a.scale_log2 : a.scale_log2 * __uint_as_float((uint32_t)(e - 11) << 23);
-            if (f < 0.f) {  // maxima are taken before the factor
-              f = -f;
-              up = -up;
-            }
-            if (sub == 0) factors[i][qr] = f;
-#pragma unroll
-            for (int c = 0; c < D / 64; ++c) {
-              const float* y = x + 8 * c;
-              *reinterpret_cast<uint4*>(tile + c * (kRows * 128) + sw128_offset(qr, 8 * sub)) =
-                  make_uint4(h2(y[0] * up, y[1] * up), h2(y[2] * up, y[3] * up), h2(y[4] * up, y[5] * up), h2(y[6] * up, y[7] * up));
-            }
-          }
-        }
-      };
-      if (a.q_type == J4B_F32)
-        rows(std::integral_constant<int, J4B_F32>{});
-      else
-        rows(std::integral_constant<int, J4B_BF16>{});
-      to_async_proxy();
-      bar_arrive(&q_ready[i]);
-      __syncwarp();  // a warp wrote the factors of its own rows
-      factor = factors[i][r];
-    }
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const uint32_t s_at = lanes + (uint32_t)(i * 128), o_at = lanes + 256u + (uint32_t)(i * 128);
-    float m = -INFINITY, l = 0.f;
-    int eref = 0;  // exponent of the value scale that O is in units of
-    uint32_t use = 0;
-    for (int j = rg.begin; j < rg.end; ++j, ++use) {
-      ok = ok && bar_wait(&info_full[j % kInfos], (uint32_t)(j / kInfos & 1));
-      ok = ok && bar_wait(&s_full[i], use & 1);
-      tc_fence_after();
-      const TileInfo& info = infos[j % kInfos];
-      int near = kNowhere, far = 0;
-#pragma unroll
-      for (int k = 0; k < kTileBlocks; ++k) {
-        near = min(near, info.pos[k]);
-        far = max(far, info.pos[k] + kKvBlock);
+    uint32_t use = 0, outs = 0, before = 0;  // tiles done, items done, key tiles of the earlier items
+    Queries<D, TYPE> queries;
+    const Item* item = next_item();
+    queries.fetch(a, item, i, warp & 3, lane);
+    while (item) {
+      const Item& it = *item;
+      const bool active = it.active(i);
+      float factor = 0.f;
+      if (active) {
+        if (outs > 0) ok = ok && kv8_wait(&q_empty[i], (outs - 1) & 1);
+        factor = fabsf(a.scale_log2) * queries.put(a, it, i, warp & 3, sq + i * Smem<D>::kQ, lane);
+        to_async_proxy();
+        warp_arrive(&q_ready[i], lane);
       }
-      const bool all = far - 1 <= least && (near >= most_lo || far <= a.sinks);
-      bool bad = false;
-      Row row;
-      row.load(s_at);
-      const float mx = all ? row.most<true>(info, view, factor, bad) : row.most<false>(info, view, factor, bad);
-      if (bad) l = NAN;
-      int ev = info.ev[0];
+      const int gr = it.first_row + i * kRows + r, tok = gr / a.group, gh = it.head * a.group + gr % a.group;
+      const bool valid = i * kRows + r < it.rows && it.row0 + tok >= 0 && it.row0 + tok < a.tokens;
+      const int64_t out_row = valid ? ((int64_t)(it.row0 + tok) * a.heads + gh) * D : -1;
+      const int qp = valid ? it.pos0 + tok : -1;
+      const View view = {a.window > 0 ? max(0, qp - a.window + 1) : 0, qp, a.sinks};
+      // every valid row of the tile sees the positions [most_lo, least]
+      const int least = it.pos0 + (it.first_row + i * kRows) / a.group;
+      const int most_lo = a.window > 0 ? max(0, it.pos0 + (it.first_row + min(it.rows, (i + 1) * kRows) - 1) / a.group - a.window + 1) : 0;
+      float m = -INFINITY, l = 0.f;
+      int eref = 0;  // exponent of the value scale that O is in units of
+      const int j0 = it.begin[i], j1 = it.end[i];
+      for (int j = j0; j < j1; ++j, ++use) {
+        const uint32_t k = before + (uint32_t)j;
+        ok = ok && kv8_wait(&s_full[i], use & 1);  // with it comes the tile's info
+        tc_fence_after();
+        const TileInfo& info = infos[k % kInfos];
+        int near = kNowhere, far = 0, ev = -127;
 #pragma unroll
-      for (int k = 1; k < kTileBlocks; ++k) ev = max(ev, info.ev[k]);
-      const bool begin = j == rg.begin;
-      const int enew = begin ? ev : max(eref, ev);
-      float mnew = m;
-      if (mx > m + kLazy || (m == -INFINITY && mx > m)) mnew = mx;
-      if (begin) {
-        m = mnew;
-      } else if (__any_sync(0xffffffffu, mnew != m || enew != eref)) {
-        const float cm = m == -INFINITY ? 0.f : exp2_ftz(m - mnew), co = cm * exp2_ftz((float)(eref - enew));
-        l *= m == mnew ? 1.f : cm;
-        m = mnew;
-        uint32_t v[32];
-#pragma unroll 1
-        for (int c = 0; c < D; c += 32) {
-          tmem_ld32(o_at + (uint32_t)c, v);
-          tmem_ld_wait();
-#pragma unroll
-          for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * co);
-          tmem_st32(o_at + (uint32_t)c, v);
+        for (int x = 0; x < kTileBlocks; ++x) {
+          near = min(near, info.pos[x]);
+          far = max(far, info.pos[x] + kKvBlock);
+          ev = max(ev, info.ev[x]);
         }
+        const bool all = far - 1 <= least && (near >= most_lo || far <= a.sinks);
+        const float mx = all ? row_max<true>(s_at, info, view, factor) : row_max<false>(s_at, info, view, factor);
+        // the last tile's values were ready before these scores were
+        if (j > j0 && sees_nan(infos[(k - 1) % kInfos], view)) l = NAN;
+        const bool begin = j == j0;
+        const int enew = begin ? ev : max(eref, ev);
+        float mnew = m;
+        if (mx > m + kLazy || (m == -INFINITY && mx > m)) mnew = mx;
+        if (begin) {
+          m = mnew;
+        } else if (__any_sync(0xffffffffu, mnew != m || enew != eref)) {
+          const float cm = m == -INFINITY ? 0.f : exp2_ftz(m - mnew), co = cm * exp2_ftz((float)(eref - enew));
+          l *= m == mnew ? 1.f : cm;
+          m = mnew;
+          rescale<D>(o_at, co);
+        }
+        eref = enew;
+        const float base = m == -INFINITY ? 0.f : m;
+        l += all ? row_exp<true>(s_at, info, view, factor, base, eref) : row_exp<false>(s_at, info, view, factor, base, eref);
+        tmem_st_wait();
+        tc_fence_before();
+        warp_arrive(&p_ready[i], lane);
       }
-      eref = enew;
-      const float base = m == -INFINITY ? 0.f : m;
-      l += all ? row.store<true>(s_at, info, factor, base, eref) : row.store<false>(s_at, info, factor, base, eref);
-      tmem_st_wait();
+      const uint32_t last_tile = before + (uint32_t)j1 - 1;
+      before += (uint32_t)it.tiles();
+      const int rows = it.rows;
+      item = next_item();
+      queries.fetch(a, item, i, warp & 3, lane);
+      // the output rows, through shared memory so that the stores are whole: 64 bytes of a row at a
+      // time
+      if (active) {
+        ok = ok && kv8_wait(&o_full[i], outs & 1);
+        ++outs;
+        tc_fence_after();
+        if (sees_nan(infos[last_tile % kInfos], view)) l = NAN;
+      }
+      if (i * kRows < rows) {
+        const bool none = m == -INFINITY;
+        const float inv = none ? 0.f : exp2_ftz((float)(eref - kShift)) / l;
+        uint8_t* stage = sout + warp * (32 * 64);
+        if (a.out_type == J4B_F32)
+          put_rows<D, J4B_F32>(a.out, stage, o_at, none, inv, out_row, lane);
+        else
+          put_rows<D, J4B_BF16>(a.out, stage, o_at, none, inv, out_row, lane);
+      }
       tc_fence_before();
-      bar_arrive(&p_ready[i]);
-    }
-    // the output row
-    if (rg.end > rg.begin) {
-      ok = ok && bar_wait(&o_full[i], 0);
-      tc_fence_after();
-    }
-    const int64_t out_row = valid ? ((int64_t)(row0 + tok) * a.heads + gh) * D : -1;
-    const float inv = m == -INFINITY ? 0.f : exp2_ftz((float)(eref - kShift)) / l;
-    // through the warp's rows of the query tile (its MMAs are done), so that the stores are whole
-    // rows: 256 bytes of a row at a time, 16-byte pieces swizzled by the row
-    uint8_t* stage = sq + i * Smem<D>::kQ + (warp & 3) * (32 * 2 * D);
-    const bool f32 = a.out_type == J4B_F32;
-    const int bytes = min(f32 ? 4 * D : 2 * D, 2 * D), passes = f32 ? 2 : 1;  // of a row and pass
-#pragma unroll 1
-    for (int pass = 0; pass < passes && i < tiles; ++pass) {
-      __syncwarp();
-#pragma unroll 1
-      for (int c = pass * (D / 2); c < (f32 ? (pass + 1) * (D / 2) : D); c += 32) {
-        uint32_t v[32];
-        if (rg.end > rg.begin) {
-          tmem_ld32(o_at + (uint32_t)c, v);
-          tmem_ld_wait();
-        }
-        float x[32];
-#pragma unroll
-        for (int e = 0; e < 32; ++e) x[e] = m == -INFINITY ? 0.f : __uint_as_float(v[e]) * inv;
-        const int first = (f32 ? 4 * (c - pass * (D / 2)) : 2 * c) / 16;  // 16-byte piece of the row
-        if (f32) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            *reinterpret_cast<float4*>(stage + lane * bytes + (((first + e) ^ (lane & 7)) << 4)) = make_float4(x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            uint32_t w[4];
-#pragma unroll
-            for (int y = 0; y < 4; ++y) {
-              const __nv_bfloat162 t = __floats2bfloat162_rn(x[8 * e + 2 * y], x[8 * e + 2 * y + 1]);
-              w[y] = *reinterpret_cast<const uint32_t*>(&t);
-            }
-            *reinterpret_cast<uint4*>(stage + lane * bytes + (((first + e) ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
-          }
-        }
-      }
-      __syncwarp();
-      constexpr int kLanes = D / 8, kAtOnce = 32 / kLanes;  // lanes of a row, rows of a store
-      uint8_t* out = static_cast<uint8_t*>(a.out) + pass * bytes;
-#pragma unroll 8
-      for (int k = 0; k < 32 / kAtOnce; ++k) {
-        const int qr = kAtOnce * k + lane / kLanes, piece = lane % kLanes;
-        const int64_t dst = __shfl_sync(0xffffffffu, out_row, qr);
-        if (dst >= 0)
-          *reinterpret_cast<uint4*>(out + dst * (f32 ? 4 : 2) + 16 * piece) =
-              *reinterpret_cast<const uint4*>(stage + qr * bytes + ((piece ^ (qr & 7)) << 4));
-      }
     }
   } else if (warp < 12) {
-    fewer_registers<104>();
     // ---- pages to operands: this warp the rows 32 w .. + 31 (2 blocks) of each key tile ----
     const int w = warp - 8;
     constexpr int kHalves = D / 64, kPieces = 4 * kHalves;  // 16-code pieces of a thread, K or V
     // piece x: row 32 w + 8 (x / kHalves) + lane / 4, codes 64 (x % kHalves) + 16 (lane % 4): 8 lanes of
     // a store phase are 2 rows x 4 pieces, whose swizzled places cover all banks
     const int pr = lane >> 2, pc = lane & 3;
-    auto block_at = [&](int j, int k) {  // block 2 w + k of tile j
-      const int x = j * kTileBlocks + 2 * w + k;
-      return x < nb ? span.block(x) : -1;
-    };
-    auto id_at = [&](int blk) { return blk < 0 ? -1 : kv8_block_id(a.c, a.t, b, head, blk); };
     auto load = [&](const uint8_t* codes, const int (&id)[2], uint4 (&dst)[kPieces]) {
 #pragma unroll
       for (int x = 0; x < kPieces; ++x) {
         const int row = 8 * (x / kHalves) + pr, k = row >> 4;  // of the warp's 32
         dst[x] = id[k] < 0 ? make_uint4(0, 0, 0, 0)
-                           : __ldg(reinterpret_cast<const uint4*>(codes + (int64_t)id[k] * (kKvBlock * D) + (row & 15) * D + 64 * (x % kHalves) + 16 * pc));
+                           : load_once(codes + (int64_t)id[k] * (kKvBlock * D) + (row & 15) * D + 64 * (x % kHalves) + 16 * pc);
       }
     };
-    auto store = [&](uint8_t* tile, const uint4 (&src)[kPieces]) {
+    // The keys' codes wait in shared memory, each thread's pieces its own (so its own wait is all they
+    // need): registers for them would be the softmax's.
+    const uint32_t mine_at = saddr(sraw) + (uint32_t)(tid & 127) * 16u;
+    auto load_keys = [&](const int (&id)[2]) {
 #pragma unroll
       for (int x = 0; x < kPieces; ++x) {
-        const int row = 32 * w + 8 * (x / kHalves) + pr;
-        uint4 lo, hi;
-        e4m3x4_f16(src[x].x, lo.x, lo.y);
-        e4m3x4_f16(src[x].y, lo.z, lo.w);
-        e4m3x4_f16(src[x].z, hi.x, hi.y);
-        e4m3x4_f16(src[x].w, hi.z, hi.w);
-        uint8_t* half = tile + (x % kHalves) * (kKeys * 128);
-        *reinterpret_cast<uint4*>(half + sw128_offset(row, 16 * pc)) = lo;
-        *reinterpret_cast<uint4*>(half + sw128_offset(row, 16 * pc + 8)) = hi;
+        const int row = 8 * (x / kHalves) + pr, k = row >> 4;
+        const uint8_t* src = a.c.k + (int64_t)max(id[k], 0) * (kKvBlock * D) + (row & 15) * D + 64 * (x % kHalves) + 16 * pc;
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(mine_at + x * 2048u), "l"(src), "r"(id[k] < 0 ? 0 : 16) : "memory");
       }
+      asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    int blk[2] = {block_at(0, 0), block_at(0, 1)};
-    int id[2] = {id_at(blk[0]), id_at(blk[1])};
-    uint4 kr[kPieces], vr[kPieces];
+    auto store_piece = [&](uint8_t* tile, int x, const uint4& src) {
+      const int row = 32 * w + 8 * (x / kHalves) + pr;
+      uint4 lo, hi;
+      e4m3x4_f16(src.x, lo.x, lo.y);
+      e4m3x4_f16(src.y, lo.z, lo.w);
+      e4m3x4_f16(src.z, hi.x, hi.y);
+      e4m3x4_f16(src.w, hi.z, hi.w);
+      uint8_t* half = tile + (x % kHalves) * (kKeys * 128);
+      *reinterpret_cast<uint4*>(half + sw128_offset(row, 16 * pc)) = lo;
+      *reinterpret_cast<uint4*>(half + sw128_offset(row, 16 * pc + 8)) = hi;
+    };
+    // (it, j) runs two tiles ahead of the operands, into the next items: its page numbers are on their
+    // way while a tile is turned, the codes and scales of the tile between from when this one's are out
+    // of the way.
+    const Item* it = next_item();
+    int j = 0;
+    // of its tile: blocks 2 w, 2 w + 1 (-1: past the end), their pages as loaded, the kv head, the length
+    int blk[2] = {-1, -1}, page[2] = {-1, -1}, head = 0, len = 0;
+    int id[2] = {-1, -1};  // the blocks' numbers, once the pages are there
+    auto find = [&]() -> bool {                        // tile j, and on to the next; false after the last
+      while (it && j >= it->tiles()) {
+        it = next_item();
+        j = 0;
+      }
+      if (!it) return false;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int x = j * kTileBlocks + 2 * w + k;
+        blk[k] = x < it->blocks() ? it->span.block(x) : -1;
+        const int at = blk[k] / a.c.bpp;
+        page[k] = blk[k] >= 0 && at < a.t.width ? __ldg(a.t.pages + it->seq * a.t.stride + at) : -1;
+      }
+      head = it->head;
+      len = it->len;
+      ++j;
+      return true;
+    };
+    auto number = [&] {
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+        id[k] = (unsigned)page[k] < (unsigned)a.c.pages ? (page[k] * a.c.kv_heads + head) * a.c.bpp + blk[k] % a.c.bpp : -1;
+    };
+    uint4 vr[kPieces];
     float ks = 1.f, vs = 0.f;
+    int now[2] = {-1, -1}, now_len = 0;  // first positions of the tile's blocks (-1: not there)
     auto scales = [&] {
-      if (lane < 2 && id[lane & 1] >= 0) {
-        ks = __ldg(a.c.ks + id[lane & 1]);
-        vs = __ldg(a.c.vs + id[lane & 1]);
-      } else {
-        ks = 1.f;
-        vs = 0.f;
+      const int mine = lane == 0 ? id[0] : id[1];
+      ks = 1.f, vs = 0.f;
+      if (lane < 2 && mine >= 0) {
+        ks = __ldg(a.c.ks + mine);
+        vs = __ldg(a.c.vs + mine);
       }
     };
-    load(a.c.k, id, kr);
-    load(a.c.v, id, vr);
-    scales();
-    int nblk[2] = {block_at(1, 0), block_at(1, 1)};
-    int nid[2] = {id_at(nblk[0]), id_at(nblk[1])};
-    for (int j = 0; j < nt; ++j) {
-      const int s = j % kStages;
-      const uint32_t parity = (uint32_t)(j / kStages - 1) & 1;
+    auto take = [&] {
+#pragma unroll
+      for (int k = 0; k < 2; ++k) now[k] = id[k] < 0 ? -1 : blk[k] * kKvBlock;
+      now_len = len;
+    };
+    bool here = find();
+    if (here) {
+      number();
+      load_keys(id);
+      load(a.c.v, id, vr);
+      scales();
+      take();
+    }
+    bool next = here && find();
+    for (uint32_t k = 0; here; ++k) {
+      const int s = k % kStages;
+      const uint32_t parity = (k / kStages - 1) & 1;
       uint8_t* kt = sk + s * 2 * Smem<D>::kOperand;
-      TileInfo& info = infos[j % kInfos];
-      if (j >= kStages) ok = ok && bar_wait(&k_empty[s], parity);
-      store(kt, kr);
+      TileInfo& info = infos[k % kInfos];
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+      if (k >= kStages) ok = ok && kv8_wait(&k_empty[s], parity);
+#pragma unroll
+      for (int x = 0; x < kPieces; ++x) store_piece(kt, x, *reinterpret_cast<const uint4*>(sraw + x * 2048 + (tid & 127) * 16));
       if (lane < 2) {
-        const int k = 2 * w + lane;
-        info.pos[k] = id[lane] < 0 ? kNowhere : blk[lane] * kKvBlock;
-        info.ks[k] = ks;
-        info.ev[k] = (int)(__float_as_uint(vs) >> 23) - 127;
+        const int x = 2 * w + lane, pos = lane == 0 ? now[0] : now[1];
+        info.pos[x] = pos < 0 ? kNowhere : pos;
+        info.ks[x] = ks;
+        info.ev[x] = (int)(__float_as_uint(vs) >> 23) - 127;
+      }
+      to_async_proxy();
+      warp_arrive(&k_full[s], lane);
+      if (next) {
+        number();
+        load_keys(id);
       }
       // the values' tokens past the length hold anything; NaNs go to the info, as zeros to the operand
-      {
-        unsigned nan = 0;
+      unsigned nan = 0;
 #pragma unroll
-        for (int x = 0; x < kPieces; ++x) {
-          const int row = 8 * (x / kHalves) + pr, k = row >> 4;
-          if (blk[k] * kKvBlock + (row & 15) >= len) vr[x] = make_uint4(0, 0, 0, 0);
-          uint32_t* q = reinterpret_cast<uint32_t*>(&vr[x]);
-          uint32_t any = 0;
+      for (int x = 0; x < kPieces; ++x) {
+        const int row = 8 * (x / kHalves) + pr;
+        if (now[row >> 4] + (row & 15) >= now_len) vr[x] = make_uint4(0, 0, 0, 0);
+        uint32_t* q = reinterpret_cast<uint32_t*>(&vr[x]);
+        uint32_t any = 0;
 #pragma unroll
-          for (int y = 0; y < 4; ++y) any |= ((q[y] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
-          if (any) {
-            nan |= 1u << row;
+        for (int e = 0; e < 4; ++e) any |= ((q[e] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+        if (any) {
+          nan |= 1u << row;
 #pragma unroll
-            for (int y = 0; y < 4; ++y) {
-              const uint32_t bytes = (((q[y] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7;
-              q[y] &= ~(bytes * 0xffu);
-            }
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t bytes = (((q[e] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7;
+            q[e] &= ~(bytes * 0xffu);
           }
         }
-        nan = __reduce_or_sync(0xffffffffu, nan);
-        if (lane == 0) info.nan[w] = nan;
       }
+      nan = __reduce_or_sync(0xffffffffu, nan);
+      if (lane == 0) info.nan[w] = nan;
+      if (k >= kStages) ok = ok && kv8_wait(&v_empty[s], parity);
+#pragma unroll
+      for (int x = 0; x < kPieces; ++x) store_piece(kt + Smem<D>::kOperand, x, vr[x]);
       to_async_proxy();
-      bar_arrive(&k_full[s]);
-      bar_arrive(&info_full[j % kInfos]);
-      if (j >= kStages) ok = ok && bar_wait(&v_empty[s], parity);
-      store(kt + Smem<D>::kOperand, vr);
-      to_async_proxy();
-      bar_arrive(&v_full[s]);
-      blk[0] = nblk[0], blk[1] = nblk[1], id[0] = nid[0], id[1] = nid[1];
-      if (j + 1 < nt) {
-        load(a.c.k, id, kr);
+      warp_arrive(&v_full[s], lane);
+      here = next;
+      if (next) {
         load(a.c.v, id, vr);
         scales();
-        nblk[0] = block_at(j + 2, 0), nblk[1] = block_at(j + 2, 1);
-        nid[0] = id_at(nblk[0]), nid[1] = id_at(nblk[1]);
+        take();
+        next = find();
       }
     }
   } else {
-    fewer_registers<56>();
     if (warp == 12 && lane == 0) {
-    // ---- the MMAs ----
-    constexpr uint32_t is = idesc_f16(kRows, kKeys, false), io = idesc_f16(kRows, D, true);
-    // descriptors count in 16-byte units: stepping one is an addition
-    uint64_t qd = kmajor_sw128(saddr(sq)), kd = kmajor_sw128(saddr(sk)), vd = rows_sw128(saddr(sk) + Smem<D>::kOperand, kKeys * 128);
-    constexpr uint32_t kStage = 2 * Smem<D>::kOperand / 16;
-    for (int i = 0; i < tiles; ++i) ok = ok && bar_wait(&q_ready[i], 0);
-    tc_fence_after();
-    uint32_t uses0 = 0, uses1 = 0;
-    for (int j = -1; j < nt && ok; ++j) {
-      if (j + 1 < nt) ok = ok && bar_wait(&k_full[(j + 1) % kStages], (uint32_t)((j + 1) / kStages & 1));
-      if (j >= 0) ok = ok && bar_wait(&v_full[j % kStages], (uint32_t)(j / kStages & 1));
-      tc_fence_after();
-      // opaque, or every step's descriptor is kept across the loop and spilled: the issue then waits for
-      // local memory (8 x 2048: PV's 8 MMAs took 2 us to issue instead of 0.3)
-      asm volatile("" : "+l"(qd), "+l"(kd), "+l"(vd));
-      const uint64_t vt = vd + (uint32_t)(j & 1) * kStage, kt = kd + (uint32_t)((j + 1) & 1) * kStage;
+      // ---- the MMAs, by one thread ----
+      constexpr uint32_t is = idesc_f16(kRows, kKeys, false), io = idesc_f16(kRows, D, true);
+      // descriptors count in 16-byte units: stepping one is an addition
+      uint64_t qd = kmajor_sw128(saddr(sq)), kd = kmajor_sw128(saddr(sk)), vd = rows_sw128(saddr(sk) + Smem<D>::kOperand, kKeys * 128);
+      constexpr uint32_t kStage = 2 * Smem<D>::kOperand / 16;
+      uint32_t p_use0 = 0, p_use1 = 0, q_use0 = 0, q_use1 = 0, before = 0;
+      while (const Item* const item = next_item(true)) {
+        const int nt = item->tiles(), b0 = item->begin[0], b1 = item->begin[1], e0 = item->end[0], e1 = item->end[1];
+        for (int j = -1; j < nt && ok; ++j) {
+          const uint32_t now = before + (uint32_t)j, next = now + 1;
+          if (j + 1 < nt) ok = ok && kv8_wait(&k_full[next & 1], next >> 1 & 1);
+          if (j >= 0) ok = ok && kv8_wait(&v_full[now & 1], now >> 1 & 1);
+          // opaque, or every step's descriptor is kept across the loop and spilled: the issue then waits
+          // for local memory (8 x 2048: PV's 8 MMAs took 2 us to issue instead of 0.3)
+          asm volatile("" : "+l"(qd), "+l"(kd), "+l"(vd));
+          const uint64_t vt = vd + (now & 1) * kStage, kt = kd + (next & 1) * kStage;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const Range rg = i ? range1 : range0;
-        uint32_t& uses = i ? uses1 : uses0;
-        const uint32_t s_at = tmem + (uint32_t)(i * 128), o_at = tmem + 256u + (uint32_t)(i * 128);
-        if (rg.has(j)) {
-          ok = ok && bar_wait(&p_ready[i], uses & 1);
-          ++uses;
-          tc_fence_after();
-          const uint32_t later = j > rg.begin;
+          for (int i = 0; i < 2; ++i) {
+            const int begin = i ? b1 : b0, end = i ? e1 : e0;
+            uint32_t &p_use = i ? p_use1 : p_use0, &q_use = i ? q_use1 : q_use0;
+            const uint32_t s_at = tmem + (uint32_t)(i * 128), o_at = tmem + 256u + (uint32_t)(i * 128);
+            if (j >= begin && j < end) {
+              ok = ok && kv8_wait(&p_ready[i], p_use & 1);
+              ++p_use;
+              tc_fence_after();
+              const uint32_t later = j > begin;
 #pragma unroll
-          for (int k = 0; k < kKeys / 16; ++k)  // 16 keys: 8 columns of P, 2 groups of 8 rows of V
-            umma_ts(o_at, s_at + 8u * k, vt + k * (2048 / 16), io, k > 0 ? 1u : later);
-          if (j + 1 == rg.end) umma_commit(&o_full[i]);
-        }
-        if (rg.has(j + 1)) {
-          const uint64_t qt = qd + (uint32_t)(i * Smem<D>::kQ / 16);
+              for (int k = 0; k < kKeys / 16; ++k)  // 16 keys: 8 columns of P, 2 groups of 8 rows of V
+                umma_ts(o_at, s_at + 8u * k, vt + k * (2048 / 16), io, k > 0 ? 1u : later);
+              if (j + 1 == end) {
+                umma_commit(&o_full[i]);
+                bar_arrive(&o_full[i]);
+              }
+            }
+            if (j + 1 >= begin && j + 1 < end) {
+              if (j + 1 == begin) {
+                ok = ok && kv8_wait(&q_ready[i], q_use & 1);
+                ++q_use;
+              }
+              tc_fence_after();
+              const uint64_t qt = qd + (uint32_t)(i * Smem<D>::kQ / 16);
 #pragma unroll
-          for (int k = 0; k < D / 16; ++k) {
-            const uint32_t off = ((k >> 2) * (kRows * 128) + (k & 3) * 32) / 16;  // kRows == kKeys
-            umma_bf16(s_at, qt + off, kt + off, is, k > 0 ? 1u : 0u);
+              for (int k = 0; k < D / 16; ++k) {
+                const uint32_t off = ((k >> 2) * (kRows * 128) + (k & 3) * 32) / 16;  // kRows == kKeys
+                umma_bf16(s_at, qt + off, kt + off, is, k > 0 ? 1u : 0u);
+              }
+              umma_commit(&s_full[i]);
+              bar_arrive(&s_full[i]);
+              if (j + 2 == end) umma_commit(&q_empty[i]);
+            }
           }
-          umma_commit(&s_full[i]);
+          if (j + 1 < nt) umma_commit(&k_empty[next & 1]);
+          if (j >= 0) umma_commit(&v_empty[now & 1]);
         }
+        before += (uint32_t)nt;
       }
-      if (j + 1 < nt) umma_commit(&k_empty[(j + 1) % kStages]);
-      if (j >= 0) umma_commit(&v_empty[j % kStages]);
-    }
+    } else if (warp == 13) {
+      // ---- items ----
+      bool more = true;
+      for (uint32_t r = 0; more && ok; ++r) {
+        Item it;
+        find_item(a, (int64_t)r * gridDim.x + (r & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x), lane, it);
+        if (r >= kItems) ok = ok && kv8_wait(&item_empty[r % kItems], (r / kItems - 1) & 1);
+        if (lane == 0) {
+          items[r % kItems] = it;
+          bar_arrive(&item_full[r % kItems]);
+        }
+        __syncwarp();
+        more = it.seq >= 0;  // a CTA's numbers rise
+      }
     }
   }
   if (!ok) *a.timeout = 1;
+  __syncwarp();
   tc_fence_before();
   __syncthreads();
   if (warp == 12) {
-    __syncwarp();
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
   }
 }
 
-template <int D>
+template <int D, int TYPE>
 int launch_prefill(const AttnArgs& a, int dev, cudaStream_t stream) {
   static bool done[kMaxDevices] = {};
   if (!done[dev]) {
-    J4B_CUDA(cudaFuncSetAttribute(kv8_prefill_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<D>::kBytes), "cudaFuncSetAttribute");
+    J4B_CUDA(cudaFuncSetAttribute(kv8_prefill_kernel<D, TYPE>, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<D>::kBytes), "cudaFuncSetAttribute");
     done[dev] = true;
   }
-  const int64_t rows = a.tokens * a.group, tiles = std::min(rows, rows / (2 * kRows) + a.batch);
-  J4B_REQUIRE(tiles <= 0x7fffffffLL, "kv8 prefill: too many rows");
-  kv8_prefill_kernel<D><<<dim3((unsigned)tiles, (unsigned)a.c.kv_heads), kThreads, Smem<D>::kBytes, stream>>>(a);
+  const int64_t rows = a.tokens * a.group, items = std::min(rows, rows / (2 * kRows) + a.batch) * a.c.kv_heads;
+  J4B_REQUIRE(rows <= 0x3fffffffLL, "kv8 prefill: too many rows");
+  const DeviceCtx* ctx = device_ctx(dev);
+  kv8_prefill_kernel<D, TYPE><<<(unsigned)std::min<int64_t>(items, ctx->sm_count), kThreads, Smem<D>::kBytes, stream>>>(a);
   J4B_CHECK_LAUNCH("kv8_prefill_kernel");
   return J4B_OK;
 }
@@ -666,5 +863,7 @@ extern "C" int j4b_kv8_attention_prefill(const j4b_kv8_cache* cache, int64_t lay
   a.offsets = (const int*)(uintptr_t)offsets;
   DeviceGuard guard(dev);
   cudaStream_t stream = resolve_stream(dev, s);
-  return cache->head_dim == 128 ? launch_prefill<128>(a, dev, stream) : launch_prefill<64>(a, dev, stream);
+  if (q_type == J4B_F32)
+    return cache->head_dim == 128 ? launch_prefill<128, J4B_F32>(a, dev, stream) : launch_prefill<64, J4B_F32>(a, dev, stream);
+  return cache->head_dim == 128 ? launch_prefill<128, J4B_BF16>(a, dev, stream) : launch_prefill<64, J4B_BF16>(a, dev, stream);
 }
