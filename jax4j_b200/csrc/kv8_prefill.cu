@@ -50,9 +50,8 @@ template <int D>
 struct Smem {
   static constexpr int kQ = kRows * D * 2;       // bytes of a query tile
   static constexpr int kOperand = kKeys * D * 2; // of K or V
-  static constexpr int kOut = 8 * 32 * 64;       // output staging: 64 bytes of each row
-  static constexpr int kRaw = kKeys * D;         // codes of the next tile's keys
-  static constexpr int kBytes = 2 * kQ + 2 * kStages * kOperand + kOut + kRaw + kInfos * (int)sizeof(TileInfo) + 1024;
+  static constexpr int kRaw = kKeys * D;         // codes of the next tile's keys, and of its values
+  static constexpr int kBytes = 2 * kQ + 2 * kStages * kOperand + 2 * kRaw + kInfos * (int)sizeof(TileInfo) + 1024;
 };
 
 // kind::f16 with f16 operands; b_rows: B's shared-memory rows run along N (its 16-bit "MN-major" form)
@@ -151,22 +150,19 @@ __device__ __forceinline__ bool sees_nan(const TileInfo& info, const View& view)
   return found != 0;
 }
 
-// Calls work(c, scores) for the four 32-key chunks of a row of scores in TMEM, the next chunk's load
-// in flight meanwhile. The loop stays rolled and the row in TMEM: a row of 128 scores in registers
-// left the kernel spilling and its code beyond the instruction cache (11 local loads a tile and
-// warp, most of them L2 round trips: 750 us for 8 x 2048).
+// Calls work(c, scores) for the four 32-key chunks of a row of scores in TMEM. The loop stays rolled
+// and the row in TMEM: what bounds this kernel is the instruction cache (its misses were the largest
+// of the warps' waits), so every loop of a role is kept short. 8 x 2048 causal took 750 us with a row
+// of 128 scores in registers (spills, too), 514 us with two chunks in turn and the page warps'
+// loops unrolled, 478 us so; chunks of 16 took 538 us, 516 us with the next one's load in flight.
 template <class Work>
 __device__ __forceinline__ void over_row(uint32_t s_at, Work work) {
-  uint32_t v0[32], v1[32];
-  tmem_ld32(s_at, v0);
 #pragma unroll 1
-  for (int c = 0; c < kKeys / 32; c += 2) {
+  for (int c = 0; c < kKeys / 32; ++c) {
+    uint32_t v[32];
+    tmem_ld32(s_at + 32u * c, v);
     tmem_ld_wait();
-    tmem_ld32(s_at + 32u * (c + 1), v1);
-    work(c, v0);
-    tmem_ld_wait();
-    if (c + 2 < kKeys / 32) tmem_ld32(s_at + 32u * (c + 2), v0);
-    work(c + 1, v1);
+    work(c, v);
   }
 }
 
@@ -331,91 +327,70 @@ __device__ __forceinline__ void rescale(uint32_t o_at, float by) {
   }
 }
 
-// A warp's 32 output rows from TMEM: each lane's times its `inv` (zeros where `none`).
+// A lane's output row from TMEM times `inv` (zeros where `none`): 64 or 128 bytes at a time, which
+// fill whole sectors.
 template <int D, int TYPE>
-__device__ __forceinline__ void put_rows(void* out, uint8_t* stage, uint32_t o_at, bool none, float inv, int64_t out_row, int lane) {
-  constexpr int kItem = TYPE == J4B_F32 ? 4 : 2, kCols = 64 / kItem;  // columns of a pass
+__device__ __forceinline__ void put_row(void* out, uint32_t o_at, bool none, float inv, int64_t out_row) {
 #pragma unroll 1
-  for (int c0 = 0; c0 < D; c0 += 32) {
+  for (int c = 0; c < D; c += 32) {
     uint32_t v[32];
-    tmem_ld32(o_at + (uint32_t)c0, v);
+    tmem_ld32(o_at + (uint32_t)c, v);
     tmem_ld_wait();
-    float x[32];
 #pragma unroll
-    for (int e = 0; e < 32; ++e) x[e] = none ? 0.f : __uint_as_float(v[e]) * inv;
+    for (int e = 0; e < 32; ++e) v[e] = none ? 0u : __float_as_uint(__uint_as_float(v[e]) * inv);
+    if (out_row >= 0) {
+      if (TYPE == J4B_F32) {
+        uint4* dst = reinterpret_cast<uint4*>(static_cast<float*>(out) + out_row + c);
 #pragma unroll
-    for (int c = 0; c < 32; c += kCols) {
-      __syncwarp();
+        for (int e = 0; e < 8; ++e) dst[e] = make_uint4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+      } else {
+        uint4* dst = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(out) + out_row + c);
 #pragma unroll
-      for (int e = 0; e < kCols; e += 16 / kItem) {
-        uint32_t w[4];
+        for (int e = 0; e < 4; ++e) {
+          uint32_t w[4];
 #pragma unroll
-        for (int y = 0; y < 4; ++y) {
-          if (TYPE == J4B_F32) {
-            w[y] = __float_as_uint(x[c + e + y]);
-          } else {
-            const __nv_bfloat162 t = __floats2bfloat162_rn(x[c + e + 2 * y], x[c + e + 2 * y + 1]);
+          for (int y = 0; y < 4; ++y) {
+            const __nv_bfloat162 t = __floats2bfloat162_rn(__uint_as_float(v[8 * e + 2 * y]), __uint_as_float(v[8 * e + 2 * y + 1]));
             w[y] = *reinterpret_cast<const uint32_t*>(&t);
           }
+          dst[e] = make_uint4(w[0], w[1], w[2], w[3]);
         }
-        // rows are 64 bytes: two of them cover the banks, so pieces are swizzled by every other row
-        *reinterpret_cast<uint4*>(stage + lane * 64 + (((e * kItem / 16) ^ (lane >> 1 & 3)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
-      }
-      __syncwarp();
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {  // 8 rows x 4 pieces
-        const int qr = 8 * k + (lane >> 2), piece = lane & 3;
-        const int64_t dst = __shfl_sync(0xffffffffu, out_row, qr);
-        if (dst >= 0)
-          *reinterpret_cast<uint4*>(static_cast<uint8_t*>(out) + (dst + c0 + c) * kItem + 16 * piece) =
-              *reinterpret_cast<const uint4*>(stage + qr * 64 + ((piece ^ (qr >> 1 & 3)) << 4));
       }
     }
+    __syncwarp();  // the loads from TMEM are the whole warp's
   }
 }
 
-// A warp's 32 query rows of a tile, 8 lanes a row, 4 rows at a time: `fetch` has the loads in
-// flight while the last item's output is written, `put` brings each row by a power of two to a
-// largest element in [2^11, 2^12), then to f16 (bf16 is exact there), in the tile's swizzled operand.
-// Returns lane's own row's power of two, by which its scores are to be multiplied.
+// A warp's 32 query rows of a tile, 8 lanes a row, into the tile's swizzled operand: each by a power
+// of two to a largest element in [2^11, 2^12), then to f16 (bf16 is exact there). `factors` takes the
+// (biased) exponent of the power of two by which a row's scores are to be multiplied. Rolled: the
+// code runs once an item and would come from beyond the instruction cache every time.
 template <int D, int TYPE>
-struct Queries {
-  static constexpr int kWords = TYPE == J4B_F32 ? D / 32 : D / 64;  // 16-byte pieces of a row and lane
-  static constexpr int kHeld = 8 / kWords;                         // rows of a lane that fetch holds
-  uint4 raw[kHeld][kWords];
-
-  static __device__ __forceinline__ void get(const AttnArgs& a, const Item& it, int i, int warp, int k, int lane, uint4 (&dst)[kWords]) {
-    const int qr = 32 * warp + 4 * k + (lane >> 3), g = it.first_row + i * kRows + qr, row = it.row0 + g / a.group;
-    const bool there = i * kRows + qr < it.rows && row >= 0 && row < a.tokens;
-    const int64_t src = (int64_t)row * a.q_stride + (int64_t)(it.head * a.group + g % a.group) * D + 8 * (lane & 7);
-#pragma unroll
-    for (int c = 0; c < kWords; ++c)
-      dst[c] = !there ? make_uint4(0, 0, 0, 0)
-               : TYPE == J4B_F32 ? load_once(static_cast<const float*>(a.q) + src + 64 * (c >> 1) + 4 * (c & 1))
-                                 : load_once(static_cast<const __nv_bfloat16*>(a.q) + src + 64 * c);
-  }
-  __device__ __forceinline__ void fetch(const AttnArgs& a, const Item* it, int i, int warp, int lane) {
+__device__ __forceinline__ void bring_queries(const AttnArgs& a, const Item& it, int i, int warp, uint8_t* tile, uint8_t* factors, int lane) {
+  constexpr int kWords = TYPE == J4B_F32 ? D / 32 : D / 64;  // 16-byte pieces of a row and lane
+  constexpr int kHeld = 8 / kWords;                          // rows of a lane in flight
+#pragma unroll 1
+  for (int k0 = 0; k0 < 8; k0 += kHeld) {
+    uint4 raw[kHeld][kWords];
 #pragma unroll
     for (int k = 0; k < kHeld; ++k) {
-      if (it) {
-        get(a, *it, i, warp, k, lane, raw[k]);
-      } else {  // all of it set anew, or it would be held through the key tiles
+      const int qr = 32 * warp + 4 * (k0 + k) + (lane >> 3), g = it.first_row + i * kRows + qr, row = it.row0 + g / a.group;
+      const bool there = i * kRows + qr < it.rows && row >= 0 && row < a.tokens;
+      const int64_t src = (int64_t)row * a.q_stride + (int64_t)(it.head * a.group + g % a.group) * D + 8 * (lane & 7);
 #pragma unroll
-        for (int c = 0; c < kWords; ++c) raw[k][c] = make_uint4(0, 0, 0, 0);
-      }
+      for (int c = 0; c < kWords; ++c)
+        raw[k][c] = !there ? make_uint4(0, 0, 0, 0)
+                    : TYPE == J4B_F32 ? load_once(static_cast<const float*>(a.q) + src + 64 * (c >> 1) + 4 * (c & 1))
+                                      : load_once(static_cast<const __nv_bfloat16*>(a.q) + src + 64 * c);
     }
-  }
-  __device__ __forceinline__ float put(const AttnArgs& a, const Item& it, int i, int warp, uint8_t* tile, int lane) {
-    float mine = 1.f;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      if (k >= kHeld) get(a, it, i, warp, k, lane, raw[k % kHeld]);
-      const int qr = 32 * warp + 4 * k + (lane >> 3);
+    for (int k = 0; k < kHeld; ++k) {
+      const int qr = 32 * warp + 4 * (k0 + k) + (lane >> 3);
       float x[D / 8];
       float most = 0.f;
 #pragma unroll
       for (int c = 0; c < kWords; ++c) {
-        const uint32_t w[4] = {raw[k % kHeld][c].x, raw[k % kHeld][c].y, raw[k % kHeld][c].z, raw[k % kHeld][c].w};
+        const uint32_t w[4] = {raw[k][c].x, raw[k][c].y, raw[k][c].z, raw[k][c].w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           if (TYPE == J4B_F32) {
@@ -433,11 +408,8 @@ struct Queries {
       const int e = (int)(__float_as_uint(most) >> 23);
       const bool plain = e < 24 || e > 240;
       float up = plain ? 1.f : __uint_as_float((uint32_t)(254 - (e - 11)) << 23);
-      const float down = plain ? 1.f : __uint_as_float((uint32_t)(e - 11) << 23);
       if (a.scale_log2 < 0.f) up = -up;  // maxima are taken before the factor
-      // row 4 k + x of the warp is handled by lanes 8 x ..: lane 4 k + x takes its factor from there
-      const float theirs = __shfl_sync(0xffffffffu, down, (lane & 3) << 3);
-      if (lane >> 2 == k) mine = theirs;
+      if ((lane & 7) == 0) factors[qr] = (uint8_t)(plain ? 127 : e - 11);
 #pragma unroll
       for (int c = 0; c < D / 64; ++c) {
         const float* y = x + 8 * c;
@@ -445,9 +417,8 @@ struct Queries {
             make_uint4(h2(y[0] * up, y[1] * up), h2(y[2] * up, y[3] * up), h2(y[4] * up, y[5] * up), h2(y[6] * up, y[7] * up));
       }
     }
-    return mine;
   }
-};
+}
 
 constexpr int kItems = 4;         // found ahead
 constexpr int kItemReaders = 13;  // warps
@@ -458,13 +429,13 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const AttnArgs
   uint8_t* smem = aligned_smem(smem_raw);
   uint8_t* sq = smem;                    // [2 tiles]
   uint8_t* sk = smem + 2 * Smem<D>::kQ;  // [stage][K | V]
-  uint8_t* sout = sk + 2 * kStages * Smem<D>::kOperand;
-  uint8_t* sraw = sout + Smem<D>::kOut;
-  TileInfo* infos = reinterpret_cast<TileInfo*>(sraw + Smem<D>::kRaw);
+  uint8_t* sraw = sk + 2 * kStages * Smem<D>::kOperand;
+  TileInfo* infos = reinterpret_cast<TileInfo*>(sraw + 2 * Smem<D>::kRaw);
   __shared__ uint64_t item_full[kItems], item_empty[kItems], q_ready[2], q_empty[2], k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages],
-      s_full[2], p_ready[2], o_full[2];
+      s_full[2], p_ready[2], o_full[2], o_seen[2];
   __shared__ uint32_t tmem_slot;
   __shared__ Item items[kItems];
+  __shared__ uint8_t factors[2][kRows];  // a warp's are its own rows'
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if (tid == 0) {
     for (int i = 0; i < kItems; ++i) {
@@ -477,6 +448,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const AttnArgs
       bar_init(&s_full[i], 2);  // the MMAs, and the thread that saw keys, info and queries ready
       bar_init(&p_ready[i], 4);
       bar_init(&o_full[i], 2);
+      bar_init(&o_seen[i], 4);
     }
     for (int s = 0; s < kStages; ++s) {
       bar_init(&k_full[s], 4);
@@ -513,19 +485,20 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const AttnArgs
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const uint32_t s_at = lanes + (uint32_t)(i * 128), o_at = lanes + 256u + (uint32_t)(i * 128);
     uint32_t use = 0, outs = 0, before = 0;  // tiles done, items done, key tiles of the earlier items
-    Queries<D, TYPE> queries;
     const Item* item = next_item();
-    queries.fetch(a, item, i, warp & 3, lane);
+    // an item's queries, into the tile's operand once the last item's scores are done with it; returns
+    // what the lane's row's scores are to be multiplied by
+    auto bring = [&](const Item& it) -> float {
+      if (outs > 0) ok = ok && kv8_wait(&q_empty[i], (outs - 1) & 1);
+      bring_queries<D, TYPE>(a, it, i, warp & 3, sq + i * Smem<D>::kQ, factors[i], lane);
+      to_async_proxy();
+      warp_arrive(&q_ready[i], lane);
+      return fabsf(a.scale_log2) * __uint_as_float((uint32_t)factors[i][r] << 23);
+    };
+    float factor = item && item->active(i) ? bring(*item) : 0.f;
     while (item) {
       const Item& it = *item;
       const bool active = it.active(i);
-      float factor = 0.f;
-      if (active) {
-        if (outs > 0) ok = ok && kv8_wait(&q_empty[i], (outs - 1) & 1);
-        factor = fabsf(a.scale_log2) * queries.put(a, it, i, warp & 3, sq + i * Smem<D>::kQ, lane);
-        to_async_proxy();
-        warp_arrive(&q_ready[i], lane);
-      }
       const int gr = it.first_row + i * kRows + r, tok = gr / a.group, gh = it.head * a.group + gr % a.group;
       const bool valid = i * kRows + r < it.rows && it.row0 + tok >= 0 && it.row0 + tok < a.tokens;
       const int64_t out_row = valid ? ((int64_t)(it.row0 + tok) * a.heads + gh) * D : -1;
@@ -575,24 +548,23 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const AttnArgs
       const uint32_t last_tile = before + (uint32_t)j1 - 1;
       before += (uint32_t)it.tiles();
       const int rows = it.rows;
+      if (active) ++outs;
       item = next_item();
-      queries.fetch(a, item, i, warp & 3, lane);
-      // the output rows, through shared memory so that the stores are whole: 64 bytes of a row at a
-      // time
+      // the next item's queries first: its scores are computed while this one's output is written
+      factor = item && item->active(i) ? bring(*item) : 0.f;
       if (active) {
-        ok = ok && kv8_wait(&o_full[i], outs & 1);
-        ++outs;
+        ok = ok && kv8_wait(&o_full[i], (outs - 1) & 1);
         tc_fence_after();
         if (sees_nan(infos[last_tile % kInfos], view)) l = NAN;
+        warp_arrive(&o_seen[i], lane);
       }
       if (i * kRows < rows) {
         const bool none = m == -INFINITY;
         const float inv = none ? 0.f : exp2_ftz((float)(eref - kShift)) / l;
-        uint8_t* stage = sout + warp * (32 * 64);
         if (a.out_type == J4B_F32)
-          put_rows<D, J4B_F32>(a.out, stage, o_at, none, inv, out_row, lane);
+          put_row<D, J4B_F32>(a.out, o_at, none, inv, out_row);
         else
-          put_rows<D, J4B_BF16>(a.out, stage, o_at, none, inv, out_row, lane);
+          put_row<D, J4B_BF16>(a.out, o_at, none, inv, out_row);
       }
       tc_fence_before();
     }
@@ -603,23 +575,16 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const AttnArgs
     // piece x: row 32 w + 8 (x / kHalves) + lane / 4, codes 64 (x % kHalves) + 16 (lane % 4): 8 lanes of
     // a store phase are 2 rows x 4 pieces, whose swizzled places cover all banks
     const int pr = lane >> 2, pc = lane & 3;
-    auto load = [&](const uint8_t* codes, const int (&id)[2], uint4 (&dst)[kPieces]) {
-#pragma unroll
-      for (int x = 0; x < kPieces; ++x) {
-        const int row = 8 * (x / kHalves) + pr, k = row >> 4;  // of the warp's 32
-        dst[x] = id[k] < 0 ? make_uint4(0, 0, 0, 0)
-                           : load_once(codes + (int64_t)id[k] * (kKvBlock * D) + (row & 15) * D + 64 * (x % kHalves) + 16 * pc);
-      }
-    };
-    // The keys' codes wait in shared memory, each thread's pieces its own (so its own wait is all they
-    // need): registers for them would be the softmax's.
+    // Codes wait in shared memory, each thread's pieces its own (so its own wait is all they need). The
+    // loops over pieces stay rolled, for the instruction cache.
     const uint32_t mine_at = saddr(sraw) + (uint32_t)(tid & 127) * 16u;
-    auto load_keys = [&](const int (&id)[2]) {
-#pragma unroll
+    auto load = [&](const uint8_t* codes, int which, const int (&id)[2]) {
+#pragma unroll 4
       for (int x = 0; x < kPieces; ++x) {
-        const int row = 8 * (x / kHalves) + pr, k = row >> 4;
-        const uint8_t* src = a.c.k + (int64_t)max(id[k], 0) * (kKvBlock * D) + (row & 15) * D + 64 * (x % kHalves) + 16 * pc;
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(mine_at + x * 2048u), "l"(src), "r"(id[k] < 0 ? 0 : 16) : "memory");
+        const int row = 8 * (x / kHalves) + pr, k = x >= kPieces / 2;
+        const int block = k ? id[1] : id[0];
+        const uint8_t* src = codes + (int64_t)max(block, 0) * (kKvBlock * D) + (row & 15) * D + 64 * (x % kHalves) + 16 * pc;
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(mine_at + (uint32_t)(which * Smem<D>::kRaw) + x * 2048u), "l"(src), "r"(block < 0 ? 0 : 16) : "memory");
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
     };
@@ -665,7 +630,6 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const AttnArgs
       for (int k = 0; k < 2; ++k)
         id[k] = (unsigned)page[k] < (unsigned)a.c.pages ? (page[k] * a.c.kv_heads + head) * a.c.bpp + blk[k] % a.c.bpp : -1;
     };
-    uint4 vr[kPieces];
     float ks = 1.f, vs = 0.f;
     int now[2] = {-1, -1}, now_len = 0;  // first positions of the tile's blocks (-1: not there)
     auto scales = [&] {
@@ -684,8 +648,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const AttnArgs
     bool here = find();
     if (here) {
       number();
-      load_keys(id);
-      load(a.c.v, id, vr);
+      load(a.c.k, 0, id);
+      load(a.c.v, 1, id);
       scales();
       take();
     }
@@ -695,9 +659,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const AttnArgs
       const uint32_t parity = (k / kStages - 1) & 1;
       uint8_t* kt = sk + s * 2 * Smem<D>::kOperand;
       TileInfo& info = infos[k % kInfos];
-      asm volatile("cp.async.wait_group 0;" ::: "memory");
+      asm volatile("cp.async.wait_group 1;" ::: "memory");  // the keys; the values may be on their way
       if (k >= kStages) ok = ok && kv8_wait(&k_empty[s], parity);
-#pragma unroll
+#pragma unroll 4
       for (int x = 0; x < kPieces; ++x) store_piece(kt, x, *reinterpret_cast<const uint4*>(sraw + x * 2048 + (tid & 127) * 16));
       if (lane < 2) {
         const int x = 2 * w + lane, pos = lane == 0 ? now[0] : now[1];
@@ -709,15 +673,22 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const AttnArgs
       warp_arrive(&k_full[s], lane);
       if (next) {
         number();
-        load_keys(id);
+        load(a.c.k, 0, id);
       }
-      // the values' tokens past the length hold anything; NaNs go to the info, as zeros to the operand
+      // the values: one group after theirs is this tile's next keys'
+      if (next)
+        asm volatile("cp.async.wait_group 1;" ::: "memory");
+      else
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+      if (k >= kStages) ok = ok && kv8_wait(&v_empty[s], parity);
+      // tokens past the length hold anything; NaNs go to the info, as zeros to the operand
       unsigned nan = 0;
-#pragma unroll
+#pragma unroll 4
       for (int x = 0; x < kPieces; ++x) {
         const int row = 8 * (x / kHalves) + pr;
-        if (now[row >> 4] + (row & 15) >= now_len) vr[x] = make_uint4(0, 0, 0, 0);
-        uint32_t* q = reinterpret_cast<uint32_t*>(&vr[x]);
+        uint4 v = *reinterpret_cast<const uint4*>(sraw + Smem<D>::kRaw + x * 2048 + (tid & 127) * 16);
+        if ((x >= kPieces / 2 ? now[1] : now[0]) + (row & 15) >= now_len) v = make_uint4(0, 0, 0, 0);
+        uint32_t* q = reinterpret_cast<uint32_t*>(&v);
         uint32_t any = 0;
 #pragma unroll
         for (int e = 0; e < 4; ++e) any |= ((q[e] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
@@ -729,17 +700,15 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const AttnArgs
             q[e] &= ~(bytes * 0xffu);
           }
         }
+        store_piece(kt + Smem<D>::kOperand, x, v);
       }
       nan = __reduce_or_sync(0xffffffffu, nan);
       if (lane == 0) info.nan[w] = nan;
-      if (k >= kStages) ok = ok && kv8_wait(&v_empty[s], parity);
-#pragma unroll
-      for (int x = 0; x < kPieces; ++x) store_piece(kt + Smem<D>::kOperand, x, vr[x]);
       to_async_proxy();
       warp_arrive(&v_full[s], lane);
       here = next;
       if (next) {
-        load(a.c.v, id, vr);
+        load(a.c.v, 1, id);
         scales();
         take();
         next = find();
@@ -753,12 +722,22 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const AttnArgs
       uint64_t qd = kmajor_sw128(saddr(sq)), kd = kmajor_sw128(saddr(sk)), vd = rows_sw128(saddr(sk) + Smem<D>::kOperand, kKeys * 128);
       constexpr uint32_t kStage = 2 * Smem<D>::kOperand / 16;
       uint32_t p_use0 = 0, p_use1 = 0, q_use0 = 0, q_use1 = 0, before = 0;
+      bool left0 = false, left1 = false;  // the last item's softmax may still need its last info
+      uint32_t s_use0 = 0, s_use1 = 0;
       while (const Item* const item = next_item(true)) {
         const int nt = item->tiles(), b0 = item->begin[0], b1 = item->begin[1], e0 = item->end[0], e1 = item->end[1];
         for (int j = -1; j < nt && ok; ++j) {
           const uint32_t now = before + (uint32_t)j, next = now + 1;
           if (j + 1 < nt) ok = ok && kv8_wait(&k_full[next & 1], next >> 1 & 1);
           if (j >= 0) ok = ok && kv8_wait(&v_full[now & 1], now >> 1 & 1);
+          // The second scores of an item free the stage of the tile whose info takes the place of the last
+          // item's last: a softmax that has no part in this item's first tiles may not have read that yet.
+          if (j == 0) {
+            if (left0) ok = ok && kv8_wait(&o_seen[0], s_use0++ & 1);
+            if (left1) ok = ok && kv8_wait(&o_seen[1], s_use1++ & 1);
+            left0 = e0 > b0;
+            left1 = e1 > b1;
+          }
           // opaque, or every step's descriptor is kept across the loop and spilled: the issue then waits
           // for local memory (8 x 2048: PV's 8 MMAs took 2 us to issue instead of 0.3)
           asm volatile("" : "+l"(qd), "+l"(kd), "+l"(vd));
