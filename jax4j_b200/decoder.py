@@ -18,6 +18,10 @@ are slices of the unsharded matrices, quantised along K in 32-column blocks that
 a shard boundary, so the sharded weights are bit-identical to the corresponding parts of the
 single-GPU block.
 
+The cache may instead be the paged 8-bit one (`kv8.Kv8Cache` under a `kv8.PageTable`): half the
+bytes of the decode step's largest traffic, sequences of their own lengths, prompts in chunks, forks
+and a sliding window (`decode_paged`, `prefill_paged`).
+
 Decode (one new token per sequence) runs the projections as batched dequant-GEMVs
 (j4b_quant_matvec, with the residual fused as its `add`); prefill runs them as dequant-GEMMs on
 the tcgen05 tensor cores (j4b_quant_gemm) and attention as the causal flash kernel.
@@ -35,6 +39,7 @@ import torch
 
 from ._lib import call
 from .backend import B200Backend, DeviceBuffer, QuantBuffer
+from .kv8 import PageTable, rope_table
 from .prng import PrngKey
 
 Q4_0 = 2
@@ -130,6 +135,7 @@ class DecoderBlock:
         """`group`: the torch.distributed process group of the ranks sharing the block (default:
         the world group) when the weights are sharded."""
         self.be, self.w, self.eps, self.theta, self.group = backend, weights, eps, theta, group
+        self._rope = None
 
     def _sum_ranks(self, partial: DeviceBuffer) -> DeviceBuffer:
         if self.w.world > 1:
@@ -196,5 +202,53 @@ class DecoderBlock:
         call("j4b_attention_prefill", q.ptr, cache.k.data_ptr(), cache.v.data_ptr(), batch, w.heads,
              HEAD_DIM, cache.capacity, seq, attn.ptr, be.stream)
         h = self._sum_ranks(self._add_residual(be.quant_gemm(w.wo, attn, precision), x))
+        gu = be.quant_gemm(w.wgu, self.rmsnorm(h, w.g_ffn), precision)
+        return self._sum_ranks(self._add_residual(be.quant_gemm(w.wd, self.swiglu(gu), precision), h))
+
+    def _rope_table(self, pages: PageTable) -> torch.Tensor:
+        positions = pages.width * pages.cache.page
+        if self._rope is None or self._rope.shape[0] < positions:
+            self._rope = rope_table(positions, HEAD_DIM, self.theta, pages.cache.device)
+        return self._rope
+
+    def _paged(self, x: DeviceBuffer, pages: PageTable, tokens: int) -> None:
+        cache = pages.cache
+        if cache.head_dim != HEAD_DIM or cache.kv_heads != self.w.heads:
+            raise ValueError("paged cache does not match the head count or the head size")
+        if tokens <= 0:
+            raise ValueError("no new tokens")
+        if x.shape[0] != tokens:
+            raise ValueError(f"x has {x.shape[0]} rows for {tokens} new tokens")
+
+    def decode_paged(self, x: DeviceBuffer, pages: PageTable, window: int = 0, sinks: int = 0, layer: int = 0) -> DeviceBuffer:
+        """One token for each slot of `pages`, x [slots, d] -> [slots, d]: its key and value join the
+        slot's sequence, and attention covers that (with window > 0, the last `window` tokens and
+        the first `sinks`). Layer 0 makes the room for a step's tokens,
+        a model's other layers take it as it is."""
+        be, w = self.be, self.w
+        self._paged(x, pages, pages.slots)
+        starts, lengths, _ = pages.extend([1] * pages.slots) if layer == 0 else pages.step
+        qkv = be.quant_matvec(w.wqkv, self.rmsnorm(x, w.g_attn))
+        q = pages.cache.append(qkv.tensor.view(pages.slots, -1), self._rope_table(pages), pages.table, starts, w.heads, layer=layer)
+        attn = pages.cache.attention_decode(q, pages.table, lengths, window, sinks, layer=layer)
+        h = self._sum_ranks(be.quant_matvec(w.wo, be.wrap(attn.view(pages.slots, -1)), self._residual(x)))
+        gu = be.quant_matvec(w.wgu, self.rmsnorm(h, w.g_ffn))
+        return self._sum_ranks(be.quant_matvec(w.wd, self.swiglu(gu), self._residual(h)))
+
+    def prefill_paged(self, x: DeviceBuffer, pages: PageTable, counts: list, window: int = 0, sinks: int = 0, layer: int = 0,
+                      precision: int = 1) -> DeviceBuffer:
+        """counts[slot] new tokens for each slot (0: none), x [sum of counts, d] slot by slot: whole
+        prompts, or the next chunks of them, of any lengths. Projections on the tensor cores at
+        `precision`; layers as in decode_paged."""
+        be, w = self.be, self.w
+        tokens = sum(counts)
+        self._paged(x, pages, tokens)
+        starts, lengths, offsets = pages.extend(counts) if layer == 0 else pages.step
+        qkv = be.quant_gemm(w.wqkv, self.rmsnorm(x, w.g_attn), precision)
+        q = pages.cache.append(qkv.tensor.view(tokens, -1), self._rope_table(pages), pages.table, starts, w.heads, offsets, layer,
+                               q_dtype=torch.bfloat16)
+        del qkv
+        attn = pages.cache.attention_prefill(q, offsets, pages.table, lengths, window, sinks, layer=layer, out_dtype=torch.float32)
+        h = self._sum_ranks(self._add_residual(be.quant_gemm(w.wo, be.wrap(attn.view(tokens, -1)), precision), x))
         gu = be.quant_gemm(w.wgu, self.rmsnorm(h, w.g_ffn), precision)
         return self._sum_ranks(self._add_residual(be.quant_gemm(w.wd, self.swiglu(gu), precision), h))

@@ -7,19 +7,20 @@ and quantisation of new tokens), `attention_decode` (one query per sequence), `a
 first tokens that stay visible. `PageTable` is the host's bookkeeping for it: which pages a
 sequence has, shared pages of forks, freed pages, compaction.
 
-Launches go to PyTorch's current stream of the cache's device; outputs and the decode workspace
-come from its allocator on that stream. The reference has no KV cache; the functions are stated in
+Launches go to PyTorch's current stream of the cache's device; outputs come from its allocator on
+that stream, and the decode workspace is kept, one per stream. The reference has no KV cache; the functions are stated in
 include/jax4j_b200.h.
 """
 from __future__ import annotations
 
 import ctypes
+import heapq
 
 import torch
 
 from . import _lib
 from ._lib import BF16, F32, call
-from .backend import torch_stream
+from .backend import CUDA_STREAM_LEGACY
 
 BLOCK = 16  # tokens that share a scale
 _TYPES = {torch.float32: F32, torch.bfloat16: BF16}
@@ -32,14 +33,10 @@ def rope_table(positions: int, head_dim: int, theta: float = 10000.0, device=Non
     return torch.stack((angle.cos(), angle.sin()), -1).float()
 
 
-def _type(t: torch.Tensor, what: str) -> int:
-    if t.dtype not in _TYPES:
-        raise ValueError(f"{what} must be float32 or bfloat16, got {t.dtype}")
-    return _TYPES[t.dtype]
-
-
 def _rows(t: torch.Tensor, what: str) -> int:
     """Row stride of a tensor [rows, heads, dim] (or [rows, width]) whose rows are dense."""
+    if t.is_contiguous():
+        return t.stride(0)
     inner = 1
     for size, stride in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
         if size != 1 and stride != inner:
@@ -82,28 +79,52 @@ class Kv8Cache:
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.layers, self.pages, self.kv_heads, self.page, self.head_dim = layers, pages, kv_heads, page, dim
         self.device = k.device
+        self._index = k.device.index if k.device.type == "cuda" else -1
+        self._need = {}  # (heads, batch) -> bytes of the decode workspace
+        self._work = {}  # stream -> workspace
         self._desc = _lib.Kv8CacheDesc(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), layers, pages, kv_heads, page, dim)
         self._ref = ctypes.byref(self._desc)
-        self._workspace = {}  # (heads, batch) -> bytes
 
-    def _ints(self, t: torch.Tensor, what: str, shape: tuple) -> int:
-        if t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous() or t.device != self.device:
-            raise ValueError(f"{what} must be a contiguous int32 tensor {shape} on {self.device}")
+    def _ints(self, t: torch.Tensor, what: str, n: int) -> int:
+        if t.dtype is not torch.int32 or t.dim() != 1 or t.shape[0] != n or t.get_device() != self._index or not t.is_contiguous():
+            raise ValueError(f"{what} must be a contiguous int32 tensor ({n},) on {self.device}")
         return t.data_ptr()
 
     def _table(self, table: torch.Tensor) -> tuple:
-        if table.dtype != torch.int32 or table.dim() != 2 or table.device != self.device or (table.shape[1] > 1 and table.stride(1) != 1):
+        if table.dtype is not torch.int32 or table.dim() != 2 or table.get_device() != self._index or (table.shape[1] > 1 and table.stride(1) != 1):
             raise ValueError(f"the page table must be an int32 tensor [batch, pages of a sequence] on {self.device}, dense within a row")
-        return table.data_ptr(), table.stride(0) if table.shape[0] > 1 else table.shape[1], table.shape[1]
+        batch, width = table.shape
+        return table.data_ptr(), table.stride(0) if batch > 1 else width, width
 
-    def _queries(self, q: torch.Tensor, out: torch.Tensor | None, out_dtype, scale) -> tuple:
-        if q.dim() != 3 or q.shape[2] != self.head_dim or q.device != self.device:
+    def _queries(self, q: torch.Tensor, out: torch.Tensor | None, out_dtype) -> torch.Tensor:
+        if q.dim() != 3 or q.shape[2] != self.head_dim or q.get_device() != self._index:
             raise ValueError(f"q must be [rows, heads, {self.head_dim}] on {self.device}, got {tuple(q.shape)}")
+        if q.dtype not in _TYPES or (out_dtype is not None and out_dtype not in _TYPES):
+            raise ValueError(f"q and the output must be float32 or bfloat16, got {q.dtype} and {out_dtype or q.dtype}")
         if out is None:
-            out = torch.empty(q.shape, dtype=out_dtype or q.dtype, device=self.device)
-        elif out.shape != q.shape or not out.is_contiguous() or out.device != self.device:
-            raise ValueError("out must be contiguous and of q's shape and device")
-        return out, self.head_dim ** -0.5 if scale is None else float(scale)
+            return q.new_empty(q.shape, dtype=out_dtype)
+        if out.shape != q.shape or not out.is_contiguous() or out.get_device() != self._index or out.dtype not in _TYPES:
+            raise ValueError("out must be contiguous, float32 or bfloat16, and of q's shape and device")
+        return out
+
+    def _stream(self) -> int:
+        """The current stream, as backend.torch_stream gives it."""
+        return torch._C._cuda_getCurrentRawStream(self._index) or CUDA_STREAM_LEGACY
+
+    def _workspace(self, heads: int, batch: int, stream: int) -> torch.Tensor:
+        """Of a decode call. One per stream, since calls on different streams may run at the same time;
+        a graph gets one of its own, which lives as long as the graph's memory."""
+        need = self._need.get((heads, batch))
+        if need is None:
+            n = ctypes.c_int64()
+            call("j4b_kv8_decode_workspace", self._ref, heads, batch, ctypes.byref(n))
+            need = self._need[heads, batch] = n.value
+        if torch.cuda.is_current_stream_capturing():
+            return torch.empty(need, dtype=torch.uint8, device=self.device)
+        work = self._work.get(stream)
+        if work is None or work.shape[0] < need:
+            work = self._work[stream] = torch.empty(need, dtype=torch.uint8, device=self.device)
+        return work
 
     def append(self, qkv: torch.Tensor, rope: torch.Tensor, table: torch.Tensor, starts: torch.Tensor, heads: int,
                offsets: torch.Tensor | None = None, layer: int = 0, q_dtype: torch.dtype = torch.float32) -> torch.Tensor:
@@ -113,18 +134,18 @@ class Kv8Cache:
         offsets[b] .. offsets[b + 1] - 1 (no offsets: row b alone) and go to positions starts[b], ...;
         rope f32 [positions, head_dim / 2, 2] (`rope_table`). Returns the rotated queries
         [tokens, heads, head_dim]."""
-        if qkv.dim() != 2 or qkv.dtype != torch.float32 or qkv.shape[1] != (heads + 2 * self.kv_heads) * self.head_dim or qkv.device != self.device:
+        if qkv.dim() != 2 or qkv.dtype != torch.float32 or qkv.shape[1] != (heads + 2 * self.kv_heads) * self.head_dim or qkv.get_device() != self._index:
             raise ValueError(f"qkv must be float32 [tokens, {(heads + 2 * self.kv_heads) * self.head_dim}] on {self.device}")
-        if rope.dim() != 3 or rope.dtype != torch.float32 or tuple(rope.shape[1:]) != (self.head_dim // 2, 2) or not rope.is_contiguous() or rope.device != self.device:
+        if rope.dim() != 3 or rope.dtype != torch.float32 or rope.shape[1] != self.head_dim // 2 or rope.shape[2] != 2 or not rope.is_contiguous() or rope.get_device() != self._index:
             raise ValueError(f"rope must be a contiguous float32 tensor [positions, {self.head_dim // 2}, 2] on {self.device}")
         if q_dtype not in _TYPES:
             raise ValueError(f"q must be float32 or bfloat16, got {q_dtype}")
-        tokens, batch = qkv.shape[0], table.shape[0]
         at, stride, width = self._table(table)
-        q = torch.empty(tokens, heads, self.head_dim, dtype=q_dtype, device=self.device)
+        tokens, batch = qkv.shape[0], table.shape[0]
+        q = qkv.new_empty((tokens, heads, self.head_dim), dtype=q_dtype)
         call("j4b_kv8_append", self._ref, layer, qkv.data_ptr(), _rows(qkv, "qkv"), tokens, heads, rope.data_ptr(), rope.shape[0], at, stride,
-             width, self._ints(starts, "starts", (batch,)), 0 if offsets is None else self._ints(offsets, "offsets", (batch + 1,)), batch,
-             q.data_ptr(), _TYPES[q_dtype], torch_stream(self.device))
+             width, self._ints(starts, "starts", batch), 0 if offsets is None else self._ints(offsets, "offsets", batch + 1), batch,
+             q.data_ptr(), _TYPES[q_dtype], self._stream())
         return q
 
     def attention_decode(self, q: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, window: int = 0, sinks: int = 0,
@@ -133,20 +154,17 @@ class Kv8Cache:
         """softmax(scale q k^T) v of one query per sequence, q [batch, heads, head_dim], at position
         lengths[b] - 1 over its cached tokens (with window > 0: the last `window` and the first
         `sinks`). Sequences that see nothing give zeros."""
-        batch, heads = table.shape[0], q.shape[1] if q.dim() == 3 else 0
-        out, scale = self._queries(q, out, out_dtype, scale)
-        if q.shape[0] != batch:
-            raise ValueError(f"q has {q.shape[0]} rows for {batch} sequences")
+        out = self._queries(q, out, out_dtype)
         at, stride, width = self._table(table)
-        if (heads, batch) not in self._workspace:
-            n = ctypes.c_int64()
-            call("j4b_kv8_decode_workspace", self._ref, heads, batch, ctypes.byref(n))
-            self._workspace[heads, batch] = n.value
-        n = self._workspace[heads, batch]
-        work = torch.empty(n, dtype=torch.uint8, device=self.device)
-        call("j4b_kv8_attention_decode", self._ref, layer, q.data_ptr(), _type(q, "q"), _rows(q, "q"), heads, at, stride, width,
-             self._ints(lengths, "lengths", (batch,)), batch, window, sinks, scale, out.data_ptr(), _type(out, "out"), work.data_ptr(), n,
-             torch_stream(self.device))
+        rows, heads, _ = q.shape
+        batch = table.shape[0]
+        if rows != batch:
+            raise ValueError(f"q has {rows} rows for {batch} sequences")
+        stream = self._stream()
+        work = self._workspace(heads, batch, stream)
+        call("j4b_kv8_attention_decode", self._ref, layer, q.data_ptr(), _TYPES[q.dtype], _rows(q, "q"), heads, at, stride, width,
+             self._ints(lengths, "lengths", batch), batch, window, sinks, self.head_dim ** -0.5 if scale is None else scale, out.data_ptr(),
+             _TYPES[out.dtype], work.data_ptr(), work.shape[0], stream)
         return out
 
     def attention_prefill(self, q: torch.Tensor, offsets: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, window: int = 0,
@@ -155,12 +173,13 @@ class Kv8Cache:
         """Causal attention of ragged chunks: sequence b's queries, the rows offsets[b] ..
         offsets[b + 1] - 1 of q [tokens, heads, head_dim], are its last tokens (lengths[b] counts
         them). Window, sinks and empty rows as in attention_decode."""
-        batch, heads = table.shape[0], q.shape[1] if q.dim() == 3 else 0
-        out, scale = self._queries(q, out, out_dtype, scale)
+        out = self._queries(q, out, out_dtype)
         at, stride, width = self._table(table)
-        call("j4b_kv8_attention_prefill", self._ref, layer, q.data_ptr(), _type(q, "q"), _rows(q, "q"), q.shape[0], heads,
-             self._ints(offsets, "offsets", (batch + 1,)), at, stride, width, self._ints(lengths, "lengths", (batch,)), batch, window, sinks,
-             scale, out.data_ptr(), _type(out, "out"), torch_stream(self.device))
+        rows, heads, _ = q.shape
+        batch = table.shape[0]
+        call("j4b_kv8_attention_prefill", self._ref, layer, q.data_ptr(), _TYPES[q.dtype], _rows(q, "q"), rows, heads,
+             self._ints(offsets, "offsets", batch + 1), at, stride, width, self._ints(lengths, "lengths", batch), batch, window, sinks,
+             self.head_dim ** -0.5 if scale is None else scale, out.data_ptr(), _TYPES[out.dtype], self._stream())
         return out
 
     def copy_pages(self, src: list, dst: list, tokens: list | None = None) -> None:
@@ -171,4 +190,139 @@ class Kv8Cache:
         if len(dst) != n or (tokens is not None and len(tokens) != n):
             raise ValueError("src, dst and tokens must have one entry per move")
         ints = ctypes.c_int32 * n
-        call("j4b_kv8_copy_pages", self._ref, n, ints(*src), ints(*dst), None if tokens is None else ints(*tokens), torch_stream(self.device))
+        call("j4b_kv8_copy_pages", self._ref, n, ints(*src), ints(*dst), None if tokens is None else ints(*tokens), self._stream())
+
+
+class PageTable:
+    """The host's bookkeeping of a `Kv8Cache`: `slots` sequences of up to `max_tokens` tokens, each a list
+    of pages in token order. Full pages of a fork are shared (counted), its partly filled last page
+    is copied. The device sees it through `table` (int32 [slots, pages of a sequence], -1: none)
+    and the arrays that `extend` returns."""
+
+    def __init__(self, cache: Kv8Cache, slots: int, max_tokens: int):
+        if slots <= 0 or max_tokens <= 0:
+            raise ValueError("slots and max_tokens must be positive")
+        self.cache, self.slots = cache, slots
+        self.width = -(-max_tokens // cache.page)
+        self.pages = [[] for _ in range(slots)]  # -1: freed by trim
+        self.lengths = [0] * slots
+        self.refs = [0] * cache.pages
+        self._free = list(range(cache.pages))  # a heap: the lowest page first, so what is in use stays low
+        self.table = torch.full((slots, self.width), -1, dtype=torch.int32, device=cache.device)
+        self._dirty = False
+        self.step = None  # what the last extend returned, for a model's other layers
+
+    def _slot(self, slot: int) -> int:
+        if not 0 <= slot < self.slots:
+            raise ValueError(f"slot {slot} outside [0, {self.slots})")
+        return slot
+
+    def _take(self, n: int) -> list:
+        if n > len(self._free):
+            raise MemoryError(f"{n} pages are needed and {len(self._free)} are free")
+        got = [heapq.heappop(self._free) for _ in range(n)]
+        for p in got:
+            self.refs[p] = 1
+        return got
+
+    def _drop(self, page: int) -> None:
+        if page < 0:
+            return
+        self.refs[page] -= 1
+        if self.refs[page] == 0:
+            heapq.heappush(self._free, page)
+
+    @property
+    def free_pages(self) -> int:
+        return len(self._free)
+
+    def extend(self, counts: list) -> tuple:
+        """Room for counts[slot] new tokens in each slot. Returns device int32 arrays (starts, lengths,
+        offsets): where each slot's new tokens begin, its length with them, and the rows of the new
+        tokens, slot by slot. Raises MemoryError, changing nothing, where pages do not suffice."""
+        if len(counts) != self.slots or any(n < 0 for n in counts):
+            raise ValueError(f"one count for each of {self.slots} slots, none negative")
+        page = self.cache.page
+        need = [max(0, -(-(m + n) // page) - len(p)) for m, n, p in zip(self.lengths, counts, self.pages)]
+        for slot, (m, n) in enumerate(zip(self.lengths, counts)):
+            if m + n > self.width * page:
+                raise ValueError(f"slot {slot} holds at most {self.width * page} tokens, {m} + {n} asked for")
+        fresh = self._take(sum(need))
+        starts = list(self.lengths)
+        for slot, n in enumerate(need):
+            if n:
+                self.pages[slot] += fresh[:n]
+                del fresh[:n]
+                self._dirty = True
+            self.lengths[slot] += counts[slot]
+        self._upload()
+        offsets = [0]
+        for n in counts:
+            offsets.append(offsets[-1] + n)
+        packed = torch.tensor(starts + self.lengths + offsets, dtype=torch.int32).to(self.cache.device)
+        self.step = packed[:self.slots], packed[self.slots:2 * self.slots], packed[2 * self.slots:]
+        return self.step
+
+    def _upload(self) -> None:
+        if self._dirty:
+            rows = [p + [-1] * (self.width - len(p)) for p in self.pages]
+            self.table.copy_(torch.tensor(rows, dtype=torch.int32))
+            self._dirty = False
+
+    def release(self, slot: int) -> None:
+        """Ends a slot's sequence: its pages that no other shares are free again."""
+        for p in self.pages[self._slot(slot)]:
+            self._drop(p)
+        self.pages[slot], self.lengths[slot], self._dirty = [], 0, True
+
+    def trim(self, window: int, sinks: int = 0) -> int:
+        """Frees the pages that no later query sees under a window with sinks; returns how many."""
+        if window <= 0 or sinks < 0:
+            raise ValueError("trim needs a positive window and no negative sinks")
+        page, freed = self.cache.page, len(self._free)
+        for slot in range(self.slots):
+            first = self.lengths[slot] - window + 1  # of the next query's window
+            for i in range(-(-sinks // page), max(0, first) // page):
+                if self.pages[slot][i] >= 0:
+                    self._drop(self.pages[slot][i])
+                    self.pages[slot][i] = -1
+                    self._dirty = True
+        return len(self._free) - freed
+
+    def fork(self, parent: int, children: list) -> None:
+        """Makes each child (a slot without a sequence) a copy of the parent's sequence: full pages are
+        shared, the partly filled last one is copied, in every layer, by one call."""
+        self._slot(parent)
+        for c in children:
+            if self.pages[self._slot(c)] or c == parent:
+                raise ValueError(f"slot {c} is in use")
+        if len(set(children)) != len(children):
+            raise ValueError("a slot is named twice")
+        rest = self.lengths[parent] % self.cache.page
+        shared, last = (self.pages[parent][:-1], self.pages[parent][-1]) if rest else (self.pages[parent], -1)
+        fresh = self._take(len(children)) if last >= 0 else []
+        for i, c in enumerate(children):
+            for p in shared:
+                if p >= 0:
+                    self.refs[p] += 1
+            self.pages[c] = list(shared) + ([fresh[i]] if last >= 0 else [])
+            self.lengths[c] = self.lengths[parent]
+        if fresh:
+            self.cache.copy_pages([last] * len(children), fresh, [rest] * len(children))
+        self._dirty = True
+
+    def compact(self) -> int:
+        """Moves pages so that the ones in use are the lowest (a pool that can then be cut, or saved
+        whole); returns how many moved."""
+        used = sum(r > 0 for r in self.refs)
+        src = [p for p in range(used, self.cache.pages) if self.refs[p] > 0]
+        dst = [p for p in range(used) if self.refs[p] == 0]
+        if src:
+            self.cache.copy_pages(src, dst)
+            to = dict(zip(src, dst))
+            self.pages = [[to.get(p, p) for p in pages] for pages in self.pages]
+            for a, b in to.items():
+                self.refs[b], self.refs[a] = self.refs[a], 0
+            self._free = list(range(used, self.cache.pages))  # ascending: a heap
+            self._dirty = True
+        return len(src)

@@ -79,3 +79,96 @@ def test_rope_table_holds_cos_and_sin():
     t = rope_table(50, 64, 500.0).double().numpy()
     ang = np.arange(50)[:, None] * 500.0 ** (-2.0 * np.arange(32) / 64)
     assert np.abs(t[..., 0] - np.cos(ang)).max() < 1e-7 and np.abs(t[..., 1] - np.sin(ang)).max() < 1e-7
+
+
+class FakeCache:
+    """A cache's sizes without its device; page copies are noted."""
+    def __init__(self, pages, page):
+        self.pages, self.page, self.device, self.copies = pages, page, torch.device("cpu"), []
+
+    def copy_pages(self, src, dst, tokens=None):
+        assert len(set(dst)) == len(dst) and not set(src) & set(dst)
+        self.copies.append((list(src), list(dst), tokens))
+
+
+def _consistent(t):
+    """Every page is free or counted as often as sequences name it; the device's table is the host's."""
+    named = [p for pages in t.pages for p in pages if p >= 0]
+    for p in range(t.cache.pages):
+        assert t.refs[p] == named.count(p)
+        assert (p in t._free) == (t.refs[p] == 0)
+    t._upload()
+    for row, pages in zip(t.table.tolist(), t.pages):
+        assert row == pages + [-1] * (t.width - len(pages))
+
+
+def test_page_table_extends_and_releases():
+    from jax4j_b200.kv8 import PageTable
+    t = PageTable(FakeCache(6, 32), 3, 100)
+    assert t.width == 4
+    starts, lengths, offsets = t.extend([33, 0, 1])
+    assert (starts.tolist(), lengths.tolist(), offsets.tolist()) == ([0, 0, 0], [33, 0, 1], [0, 33, 33, 34])
+    assert [len(p) for p in t.pages] == [2, 0, 1] and t.free_pages == 3
+    _consistent(t)
+    starts, lengths, _ = t.extend([31, 64, 0])  # the first fills its second page
+    assert starts.tolist() == [33, 0, 1] and lengths.tolist() == [64, 64, 1] and t.free_pages == 1
+    with pytest.raises(MemoryError, match="2 pages are needed and 1 are free"):
+        t.extend([1, 1, 0])
+    assert t.lengths == [64, 64, 1] and t.free_pages == 1
+    with pytest.raises(ValueError, match="at most 128 tokens"):
+        t.extend([65, 0, 0])
+    with pytest.raises(ValueError, match="one count"):
+        t.extend([1, 1])
+    t.release(1)
+    _consistent(t)
+    assert t.lengths[1] == 0 and t.free_pages == 3
+    with pytest.raises(ValueError, match="slot 3"):
+        t.release(3)
+
+
+def test_page_table_forks_share_full_pages_and_copy_the_last():
+    from jax4j_b200.kv8 import PageTable
+    t = PageTable(FakeCache(8, 16), 4, 64)
+    t.extend([40, 0, 0, 0])
+    t.fork(0, [1, 3])
+    assert t.cache.copies == [([t.pages[0][2]] * 2, [t.pages[1][2], t.pages[3][2]], [8, 8])]
+    assert t.pages[1][:2] == t.pages[0][:2] == t.pages[3][:2] and len({t.pages[s][2] for s in (0, 1, 3)}) == 3
+    assert t.lengths == [40, 40, 0, 40] and [t.refs[p] for p in t.pages[0]] == [3, 3, 1]
+    _consistent(t)
+    t.release(0)
+    _consistent(t)
+    with pytest.raises(ValueError, match="in use"):
+        t.fork(1, [3])
+    with pytest.raises(ValueError, match="named twice"):
+        t.fork(1, [0, 0])
+    t.extend([0, 8, 0, 0])  # 48 tokens: a whole number of pages, nothing to copy
+    copies = len(t.cache.copies)
+    t.fork(1, [2])
+    assert len(t.cache.copies) == copies and t.pages[2] == t.pages[1]
+    _consistent(t)
+
+
+def test_page_table_trims_a_window_and_compacts():
+    from jax4j_b200.kv8 import PageTable
+    t = PageTable(FakeCache(20, 16), 2, 200)
+    t.extend([150, 30])
+    # the next query of slot 0 is at 150 and sees 111 .. 150 and the first 20: pages 2 .. 5 are not needed
+    assert t.trim(40, 20) == 4
+    assert [i for i, p in enumerate(t.pages[0]) if p < 0] == [2, 3, 4, 5]
+    assert t.trim(40, 20) == 0
+    _consistent(t)
+    before = [list(p) for p in t.pages]
+    moved = t.compact()
+    used = 20 - t.free_pages
+    assert moved > 0 and t.cache.copies[-1][2] is None
+    assert all(p < used for pages in t.pages for p in pages)
+    src, dst, _ = t.cache.copies[-1]
+    to = dict(zip(src, dst))
+    assert [[to.get(p, p) for p in pages] for pages in before] == t.pages
+    _consistent(t)
+    assert t.compact() == 0
+    t.release(0)
+    t.extend([1, 1])
+    _consistent(t)
+    with pytest.raises(ValueError, match="positive window"):
+        t.trim(0)

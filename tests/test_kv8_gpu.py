@@ -427,3 +427,88 @@ def test_refusals():
     empty = cache.attention_decode(torch.zeros(0, 4, 128, device="cuda"), table[:0], n[:0])
     assert empty.shape == (0, 4, 128)
     cache.copy_pages([], [])
+
+
+def test_prefill_keeps_nan_values_from_the_queries_before_them():
+    """A NaN among the values makes NaN of the queries that see it, and of no other: those before it
+    (causal, in the same tile) and those whose window has passed it."""
+    rng = np.random.default_rng(23)
+    n, window = 300, 60
+    for w in (0, window):
+        pool, offsets, q = prefill_inputs(rng, [(0, n)], 4, 2, 128, 32, torch.bfloat16)
+        for at in (150, 290):
+            pool.cache.v.view(torch.uint8)[0, int(pool.table[0, at // 32]), 1, at % 32, 7] = 0xff
+        got = pool.cache.attention_prefill(q, ints(offsets), ints(pool.table), ints(pool.lengths), window=w)
+        bad = torch.isnan(got[:, 2:]).any(-1).cpu().numpy()  # heads of kv head 1
+        pos = np.arange(n)
+        sees = (pos >= 150) & ((w == 0) | (pos < 150 + window)) | (pos >= 290)
+        assert np.array_equal(bad[:, 0], sees) and np.array_equal(bad[:, 1], sees)
+        assert torch.isfinite(got[:, :2]).all()
+        ref = pool.reference(q.double().cpu().numpy()[:150], 0, 0, w, 0)
+        assert normwise(got[:150].double().cpu().numpy(), ref) <= PREFILL_BAR
+
+
+@pytest.mark.parametrize("spans", [[(0, 1)] * 3, [(1000, 1), (0, 500), (3, 2)], [(0, 1300)], [(31, 1), (0, 0), (500, 600), (7, 257), (0, 256), (0, 255)]])
+def test_prefill_many_items_and_tiles(spans):
+    """Enough rows for several items of 256 a sequence, and for CTAs that take more than one."""
+    rng = np.random.default_rng(sum(n for _, n in spans))
+    pool, offsets, q = prefill_inputs(rng, spans, 24, 8, 64, 32, torch.bfloat16)
+    got = pool.cache.attention_prefill(q, ints(offsets), ints(pool.table), ints(pool.lengths)).double().cpu().numpy()
+    qh = q.double().cpu().numpy()
+    for b, (past, n) in enumerate(spans):
+        for i in sorted({0, n // 3, n - 1} if n else ()):
+            row = offsets[b] + i
+            assert normwise(got[row], pool.reference(qh[row:row + 1], b, past + i, 0, 0)[0]) <= PREFILL_BAR, (b, i)
+
+
+def test_decoder_block_on_the_paged_cache(backend):
+    """Prompts in chunks, a fork, a window that frees pages, then decode steps, through DecoderBlock.
+    The engine's cache holds the float64 oracle's keys and values within the format's rounding (and
+    the projections' bar); attention over what it holds and the rest of the block are the oracle's,
+    at the block's bars: 1e-2 for prefill, 1e-4 for decode."""
+    from jax4j_b200.decoder import DecoderBlock, DecoderWeights
+    from jax4j_b200.kv8 import Kv8Cache, PageTable
+    from jax4j_b200.prng import PrngKey
+    from oracle import kv8 as O
+    from oracle.decoder import Block, rope
+    d, heads, ffn, window, sinks = 256, 2, 512, 48, 5
+    w = DecoderWeights.random(backend, d, heads, ffn, PrngKey.of(7), keep_blobs=True)
+    ref = Block({k: v.cpu().numpy() for k, v in w.blobs.items()}, d, heads, ffn, backend.download(w.g_attn), backend.download(w.g_ffn))
+    block, rng = DecoderBlock(backend, w), np.random.default_rng(41)
+    cache = Kv8Cache(24, heads, 32, 128)
+    pages = PageTable(cache, 4, 300)
+
+    def check(x, counts, out, bar):
+        q, k, v = ref.qkv(x)
+        kh, vh = (O.values(c[0].double().cpu().numpy(), s[0].double().cpu().numpy()) for c, s in ((cache.k, cache.k_scale), (cache.v, cache.v_scale)))
+        attn, row = np.zeros((len(x), heads, 128)), 0
+        for slot, n in enumerate(counts):
+            first = pages.lengths[slot] - n
+            pos = np.broadcast_to(first + np.arange(n)[:, None], (n, heads))
+            rows = slice(row, row + n)
+            qr, kr = rope(q[rows], pos, 10000.0), rope(k[rows], pos, 10000.0)
+            for i in range(n):
+                page, at = pages.pages[slot][(first + i) // 32], (first + i) % 32
+                for got, want, scales in ((kh[page, :, at], kr[i], cache.k_scale), (vh[page, :, at], v[rows][i], cache.v_scale)):
+                    step = np.maximum(np.abs(want) * 2.0 ** -4, scales[0, page, :, at // 16].cpu().numpy()[:, None] * 2.0 ** -9)
+                    assert np.all(np.abs(got - want) <= step + bar * np.abs(want).max())
+            attn[rows] = O.attention(qr, kh, vh, pages.pages[slot], pages.lengths[slot], first, window, sinks)
+            row += n
+        assert normwise(out, ref.finish(x, attn.reshape(len(x), d))) <= bar
+
+    for counts in ([37, 0, 70, 0], [5, 16, 1, 0], [0, 100, 0, 0]):
+        x = rng.standard_normal((sum(counts), d)).astype(np.float32)
+        out = backend.download(block.prefill_paged(backend.upload(x, x.shape), pages, counts, window, sinks, precision=2))
+        check(x, counts, out, 1e-2)
+    pages.fork(1, [3])
+    for step in range(4):
+        x = rng.standard_normal((4, d)).astype(np.float32)
+        out = backend.download(block.decode_paged(backend.upload(x, x.shape), pages, window, sinks))
+        check(x, [1] * 4, out, 1e-4)
+        if step == 1:
+            assert pages.trim(window, sinks) > 0
+        if step == 2:
+            pages.release(0)
+            assert pages.compact() >= 0
+    with pytest.raises(ValueError, match="rows for"):
+        block.decode_paged(backend.upload(np.zeros((3, d), np.float32), (3, d)), pages)
