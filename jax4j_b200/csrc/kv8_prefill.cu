@@ -10,7 +10,7 @@
 //   O_i += P_i V    (P from TMEM, V f16 codes in shared memory, dims contiguous)    -> TMEM
 // Scales never touch the operands: a block's key scale multiplies its scores, and its value scale,
 // over the largest seen, is the w of its probabilities (both powers of two). The running maximum m
-// moves only when a row outgrows it by 2^kLazy, so O is seldom rescaled.
+// moves only when f16 would not hold a row's probabilities, so O is seldom rescaled.
 //
 // Warps: 0-3 and 4-7 queries, softmax and output of tile 0 and 1; 8-11 bring pages: each thread loads
 // 16-code pieces of the next tile while it turns this one's into the swizzled f16 operands; 12 issues
@@ -34,9 +34,11 @@ constexpr int kKeys = 128;           // of a key tile
 constexpr int kTileBlocks = kKeys / kKvBlock;
 constexpr int kThreads = 14 * 32;
 constexpr int kStages = 2;           // of K and of V (their parity is counted with & 1)
-constexpr int kInfos = 4;            // of what is known of a key tile: the softmax may be two behind
-constexpr float kLazy = 5.f;         // log2: P <= 2^(kShift + kLazy) = 2^15, inside f16
-constexpr int kShift = 10;           // log2: keeps f16's bits for blocks of small value scale
+constexpr int kInfos = 8;            // of what is known of a key tile: the softmax may be some behind
+constexpr float kMost = 65504.f;     // f16's largest
+// log2 of the probability that stands for 1. Above it is room for a maximum outgrown 2^12 times; below
+// it f16 has all its bits down to 2^-18 and some to 2^-28, for far keys and blocks of small value scale.
+constexpr int kShift = 4;
 
 // What the softmax needs of a key tile.
 struct __align__(16) TileInfo {
@@ -66,11 +68,35 @@ __device__ __forceinline__ uint64_t rows_sw128(uint32_t at, uint32_t n_stride) {
 }
 // A from TMEM
 __device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-  const uint32_t z = 0;
   asm volatile(
       "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n}\n" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(z));
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate));
+}
+__device__ __forceinline__ void umma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate));
+}
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.b32 %0, 1, 0, p;\n}\n" : "=r"(p));
+  return p != 0;
+}
+
+__device__ __forceinline__ void tmem_ld16(uint32_t addr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(addr));
+}
+
+__device__ __forceinline__ uint32_t mul2h(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
 }
 
 __device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t (&r)[32]) {
@@ -83,15 +109,6 @@ __device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t (&r)[32]) {
         "=r"(r[30]), "=r"(r[31])
       : "r"(addr));
 }
-__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, "
-      "%19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};\n" ::"r"(r[0]),
-      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]),
-      "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
-      "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(addr)
-      : "memory");
-}
 __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};\n" ::"r"(r[0]),
@@ -99,11 +116,23 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]
       "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(addr)
       : "memory");
 }
+__device__ __forceinline__ void store_shared(uint32_t at, const uint4& v) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+// acc + 0 * v in f16x2
+__device__ __forceinline__ uint32_t zeros_of(const uint4& v, uint32_t acc) {
+  const uint32_t z = 0;
+  asm("fma.rn.f16x2 %0, %1, %2, %0;" : "+r"(acc) : "r"(v.x), "r"(z));
+  asm("fma.rn.f16x2 %0, %1, %2, %0;" : "+r"(acc) : "r"(v.y), "r"(z));
+  asm("fma.rn.f16x2 %0, %1, %2, %0;" : "+r"(acc) : "r"(v.z), "r"(z));
+  asm("fma.rn.f16x2 %0, %1, %2, %0;" : "+r"(acc) : "r"(v.w), "r"(z));
+  return acc;
+}
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void to_async_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-// 16 bytes that are read once: past L1, which shared memory leaves little of and the spilled registers need
+// 16 bytes that are read once: past L1, which shared memory leaves little of
 __device__ __forceinline__ uint4 load_once(const void* p) {
   uint4 v;
   asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
@@ -150,60 +179,55 @@ __device__ __forceinline__ bool sees_nan(const TileInfo& info, const View& view)
   return found != 0;
 }
 
-// Calls work(c, scores) for the four 32-key chunks of a row of scores in TMEM. The loop stays rolled
-// and the row in TMEM: what bounds this kernel is the instruction cache (its misses were the largest
-// of the warps' waits), so every loop of a role is kept short. 8 x 2048 causal took 750 us with a row
-// of 128 scores in registers (spills, too), 514 us with two chunks in turn and the page warps'
-// loops unrolled, 478 us so; chunks of 16 took 538 us, 516 us with the next one's load in flight.
-template <class Work>
-__device__ __forceinline__ void over_row(uint32_t s_at, Work work) {
+// Columns of TMEM of a warp's rows times a factor of each: f32, or pairs of f16.
+template <bool HALF>
+__device__ __forceinline__ void rescale(uint32_t at, int columns, float by) {
+  const uint32_t by2 = h2(by, by);
 #pragma unroll 1
-  for (int c = 0; c < kKeys / 32; ++c) {
-    uint32_t v[32];
-    tmem_ld32(s_at + 32u * c, v);
+  for (int c = 0; c < columns; c += 16) {
+    uint32_t v[16];
+    tmem_ld16(at + (uint32_t)c, v);
     tmem_ld_wait();
-    work(c, v);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) v[e] = HALF ? mul2h(v[e], by2) : __float_as_uint(__uint_as_float(v[e]) * by);
+    tmem_st16(at + (uint32_t)c, v);
   }
+  tmem_st_wait();
 }
 
-// The largest score of a row, times its factor. ALL: it sees the whole tile.
-template <bool ALL>
-__device__ __forceinline__ float row_max(uint32_t s_at, const TileInfo& info, const View& view, float factor) {
-  float mx = -INFINITY;
-  over_row(s_at, [&](int c, const uint32_t (&v)[32]) {
+
+// A row of scores becomes a row of probabilities, in f16 and over them, in one pass: 32 keys at a time,
+// each block's weighed by its value scale, their sum without the weights added to l. ALL: the row sees
+// the whole tile.
+//
+// No maximum is taken on the way: the last one stands until a chunk's sum shows that f16 would not
+// hold its probabilities (or the row has none yet). The chunk's maximum is then found, what was made
+// with the old one is brought to it, and the chunk done again. A maximum of every chunk beforehand
+// cost a third of the pass (16 lanes' maxima a clock and a second read of the scores: 8 x 2048 causal
+// 440 us against 414). With kShift 10 a chunk in nine was done again (539 us), with 4 hardly any.
+//
+// The loop stays rolled and short: its misses in the instruction cache cost more than a longer
+// loop's parallelism gains (64 keys at a time: 491 us).
+template <int D, bool ALL>
+__device__ __forceinline__ void row_pass(uint32_t s_at, uint32_t o_at, const TileInfo& info, const View& view, float factor, bool begin, int eref, float& m, float& l) {
+  bool again = false;
+#pragma unroll 1
+  for (int c = 0; c < kKeys / 32;) {
+    uint32_t v[32], p[16], seen = 0;
+    tmem_ld32(s_at + 32u * c, v);
+    const float2 ks = *reinterpret_cast<const float2*>(info.ks + 2 * c);
+    const int2 ev = *reinterpret_cast<const int2*>(info.ev + 2 * c);
+    const float base = m == -INFINITY ? 0.f : m;
+    float total = 0.f, part = 0.f;
+    tmem_ld_wait();
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const uint32_t* x = v + 16 * h;
-      const float f = factor * info.ks[2 * c + h];
-      float t = -INFINITY;
-      if (ALL) {
-#pragma unroll
-        for (int e = 0; e < 16; e += 2) t = fmaxf(t, fmaxf(__uint_as_float(x[e]), __uint_as_float(x[e + 1])));
-      } else {
-        const uint32_t see = view.mask(info.pos[2 * c + h]);
-#pragma unroll
-        for (int e = 0; e < 16; ++e) t = fmaxf(t, see >> e & 1 ? __uint_as_float(x[e]) : -INFINITY);
-      }
-      mx = fmaxf(mx, t == -INFINITY ? t : t * f);
-    }
-  });
-  return mx;
-}
-
-// The probabilities, in f16, each block's weighed by its value scale, go over the scores in TMEM;
-// returns their sum without the weights.
-template <bool ALL>
-__device__ __forceinline__ float row_exp(uint32_t s_at, const TileInfo& info, const View& view, float factor, float base, int eref) {
-  float l = 0.f;
-  over_row(s_at, [&](int c, const uint32_t (&v)[32]) {
-    uint32_t p[16];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const uint32_t* x = v + 16 * h;
-      const float f = factor * info.ks[2 * c + h];
-      const int w = max(-60, info.ev[2 * c + h] - eref) + kShift;
+      const float f = factor * (h ? ks.y : ks.x);
+      const int w = max(-60, (h ? ev.y : ev.x) - eref) + kShift;
+      const uint32_t see = ALL ? 0xffffu : view.mask(info.pos[2 * c + h]);
+      seen |= see;
       const uint64_t ff = pair(f, f), add = pair((float)w - base, (float)w - base);
-      const uint32_t see = ALL ? 0 : view.mask(info.pos[2 * c + h]);
       uint64_t sum = 0;
 #pragma unroll
       for (int e = 0; e < 16; e += 2) {
@@ -217,12 +241,38 @@ __device__ __forceinline__ float row_exp(uint32_t s_at, const TileInfo& info, co
         sum = add2(sum, pair(y.x, y.y));
         p[8 * h + e / 2] = h2(y.x, y.y);
       }
-      const float2 t = unpair(sum);
-      l = fmaf(t.x + t.y, __uint_as_float((uint32_t)(127 - w) << 23), l);
+      const float2 s = unpair(sum);
+      total += s.x + s.y;
+      part = fmaf(s.x + s.y, __uint_as_float((uint32_t)(127 - w) << 23), part);
+    }
+    const bool outgrown = !(total <= kMost) || (m == -INFINITY && seen != 0);  // NaN, too: once
+    if (__any_sync(0xffffffffu, outgrown) && !again) {
+      float mx = m;
+#pragma unroll 1
+      for (int k = 2 * c; k < 2 * c + 2; ++k) {
+        uint32_t x[16];
+        tmem_ld16(s_at + 16u * k, x);
+        tmem_ld_wait();
+        const uint32_t see = ALL ? 0xffffu : view.mask(info.pos[k]);
+        float t = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) t = fmaxf(t, see >> e & 1 ? __uint_as_float(x[e]) : -INFINITY);
+        mx = fmaxf(mx, t == -INFINITY ? t : t * (factor * info.ks[k]));
+      }
+      const float mnew = outgrown ? mx : m, by = m == mnew ? 1.f : m == -INFINITY ? 0.f : exp2_ftz(m - mnew);
+      l *= by;
+      m = mnew;
+      tmem_st_wait();
+      rescale<true>(s_at, 16 * c, by);
+      if (!begin) rescale<false>(o_at, D, by);
+      again = true;
+      continue;
     }
     tmem_st16(s_at + 16u * c, p);
-  });
-  return l;
+    l += part;
+    ++c;
+    again = false;
+  }
 }
 
 // One arrival for a warp: 32 threads' arrivals on one word are 32 operations one after the other,
@@ -313,20 +363,6 @@ __device__ __forceinline__ void find_item(const AttnArgs& a, int64_t f, int lane
   }
 }
 
-// O of a warp's rows times a factor of each.
-template <int D>
-__device__ __forceinline__ void rescale(uint32_t o_at, float by) {
-#pragma unroll 1
-  for (int c = 0; c < D; c += 32) {
-    uint32_t v[32];
-    tmem_ld32(o_at + (uint32_t)c, v);
-    tmem_ld_wait();
-#pragma unroll
-    for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * by);
-    tmem_st32(o_at + (uint32_t)c, v);
-  }
-}
-
 // A lane's output row from TMEM times `inv` (zeros where `none`): 64 or 128 bytes at a time, which
 // fill whole sectors.
 template <int D, int TYPE>
@@ -369,19 +405,28 @@ template <int D, int TYPE>
 __device__ __forceinline__ void bring_queries(const AttnArgs& a, const Item& it, int i, int warp, uint8_t* tile, uint8_t* factors, int lane) {
   constexpr int kWords = TYPE == J4B_F32 ? D / 32 : D / 64;  // 16-byte pieces of a row and lane
   constexpr int kHeld = 8 / kWords;                          // rows of a lane in flight
+  // rows 4 apart, without a division each
+  const int g0 = it.first_row + i * kRows + 32 * warp + (lane >> 3), on = 4 / a.group, over = 4 - on * a.group;
+  int row = it.row0 + g0 / a.group, sub = g0 % a.group;
 #pragma unroll 1
   for (int k0 = 0; k0 < 8; k0 += kHeld) {
     uint4 raw[kHeld][kWords];
 #pragma unroll
     for (int k = 0; k < kHeld; ++k) {
-      const int qr = 32 * warp + 4 * (k0 + k) + (lane >> 3), g = it.first_row + i * kRows + qr, row = it.row0 + g / a.group;
+      const int qr = 32 * warp + 4 * (k0 + k) + (lane >> 3);
       const bool there = i * kRows + qr < it.rows && row >= 0 && row < a.tokens;
-      const int64_t src = (int64_t)row * a.q_stride + (int64_t)(it.head * a.group + g % a.group) * D + 8 * (lane & 7);
+      const int64_t src = (int64_t)row * a.q_stride + (int64_t)(it.head * a.group + sub) * D + 8 * (lane & 7);
 #pragma unroll
       for (int c = 0; c < kWords; ++c)
         raw[k][c] = !there ? make_uint4(0, 0, 0, 0)
                     : TYPE == J4B_F32 ? load_once(static_cast<const float*>(a.q) + src + 64 * (c >> 1) + 4 * (c & 1))
                                       : load_once(static_cast<const __nv_bfloat16*>(a.q) + src + 64 * c);
+      row += on;
+      sub += over;
+      if (sub >= a.group) {
+        sub -= a.group;
+        ++row;
+      }
     }
 #pragma unroll
     for (int k = 0; k < kHeld; ++k) {
@@ -417,6 +462,21 @@ __device__ __forceinline__ void bring_queries(const AttnArgs& a, const Item& it,
             make_uint4(h2(y[0] * up, y[1] * up), h2(y[2] * up, y[3] * up), h2(y[4] * up, y[5] * up), h2(y[6] * up, y[7] * up));
       }
     }
+  }
+}
+
+// An item's queries on their way to L2 (8 x 2048 401 -> 397 us).
+template <int D, int TYPE>
+__device__ __forceinline__ void prefetch_queries(const AttnArgs& a, const Item& it, int lane) {
+  constexpr int kSize = TYPE == J4B_F32 ? 4 : 2;
+  if (it.seq < 0) return;
+#pragma unroll 1
+  for (int r = lane; r < it.rows; r += 32) {
+    const int g = it.first_row + r, row = it.row0 + g / a.group;
+    if (row < 0 || row >= a.tokens) continue;
+    const char* src = static_cast<const char*>(a.q) + ((int64_t)row * a.q_stride + (int64_t)(it.head * a.group + g % a.group) * D) * kSize;
+#pragma unroll
+    for (int c = 0; c < D * kSize; c += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(src + c));
   }
 }
 
@@ -470,10 +530,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const AttnArgs
   // The next item, for every warp but the one that finds them (null after the last); the one before
   // is given back. Read where it is: a copy would cost registers.
   uint32_t nth = 0;
-  auto next_item = [&](bool alone = false) -> const Item* {
-    if (!alone) __syncwarp();
+  auto next_item = [&]() -> const Item* {
+    __syncwarp();
     if (nth > 0 && lane == 0) bar_arrive(&item_empty[(nth - 1) % kItems]);
-    ok = ok && kv8_wait(&item_full[nth % kItems], nth / kItems & 1);
+    ok = __all_sync(0xffffffffu, ok && kv8_wait(&item_full[nth % kItems], nth / kItems & 1));  // the warp stays together
     const Item* it = &items[nth % kItems];
     ++nth;
     return ok && it->seq >= 0 ? it : nullptr;
@@ -523,24 +583,19 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const AttnArgs
           ev = max(ev, info.ev[x]);
         }
         const bool all = far - 1 <= least && (near >= most_lo || far <= a.sinks);
-        const float mx = all ? row_max<true>(s_at, info, view, factor) : row_max<false>(s_at, info, view, factor);
         // the last tile's values were ready before these scores were
         if (j > j0 && sees_nan(infos[(k - 1) % kInfos], view)) l = NAN;
         const bool begin = j == j0;
-        const int enew = begin ? ev : max(eref, ev);
-        float mnew = m;
-        if (mx > m + kLazy || (m == -INFINITY && mx > m)) mnew = mx;
         if (begin) {
-          m = mnew;
-        } else if (__any_sync(0xffffffffu, mnew != m || enew != eref)) {
-          const float cm = m == -INFINITY ? 0.f : exp2_ftz(m - mnew), co = cm * exp2_ftz((float)(eref - enew));
-          l *= m == mnew ? 1.f : cm;
-          m = mnew;
-          rescale<D>(o_at, co);
+          eref = ev;
+        } else if (ev > eref) {
+          rescale<false>(o_at, D, exp2_ftz((float)(eref - ev)));
+          eref = ev;
         }
-        eref = enew;
-        const float base = m == -INFINITY ? 0.f : m;
-        l += all ? row_exp<true>(s_at, info, view, factor, base, eref) : row_exp<false>(s_at, info, view, factor, base, eref);
+        if (all)
+          row_pass<D, true>(s_at, o_at, info, view, factor, begin, eref, m, l);
+        else
+          row_pass<D, false>(s_at, o_at, info, view, factor, begin, eref, m, l);
         tmem_st_wait();
         tc_fence_before();
         warp_arrive(&p_ready[i], lane);
@@ -575,29 +630,43 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const AttnArgs
     // piece x: row 32 w + 8 (x / kHalves) + lane / 4, codes 64 (x % kHalves) + 16 (lane % 4): 8 lanes of
     // a store phase are 2 rows x 4 pieces, whose swizzled places cover all banks
     const int pr = lane >> 2, pc = lane & 3;
-    // Codes wait in shared memory, each thread's pieces its own (so its own wait is all they need). The
-    // loops over pieces stay rolled, for the instruction cache.
+    // Codes wait in shared memory, each thread's pieces its own (so its own wait is all they need).
     const uint32_t mine_at = saddr(sraw) + (uint32_t)(tid & 127) * 16u;
     auto load = [&](const uint8_t* codes, int which, const int (&id)[2]) {
-#pragma unroll 4
+      const uint8_t* from = codes + pr * D + 16 * pc;
+      const uint8_t* const src[2] = {from + (int64_t)max(id[0], 0) * (kKvBlock * D), from + (int64_t)max(id[1], 0) * (kKvBlock * D)};
+      const uint32_t to = mine_at + (uint32_t)(which * Smem<D>::kRaw);
+#pragma unroll
       for (int x = 0; x < kPieces; ++x) {
-        const int row = 8 * (x / kHalves) + pr, k = x >= kPieces / 2;
-        const int block = k ? id[1] : id[0];
-        const uint8_t* src = codes + (int64_t)max(block, 0) * (kKvBlock * D) + (row & 15) * D + 64 * (x % kHalves) + 16 * pc;
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(mine_at + (uint32_t)(which * Smem<D>::kRaw) + x * 2048u), "l"(src), "r"(block < 0 ? 0 : 16) : "memory");
+        const int k = x >= kPieces / 2;
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + x * 2048u), "l"(src[k] + (x / kHalves & 1) * (8 * D) + 64 * (x % kHalves)), "r"(id[k] < 0 ? 0 : 16) : "memory");
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    auto store_piece = [&](uint8_t* tile, int x, const uint4& src) {
-      const int row = 32 * w + 8 * (x / kHalves) + pr;
+    // Where the first half of piece 0 goes in an operand (the second is 16 bytes across); piece x's are 1024 (x / kHalves) + kKeys * 128 (x % kHalves) further.
+    const uint32_t lo_at = (uint32_t)(w * 4096 + pr * 128 + (((2 * pc) ^ pr) << 4));
+    auto turn = [&](uint32_t operand, int x, const uint4& src) -> uint32_t {
       uint4 lo, hi;
       e4m3x4_f16(src.x, lo.x, lo.y);
       e4m3x4_f16(src.y, lo.z, lo.w);
       e4m3x4_f16(src.z, hi.x, hi.y);
       e4m3x4_f16(src.w, hi.z, hi.w);
-      uint8_t* half = tile + (x % kHalves) * (kKeys * 128);
-      *reinterpret_cast<uint4*>(half + sw128_offset(row, 16 * pc)) = lo;
-      *reinterpret_cast<uint4*>(half + sw128_offset(row, 16 * pc + 8)) = hi;
+      const uint32_t at = operand + lo_at + (uint32_t)(1024 * (x / kHalves) + kKeys * 128 * (x % kHalves));
+      store_shared(at, lo);
+      store_shared(at ^ 16u, hi);
+      // 0, or NaN where a code is one (the FMA units have room, the integer ones less)
+      return zeros_of(lo, zeros_of(hi, 0));
+    };
+    // four pieces at a time, for the instruction cache (all eight: 8 x 2048 405 -> 414 us)
+    auto turn_all = [&](uint32_t operand, int which) -> uint32_t {
+      const uint8_t* from = sraw + which * Smem<D>::kRaw + (tid & 127) * 16;
+      uint32_t any = 0;
+#pragma unroll 4
+      for (int x = 0; x < kPieces; ++x) {
+        const uint32_t z = turn(operand, x, *reinterpret_cast<const uint4*>(from + x * 2048));
+        if (which) any |= z;
+      }
+      return any;
     };
     // (it, j) runs two tiles ahead of the operands, into the next items: its page numbers are on their
     // way while a tile is turned, the codes and scales of the tile between from when this one's are out
@@ -657,12 +726,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const AttnArgs
     for (uint32_t k = 0; here; ++k) {
       const int s = k % kStages;
       const uint32_t parity = (k / kStages - 1) & 1;
-      uint8_t* kt = sk + s * 2 * Smem<D>::kOperand;
+      const uint32_t kt = saddr(sk) + (uint32_t)(s * 2 * Smem<D>::kOperand);
       TileInfo& info = infos[k % kInfos];
       asm volatile("cp.async.wait_group 1;" ::: "memory");  // the keys; the values may be on their way
       if (k >= kStages) ok = ok && kv8_wait(&k_empty[s], parity);
-#pragma unroll 4
-      for (int x = 0; x < kPieces; ++x) store_piece(kt, x, *reinterpret_cast<const uint4*>(sraw + x * 2048 + (tid & 127) * 16));
+      turn_all(kt, 0);
       if (lane < 2) {
         const int x = 2 * w + lane, pos = lane == 0 ? now[0] : now[1];
         info.pos[x] = pos < 0 ? kNowhere : pos;
@@ -683,26 +751,24 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const AttnArgs
       if (k >= kStages) ok = ok && kv8_wait(&v_empty[s], parity);
       // tokens past the length hold anything; NaNs go to the info, as zeros to the operand
       unsigned nan = 0;
-#pragma unroll 4
-      for (int x = 0; x < kPieces; ++x) {
-        const int row = 8 * (x / kHalves) + pr;
-        uint4 v = *reinterpret_cast<const uint4*>(sraw + Smem<D>::kRaw + x * 2048 + (tid & 127) * 16);
-        if ((x >= kPieces / 2 ? now[1] : now[0]) + (row & 15) >= now_len) v = make_uint4(0, 0, 0, 0);
-        uint32_t* q = reinterpret_cast<uint32_t*>(&v);
-        uint32_t any = 0;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) any |= ((q[e] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
-        if (any) {
-          nan |= 1u << row;
+      const uint32_t any = turn_all(kt + Smem<D>::kOperand, 1);
+      if (__any_sync(0xffffffffu, any != 0) || max(now[0], now[1]) + kKvBlock > now_len) {
+#pragma unroll 1
+        for (int x = 0; x < kPieces; ++x) {
+          const int row = 8 * (x / kHalves) + pr;
+          uint4 v = *reinterpret_cast<const uint4*>(sraw + Smem<D>::kRaw + x * 2048 + (tid & 127) * 16);
+          if ((x >= kPieces / 2 ? now[1] : now[0]) + (row & 15) >= now_len) v = make_uint4(0, 0, 0, 0);
+          uint32_t* q = reinterpret_cast<uint32_t*>(&v);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const uint32_t bytes = (((q[e] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7;
             q[e] &= ~(bytes * 0xffu);
+            if (bytes) nan |= 1u << row;
           }
+          turn(kt + Smem<D>::kOperand, x, v);
         }
-        store_piece(kt + Smem<D>::kOperand, x, v);
+        nan = __reduce_or_sync(0xffffffffu, nan);
       }
-      nan = __reduce_or_sync(0xffffffffu, nan);
       if (lane == 0) info.nan[w] = nan;
       to_async_proxy();
       warp_arrive(&v_full[s], lane);
@@ -715,8 +781,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const AttnArgs
       }
     }
   } else {
-    if (warp == 12 && lane == 0) {
-      // ---- the MMAs, by one thread ----
+    if (warp == 12) {
+      // ---- the MMAs: the warp waits as one, an elected thread issues ----
+      // One thread's branch would keep the descriptors out of uniform registers (8 x 2048 456 against 441 us).
+      auto uni = [](int x) { return __shfl_sync(0xffffffffu, x, 0); };
+      auto wait = [&](uint64_t* bar, uint32_t parity) { ok = __all_sync(0xffffffffu, ok && kv8_wait(bar, parity)); };
       constexpr uint32_t is = idesc_f16(kRows, kKeys, false), io = idesc_f16(kRows, D, true);
       // descriptors count in 16-byte units: stepping one is an addition
       uint64_t qd = kmajor_sw128(saddr(sq)), kd = kmajor_sw128(saddr(sk)), vd = rows_sw128(saddr(sk) + Smem<D>::kOperand, kKeys * 128);
@@ -724,23 +793,20 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const AttnArgs
       uint32_t p_use0 = 0, p_use1 = 0, q_use0 = 0, q_use1 = 0, before = 0;
       bool left0 = false, left1 = false;  // the last item's softmax may still need its last info
       uint32_t s_use0 = 0, s_use1 = 0;
-      while (const Item* const item = next_item(true)) {
-        const int nt = item->tiles(), b0 = item->begin[0], b1 = item->begin[1], e0 = item->end[0], e1 = item->end[1];
+      while (const Item* const item = next_item()) {
+        const int nt = uni(item->tiles()), b0 = uni(item->begin[0]), b1 = uni(item->begin[1]), e0 = uni(item->end[0]), e1 = uni(item->end[1]);
         for (int j = -1; j < nt && ok; ++j) {
           const uint32_t now = before + (uint32_t)j, next = now + 1;
-          if (j + 1 < nt) ok = ok && kv8_wait(&k_full[next & 1], next >> 1 & 1);
-          if (j >= 0) ok = ok && kv8_wait(&v_full[now & 1], now >> 1 & 1);
-          // The second scores of an item free the stage of the tile whose info takes the place of the last
-          // item's last: a softmax that has no part in this item's first tiles may not have read that yet.
+          if (j + 1 < nt) wait(&k_full[next & 1], next >> 1 & 1);
+          if (j >= 0) wait(&v_full[now & 1], now >> 1 & 1);
+          // No further until the last item's infos are read: a softmax that has no part in this item could
+          // fall behind by more than kInfos tiles (three of this and the next item may have infos by now).
           if (j == 0) {
-            if (left0) ok = ok && kv8_wait(&o_seen[0], s_use0++ & 1);
-            if (left1) ok = ok && kv8_wait(&o_seen[1], s_use1++ & 1);
+            if (left0) wait(&o_seen[0], s_use0++ & 1);
+            if (left1) wait(&o_seen[1], s_use1++ & 1);
             left0 = e0 > b0;
             left1 = e1 > b1;
           }
-          // opaque, or every step's descriptor is kept across the loop and spilled: the issue then waits
-          // for local memory (8 x 2048: PV's 8 MMAs took 2 us to issue instead of 0.3)
-          asm volatile("" : "+l"(qd), "+l"(kd), "+l"(vd));
           const uint64_t vt = vd + (now & 1) * kStage, kt = kd + (next & 1) * kStage;
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
@@ -748,37 +814,44 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const AttnArgs
             uint32_t &p_use = i ? p_use1 : p_use0, &q_use = i ? q_use1 : q_use0;
             const uint32_t s_at = tmem + (uint32_t)(i * 128), o_at = tmem + 256u + (uint32_t)(i * 128);
             if (j >= begin && j < end) {
-              ok = ok && kv8_wait(&p_ready[i], p_use & 1);
+              wait(&p_ready[i], p_use & 1);
               ++p_use;
               tc_fence_after();
-              const uint32_t later = j > begin;
+              if (elect_one()) {
+                const uint32_t later = j > begin;
 #pragma unroll
-              for (int k = 0; k < kKeys / 16; ++k)  // 16 keys: 8 columns of P, 2 groups of 8 rows of V
-                umma_ts(o_at, s_at + 8u * k, vt + k * (2048 / 16), io, k > 0 ? 1u : later);
-              if (j + 1 == end) {
-                umma_commit(&o_full[i]);
-                bar_arrive(&o_full[i]);
+                for (int k = 0; k < kKeys / 16; ++k)  // 16 keys: 8 columns of P, 2 groups of 8 rows of V
+                  umma_ts(o_at, s_at + 8u * k, vt + k * (2048 / 16), io, k > 0 ? 1u : later);
+                if (j + 1 == end) {
+                  umma_commit(&o_full[i]);
+                  bar_arrive(&o_full[i]);
+                }
               }
             }
             if (j + 1 >= begin && j + 1 < end) {
               if (j + 1 == begin) {
-                ok = ok && kv8_wait(&q_ready[i], q_use & 1);
+                wait(&q_ready[i], q_use & 1);
                 ++q_use;
               }
               tc_fence_after();
-              const uint64_t qt = qd + (uint32_t)(i * Smem<D>::kQ / 16);
+              if (elect_one()) {
+                const uint64_t qt = qd + (uint32_t)(i * Smem<D>::kQ / 16);
 #pragma unroll
-              for (int k = 0; k < D / 16; ++k) {
-                const uint32_t off = ((k >> 2) * (kRows * 128) + (k & 3) * 32) / 16;  // kRows == kKeys
-                umma_bf16(s_at, qt + off, kt + off, is, k > 0 ? 1u : 0u);
+                for (int k = 0; k < D / 16; ++k) {
+                  const uint32_t off = ((k >> 2) * (kRows * 128) + (k & 3) * 32) / 16;  // kRows == kKeys
+                  umma_ss(s_at, qt + off, kt + off, is, k > 0 ? 1u : 0u);
+                }
+                umma_commit(&s_full[i]);
+                bar_arrive(&s_full[i]);
+                if (j + 2 == end) umma_commit(&q_empty[i]);
               }
-              umma_commit(&s_full[i]);
-              bar_arrive(&s_full[i]);
-              if (j + 2 == end) umma_commit(&q_empty[i]);
             }
           }
-          if (j + 1 < nt) umma_commit(&k_empty[next & 1]);
-          if (j >= 0) umma_commit(&v_empty[now & 1]);
+          if (elect_one()) {
+            if (j + 1 < nt) umma_commit(&k_empty[next & 1]);
+            if (j >= 0) umma_commit(&v_empty[now & 1]);
+          }
+          __syncwarp();
         }
         before += (uint32_t)nt;
       }
@@ -788,13 +861,14 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const AttnArgs
       for (uint32_t r = 0; more && ok; ++r) {
         Item it;
         find_item(a, (int64_t)r * gridDim.x + (r & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x), lane, it);
-        if (r >= kItems) ok = ok && kv8_wait(&item_empty[r % kItems], (r / kItems - 1) & 1);
+        if (r >= kItems) ok = __all_sync(0xffffffffu, ok && kv8_wait(&item_empty[r % kItems], (r / kItems - 1) & 1));
         if (lane == 0) {
           items[r % kItems] = it;
           bar_arrive(&item_full[r % kItems]);
         }
         __syncwarp();
-        more = it.seq >= 0;  // a CTA's numbers rise
+        more = it.seq >= 0;
+        prefetch_queries<D, TYPE>(a, it, lane);  // a CTA's numbers rise
       }
     }
   }

@@ -512,3 +512,45 @@ def test_decoder_block_on_the_paged_cache(backend):
             assert pages.compact() >= 0
     with pytest.raises(ValueError, match="rows for"):
         block.decode_paged(backend.upload(np.zeros((3, d), np.float32), (3, d)), pages)
+
+
+@pytest.mark.parametrize("rising", [True, False])
+@pytest.mark.parametrize("window", [0, 150])
+def test_prefill_maxima_that_are_outgrown_many_times(rising, window):
+    """Keys that get louder (or quieter) block by block, the values the other way round: with rising
+    keys a row's maximum moves in tile after tile, and what counts in the end lies in blocks whose
+    value scale is 2^14 below the first ones'. Scores of an rms of 2^-4 to 2^2.5: the queries' f16
+    (2^-12) moves the loudest by some 1e-3 and so the probabilities; these keep 11 bits down to
+    2^-18, where what is lost, 2^-29 of each of a few hundred early values 2^14 times as large as the
+    last, is below 1e-3 of the sum, too."""
+    rng = np.random.default_rng(31 + rising)
+    n, dim, page = 500, 128, 32
+    pool, offsets, q = prefill_inputs(rng, [(0, n)], 4, 2, dim, page, torch.bfloat16)
+    blocks = -(-n // 16)
+    for j in range(blocks):
+        at = (pool.table[0, j * 16 // page], slice(None), j * 16 % page // 16)
+        t = j / (blocks - 1) if rising else 1 - j / (blocks - 1)
+        pool.ks[at] = 2.0 ** round(-11 + 6.5 * t)
+        pool.vs[at] = 2.0 ** round(-14 * t)
+    pool.cache.k_scale[0] = torch.from_numpy(pool.ks).float()
+    pool.cache.v_scale[0] = torch.from_numpy(pool.vs).float()
+    got = pool.cache.attention_prefill(q, ints(offsets), ints(pool.table), ints(pool.lengths), window=window, out_dtype=torch.float32)
+    ref = pool.reference(q.double().cpu().numpy(), 0, 0, window, 0)
+    for rows in (slice(0, 100), slice(100, 300), slice(300, n), slice(n - 1, n)):
+        assert normwise(got[rows].double().cpu().numpy(), ref[rows]) <= PREFILL_BAR, rows
+
+
+def test_prefill_of_infinite_scores():
+    """Queries so large that scores overflow: rows of infinities are NaN or finite, and never touch
+    other rows."""
+    rng = np.random.default_rng(33)
+    pool, offsets, q = prefill_inputs(rng, [(0, 200)], 4, 2, 128, 32, torch.float32)
+    loud = q.clone()
+    loud[50:60] *= 1e38
+    got = pool.cache.attention_prefill(loud, ints(offsets), ints(pool.table), ints(pool.lengths))
+    calm = pool.cache.attention_prefill(q, ints(offsets), ints(pool.table), ints(pool.lengths))
+    ref = pool.reference(q.double().cpu().numpy(), 0, 0, 0, 0)
+    others = [i for i in range(200) if not 50 <= i < 60]
+    assert torch.isfinite(got[others]).all()
+    assert normwise(got[others].cpu().numpy(), ref[others]) <= PREFILL_BAR
+    assert normwise(calm.cpu().numpy(), ref) <= PREFILL_BAR
