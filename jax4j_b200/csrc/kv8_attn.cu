@@ -59,17 +59,16 @@ struct Piece {
   }
 };
 
-// A warp's online softmax over the blocks it visits. SPLIT: the 16 rows of the MMAs are 8 queries,
-// rows 0-7 the f16 values of Q (and P), rows 8-15 what the rounding left, so that every product is
-// f32-accurate at no extra MMA (a group of up to 8 heads leaves those rows idle otherwise); a
-// thread's query is row g alone. Otherwise 16 queries; a thread's are g and g + 8.
-template <int D, bool SPLIT>
+// A warp's online softmax over the blocks it visits. The 16 rows of the MMAs are 8 queries: rows 0-7
+// the f16 values of Q (and P), rows 8-15 what the rounding left, so that every product is
+// f32-accurate at no extra MMA (a group of up to 8 heads leaves those rows idle otherwise). A thread's
+// query is row g = lane / 4.
+template <int D>
 struct Warp {
-  static constexpr int kRows = SPLIT ? 1 : 2;
   const uint4* q;  // the A operands of the D / 16 k steps, [step][lane], in shared memory
   float o[D / 8][4];
-  float factor[kRows];  // scores in log2 units per unit of the MMA's result and of key scale
-  float m[kRows], l[kRows];
+  float factor;  // scores in log2 units per unit of the MMA's result and of key scale
+  float m, l;
   float ref;  // value scale that the accumulators are in units of (times 2^-kPShift)
 
   // probabilities enter the second product as p 2^kPShift <= 4096: f16 keeps p's bits down to
@@ -79,59 +78,52 @@ struct Warp {
   __device__ __forceinline__ void reset() {
 #pragma unroll
     for (int j = 0; j < D / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
-#pragma unroll
-    for (int r = 0; r < kRows; ++r) m[r] = -INFINITY, l[r] = 0.f;
+    m = -INFINITY, l = 0.f;
     ref = 0.f;
   }
 
-  // Writes the operands of the query rows (row < 0: zeros) to `dst`, and keeps it. Each row is first
-  // brought to a largest element in [2^11, 2^12) by a power of two, so f16's range does not limit
-  // queries. `warps` warps with the same rows share the operands, each writes every warps-th step.
-  __device__ __forceinline__ void load_q(uint4* dst, const void* base, int type, const int64_t (&row)[kRows], float scale_log2, int lane,
-                                         int warp = 0, int warps = 1) {
+  // A query row's elements of a lane (row < 0: zeros), on their way.
+  struct Query {
+    float4 x[D / 16];
+  };
+  __device__ __forceinline__ static void fetch_q(Query& f, const void* base, int type, int64_t row, int lane) {
     const int t = lane & 3;
-    uint32_t frag[D / 16][4];
-#pragma unroll
-    for (int r = 0; r < kRows; ++r) {
-      float4 x[D / 16];
-      float most = 0.f;
-#pragma unroll
-      for (int i = 0; i < D / 16; ++i) {
-        x[i] = row[r] >= 0 ? load4(base, type, row[r] + 16 * (Piece<D>::kK * t + (i >> 2)) + 4 * (i & 3)) : make_float4(0.f, 0.f, 0.f, 0.f);
-        most = fmaxf(most, fmaxf(fmaxf(fabsf(x[i].x), fabsf(x[i].y)), fmaxf(fabsf(x[i].z), fabsf(x[i].w))));
-      }
-      most = quad_max(most);
-      // the power of two below `most`, biased; queries of tiny, infinite or no magnitude stay as they are
-      const int e = (int)(__float_as_uint(most) >> 23);
-      const float down = e < 24 || e > 240 ? 1.f : __uint_as_float((uint32_t)(e - 11) << 23);
-      const float up = e < 24 || e > 240 ? 1.f : __uint_as_float((uint32_t)(254 - (e - 11)) << 23);
-      factor[r] = scale_log2 * down;
-#pragma unroll
-      for (int i = 0; i < D / 16; ++i) {
-        const float4 y = make_float4(x[i].x * up, x[i].y * up, x[i].z * up, x[i].w * up);
-        frag[i][r] = h2(y.x, y.y);
-        frag[i][2 + r] = h2(y.z, y.w);
-        if (SPLIT) {
-          frag[i][1] = h2_rest(y.x, y.y, frag[i][0]);
-          frag[i][3] = h2_rest(y.z, y.w, frag[i][2]);
-        }
-      }
-    }
 #pragma unroll
     for (int i = 0; i < D / 16; ++i)
-      if (i % warps == warp) dst[i * 32 + lane] = make_uint4(frag[i][0], frag[i][1], frag[i][2], frag[i][3]);
+      f.x[i] = row >= 0 ? load4(base, type, row + 16 * (Piece<D>::kK * t + (i >> 2)) + 4 * (i & 3)) : make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  // Writes the operands of the query rows to `dst`, and keeps it. Each row is first brought to a
+  // largest element in [2^11, 2^12) by a power of two, so f16's range does not limit queries. `warps`
+  // warps with the same rows share the operands, each writes every warps-th step.
+  __device__ __forceinline__ void load_q(uint4* dst, const Query& f, float scale_log2, int lane, int warp, int warps) {
+    float most = 0.f;
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i)
+      most = fmaxf(most, fmaxf(fmaxf(fabsf(f.x[i].x), fabsf(f.x[i].y)), fmaxf(fabsf(f.x[i].z), fabsf(f.x[i].w))));
+    most = quad_max(most);
+    // the power of two below `most`, biased; queries of tiny, infinite or no magnitude stay as they are
+    const int e = (int)(__float_as_uint(most) >> 23);
+    const float down = e < 24 || e > 240 ? 1.f : __uint_as_float((uint32_t)(e - 11) << 23);
+    const float up = e < 24 || e > 240 ? 1.f : __uint_as_float((uint32_t)(254 - (e - 11)) << 23);
+    factor = scale_log2 * down;
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) {
+      const float4 y = make_float4(f.x[i].x * up, f.x[i].y * up, f.x[i].z * up, f.x[i].w * up);
+      const uint32_t lo = h2(y.x, y.y), hi = h2(y.z, y.w);
+      if (i % warps == warp) dst[i * 32 + lane] = make_uint4(lo, h2_rest(y.x, y.y, lo), hi, h2_rest(y.z, y.w, hi));
+    }
     q = dst + lane;
   }
 
   // Two blocks, first half: their key codes in the lane's buffer, their scales, and which of their
-  // tokens row r sees: tokens j with (first[r] <= j or j < sinks) and j <= last[r] (a block that is
+  // tokens the lane's row sees: tokens j with (first <= j or j < sinks) and j <= last (a block that is
   // not there has p0 far past every row). `all`: every row sees every token of both. Two at a time:
   // their MMA chains are independent, and one maximum, one vote on rescaling serve both.
   // Leaves the probabilities in p, and in `seen` (bit 4 u + j) which of the lane's tokens any row
   // sees: a masked token's value codes are replaced by zeros in the second half, since they may
   // hold anything, NaN too, in a page that is not full.
-  __device__ __forceinline__ void scores(const uint8_t* stage, const float (&ks)[2], const float (&vs)[2], bool all, const int (&first)[kRows],
-                                         const int (&last)[kRows], int sinks, const int (&p0)[2], int lane, uint32_t (&p)[2][4], uint32_t& seen) {
+  __device__ __forceinline__ void scores(const uint8_t* stage, const float (&ks)[2], const float (&vs)[2], bool all, int first, int last,
+                                         int sinks, const int (&p0)[2], int lane, uint32_t (&p)[2][4], uint32_t& seen) {
     const int t = lane & 3;
     float s[2][2][4];
 #pragma unroll
@@ -161,31 +153,23 @@ struct Warp {
           }
       }
     }
-    float x[kRows][2][4];  // scores of tokens 2t, 2t + 1, 2t + 8, 2t + 9 of each block
+    float x[2][4];  // scores of tokens 2t, 2t + 1, 2t + 8, 2t + 9 of each block
     seen = all ? 0xffu : 0u;
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
+    for (int u = 0; u < 2; ++u) {
+      const float f = factor * ks[u];
 #pragma unroll
-      for (int r = 0; r < kRows; ++r) {
-        const float f = factor[r] * ks[u];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float raw = SPLIT ? s[u][j >> 1][j & 1] + s[u][j >> 1][2 + (j & 1)] : s[u][j >> 1][2 * r + (j & 1)];
-          x[r][u][j] = raw * f;
-        }
-      }
+      for (int j = 0; j < 4; ++j) x[u][j] = (s[u][j >> 1][j & 1] + s[u][j >> 1][2 + (j & 1)]) * f;
+    }
     if (!all) {
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int tok = p0[u] + 2 * t + (j & 1) + 8 * (j >> 1);
-#pragma unroll
-          for (int r = 0; r < kRows; ++r) {
-            const bool see = (tok >= first[r] || tok < sinks) && tok <= last[r];
-            if (!see) x[r][u][j] = -INFINITY;
-            seen |= (uint32_t)see << (4 * u + j);
-          }
+          const bool see = (tok >= first || tok < sinks) && tok <= last;
+          if (!see) x[u][j] = -INFINITY;
+          seen |= (uint32_t)see << (4 * u + j);
         }
       // the lanes of the same t hold the other rows
       seen |= __shfl_xor_sync(0xffffffffu, seen, 4);
@@ -193,55 +177,34 @@ struct Warp {
       seen |= __shfl_xor_sync(0xffffffffu, seen, 16);
     }
     const float vmax = fmaxf(vs[0], vs[1]);
-    bool grown = vmax > ref;
-    float mn[kRows];
-#pragma unroll
-    for (int r = 0; r < kRows; ++r) {
-      float v = fmaxf(fmaxf(fmaxf(x[r][0][0], x[r][0][1]), fmaxf(x[r][0][2], x[r][0][3])),
-                      fmaxf(fmaxf(x[r][1][0], x[r][1][1]), fmaxf(x[r][1][2], x[r][1][3])));
-      mn[r] = fmaxf(m[r], quad_max(v));
-      grown |= mn[r] > m[r];
-    }
-    if (__any_sync(0xffffffffu, grown)) {
+    const float mn = fmaxf(m, quad_max(fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])), fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3])))));
+    if (__any_sync(0xffffffffu, vmax > ref || mn > m)) {
       const float now = fmaxf(ref, vmax);
       const float down = ref * kv8_inverse(now);  // 0 at the first block
       ref = now;
+      const float c = mn == -INFINITY ? 1.f : exp2f(m - mn);
+      l *= c;
+      m = mn;
 #pragma unroll
-      for (int r = 0; r < kRows; ++r) {
-        const float c = mn[r] == -INFINITY ? 1.f : exp2f(m[r] - mn[r]);
-        l[r] *= c;
-        m[r] = mn[r];
+      for (int j = 0; j < D / 8; ++j)
 #pragma unroll
-        for (int j = 0; j < D / 8; ++j) {
-          o[j][2 * r] *= c * down;
-          o[j][2 * r + 1] *= c * down;
-          if (SPLIT) {
-            o[j][2] *= c * down;
-            o[j][3] *= c * down;
-          }
-        }
-      }
+        for (int e = 0; e < 4; ++e) o[j][e] *= c * down;
     }
+    const float base = m == -INFINITY ? 0.f : m;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const float weight = (float)(1 << kPShift) * vs[u] * kv8_inverse(ref);
+      float e[4];
 #pragma unroll
-      for (int r = 0; r < kRows; ++r) {
-        const float base = m[r] == -INFINITY ? 0.f : m[r];
-        float e[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          e[j] = exp2_ftz(x[r][u][j] - base);
-          l[r] += e[j];
-          e[j] *= weight;
-        }
-        p[u][r] = h2(e[0], e[1]);
-        p[u][2 + r] = h2(e[2], e[3]);
-        if (SPLIT) {
-          p[u][1] = h2_rest(e[0], e[1], p[u][0]);
-          p[u][3] = h2_rest(e[2], e[3], p[u][2]);
-        }
+      for (int j = 0; j < 4; ++j) {
+        e[j] = exp2_ftz(x[u][j] - base);
+        l += e[j];
+        e[j] *= weight;
       }
+      p[u][0] = h2(e[0], e[1]);
+      p[u][2] = h2(e[2], e[3]);
+      p[u][1] = h2_rest(e[0], e[1], p[u][0]);
+      p[u][3] = h2_rest(e[2], e[3], p[u][2]);
     }
   }
 
@@ -349,9 +312,12 @@ struct Copies {
 // Bound by HBM once the rows are long: 2 x 16 D bytes a block against ~430 warp instructions at 12
 // warps an SM. What the short ones cost is latency, so a warp never lets its copies run dry: it looks
 // up the next 32 blocks, of its next segment too, while it works on these, and fetches the first
-// pair's keys of the next segment before it merges.
+// pair's keys of the next segment before it merges. At the start the pages and the queries are asked
+// for together, and codes before scales (1 x 517 tokens 11.0 -> 10.4 us, ragged batch 61.8 -> 60.0).
 constexpr int kDecWarps = 4;
-constexpr int kDecCtas = 3;  // of an SM
+// CTAs of an SM: D = 128 fills the registers at 3; with D = 64 (bound by instructions) 4 fit, too:
+// 32 x window 4096, 40/8 heads of 64: 3 43.2 us, 4 41.0, 5 (spilling) 44.6.
+constexpr int dec_ctas(int dim) { return dim == 64 ? 4 : 3; }
 constexpr int kDecHeads = 8;
 constexpr int kWholeTokens = 576;
 constexpr int kRowUnits = 20;  // 4: ragged batch (48 x up to 8191 tokens) 78.9 us, 12: 67.8, 20: 61.6, 28: 61.7, 40: 63.5
@@ -367,10 +333,14 @@ __device__ __forceinline__ int64_t row_units(const AttnArgs& a, int b) {
   const int len = __ldg(a.lengths + b), n = span_of(len - 1, len - 1, a.window, a.sinks).count();
   return n > 0 ? n + kRowUnits : 0;
 }
+// Of numbers that are not negative, and seldom past 31 bits: a 64-bit division takes as long as a load.
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+  return ((a | b) >> 31) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
+}
 // Units of a CTA: a whole number for each of its warps, the same for all CTAs (the last ones may get none).
 __device__ __forceinline__ int64_t share_of(int64_t units, int ctas) {
   const int64_t each = (int64_t)ctas * kDecWarps;
-  return (units + each - 1) / each * kDecWarps;
+  return quotient(units + each - 1, each) * kDecWarps;
 }
 
 // A CTA's part of a row: its blocks begin .. end - 1 of the row's nb.
@@ -396,7 +366,7 @@ struct Share {
         continue;
       }
       s.b = b;
-      s.row = (int)(at / units);
+      s.row = (int)quotient(at, units);
       const int from = (int)(at - (int64_t)s.row * units), to = (int)min((int64_t)units, from + left);
       left -= to - from;
       at += to - from;
@@ -442,7 +412,7 @@ __device__ __forceinline__ Kv8Place find_share(const DecArgs& d, int rows, bool 
 
 // WHOLE: a CTA per row, no shares and no join.
 template <int D, bool WHOLE>
-__global__ void __launch_bounds__(kDecWarps * 32, kDecCtas) kv8_decode_kernel(const DecArgs d, const __grid_constant__ CUtensorMap mk,
+__global__ void __launch_bounds__(kDecWarps * 32, dec_ctas(D)) kv8_decode_kernel(const DecArgs d, const __grid_constant__ CUtensorMap mk,
                                                                               const __grid_constant__ CUtensorMap mv) {
   const AttnArgs& a = d.a;
   extern __shared__ uint8_t smem_raw[];
@@ -473,7 +443,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, kDecCtas) kv8_decode_kernel(co
     const int pg = s.span.block(s.begin + warp + kDecWarps * i) / a.c.bpp;
     return pg < a.t.width ? __ldg(a.t.pages + s.b * a.t.stride + pg) : -1;
   };
-  auto look_up = [&](const Segment& s, int i, int page, Block* dst) {
+  auto look_up = [&](const Segment& s, int i, int page, Block* dst, auto numbered) {
     Block k = {-1, kNowhere, 0.f, 0.f};
     if ((unsigned)page < (unsigned)a.c.pages) {
       const int blk = s.span.block(s.begin + warp + kDecWarps * i);
@@ -482,31 +452,41 @@ __global__ void __launch_bounds__(kDecWarps * 32, kDecCtas) kv8_decode_kernel(co
       k.ks = __ldg(a.c.ks + k.id);
       k.vs = __ldg(a.c.vs + k.id);
     }
-    dst[lane] = k;
+    // the numbers are there before the scales arrive, so that the first copies need not wait for those
+    *reinterpret_cast<int2*>(&dst[lane]) = make_int2(k.id, k.pos);
+    numbered();
+    *reinterpret_cast<float2*>(&dst[lane].ks) = make_float2(k.ks, k.vs);
+  };
+
+  auto q_row = [&](const Segment& s) -> int64_t {  // of the lane's row, -1: none
+    const int head = s.row / d.chunks, h = head * a.group + s.row % d.chunks * kDecHeads + g;
+    return h < (head + 1) * a.group ? (int64_t)s.b * a.q_stride + (int64_t)h * D : -1;
   };
 
   Segment cur, nxt;
+  Warp<D> w;
   bool more = work.next(a, rows, cur);
   int which = 0;  // half of `blocks` in use
   if (more) {
-    look_up(cur, lane, page_of(cur, lane, cur.mine(warp)), blocks);
+    const int page = page_of(cur, lane, cur.mine(warp));
+    typename Warp<D>::Query query;
+    Warp<D>::fetch_q(query, a.q, a.q_type, q_row(cur), lane);  // on their way with the pages, then the codes and scales
+    look_up(cur, lane, page, blocks, [&] {
+      __syncwarp();
+      if (cur.mine(warp) > 0) {
+        copies.fetch(0, blocks, lane);
+        copies.fetch(1, blocks, lane);
+      }
+    });
+    w.load_q(queries, query, a.scale_log2, lane, warp, kDecWarps);
     __syncwarp();
-    if (cur.mine(warp) > 0) {
-      copies.fetch(0, blocks, lane);
-      copies.fetch(1, blocks, lane);
-    }
   }
-  Warp<D, true> w;
   for (int done = 0; more; ++done, cur = nxt) {
     more = !WHOLE && work.next(a, rows, nxt);
     const int head = cur.row / d.chunks, h0 = head * a.group + cur.row % d.chunks * kDecHeads;
     const int nh = min(kDecHeads, (head + 1) * a.group - h0);
-    const int first[1] = {a.window > 0 ? max(0, cur.len - a.window) : 0}, last[1] = {cur.len - 1};
+    const int first = a.window > 0 ? max(0, cur.len - a.window) : 0, last = cur.len - 1;
     w.reset();
-    {
-      const int64_t qrow[1] = {g < nh ? (int64_t)cur.b * a.q_stride + (int64_t)(h0 + g) * D : -1};
-      w.load_q(queries, a.q, a.q_type, qrow, a.scale_log2, lane, warp, kDecWarps);
-    }
     __syncthreads();
     const int mine = cur.mine(warp), next_mine = more ? nxt.mine(warp) : 0;
     for (int base = 0; base < mine; base += kBatch) {
@@ -523,8 +503,8 @@ __global__ void __launch_bounds__(kDecWarps * 32, kDecCtas) kv8_decode_kernel(co
         const float kk[2] = {b0.ks, b1.ks}, vv[2] = {b0.vs, b1.vs};
         const bool any = b0.id >= 0 || b1.id >= 0;
         const int far = max(p0[0], p0[1]) + kKvBlock, near = min(p0[0], p0[1]);
-        const bool all = far <= cur.len && (near >= first[0] || far <= a.sinks);
-        if (i == look_at) look_up(same ? cur : nxt, next_base + lane, page, then);
+        const bool all = far <= cur.len && (near >= first || far <= a.sinks);
+        if (i == look_at) look_up(same ? cur : nxt, next_base + lane, page, then, [] {});
         uint32_t p[2][4], seen;
         copies.wait(0);
         if (any) w.scores(buffer, kk, vv, all, first, last, a.sinks, p0, lane, p, seen);
@@ -547,15 +527,15 @@ __global__ void __launch_bounds__(kDecWarps * 32, kDecCtas) kv8_decode_kernel(co
     }
     if (mine == 0 && next_mine > 0) {  // a segment of fewer blocks than warps
       Block* then = blocks + (which ^ 1) * kBatch;
-      look_up(nxt, lane, page_of(nxt, lane, next_mine), then);
+      look_up(nxt, lane, page_of(nxt, lane, next_mine), then, [] {});
       __syncwarp();
       copies.fetch(0, then, lane);
       which ^= 1;
     }
     // merge the warps
-    const float l = quad_sum(w.l[0]), unit = w.unit();
+    const float l = quad_sum(w.l), unit = w.unit();
     if (g < nh) {
-      if (t == 0) states[warp][g] = make_float2(w.m[0], l);
+      if (t == 0) states[warp][g] = make_float2(w.m, l);
       // columns of tile j are dims (D / 8) n + j: this thread's n are 2t and 2t + 1
 #pragma unroll
       for (int n = 0; n < 2; ++n)
@@ -600,6 +580,11 @@ __global__ void __launch_bounds__(kDecWarps * 32, kDecCtas) kv8_decode_kernel(co
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the values' half goes back to TMA
     __syncthreads();
     if (next_mine > 0) copies.fetch(1, blocks + which * kBatch, lane);
+    if (more) {
+      typename Warp<D>::Query query;
+      Warp<D>::fetch_q(query, a.q, a.q_type, q_row(nxt), lane);
+      w.load_q(queries, query, a.scale_log2, lane, warp, kDecWarps);
+    }
   }
   copies.finish(a.timeout);
 }
@@ -617,7 +602,7 @@ __global__ void __launch_bounds__(128) kv8_join_kernel(const DecArgs d, int ctas
   __shared__ float2 states[4];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int64_t before = d.cum[b], units = d.cum[a.batch];
-  const int64_t row = (d.cum[b + 1] - before) / (a.c.kv_heads * d.chunks);
+  const int64_t row = quotient(d.cum[b + 1] - before, a.c.kv_heads * d.chunks);
   constexpr int kPer = D / 32;
   float acc[kPer];
 #pragma unroll
@@ -625,13 +610,16 @@ __global__ void __launch_bounds__(128) kv8_join_kernel(const DecArgs d, int ctas
   float lt = 0.f, mt = -INFINITY;
   if (row > 0) {
     const int64_t share = share_of(units, ctas), u0 = before + (head * d.chunks + chunk) * row;
-    const int c0 = (int)((u0 + kRowUnits) / share), c1 = (int)((u0 + row - 1) / share);
+    const int c0 = (int)quotient(u0 + kRowUnits, share), c1 = (int)quotient(u0 + row - 1, share);
     if (c0 == c1) return;  // finished by its CTA
     // part i of the row is the first segment of CTA c0 + i, but for part 0 when c0 starts before the row
     const float* first = d.part + ((int64_t)(2 * c0 + (share * c0 < u0)) * kDecHeads + h) * (D + 2);
     const float* rest = d.part + ((int64_t)2 * (c0 + 1) * kDecHeads + h) * (D + 2);
     constexpr int64_t kNext = (int64_t)2 * kDecHeads * (D + 2);
     const int parts = c1 - c0 + 1;
+    float head_start[kPer];  // of the warp's first part, while its state is on its way
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) head_start[e] = warp < parts ? (warp == 0 ? first : rest + (warp - 1) * kNext)[2 + lane + 32 * e] : 0.f;
     // warp w takes parts w, w + 4, ..: lane j looks at the j-th of 32
     for (int base = 0; base * 4 < parts; base += 32) {
       const int mine = warp + 4 * (base + lane), n = min(32, (parts - warp + 3) / 4 - base);
@@ -656,7 +644,7 @@ __global__ void __launch_bounds__(128) kv8_join_kernel(const DecArgs d, int ctas
         const float fp = __shfl_sync(0xffffffffu, f, p);
         const float* src = (at == 0 ? first : rest + (at - 1) * kNext) + 2 + lane;
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) acc[e] = fmaf(fp, src[32 * e], acc[e]);
+        for (int e = 0; e < kPer; ++e) acc[e] = fmaf(fp, at == warp ? head_start[e] : src[32 * e], acc[e]);
       }
     }
   }
@@ -708,9 +696,9 @@ int* timeout_word() {
   return word;
 }
 
-int decode_ctas(int dev) {
+int decode_ctas(int dev, int dim) {
   const DeviceCtx* ctx = device_ctx(dev);
-  return kDecCtas * (ctx && ctx->sm_count > 0 ? ctx->sm_count : 148);
+  return dec_ctas(dim) * (ctx && ctx->sm_count > 0 ? ctx->sm_count : 148);
 }
 
 int64_t decode_bytes(int dim, int64_t batch, int ctas) {
@@ -814,7 +802,7 @@ extern "C" int j4b_kv8_decode_workspace(const j4b_kv8_cache* cache, int64_t head
   J4B_REQUIRE(heads > 0 && heads <= 65536 && heads % cache->kv_heads == 0, "kv8 decode: heads (%lld) must be a multiple of kv_heads (%d)",
               (long long)heads, cache->kv_heads);
   J4B_REQUIRE(batch >= 0 && batch <= 0xffffff, "kv8 decode: bad batch");
-  *bytes = decode_bytes(cache->head_dim, batch, decode_ctas(dev));
+  *bytes = decode_bytes(cache->head_dim, batch, decode_ctas(dev, cache->head_dim));
   return J4B_OK;
 }
 
@@ -829,7 +817,7 @@ extern "C" int j4b_kv8_attention_decode(const j4b_kv8_cache* cache, int64_t laye
     return st;
   J4B_REQUIRE(batch * heads <= 0x7fffffffLL, "kv8 decode: too many rows");
   if (batch == 0) return J4B_OK;
-  const int ctas = decode_ctas(dev);
+  const int ctas = decode_ctas(dev, cache->head_dim);
   J4B_REQUIRE(workspace && (workspace & 15) == 0 && workspace_bytes >= decode_bytes(cache->head_dim, batch, ctas),
               "kv8 decode: workspace must be 16-byte aligned and hold %lld bytes", (long long)decode_bytes(cache->head_dim, batch, ctas));
   DeviceGuard guard(dev);
