@@ -333,14 +333,10 @@ __device__ __forceinline__ int64_t row_units(const AttnArgs& a, int b) {
   const int len = __ldg(a.lengths + b), n = span_of(len - 1, len - 1, a.window, a.sinks).count();
   return n > 0 ? n + kRowUnits : 0;
 }
-// Of numbers that are not negative, and seldom past 31 bits: a 64-bit division takes as long as a load.
-__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
-  return ((a | b) >> 31) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
-}
 // Units of a CTA: a whole number for each of its warps, the same for all CTAs (the last ones may get none).
 __device__ __forceinline__ int64_t share_of(int64_t units, int ctas) {
   const int64_t each = (int64_t)ctas * kDecWarps;
-  return quotient(units + each - 1, each) * kDecWarps;
+  return kv8_quotient(units + each - 1, each) * kDecWarps;
 }
 
 // A CTA's part of a row: its blocks begin .. end - 1 of the row's nb.
@@ -366,7 +362,7 @@ struct Share {
         continue;
       }
       s.b = b;
-      s.row = (int)quotient(at, units);
+      s.row = (int)kv8_quotient(at, units);
       const int from = (int)(at - (int64_t)s.row * units), to = (int)min((int64_t)units, from + left);
       left -= to - from;
       at += to - from;
@@ -602,7 +598,7 @@ __global__ void __launch_bounds__(128) kv8_join_kernel(const DecArgs d, int ctas
   __shared__ float2 states[4];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int64_t before = d.cum[b], units = d.cum[a.batch];
-  const int64_t row = quotient(d.cum[b + 1] - before, a.c.kv_heads * d.chunks);
+  const int64_t row = kv8_quotient(d.cum[b + 1] - before, a.c.kv_heads * d.chunks);
   constexpr int kPer = D / 32;
   float acc[kPer];
 #pragma unroll
@@ -610,7 +606,7 @@ __global__ void __launch_bounds__(128) kv8_join_kernel(const DecArgs d, int ctas
   float lt = 0.f, mt = -INFINITY;
   if (row > 0) {
     const int64_t share = share_of(units, ctas), u0 = before + (head * d.chunks + chunk) * row;
-    const int c0 = (int)quotient(u0 + kRowUnits, share), c1 = (int)quotient(u0 + row - 1, share);
+    const int c0 = (int)kv8_quotient(u0 + kRowUnits, share), c1 = (int)kv8_quotient(u0 + row - 1, share);
     if (c0 == c1) return;  // finished by its CTA
     // part i of the row is the first segment of CTA c0 + i, but for part 0 when c0 starts before the row
     const float* first = d.part + ((int64_t)(2 * c0 + (share * c0 < u0)) * kDecHeads + h) * (D + 2);

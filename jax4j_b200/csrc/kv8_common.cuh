@@ -141,8 +141,14 @@ struct AttnArgs {
   float scale_log2;
   void* out;
   int out_type;
-  int* timeout;  // host memory; set when a wait gave up
+  int* timeout;   // host memory; set when a wait gave up
+  int item_log2;  // prefill: rows of an item
 };
+
+// Of numbers that are not negative, and seldom past 31 bits: a 64-bit division takes as long as a load.
+__device__ __forceinline__ int64_t kv8_quotient(int64_t a, int64_t b) {
+  return ((a | b) >> 31) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
+}
 
 __device__ __forceinline__ uint8_t* aligned_smem(uint8_t* raw) {  // the swizzle goes by address bits
   return raw + ((1024u - ((uint32_t)__cvta_generic_to_shared(raw) & 1023u)) & 1023u);

@@ -282,7 +282,7 @@ __device__ __forceinline__ void warp_arrive(uint64_t* bar, int lane) {
   if (lane == 0) bar_arrive(bar);
 }
 
-// 256 rows of one (sequence, kv head).
+// 256 rows (or 128: AttnArgs.item_log2) of one (sequence, kv head).
 struct Item {
   int seq, head;               // seq -1: no more
   int row0, len, pos0;         // the sequence's first row of q, its length, the position of its query 0
@@ -297,38 +297,36 @@ struct Item {
 // Items of a sequence, before its kv heads.
 __device__ __forceinline__ int items_of(const AttnArgs& a, int b) {
   const int64_t rows = (int64_t)max(0, __ldg(a.offsets + b + 1) - __ldg(a.offsets + b)) * a.group;
-  return (int)((rows + 2 * kRows - 1) / (2 * kRows));
+  return (int)((rows + (1 << a.item_log2) - 1) >> a.item_log2);
 }
-// Sum over the sequences of min(items, most), by a warp.
-__device__ __forceinline__ int64_t items_up_to(const AttnArgs& a, int most, int lane) {
-  int64_t n = 0;
-  for (int b = lane; b < a.batch; b += 32) n += min(most, items_of(a, b));
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
-  return n;
-}
-
 // Item number f of the call, for a warp: all last items of the sequences, then all last but one, ...
 __device__ __forceinline__ void find_item(const AttnArgs& a, int64_t f, int lane, Item& it) {
   it.seq = -1;
-  const int64_t m = f / a.c.kv_heads;
-  if (m >= items_up_to(a, 0x7fffffff, lane)) return;
+  const int64_t m = kv8_quotient(f, a.c.kv_heads);
+  // of the first 32 sequences, which are mostly all
+  const int own = lane < a.batch ? items_of(a, lane) : 0, own_len = lane < a.batch ? __ldg(a.lengths + lane) : 0;
+  auto items_up_to = [&](int most) -> int64_t {            // sum over the sequences of min(items, most)
+    unsigned n = (unsigned)min(most, own);
+    for (int b = lane + 32; b < a.batch; b += 32) n += (unsigned)min(most, items_of(a, b));
+    return __reduce_add_sync(0xffffffffu, n);
+  };
+  if (m >= items_up_to(0x7fffffff)) return;
   int lo = 0, hi = 1;  // items_up_to(lo) <= m < items_up_to(hi)
-  while (items_up_to(a, hi, lane) <= m) {
+  while (items_up_to(hi) <= m) {
     lo = hi;
     hi *= 2;
   }
   while (hi - lo > 1) {
     const int mid = (lo + hi) / 2;
-    if (items_up_to(a, mid, lane) <= m)
+    if (items_up_to(mid) <= m)
       lo = mid;
     else
       hi = mid;
   }
-  int64_t left = m - items_up_to(a, lo, lane);  // this many sequences of more than lo items come before
+  int64_t left = m - items_up_to(lo);  // this many sequences of more than lo items come before
   int b = 0;
   for (int base = 0;; base += 32) {
-    const uint32_t has = __ballot_sync(0xffffffffu, base + lane < a.batch && items_of(a, min(base + lane, a.batch - 1)) > lo);
+    const uint32_t has = __ballot_sync(0xffffffffu, (base == 0 ? own : base + lane < a.batch ? items_of(a, base + lane) : 0) > lo);
     if (left >= __popc(has)) {
       left -= __popc(has);
       continue;
@@ -337,13 +335,13 @@ __device__ __forceinline__ void find_item(const AttnArgs& a, int64_t f, int lane
     break;
   }
   it.seq = b;
-  it.head = (int)(f % a.c.kv_heads);
+  it.head = (int)(f - m * a.c.kv_heads);
   it.row0 = __ldg(a.offsets + b);
   const int n = __ldg(a.offsets + b + 1) - it.row0;
-  it.len = __ldg(a.lengths + b);
+  it.len = b < 32 ? __shfl_sync(0xffffffffu, own_len, b) : __ldg(a.lengths + b);
   it.pos0 = it.len - n;  // negative: the first queries are before the cache and see nothing
-  it.first_row = (items_of(a, b) - 1 - lo) * (2 * kRows);
-  it.rows = (int)min((int64_t)2 * kRows, (int64_t)n * a.group - it.first_row);
+  it.first_row = (items_of(a, b) - 1 - lo) << a.item_log2;
+  it.rows = (int)min((int64_t)1 << a.item_log2, (int64_t)n * a.group - it.first_row);
   auto span_of_tile = [&](int i, int tiles) {  // of tiles i .. i + tiles - 1
     const int from = it.first_row + i * kRows, to = it.first_row + min(it.rows, (i + tiles) * kRows) - 1;
     return span_of(max(0, it.pos0 + from / a.group), min(it.len - 1, it.pos0 + to / a.group), a.window, a.sinks);
@@ -883,15 +881,21 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const AttnArgs
 }
 
 template <int D, int TYPE>
-int launch_prefill(const AttnArgs& a, int dev, cudaStream_t stream) {
+int launch_prefill(AttnArgs& a, int dev, cudaStream_t stream) {
   static bool done[kMaxDevices] = {};
   if (!done[dev]) {
     J4B_CUDA(cudaFuncSetAttribute(kv8_prefill_kernel<D, TYPE>, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<D>::kBytes), "cudaFuncSetAttribute");
     done[dev] = true;
   }
-  const int64_t rows = a.tokens * a.group, items = std::min(rows, rows / (2 * kRows) + a.batch) * a.c.kv_heads;
+  const int64_t rows = a.tokens * a.group;
   J4B_REQUIRE(rows <= 0x3fffffffLL, "kv8 prefill: too many rows");
   const DeviceCtx* ctx = device_ctx(dev);
+  auto items_of_rows = [&](int log2) { return std::min(rows, (rows >> log2) + a.batch) * a.c.kv_heads; };  // at most
+  // A tile of 128 rows alone walks its keys faster than one of two, so where every such tile has an SM
+  // to itself, items are one tile (5 turns of up to 77 tokens on up to 1000: 31.6 -> 27.0 us). Two
+  // share the work on the pages elsewhere (8 x 2048: 396 us, by single tiles 642).
+  a.item_log2 = items_of_rows(7) <= ctx->sm_count ? 7 : 8;
+  const int64_t items = items_of_rows(a.item_log2);
   kv8_prefill_kernel<D, TYPE><<<(unsigned)std::min<int64_t>(items, ctx->sm_count), kThreads, Smem<D>::kBytes, stream>>>(a);
   J4B_CHECK_LAUNCH("kv8_prefill_kernel");
   return J4B_OK;

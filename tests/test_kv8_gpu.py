@@ -554,3 +554,29 @@ def test_prefill_of_infinite_scores():
     assert torch.isfinite(got[others]).all()
     assert normwise(got[others].cpu().numpy(), ref[others]) <= PREFILL_BAR
     assert normwise(calm.cpu().numpy(), ref) <= PREFILL_BAR
+
+
+@pytest.mark.parametrize("window,sinks", [(0, 0), (300, 20)])
+def test_prefill_of_two_tiles_an_item_with_nan_and_unmapped_pages(window, sinks):
+    """More rows than one tile an SM: NaN values, pages that are not there, a window and sinks, where
+    two tiles of rows share the key tiles."""
+    rng = np.random.default_rng(41 + window)
+    spans, heads, kv, dim, page = [(0, 700), (900, 333)], 32, 8, 128, 64
+    pool, offsets, q = prefill_inputs(rng, spans, heads, kv, dim, page, torch.bfloat16)
+    pool.unmap(1, [1, 5, 6])
+    at = 450
+    pool.cache.v.view(torch.uint8)[0, int(pool.table[0, at // page]), 3, at % page, 100] = 0x7f
+    got = pool.cache.attention_prefill(q, ints(offsets), ints(pool.table), ints(pool.lengths), window=window, sinks=sinks).double().cpu().numpy()
+    bad = np.isnan(got).any(-1)
+    pos = np.arange(700)
+    sees = (pos >= at) & ((window == 0) | (pos < at + window))
+    want = np.zeros_like(bad)
+    want[:700, 12:16] = sees[:, None]  # the query heads of kv head 3
+    assert np.array_equal(bad, want)
+    qh = q.double().cpu().numpy()
+    for b, (past, n) in enumerate(spans):
+        ref = pool.reference(qh[offsets[b]:offsets[b + 1]], b, past, window, sinks)
+        mine = got[offsets[b]:offsets[b + 1]]
+        for part in (slice(0, 128), slice(128, 256), slice(256, n)):
+            keep = ~want[offsets[b]:offsets[b + 1]][part]
+            assert normwise(mine[part][keep], ref[part][keep]) <= PREFILL_BAR, (b, part)
