@@ -671,8 +671,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const AttnArgs
     // of the way.
     const Item* it = next_item();
     int j = 0;
-    // of its tile: blocks 2 w, 2 w + 1 (-1: past the end), their pages as loaded, the kv head, the length
-    int blk[2] = {-1, -1}, page[2] = {-1, -1}, head = 0, len = 0;
+    // of its tile, for an even lane block 2 w, for an odd one 2 w + 1 (-1: past the end): its page as
+    // loaded, its number in the page; the kv head, the length
+    int blk = -1, page = -1, in_page = 0, head = 0, len = 0;
     int id[2] = {-1, -1};  // the blocks' numbers, once the pages are there
     auto find = [&]() -> bool {                        // tile j, and on to the next; false after the last
       while (it && j >= it->tiles()) {
@@ -680,22 +681,20 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const AttnArgs
         j = 0;
       }
       if (!it) return false;
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const int x = j * kTileBlocks + 2 * w + k;
-        blk[k] = x < it->blocks() ? it->span.block(x) : -1;
-        const int at = blk[k] / a.c.bpp;
-        page[k] = blk[k] >= 0 && at < a.t.width ? __ldg(a.t.pages + it->seq * a.t.stride + at) : -1;
-      }
+      const int x = j * kTileBlocks + 2 * w + (lane & 1);
+      blk = x < it->blocks() ? it->span.block(x) : -1;
+      const int at = blk / a.c.bpp;
+      in_page = blk - at * a.c.bpp;
+      page = blk >= 0 && at < a.t.width ? __ldg(a.t.pages + it->seq * a.t.stride + at) : -1;
       head = it->head;
       len = it->len;
       ++j;
       return true;
     };
     auto number = [&] {
+      const int mine = (unsigned)page < (unsigned)a.c.pages ? (page * a.c.kv_heads + head) * a.c.bpp + in_page : -1;
 #pragma unroll
-      for (int k = 0; k < 2; ++k)
-        id[k] = (unsigned)page[k] < (unsigned)a.c.pages ? (page[k] * a.c.kv_heads + head) * a.c.bpp + blk[k] % a.c.bpp : -1;
+      for (int k = 0; k < 2; ++k) id[k] = __shfl_sync(0xffffffffu, mine, k);
     };
     float ks = 1.f, vs = 0.f;
     int now[2] = {-1, -1}, now_len = 0;  // first positions of the tile's blocks (-1: not there)
@@ -709,7 +708,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const AttnArgs
     };
     auto take = [&] {
 #pragma unroll
-      for (int k = 0; k < 2; ++k) now[k] = id[k] < 0 ? -1 : blk[k] * kKvBlock;
+      for (int k = 0; k < 2; ++k) {
+        const int b = __shfl_sync(0xffffffffu, blk, k);
+        now[k] = id[k] < 0 ? -1 : b * kKvBlock;
+      }
       now_len = len;
     };
     bool here = find();
