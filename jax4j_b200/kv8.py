@@ -91,10 +91,11 @@ class Kv8Cache:
         return t.data_ptr()
 
     def _table(self, table: torch.Tensor) -> tuple:
-        if table.dtype is not torch.int32 or table.dim() != 2 or table.get_device() != self._index or (table.shape[1] > 1 and table.stride(1) != 1):
+        shape, strides = table.shape, table.stride()
+        if len(shape) != 2 or table.dtype is not torch.int32 or table.get_device() != self._index or (strides[1] != 1 and shape[1] > 1):
             raise ValueError(f"the page table must be an int32 tensor [batch, pages of a sequence] on {self.device}, dense within a row")
-        batch, width = table.shape
-        return table.data_ptr(), table.stride(0) if batch > 1 else width, width
+        batch, width = shape
+        return table.data_ptr(), strides[0] if batch > 1 else width, batch, width
 
     def _queries(self, q: torch.Tensor, out: torch.Tensor | None, out_dtype) -> torch.Tensor:
         if q.dim() != 3 or q.shape[2] != self.head_dim or q.get_device() != self._index:
@@ -102,7 +103,8 @@ class Kv8Cache:
         if q.dtype not in _TYPES or (out_dtype is not None and out_dtype not in _TYPES):
             raise ValueError(f"q and the output must be float32 or bfloat16, got {q.dtype} and {out_dtype or q.dtype}")
         if out is None:
-            return q.new_empty(q.shape, dtype=out_dtype)
+            same = (out_dtype is None or out_dtype is q.dtype) and q.is_contiguous()
+            return torch.empty_like(q) if same else q.new_empty(q.shape, dtype=out_dtype)  # the former takes half the time
         if out.shape != q.shape or not out.is_contiguous() or out.get_device() != self._index or out.dtype not in _TYPES:
             raise ValueError("out must be contiguous, float32 or bfloat16, and of q's shape and device")
         return out
@@ -119,7 +121,7 @@ class Kv8Cache:
             n = ctypes.c_int64()
             call("j4b_kv8_decode_workspace", self._ref, heads, batch, ctypes.byref(n))
             need = self._need[heads, batch] = n.value
-        if torch.cuda.is_current_stream_capturing():
+        if torch._C._cuda_isCurrentStreamCapturing():
             return torch.empty(need, dtype=torch.uint8, device=self.device)
         work = self._work.get(stream)
         if work is None or work.shape[0] < need:
@@ -140,9 +142,12 @@ class Kv8Cache:
             raise ValueError(f"rope must be a contiguous float32 tensor [positions, {self.head_dim // 2}, 2] on {self.device}")
         if q_dtype not in _TYPES:
             raise ValueError(f"q must be float32 or bfloat16, got {q_dtype}")
-        at, stride, width = self._table(table)
-        tokens, batch = qkv.shape[0], table.shape[0]
-        q = qkv.new_empty((tokens, heads, self.head_dim), dtype=q_dtype)
+        at, stride, batch, width = self._table(table)
+        tokens = qkv.shape[0]
+        if q_dtype is torch.float32:
+            q = qkv.new_empty((tokens, heads, self.head_dim))
+        else:
+            q = qkv.new_empty((tokens, heads, self.head_dim), dtype=q_dtype)
         call("j4b_kv8_append", self._ref, layer, qkv.data_ptr(), _rows(qkv, "qkv"), tokens, heads, rope.data_ptr(), rope.shape[0], at, stride,
              width, self._ints(starts, "starts", batch), 0 if offsets is None else self._ints(offsets, "offsets", batch + 1), batch,
              q.data_ptr(), _TYPES[q_dtype], self._stream())
@@ -155,9 +160,8 @@ class Kv8Cache:
         lengths[b] - 1 over its cached tokens (with window > 0: the last `window` and the first
         `sinks`). Sequences that see nothing give zeros."""
         out = self._queries(q, out, out_dtype)
-        at, stride, width = self._table(table)
+        at, stride, batch, width = self._table(table)
         rows, heads, _ = q.shape
-        batch = table.shape[0]
         if rows != batch:
             raise ValueError(f"q has {rows} rows for {batch} sequences")
         stream = self._stream()
@@ -174,9 +178,8 @@ class Kv8Cache:
         offsets[b + 1] - 1 of q [tokens, heads, head_dim], are its last tokens (lengths[b] counts
         them). Window, sinks and empty rows as in attention_decode."""
         out = self._queries(q, out, out_dtype)
-        at, stride, width = self._table(table)
+        at, stride, batch, width = self._table(table)
         rows, heads, _ = q.shape
-        batch = table.shape[0]
         call("j4b_kv8_attention_prefill", self._ref, layer, q.data_ptr(), _TYPES[q.dtype], _rows(q, "q"), rows, heads,
              self._ints(offsets, "offsets", batch + 1), at, stride, width, self._ints(lengths, "lengths", batch), batch, window, sinks,
              self.head_dim ** -0.5 if scale is None else scale, out.data_ptr(), _TYPES[out.dtype], self._stream())
