@@ -309,8 +309,10 @@ struct Copies {
 // in one share is finished there; one cut by a share's end leaves an unnormalised part (running
 // maximum, sum, 8 x D) in the workspace for kv8_join_kernel.
 //
-// Bound by HBM once the rows are long: 2 x 16 D bytes a block against ~430 warp instructions at 12
-// warps an SM. What the short ones cost is latency, so a warp never lets its copies run dry: it looks
+// Bound by HBM once the rows are long and D = 128: 64 x 2049 tokens of 32 heads in 180 us, 5.98 TB/s of
+// the 6.55 that a copy reaches; 2 x 131071 of 8 heads 92 us. With D = 64 the ~290 warp instructions of
+// a block (its scores cost as many at any D) bound it: window 4096 of 32 sequences, 41 us against 21
+// of traffic. What the short ones cost is latency, so a warp never lets its copies run dry: it looks
 // up the next 32 blocks, of its next segment too, while it works on these, and fetches the first
 // pair's keys of the next segment before it merges. At the start the pages and the queries are asked
 // for together, and codes before scales (1 x 517 tokens 11.0 -> 10.4 us, ragged batch 61.8 -> 60.0).
@@ -820,8 +822,8 @@ extern "C" int j4b_kv8_attention_decode(const j4b_kv8_cache* cache, int64_t laye
   cudaStream_t stream = resolve_stream(dev, s);
   d.chunks = (d.a.group + kDecHeads - 1) / kDecHeads;
   // Few and short rows are done by a CTA each: no search for its share, no second launch. Measured on
-  // 1 x 32/8 heads, whole against shared out: 1 token 5.9 against 8.7 us, 256 7.7 against 10.4, 517 11.5
-  // against 10.9 (but 3 us less on the host), 1000 15.5 against 12.2.
+  // 1 x 32/8 heads, whole against shared out: 1 token 5.1 against 7.9 us, 256 6.6 against 9.9, 517 10.4
+  // against 10.3 (but 3 us less on the host), 768 11.8 against 10.4.
   const bool whole = batch * cache->kv_heads * d.chunks <= ctas && table_width * cache->page <= kWholeTokens;
   d.part = (float*)(uintptr_t)workspace;
   d.cum = (int64_t*)((uintptr_t)workspace + ((int64_t)2 * ctas * kDecHeads * (cache->head_dim + 2) * 4 + 15) / 16 * 16);

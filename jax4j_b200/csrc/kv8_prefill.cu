@@ -16,6 +16,12 @@
 // 16-code pieces of the next tile while it turns this one's into the swizzled f16 operands; 12 issues
 // the MMAs; 13 finds the next item. S of one tile is computed while the other's softmax runs.
 //
+// Measured: 8 x 2048 causal, 32 heads of 128: 390 us, 705 TFLOP/s (a bf16 product of matrices reaches
+// 1672); 8001 tokens under a window of 1024, 32/8 heads: 198 us. A step of 128 keys takes 2.3 us, of
+// which the tensor cores work 0.6: it is a chain of softmax (1.6, its warps waiting on one another's
+// issue slots, MUFU a third busy) and MMAs (0.7 from the last probability to the next scores). What
+// shortened it most was fewer instructions in the softmax and page warps, which share 4 schedulers.
+//
 // One CTA an SM stays for the whole call and takes items (256 rows of a sequence and kv head): the
 // pages and queries of the next item come while this one's last tiles are worked on. Items are
 // numbered by how far from their sequence's end they lie, so the longest come first, and dealt out
