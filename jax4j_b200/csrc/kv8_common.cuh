@@ -141,8 +141,7 @@ struct AttnArgs {
   float scale_log2;
   void* out;
   int out_type;
-  int* timeout;   // host memory; set when a wait gave up
-  int item_log2;  // prefill: rows of an item
+  int* timeout;  // host memory; set when a wait gave up
 };
 
 // Of numbers that are not negative, and seldom past 31 bits: a 64-bit division takes as long as a load.

@@ -214,8 +214,8 @@ __device__ __forceinline__ void rescale(uint32_t at, int columns, float by) {
 //
 // The loop stays rolled and short: its misses in the instruction cache cost more than a longer
 // loop's parallelism gains (64 keys at a time: 491 us).
-template <int D, bool ALL>
-__device__ __forceinline__ void row_pass(uint32_t s_at, uint32_t o_at, const TileInfo& info, const View& view, float factor, bool begin, int eref, float& m, float& l) {
+template <int D, bool ALL, class Settle>
+__device__ __forceinline__ void row_pass(uint32_t s_at, uint32_t o_at, const TileInfo& info, const View& view, float factor, bool begin, int eref, float& m, float& l, Settle settle) {
   bool again = false;
 #pragma unroll 1
   for (int c = 0; c < kKeys / 32;) {
@@ -270,7 +270,10 @@ __device__ __forceinline__ void row_pass(uint32_t s_at, uint32_t o_at, const Til
       m = mnew;
       tmem_st_wait();
       rescale<true>(s_at, 16 * c, by);
-      if (!begin) rescale<false>(o_at, D, by);
+      if (!begin) {
+        settle();
+        rescale<false>(o_at, D, by);
+      }
       again = true;
       continue;
     }
@@ -288,7 +291,7 @@ __device__ __forceinline__ void warp_arrive(uint64_t* bar, int lane) {
   if (lane == 0) bar_arrive(bar);
 }
 
-// 256 rows (or 128: AttnArgs.item_log2) of one (sequence, kv head).
+// 256 rows (or 128, LOG2 7) of one (sequence, kv head).
 struct Item {
   int seq, head;               // seq -1: no more
   int row0, len, pos0;         // the sequence's first row of q, its length, the position of its query 0
@@ -301,19 +304,21 @@ struct Item {
 };
 
 // Items of a sequence, before its kv heads.
+template <int LOG2>
 __device__ __forceinline__ int items_of(const AttnArgs& a, int b) {
   const int64_t rows = (int64_t)max(0, __ldg(a.offsets + b + 1) - __ldg(a.offsets + b)) * a.group;
-  return (int)((rows + (1 << a.item_log2) - 1) >> a.item_log2);
+  return (int)((rows + (1 << LOG2) - 1) >> LOG2);
 }
 // Item number f of the call, for a warp: all last items of the sequences, then all last but one, ...
+template <int LOG2>
 __device__ __forceinline__ void find_item(const AttnArgs& a, int64_t f, int lane, Item& it) {
   it.seq = -1;
   const int64_t m = kv8_quotient(f, a.c.kv_heads);
   // of the first 32 sequences, which are mostly all
-  const int own = lane < a.batch ? items_of(a, lane) : 0, own_len = lane < a.batch ? __ldg(a.lengths + lane) : 0;
+  const int own = lane < a.batch ? items_of<LOG2>(a, lane) : 0, own_len = lane < a.batch ? __ldg(a.lengths + lane) : 0;
   auto items_up_to = [&](int most) -> int64_t {            // sum over the sequences of min(items, most)
     unsigned n = (unsigned)min(most, own);
-    for (int b = lane + 32; b < a.batch; b += 32) n += (unsigned)min(most, items_of(a, b));
+    for (int b = lane + 32; b < a.batch; b += 32) n += (unsigned)min(most, items_of<LOG2>(a, b));
     return __reduce_add_sync(0xffffffffu, n);
   };
   if (m >= items_up_to(0x7fffffff)) return;
@@ -332,7 +337,7 @@ __device__ __forceinline__ void find_item(const AttnArgs& a, int64_t f, int lane
   int64_t left = m - items_up_to(lo);  // this many sequences of more than lo items come before
   int b = 0;
   for (int base = 0;; base += 32) {
-    const uint32_t has = __ballot_sync(0xffffffffu, (base == 0 ? own : base + lane < a.batch ? items_of(a, base + lane) : 0) > lo);
+    const uint32_t has = __ballot_sync(0xffffffffu, (base == 0 ? own : base + lane < a.batch ? items_of<LOG2>(a, base + lane) : 0) > lo);
     if (left >= __popc(has)) {
       left -= __popc(has);
       continue;
@@ -346,8 +351,8 @@ __device__ __forceinline__ void find_item(const AttnArgs& a, int64_t f, int lane
   const int n = __ldg(a.offsets + b + 1) - it.row0;
   it.len = b < 32 ? __shfl_sync(0xffffffffu, own_len, b) : __ldg(a.lengths + b);
   it.pos0 = it.len - n;  // negative: the first queries are before the cache and see nothing
-  it.first_row = (items_of(a, b) - 1 - lo) << a.item_log2;
-  it.rows = (int)min((int64_t)1 << a.item_log2, (int64_t)n * a.group - it.first_row);
+  it.first_row = (items_of<LOG2>(a, b) - 1 - lo) << LOG2;
+  it.rows = (int)min((int64_t)1 << LOG2, (int64_t)n * a.group - it.first_row);
   auto span_of_tile = [&](int i, int tiles) {  // of tiles i .. i + tiles - 1
     const int from = it.first_row + i * kRows, to = it.first_row + min(it.rows, (i + tiles) * kRows) - 1;
     return span_of(max(0, it.pos0 + from / a.group), min(it.len - 1, it.pos0 + to / a.group), a.window, a.sinks);
@@ -487,7 +492,8 @@ __device__ __forceinline__ void prefetch_queries(const AttnArgs& a, const Item& 
 constexpr int kItems = 4;         // found ahead
 constexpr int kItemReaders = 13;  // warps
 
-template <int D, int TYPE>
+// SINGLE: items of one tile of rows.
+template <int D, int TYPE, bool SINGLE>
 __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const AttnArgs a) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = aligned_smem(smem_raw);
@@ -496,12 +502,13 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const AttnArgs
   uint8_t* sraw = sk + 2 * kStages * Smem<D>::kOperand;
   TileInfo* infos = reinterpret_cast<TileInfo*>(sraw + 2 * Smem<D>::kRaw);
   __shared__ uint64_t item_full[kItems], item_empty[kItems], q_ready[2], q_empty[2], k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages],
-      s_full[2], p_ready[2], o_full[2], o_seen[2];
+      s_full[2], p_ready[2], o_step, o_full[2], o_seen[2];
   __shared__ uint32_t tmem_slot;
   __shared__ Item items[kItems];
   __shared__ uint8_t factors[2][kRows];  // a warp's are its own rows'
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if (tid == 0) {
+    bar_init(&o_step, 1);
     for (int i = 0; i < kItems; ++i) {
       bar_init(&item_full[i], 1);
       bar_init(&item_empty[i], kItemReaders);
@@ -531,6 +538,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const AttnArgs
   tc_fence_after();
   const uint32_t tmem = tmem_slot;  // S0, S1 at columns 0, 128 (P over them); O0, O1 at 256, 384
   bool ok = true;
+  // An item of one tile has the other's columns, too: its scores, and the barriers s_full and p_ready,
+  // alternate between the two, and a key tile's are there before the last one's softmax ends (5 turns
+  // of up to 77 tokens on up to 1000: 27.0 -> 24.5 us).
   // The next item, for every warp but the one that finds them (null after the last); the one before
   // is given back. Read where it is: a copy would cost registers.
   uint32_t nth = 0;
@@ -576,7 +586,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const AttnArgs
       const int j0 = it.begin[i], j1 = it.end[i];
       for (int j = j0; j < j1; ++j, ++use) {
         const uint32_t k = before + (uint32_t)j;
-        ok = ok && kv8_wait(&s_full[i], use & 1);  // with it comes the tile's info
+        const uint32_t buffer = SINGLE ? use & 1 : (uint32_t)i, parity = SINGLE ? use >> 1 & 1 : use & 1;
+        const uint32_t s_now = SINGLE ? s_at + buffer * 128u : s_at;
+        ok = ok && kv8_wait(&s_full[buffer], parity);  // with it comes the tile's info
         tc_fence_after();
         const TileInfo& info = infos[k % kInfos];
         int near = kNowhere, far = 0, ev = -127;
@@ -587,22 +599,30 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const AttnArgs
           ev = max(ev, info.ev[x]);
         }
         const bool all = far - 1 <= least && (near >= most_lo || far <= a.sinks);
-        // the last tile's values were ready before these scores were
-        if (j > j0 && sees_nan(infos[(k - 1) % kInfos], view)) l = NAN;
+        // the last tile's values (with a tile alone the last but one's) were ready before these scores were
+        const int late = SINGLE ? 2 : 1;
+        if (j - late >= j0 && sees_nan(infos[(k - late) % kInfos], view)) l = NAN;
+        auto settle = [&] {  // the MMAs on O are done; of two tiles, before these scores
+          if (SINGLE) {
+            ok = ok && kv8_wait(&o_step, (use - 1) & 1);
+            tc_fence_after();
+          }
+        };
         const bool begin = j == j0;
         if (begin) {
           eref = ev;
         } else if (ev > eref) {
+          settle();
           rescale<false>(o_at, D, exp2_ftz((float)(eref - ev)));
           eref = ev;
         }
         if (all)
-          row_pass<D, true>(s_at, o_at, info, view, factor, begin, eref, m, l);
+          row_pass<D, true>(s_now, o_at, info, view, factor, begin, eref, m, l, settle);
         else
-          row_pass<D, false>(s_at, o_at, info, view, factor, begin, eref, m, l);
+          row_pass<D, false>(s_now, o_at, info, view, factor, begin, eref, m, l, settle);
         tmem_st_wait();
         tc_fence_before();
-        warp_arrive(&p_ready[i], lane);
+        warp_arrive(&p_ready[buffer], lane);
       }
       const uint32_t last_tile = before + (uint32_t)j1 - 1;
       before += (uint32_t)it.tiles();
@@ -614,7 +634,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const AttnArgs
       if (active) {
         ok = ok && kv8_wait(&o_full[i], (outs - 1) & 1);
         tc_fence_after();
-        if (sees_nan(infos[last_tile % kInfos], view)) l = NAN;
+        if (sees_nan(infos[last_tile % kInfos], view) || (SINGLE && j1 - 1 > j0 && sees_nan(infos[(last_tile - 1) % kInfos], view))) l = NAN;
         warp_arrive(&o_seen[i], lane);
       }
       if (i * kRows < rows) {
@@ -798,66 +818,116 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const AttnArgs
       constexpr uint32_t kStage = 2 * Smem<D>::kOperand / 16;
       uint32_t p_use0 = 0, p_use1 = 0, q_use0 = 0, q_use1 = 0, before = 0;
       bool left0 = false, left1 = false;  // the last item's softmax may still need its last info
-      uint32_t s_use0 = 0, s_use1 = 0;
+      uint32_t s_use0 = 0, s_use1 = 0, scores = 0;
       while (const Item* const item = next_item()) {
         const int nt = uni(item->tiles()), b0 = uni(item->begin[0]), b1 = uni(item->begin[1]), e0 = uni(item->end[0]), e1 = uni(item->end[1]);
-        for (int j = -1; j < nt && ok; ++j) {
-          const uint32_t now = before + (uint32_t)j, next = now + 1;
-          if (j + 1 < nt) wait(&k_full[next & 1], next >> 1 & 1);
-          if (j >= 0) wait(&v_full[now & 1], now >> 1 & 1);
-          // No further until the last item's infos are read: a softmax that has no part in this item could
-          // fall behind by more than kInfos tiles (three of this and the next item may have infos by now).
-          if (j == 0) {
-            if (left0) wait(&o_seen[0], s_use0++ & 1);
-            if (left1) wait(&o_seen[1], s_use1++ & 1);
-            left0 = e0 > b0;
-            left1 = e1 > b1;
-          }
-          const uint64_t vt = vd + (now & 1) * kStage, kt = kd + (next & 1) * kStage;
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int begin = i ? b1 : b0, end = i ? e1 : e0;
-            uint32_t &p_use = i ? p_use1 : p_use0, &q_use = i ? q_use1 : q_use0;
-            const uint32_t s_at = tmem + (uint32_t)(i * 128), o_at = tmem + 256u + (uint32_t)(i * 128);
-            if (j >= begin && j < end) {
-              wait(&p_ready[i], p_use & 1);
-              ++p_use;
-              tc_fence_after();
-              if (elect_one()) {
-                const uint32_t later = j > begin;
-#pragma unroll
-                for (int k = 0; k < kKeys / 16; ++k)  // 16 keys: 8 columns of P, 2 groups of 8 rows of V
-                  umma_ts(o_at, s_at + 8u * k, vt + k * (2048 / 16), io, k > 0 ? 1u : later);
-                if (j + 1 == end) {
-                  umma_commit(&o_full[i]);
-                  bar_arrive(&o_full[i]);
-                }
-              }
+        if constexpr (SINGLE) {
+          for (int j = -1; j < nt && ok; ++j) {
+            const uint32_t now = before + (uint32_t)j, next = now + 1;
+            if (j + 1 < nt) wait(&k_full[next & 1], next >> 1 & 1);
+            if (j == 0) {  // as below
+              if (left0) wait(&o_seen[0], s_use0++ & 1);
+              left0 = e0 > b0;
             }
-            if (j + 1 >= begin && j + 1 < end) {
-              if (j + 1 == begin) {
-                wait(&q_ready[i], q_use & 1);
-                ++q_use;
-              }
+            if (j + 1 >= b0 && j + 1 < e0) {
+              if (j + 1 == b0) wait(&q_ready[0], q_use0++ & 1);
               tc_fence_after();
               if (elect_one()) {
-                const uint64_t qt = qd + (uint32_t)(i * Smem<D>::kQ / 16);
+                const uint64_t kt = kd + (next & 1) * kStage;
+                const uint32_t s_at = tmem + (scores & 1) * 128u;
 #pragma unroll
                 for (int k = 0; k < D / 16; ++k) {
-                  const uint32_t off = ((k >> 2) * (kRows * 128) + (k & 3) * 32) / 16;  // kRows == kKeys
-                  umma_ss(s_at, qt + off, kt + off, is, k > 0 ? 1u : 0u);
+                  const uint32_t off = ((k >> 2) * (kRows * 128) + (k & 3) * 32) / 16;
+                  umma_ss(s_at, qd + off, kt + off, is, k > 0 ? 1u : 0u);
                 }
-                umma_commit(&s_full[i]);
-                bar_arrive(&s_full[i]);
-                if (j + 2 == end) umma_commit(&q_empty[i]);
+                umma_commit(&s_full[scores & 1]);
+                bar_arrive(&s_full[scores & 1]);
+                if (j + 2 == e0) umma_commit(&q_empty[0]);
+              }
+              ++scores;
+            }
+            if (j + 1 < nt && elect_one()) umma_commit(&k_empty[next & 1]);
+            __syncwarp();
+            if (j < 0) continue;
+            wait(&v_full[now & 1], now >> 1 & 1);
+            if (j >= b0 && j < e0) {
+              wait(&p_ready[p_use0 & 1], p_use0 >> 1 & 1);
+              tc_fence_after();
+              if (elect_one()) {
+                const uint64_t vt = vd + (now & 1) * kStage;
+                const uint32_t later = j > b0;
+#pragma unroll
+                for (int k = 0; k < kKeys / 16; ++k) umma_ts(tmem + 256u, tmem + (p_use0 & 1) * 128u + 8u * k, vt + k * (2048 / 16), io, k > 0 ? 1u : later);
+                umma_commit(&o_step);
+                if (j + 1 == e0) {
+                  umma_commit(&o_full[0]);
+                  bar_arrive(&o_full[0]);
+                }
+              }
+              ++p_use0;
+            }
+            if (elect_one()) umma_commit(&v_empty[now & 1]);
+            __syncwarp();
+          }
+        } else {
+          for (int j = -1; j < nt && ok; ++j) {
+            const uint32_t now = before + (uint32_t)j, next = now + 1;
+            if (j + 1 < nt) wait(&k_full[next & 1], next >> 1 & 1);
+            if (j >= 0) wait(&v_full[now & 1], now >> 1 & 1);
+            // No further until the last item's infos are read: a softmax that has no part in this item could
+            // fall behind by more than kInfos tiles (three of this and the next item may have infos by now).
+            if (j == 0) {
+              if (left0) wait(&o_seen[0], s_use0++ & 1);
+              if (left1) wait(&o_seen[1], s_use1++ & 1);
+              left0 = e0 > b0;
+              left1 = e1 > b1;
+            }
+            const uint64_t vt = vd + (now & 1) * kStage, kt = kd + (next & 1) * kStage;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const int begin = i ? b1 : b0, end = i ? e1 : e0;
+              uint32_t &p_use = i ? p_use1 : p_use0, &q_use = i ? q_use1 : q_use0;
+              const uint32_t s_at = tmem + (uint32_t)(i * 128), o_at = tmem + 256u + (uint32_t)(i * 128);
+              if (j >= begin && j < end) {
+                wait(&p_ready[i], p_use & 1);
+                ++p_use;
+                tc_fence_after();
+                if (elect_one()) {
+                  const uint32_t later = j > begin;
+#pragma unroll
+                  for (int k = 0; k < kKeys / 16; ++k)  // 16 keys: 8 columns of P, 2 groups of 8 rows of V
+                    umma_ts(o_at, s_at + 8u * k, vt + k * (2048 / 16), io, k > 0 ? 1u : later);
+                  if (j + 1 == end) {
+                    umma_commit(&o_full[i]);
+                    bar_arrive(&o_full[i]);
+                  }
+                }
+              }
+              if (j + 1 >= begin && j + 1 < end) {
+                if (j + 1 == begin) {
+                  wait(&q_ready[i], q_use & 1);
+                  ++q_use;
+                }
+                tc_fence_after();
+                if (elect_one()) {
+                  const uint64_t qt = qd + (uint32_t)(i * Smem<D>::kQ / 16);
+#pragma unroll
+                  for (int k = 0; k < D / 16; ++k) {
+                    const uint32_t off = ((k >> 2) * (kRows * 128) + (k & 3) * 32) / 16;  // kRows == kKeys
+                    umma_ss(s_at, qt + off, kt + off, is, k > 0 ? 1u : 0u);
+                  }
+                  umma_commit(&s_full[i]);
+                  bar_arrive(&s_full[i]);
+                  if (j + 2 == end) umma_commit(&q_empty[i]);
+                }
               }
             }
+            if (elect_one()) {
+              if (j + 1 < nt) umma_commit(&k_empty[next & 1]);
+              if (j >= 0) umma_commit(&v_empty[now & 1]);
+            }
+            __syncwarp();
           }
-          if (elect_one()) {
-            if (j + 1 < nt) umma_commit(&k_empty[next & 1]);
-            if (j >= 0) umma_commit(&v_empty[now & 1]);
-          }
-          __syncwarp();
         }
         before += (uint32_t)nt;
       }
@@ -866,7 +936,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const AttnArgs
       bool more = true;
       for (uint32_t r = 0; more && ok; ++r) {
         Item it;
-        find_item(a, (int64_t)r * gridDim.x + (r & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x), lane, it);
+        find_item<SINGLE ? 7 : 8>(a, (int64_t)r * gridDim.x + (r & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x), lane, it);
         if (r >= kItems) ok = __all_sync(0xffffffffu, ok && kv8_wait(&item_empty[r % kItems], (r / kItems - 1) & 1));
         if (lane == 0) {
           items[r % kItems] = it;
@@ -888,25 +958,28 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const AttnArgs
   }
 }
 
-template <int D, int TYPE>
-int launch_prefill(AttnArgs& a, int dev, cudaStream_t stream) {
+template <int D, int TYPE, bool SINGLE>
+int launch_prefill_kernel(const AttnArgs& a, int64_t items, int dev, cudaStream_t stream) {
   static bool done[kMaxDevices] = {};
   if (!done[dev]) {
-    J4B_CUDA(cudaFuncSetAttribute(kv8_prefill_kernel<D, TYPE>, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<D>::kBytes), "cudaFuncSetAttribute");
+    J4B_CUDA(cudaFuncSetAttribute(kv8_prefill_kernel<D, TYPE, SINGLE>, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<D>::kBytes), "cudaFuncSetAttribute");
     done[dev] = true;
   }
-  const int64_t rows = a.tokens * a.group;
-  J4B_REQUIRE(rows <= 0x3fffffffLL, "kv8 prefill: too many rows");
-  const DeviceCtx* ctx = device_ctx(dev);
-  auto items_of_rows = [&](int log2) { return std::min(rows, (rows >> log2) + a.batch) * a.c.kv_heads; };  // at most
-  // A tile of 128 rows alone walks its keys faster than one of two, so where every such tile has an SM
-  // to itself, items are one tile (5 turns of up to 77 tokens on up to 1000: 31.6 -> 27.0 us). Two
-  // share the work on the pages elsewhere (8 x 2048: 396 us, by single tiles 642).
-  a.item_log2 = items_of_rows(7) <= ctx->sm_count ? 7 : 8;
-  const int64_t items = items_of_rows(a.item_log2);
-  kv8_prefill_kernel<D, TYPE><<<(unsigned)std::min<int64_t>(items, ctx->sm_count), kThreads, Smem<D>::kBytes, stream>>>(a);
+  kv8_prefill_kernel<D, TYPE, SINGLE><<<(unsigned)std::min<int64_t>(items, device_ctx(dev)->sm_count), kThreads, Smem<D>::kBytes, stream>>>(a);
   J4B_CHECK_LAUNCH("kv8_prefill_kernel");
   return J4B_OK;
+}
+
+template <int D, int TYPE>
+int launch_prefill(const AttnArgs& a, int dev, cudaStream_t stream) {
+  const int64_t rows = a.tokens * a.group;
+  J4B_REQUIRE(rows <= 0x3fffffffLL, "kv8 prefill: too many rows");
+  auto items = [&](int log2) { return std::min(rows, (rows >> log2) + a.batch) * a.c.kv_heads; };  // at most
+  // A tile of 128 rows alone walks its keys faster than one of two, so where every such tile has an SM
+  // to itself, items are one tile (5 turns of up to 77 tokens on up to 1000: 31.6 -> 24.5 us). Two
+  // share the work on the pages elsewhere (8 x 2048: 390 us, by tiles alone 642).
+  if (items(7) <= device_ctx(dev)->sm_count) return launch_prefill_kernel<D, TYPE, true>(a, items(7), dev, stream);
+  return launch_prefill_kernel<D, TYPE, false>(a, items(8), dev, stream);
 }
 
 }  // namespace
