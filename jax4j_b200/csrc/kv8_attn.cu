@@ -322,7 +322,7 @@ constexpr int kDecWarps = 4;
 constexpr int dec_ctas(int dim) { return dim == 64 ? 4 : 3; }
 constexpr int kDecHeads = 8;
 constexpr int kWholeTokens = 576;
-constexpr int kRowUnits = 20;  // 4: ragged batch (48 x up to 8191 tokens) 78.9 us, 12: 67.8, 20: 61.6, 28: 61.7, 40: 63.5
+constexpr int kRowUnits = 20;  // 12: ragged batch (48 x up to 8191 tokens) 64.2 us, 20: 60.0, 28: 61.1
 
 struct DecArgs {
   AttnArgs a;
