@@ -15,6 +15,7 @@ from __future__ import annotations
 
 import ctypes
 import heapq
+import threading
 
 import torch
 
@@ -82,6 +83,7 @@ class Kv8Cache:
         self._index = k.device.index if k.device.type == "cuda" else -1
         self._need = {}  # (heads, batch) -> bytes of the decode workspace
         self._work = {}  # stream -> workspace
+        self._lock = threading.Lock()  # of the two
         self._desc = _lib.Kv8CacheDesc(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), layers, pages, kv_heads, page, dim)
         self._ref = ctypes.byref(self._desc)
 
@@ -165,10 +167,13 @@ class Kv8Cache:
         if rows != batch:
             raise ValueError(f"q has {rows} rows for {batch} sequences")
         stream = self._stream()
-        work = self._workspace(heads, batch, stream)
-        call("j4b_kv8_attention_decode", self._ref, layer, q.data_ptr(), _TYPES[q.dtype], _rows(q, "q"), heads, at, stride, width,
-             self._ints(lengths, "lengths", batch), batch, window, sinks, self.head_dim ** -0.5 if scale is None else scale, out.data_ptr(),
-             _TYPES[out.dtype], work.data_ptr(), work.shape[0], stream)
+        # A call may be two launches that share the workspace. ctypes runs it without the interpreter's
+        # lock, so another thread's call on the same stream could come between them.
+        with self._lock:
+            work = self._workspace(heads, batch, stream)
+            call("j4b_kv8_attention_decode", self._ref, layer, q.data_ptr(), _TYPES[q.dtype], _rows(q, "q"), heads, at, stride, width,
+                 self._ints(lengths, "lengths", batch), batch, window, sinks, self.head_dim ** -0.5 if scale is None else scale,
+                 out.data_ptr(), _TYPES[out.dtype], work.data_ptr(), work.shape[0], stream)
         return out
 
     def attention_prefill(self, q: torch.Tensor, offsets: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, window: int = 0,

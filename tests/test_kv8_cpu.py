@@ -1,6 +1,8 @@
 """CPU tests of the 8-bit KV cache: the float64 oracle's format against PyTorch's float8, the scale
 rule, and what the C ABI and the host classes refuse before they touch a device."""
 import ctypes
+import threading
+import time
 
 import numpy as np
 import pytest
@@ -172,3 +174,33 @@ def test_page_table_trims_a_window_and_compacts():
     _consistent(t)
     with pytest.raises(ValueError, match="positive window"):
         t.trim(0)
+
+
+def test_decode_calls_of_two_threads_never_share_a_workspace(monkeypatch):
+    """A decode call is two launches around one workspace: until it has returned, no other thread's
+    call on the stream may be given the same."""
+    from jax4j_b200 import kv8
+    busy, clashes = [], []
+
+    def fake(name, *args):
+        if name == "j4b_kv8_decode_workspace":
+            args[-1]._obj.value = 256
+            return
+        work = args[-3]
+        if work in busy:
+            clashes.append(work)
+        busy.append(work)
+        time.sleep(0.01)
+        busy.remove(work)
+    monkeypatch.setattr(kv8, "call", fake)
+    monkeypatch.setattr(torch._C, "_cuda_isCurrentStreamCapturing", lambda: False, raising=False)
+    monkeypatch.setattr(kv8.Kv8Cache, "_stream", lambda self: 7)
+    codes = torch.zeros(1, 3, 2, 32, 64, dtype=torch.uint8).view(torch.float8_e4m3fn)
+    cache = kv8.Kv8Cache.wrap(codes, codes, torch.zeros(1, 3, 2, 2), torch.zeros(1, 3, 2, 2))
+    q, table, lengths = torch.zeros(1, 2, 64), torch.zeros(1, 1, dtype=torch.int32), torch.ones(1, dtype=torch.int32)
+    threads = [threading.Thread(target=lambda: [cache.attention_decode(q, table, lengths) for _ in range(5)]) for _ in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not clashes

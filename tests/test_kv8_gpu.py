@@ -580,3 +580,28 @@ def test_prefill_of_two_tiles_an_item_with_nan_and_unmapped_pages(window, sinks)
         for part in (slice(0, 128), slice(128, 256), slice(256, n)):
             keep = ~want[offsets[b]:offsets[b + 1]][part]
             assert normwise(mine[part][keep], ref[part][keep]) <= PREFILL_BAR, (b, part)
+
+
+def test_decode_of_two_threads_on_one_stream():
+    """Threads share PyTorch's default stream and the cache: each gets its own results."""
+    import threading
+    rng = np.random.default_rng(51)
+    pool = Pool(rng, [4000, 17, 900, 2500], 2, 64, 128)
+    table = ints(pool.table)
+    jobs = []
+    for i in range(4):
+        lengths = ints([int(n * f) for n, f in zip(pool.lengths, rng.uniform(0.1, 1, 4))])
+        q = torch.from_numpy(rng.standard_normal((4, 8, 128)).astype(np.float32)).cuda()
+        jobs.append((q, lengths, pool.cache.attention_decode(q, table, lengths)))
+    bad = []
+
+    def work(q, lengths, want):
+        outs = [pool.cache.attention_decode(q, table, lengths) for _ in range(200)]
+        torch.cuda.synchronize()
+        bad.extend(i for i, o in enumerate(outs) if not torch.equal(o, want))
+    threads = [threading.Thread(target=work, args=job) for job in jobs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
