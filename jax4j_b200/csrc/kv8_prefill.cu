@@ -45,6 +45,10 @@ constexpr float kMost = 65504.f;     // f16's largest
 // log2 of the probability that stands for 1. Above it is room for a maximum outgrown 2^12 times; below
 // it f16 has all its bits down to 2^-18 and some to 2^-28, for far keys and blocks of small value scale.
 constexpr int kShift = 4;
+// A block that a row sees a part of may outweigh the row's reference by this many binades: its scale
+// may come from tokens that the row does not see. Such a probability of 1 is 2^15.
+constexpr int kPartRoom = 11;
+constexpr int kNoScale = -127;       // below every exponent of a scale
 
 // What the softmax needs of a key tile.
 struct __align__(16) TileInfo {
@@ -185,6 +189,60 @@ __device__ __forceinline__ bool sees_nan(const TileInfo& info, const View& view)
   return found != 0;
 }
 
+// 256 rows (or 128, LOG2 7) of one (sequence, kv head).
+struct Item {
+  int seq, head;               // seq -1: no more
+  int row0, len, pos0;         // the sequence's first row of q, its length, the position of its query 0
+  int first_row, rows;         // this item's first row, and its number of rows
+  Span span;                   // blocks that any of them sees
+  int begin[2], end[2];        // key tiles of each tile of 128 rows: [begin, end) of the span's list
+  __device__ __forceinline__ bool active(int i) const { return end[i] > begin[i]; }
+  __device__ __forceinline__ int blocks() const { return max(0, span.count()); }
+  __device__ __forceinline__ int tiles() const { return (blocks() + kTileBlocks - 1) / kTileBlocks; }
+};
+
+// Whether a value of the block's tokens in `see` has a code that is not zero.
+__device__ __forceinline__ bool holds_values(const AttnArgs& a, int seq, int head, int pos, uint32_t see, int dim) {
+  const int id = kv8_block_id(a.c, a.t, seq, head, pos / kKvBlock);
+  uint32_t any = 0;
+  if (id < 0) return false;
+#pragma unroll 1
+  for (; see != 0 && any == 0; see &= see - 1) {
+    const uint4* v = reinterpret_cast<const uint4*>(a.c.v + ((int64_t)id * kKvBlock + (__ffs(see) - 1)) * dim);
+#pragma unroll 1
+    for (int i = 0; i < dim / 16; ++i) any |= (v[i].x | v[i].y | v[i].z | v[i].w) & 0x7f7f7f7fu;
+  }
+  return any != 0;
+}
+
+// The exponent of the value scale that a row's probabilities are weighed by: the largest of the blocks
+// it sees, `before` or here. What it does not see must not count, or a loud value among it would
+// shift the row's probabilities out of f16. A block seen in part has kPartRoom, and beyond that
+// counts only if one of its seen values is not zero (next to a token that much louder, few are
+// anything else). Runs where a tile's scales exceed a row's reference, so seldom.
+__device__ __forceinline__ int seen_exponent(const AttnArgs& a, const Item& it, const TileInfo& info, const View& view, int before, int dim) {
+  int most = before, part = before;
+#pragma unroll 1
+  for (int k = 0; k < kTileBlocks; ++k) {
+    const int ev = info.ev[k];
+    if (ev <= most) continue;
+    const uint32_t see = view.mask(info.pos[k]);
+    if (see == 0xffffu)
+      most = ev;
+    else if (see != 0)
+      part = max(part, ev - kPartRoom);
+  }
+  if (part <= most) return most;
+#pragma unroll 1
+  for (int k = 0; k < kTileBlocks; ++k) {
+    const int ev = info.ev[k] - kPartRoom;
+    if (ev <= most) continue;
+    const uint32_t see = view.mask(info.pos[k]);
+    if (see != 0 && see != 0xffffu && holds_values(a, it.seq, it.head, info.pos[k], see, dim)) most = ev;
+  }
+  return most;
+}
+
 // Columns of TMEM of a warp's rows times a factor of each: f32, or pairs of f16.
 template <bool HALF>
 __device__ __forceinline__ void rescale(uint32_t at, int columns, float by) {
@@ -230,7 +288,8 @@ __device__ __forceinline__ void row_pass(uint32_t s_at, uint32_t o_at, const Til
     for (int h = 0; h < 2; ++h) {
       const uint32_t* x = v + 16 * h;
       const float f = factor * (h ? ks.y : ks.x);
-      const int w = max(-60, (h ? ev.y : ev.x) - eref) + kShift;
+      int w = max(-60, (h ? ev.y : ev.x) - eref) + kShift;
+      if (!ALL) w = min(w, kShift + kPartRoom);  // more: nothing of the block is seen, or only zeros
       const uint32_t see = ALL ? 0xffffu : view.mask(info.pos[2 * c + h]);
       seen |= see;
       const uint64_t ff = pair(f, f), add = pair((float)w - base, (float)w - base);
@@ -290,18 +349,6 @@ __device__ __forceinline__ void warp_arrive(uint64_t* bar, int lane) {
   __syncwarp();
   if (lane == 0) bar_arrive(bar);
 }
-
-// 256 rows (or 128, LOG2 7) of one (sequence, kv head).
-struct Item {
-  int seq, head;               // seq -1: no more
-  int row0, len, pos0;         // the sequence's first row of q, its length, the position of its query 0
-  int first_row, rows;         // this item's first row, and its number of rows
-  Span span;                   // blocks that any of them sees
-  int begin[2], end[2];        // key tiles of each tile of 128 rows: [begin, end) of the span's list
-  __device__ __forceinline__ bool active(int i) const { return end[i] > begin[i]; }
-  __device__ __forceinline__ int blocks() const { return max(0, span.count()); }
-  __device__ __forceinline__ int tiles() const { return (blocks() + kTileBlocks - 1) / kTileBlocks; }
-};
 
 // Items of a sequence, before its kv heads.
 template <int LOG2>
@@ -582,7 +629,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const AttnArgs
       const int least = it.pos0 + (it.first_row + i * kRows) / a.group;
       const int most_lo = a.window > 0 ? max(0, it.pos0 + (it.first_row + min(it.rows, (i + 1) * kRows) - 1) / a.group - a.window + 1) : 0;
       float m = -INFINITY, l = 0.f;
-      int eref = 0;  // exponent of the value scale that O is in units of
+      int eref = valid ? kNoScale : -kNoScale;  // exponent of the value scale that O is in units of
       const int j0 = it.begin[i], j1 = it.end[i];
       for (int j = j0; j < j1; ++j, ++use) {
         const uint32_t k = before + (uint32_t)j;
@@ -609,12 +656,13 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const AttnArgs
           }
         };
         const bool begin = j == j0;
-        if (begin) {
-          eref = ev;
-        } else if (ev > eref) {
-          settle();
-          rescale<false>(o_at, D, exp2_ftz((float)(eref - ev)));
-          eref = ev;
+        if (__any_sync(0xffffffffu, ev > eref)) {
+          const int now = all ? max(ev, eref) : seen_exponent(a, it, info, view, eref, D);
+          if (!begin && __any_sync(0xffffffffu, now > eref)) {
+            settle();
+            rescale<false>(o_at, D, exp2_ftz((float)(eref - now)));
+          }
+          eref = now;
         }
         if (all)
           row_pass<D, true>(s_now, o_at, info, view, factor, begin, eref, m, l, settle);
@@ -761,7 +809,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const AttnArgs
         const int x = 2 * w + lane, pos = lane == 0 ? now[0] : now[1];
         info.pos[x] = pos < 0 ? kNowhere : pos;
         info.ks[x] = ks;
-        info.ev[x] = (int)(__float_as_uint(vs) >> 23) - 127;
+        info.ev[x] = (int)(__float_as_uint(vs) >> 23) + kNoScale;
       }
       to_async_proxy();
       warp_arrive(&k_full[s], lane);

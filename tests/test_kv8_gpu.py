@@ -605,3 +605,46 @@ def test_decode_of_two_threads_on_one_stream():
     for t in threads:
         t.join()
     assert not bad
+
+
+def hide_loud_values(pool, b, at, up, alone):
+    """Makes the value of token `at` of sequence b 2^up times as loud as its block's scale has the
+    others: with its whole block, or (`alone`) by itself, and the block's other values are then below
+    the format's smallest."""
+    from oracle.kv8 import BLOCK
+    pg, blk = pool.table[b, at // pool.page], at % pool.page // BLOCK
+    rows = slice(blk * BLOCK, (blk + 1) * BLOCK)
+    pool.vs[pg, :, blk] *= 2.0 ** up
+    if alone:
+        keep = pool.v[pg, :, at % pool.page].copy()
+        pool.v[pg, :, rows] = 0
+        pool.v[pg, :, at % pool.page] = keep
+    codes = to_f8(pool.v[pg])
+    pool.cache.v[pool.layer, int(pg)].view(torch.uint8).copy_(codes.view(torch.uint8))
+    pool.cache.v_scale[pool.layer, int(pg)] = torch.from_numpy(pool.vs[pg]).float()
+
+
+def quiet_keys(pool):
+    """Scores near zero, so that every seen token counts."""
+    pool.ks *= 2.0 ** np.round(np.log2(0.05) - np.log2(np.abs(pool.k).max((-1, -2)).reshape(pool.ks.shape[0], pool.ks.shape[1], 1) * pool.ks))
+    pool.cache.k_scale[pool.layer] = torch.from_numpy(pool.ks).float()
+
+
+@pytest.mark.parametrize("up,alone", [(24, False), (24, True), (40, False), (40, True)])
+@pytest.mark.parametrize("heads,kv,dim,window,sinks", [(2, 1, 64, 0, 0), (8, 2, 128, 70, 0), (8, 2, 128, 70, 21), (32, 16, 64, 90, 5), (32, 32, 128, 0, 0)])
+def test_prefill_rows_do_not_feel_loud_values_they_do_not_see(heads, kv, dim, window, sinks, up, alone):
+    """f16 probabilities are weighed by the largest value scale that a row sees: one that it does not
+    see may not push them out of f16's range. Every row by itself, those just before a loud token in
+    its own block, too."""
+    rng = np.random.default_rng(heads + dim + window + up)
+    n = 420
+    pool, offsets, q = prefill_inputs(rng, [(0, n)], heads, kv, dim, 32, torch.float32)
+    quiet_keys(pool)
+    for at in (23, 201, 333):
+        hide_loud_values(pool, 0, at, up, alone)
+    got = pool.cache.attention_prefill(q, ints(offsets), ints(pool.table), ints(pool.lengths), window=window, sinks=sinks).double().cpu().numpy()
+    rows = np.unique(np.concatenate([np.arange(0, n, 37), np.arange(16, 40), np.arange(190, 225), np.arange(200 + 60, 200 + 95), np.arange(320, 345), [n - 1]]))
+    qh = q.double().cpu().numpy()
+    for i in rows:
+        want = pool.reference(qh[i:i + 1], 0, i, window, sinks)[0]
+        assert normwise(got[i], want) <= PREFILL_BAR, i
