@@ -74,6 +74,9 @@ struct Warp {
   // probabilities enter the second product as p 2^kPShift <= 4096: f16 keeps p's bits down to
   // 2^-24 / 4096, below f32's for a row of a million tokens
   static constexpr int kPShift = 12;
+  // A block that is seen in part may outweigh `ref` by this factor (f16 holds 2^12 times it): its
+  // scale may come from tokens that are not seen.
+  static constexpr float kPartRoom = 8.f;
 
   __device__ __forceinline__ void reset() {
 #pragma unroll
@@ -121,9 +124,12 @@ struct Warp {
   // their MMA chains are independent, and one maximum, one vote on rescaling serve both.
   // Leaves the probabilities in p, and in `seen` (bit 4 u + j) which of the lane's tokens any row
   // sees: a masked token's value codes are replaced by zeros in the second half, since they may
-  // hold anything, NaN too, in a page that is not full.
-  __device__ __forceinline__ void scores(const uint8_t* stage, const float (&ks)[2], const float (&vs)[2], bool all, int first, int last,
-                                         int sinks, const int (&p0)[2], int lane, uint32_t (&p)[2][4], uint32_t& seen) {
+  // hold anything, NaN too, in a page that is not full. What is not seen does not count for `ref`
+  // either: a block seen in part has kPartRoom, and beyond that counts only if one of its seen
+  // values is not zero (`holds`, which waits for the values' codes).
+  template <class Holds>
+  __device__ __forceinline__ void scores(const uint8_t* stage, const float (&ks)[2], float (&vs)[2], bool all, int first, int last,
+                                         int sinks, const int (&p0)[2], int lane, uint32_t (&p)[2][4], uint32_t& seen, Holds holds) {
     const int t = lane & 3;
     float s[2][2][4];
 #pragma unroll
@@ -176,7 +182,25 @@ struct Warp {
       seen |= __shfl_xor_sync(0xffffffffu, seen, 8);
       seen |= __shfl_xor_sync(0xffffffffu, seen, 16);
     }
-    const float vmax = fmaxf(vs[0], vs[1]);
+    float vmax = fmaxf(vs[0], vs[1]);
+    if (!all) {
+      const uint32_t some = __reduce_or_sync(0xffffffffu, seen), full = __reduce_and_sync(0xffffffffu, seen);
+      float most = ref;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        if ((some >> (4 * u) & 15u) == 0) vs[u] = 0.f;
+        if ((full >> (4 * u) & 15u) == 15u) most = fmaxf(most, vs[u]);
+      }
+      vmax = most;
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+        if (vs[u] > kPartRoom * most) {
+          if (holds(u, seen))
+            vmax = fmaxf(vmax, vs[u] * (1.f / kPartRoom));
+          else
+            vs[u] = 0.f;
+        }
+    }
     const float mn = fmaxf(m, quad_max(fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])), fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3])))));
     if (__any_sync(0xffffffffu, vmax > ref || mn > m)) {
       const float now = fmaxf(ref, vmax);
@@ -193,7 +217,7 @@ struct Warp {
     const float base = m == -INFINITY ? 0.f : m;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const float weight = (float)(1 << kPShift) * vs[u] * kv8_inverse(ref);
+      const float weight = (float)(1 << kPShift) * (vs[u] * kv8_inverse(ref));
       float e[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -206,6 +230,21 @@ struct Warp {
       p[u][1] = h2_rest(e[0], e[1], p[u][0]);
       p[u][3] = h2_rest(e[2], e[3], p[u][2]);
     }
+  }
+
+  // Whether any value code of block u's tokens in `seen` is not zero.
+  __device__ __forceinline__ static bool holds_values(const uint8_t* stage, int u, uint32_t seen, int lane) {
+    const uint8_t* vb = stage + u * Piece<D>::kBytes;
+    uint32_t any = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint8_t* at = vb + (j >> 1) * (8 * D) + Piece<D>::value(lane, j & 1);
+      uint32_t w = 0;
+#pragma unroll
+      for (int i = 0; i < Piece<D>::kW; ++i) w |= reinterpret_cast<const uint32_t*>(at)[i];
+      if (seen >> (4 * u + j) & 1) any |= w & 0x7f7f7f7fu;
+    }
+    return __any_sync(0xffffffffu, any != 0);
   }
 
   // Second half: the accumulators take the two blocks' values, their codes in the lane's buffer.
@@ -498,14 +537,19 @@ __global__ void __launch_bounds__(kDecWarps * 32, dec_ctas(D)) kv8_decode_kernel
       for (int i = 0; i < n; i += 2) {
         const Block b0 = now[i], b1 = now[i + 1];  // past n: not there
         const int p0[2] = {b0.pos, b1.pos};
-        const float kk[2] = {b0.ks, b1.ks}, vv[2] = {b0.vs, b1.vs};
+        const float kk[2] = {b0.ks, b1.ks};
+        float vv[2] = {b0.vs, b1.vs};
         const bool any = b0.id >= 0 || b1.id >= 0;
         const int far = max(p0[0], p0[1]) + kKvBlock, near = min(p0[0], p0[1]);
         const bool all = far <= cur.len && (near >= first || far <= a.sinks);
         if (i == look_at) look_up(same ? cur : nxt, next_base + lane, page, then, [] {});
         uint32_t p[2][4], seen;
         copies.wait(0);
-        if (any) w.scores(buffer, kk, vv, all, first, last, a.sinks, p0, lane, p, seen);
+        if (any)
+          w.scores(buffer, kk, vv, all, first, last, a.sinks, p0, lane, p, seen, [&](int u, uint32_t see) {
+            copies.wait(1);
+            return Warp<D>::holds_values(buffer + 2 * Piece<D>::kBytes, u, see, lane);
+          });
         __syncwarp();
         const bool end = i + 2 >= n;
         if (!end)

@@ -648,3 +648,44 @@ def test_prefill_rows_do_not_feel_loud_values_they_do_not_see(heads, kv, dim, wi
     for i in rows:
         want = pool.reference(qh[i:i + 1], 0, i, window, sinks)[0]
         assert normwise(got[i], want) <= PREFILL_BAR, i
+
+
+@pytest.mark.parametrize("up,alone", [(24, False), (28, True), (40, False), (40, True), (60, True)])
+@pytest.mark.parametrize("heads,kv,dim,window,sinks", [(4, 2, 64, 0, 0), (6, 2, 128, 70, 0), (6, 2, 64, 70, 21), (8, 8, 128, 90, 5)])
+def test_decode_does_not_feel_loud_values_it_does_not_see(heads, kv, dim, window, sinks, up, alone):
+    """Loud values just past the length (what the page held before), just before the window and just
+    behind the sinks, in blocks that are seen in part."""
+    rng = np.random.default_rng(heads + dim + window + up)
+    lengths = [100, 417, 31, 50, 2001, 7]
+    pool = Pool(rng, lengths, kv, 32, dim, room=16)
+    quiet_keys(pool)
+    for b, n in enumerate(lengths):
+        for at in [n] + ([n - window - 1, sinks] if window and n > window + sinks else []):
+            hide_loud_values(pool, b, at, up, alone)
+    q = torch.from_numpy(rng.standard_normal((len(lengths), heads, dim)).astype(np.float32)).cuda()
+    table = ints(pool.table)
+    for rows in (slice(0, len(lengths)), slice(0, 2), slice(2, 4)):  # shared out, and by a CTA each
+        width = max(-(-n // 32) for n in lengths[rows])
+        got = pool.cache.attention_decode(q[rows], table[rows, :width], ints(lengths[rows]), window=window, sinks=sinks).double().cpu().numpy()
+        for i, b in enumerate(range(len(lengths))[rows]):
+            want = pool.reference(q[b:b + 1].double().cpu().numpy(), b, lengths[b] - 1, window, sinks)[0]
+            assert normwise(got[i], want) <= DECODE_BAR, b
+
+
+@pytest.mark.parametrize("up,alone", [(28, False), (40, True)])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_decode_in_shares_does_not_feel_loud_values_it_does_not_see(dim, up, alone):
+    """As above, with enough rows for each warp to have many blocks of one."""
+    rng = np.random.default_rng(dim + up)
+    kv, window, sinks = 16, 1000, 6
+    lengths = [1300 + 13 * b for b in range(24)]
+    pool = Pool(rng, lengths, kv, 32, dim, room=16)
+    quiet_keys(pool)
+    for b, n in enumerate(lengths):
+        for at in (n, n - window - 1, sinks):
+            hide_loud_values(pool, b, at, up, alone)
+    q = torch.from_numpy(rng.standard_normal((len(lengths), kv, dim)).astype(np.float32)).cuda()
+    got = pool.cache.attention_decode(q, ints(pool.table), ints(lengths), window=window, sinks=sinks).double().cpu().numpy()
+    for b in range(0, len(lengths), 8):
+        want = pool.reference(q[b:b + 1].double().cpu().numpy(), b, lengths[b] - 1, window, sinks)[0]
+        assert normwise(got[b], want) <= DECODE_BAR, b
