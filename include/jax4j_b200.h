@@ -304,7 +304,10 @@ int j4b_swiglu(j4b_buf gate_up, int64_t rows, int64_t width, j4b_buf out, j4b_st
  * table_stride apart); an entry outside [0, pages) is unmapped: its tokens are neither written nor
  * seen. Lengths, starts and offsets are int32 arrays on the device, so a call can be captured in a
  * graph and replayed while they change; a call like it has to have run on the device before (the first
- * of its types and sizes sets its kernel up). heads is a multiple of kv_heads (grouped heads: query head
+ * of its types and sizes sets its kernel up). They are not checked, but lead nowhere: a negative length
+ * is 0, one past the table's pages sees what these hold, a sequence with a negative start or offset
+ * has no rows, and rows past `tokens` are not there. Rows of q, q_out and out that no sequence has
+ * are left as they are. heads is a multiple of kv_heads (grouped heads: query head
  * h reads kv head h / (heads / kv_heads)). Activation types: J4B_F32, J4B_BF16. ---- */
 #define J4B_F32 0
 #define J4B_BF16 1

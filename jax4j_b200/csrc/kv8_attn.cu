@@ -371,7 +371,7 @@ struct DecArgs {
 };
 
 __device__ __forceinline__ int64_t row_units(const AttnArgs& a, int b) {
-  const int len = __ldg(a.lengths + b), n = span_of(len - 1, len - 1, a.window, a.sinks).count();
+  const int len = kv8_length(a.lengths, b), n = span_of(len - 1, len - 1, a.window, a.sinks, a.cap).count();
   return n > 0 ? n + kRowUnits : 0;
 }
 // Units of a CTA: a whole number for each of its warps, the same for all CTAs (the last ones may get none).
@@ -393,8 +393,8 @@ struct Share {
   int64_t at, left;  // the next unit among sequence b's, units left
   __device__ __forceinline__ bool next(const AttnArgs& a, int rows, Segment& s) {
     while (left > 0) {
-      s.len = __ldg(a.lengths + b);
-      s.span = span_of(s.len - 1, s.len - 1, a.window, a.sinks);
+      s.len = kv8_length(a.lengths, b);
+      s.span = span_of(s.len - 1, s.len - 1, a.window, a.sinks, a.cap);
       s.nb = s.span.count();
       const int units = s.nb > 0 ? s.nb + kRowUnits : 0;
       if (at >= (int64_t)units * rows) {
@@ -820,6 +820,7 @@ int kv8_check_attention(const j4b_kv8_cache* cache, int64_t layer, j4b_buf q, in
         (int)(heads / cache->kv_heads),
         (int)std::min(window, far),
         window > 0 ? (int)std::min(sinks, far) : 0,
+        (int)std::min<int64_t>(table_width * view.bpp, 0x7fffffff / kKvBlock),
         (float)(scale * 1.4426950408889634),
         (void*)(uintptr_t)out,
         out_type,

@@ -44,22 +44,26 @@ template <int D>
 __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const AppendArgs a) {
   constexpr int kLanes = kAppendThreads / kKvBlock;  // threads of a token: D / 8 values each
   constexpr int kVec = D / (4 * kLanes);             // as float4
+  auto rows_of = [&](int b) -> int {  // new tokens of sequence b
+    const int n = kv8_rows(a.offsets, b, a.tokens), s = __ldg(a.starts + b);  // loads side by side
+    return s < 0 ? 0 : min(n, kMaxLength - min(s, kMaxLength));
+  };
   const Kv8Place at = kv8_find<kAppendThreads>(
       a.batch,
       [&](int b) -> int64_t {
-        const int n = a.offsets[b + 1] - a.offsets[b], s = a.starts[b];
-        return n > 0 && s >= 0 ? (s + n + kKvBlock - 1) / kKvBlock - s / kKvBlock : 0;
+        const int n = rows_of(b), s = a.starts[b];
+        return n > 0 ? (s + n + kKvBlock - 1) / kKvBlock - s / kKvBlock : 0;
       },
       [&](int64_t) -> int64_t { return blockIdx.x; });
   if (at.seq < 0) return;
   const int b = at.seq, start = a.starts[b];
-  const int row0 = a.offsets[b], n = a.offsets[b + 1] - row0;
+  const int row0 = a.offsets[b], n = rows_of(b);
   const int blk = start / kKvBlock + (int)at.at;     // block of the sequence
   const int p0 = max(start, blk * kKvBlock);         // first position written
   const int cnt = min(start + n, (blk + 1) * kKvBlock) - p0;
   const int slot0 = p0 - blk * kKvBlock;             // tokens that the block holds already
   const int tid = threadIdx.x, tok = tid / kLanes, sub = tid % kLanes;
-  const int64_t row = row0 + (p0 - start) + tok;
+  const int64_t row = (int64_t)row0 + (p0 - start) + tok;
   // a token past the rope table or the input is not written; its q is zero
   const bool mine = tok < cnt && row >= 0 && row < a.tokens;
   const bool known = mine && p0 + tok < a.positions;

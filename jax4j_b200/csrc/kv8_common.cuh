@@ -109,7 +109,17 @@ __device__ __forceinline__ float exp2_ftz(float x) {
   return y;
 }
 
-constexpr int kNowhere = 0x3fffffff;  // the position of what is not there: past every query
+// Lengths, starts and offsets come from device memory, where nobody has looked at them: the kernels
+// take them as they are within these bounds, so that no value leads out of a buffer or keeps a
+// kernel walking over blocks that no table can name.
+constexpr int kMaxLength = 0x7fffffc0;
+constexpr int kNowhere = 0x7fffffe0;  // the position of what is not there: past every query
+__device__ __forceinline__ int kv8_length(const int* lengths, int b) { return min(max(__ldg(lengths + b), 0), kMaxLength); }
+// Rows of sequence b among the call's: what its offsets name past the `tokens` there are is not there.
+__device__ __forceinline__ int kv8_rows(const int* offsets, int b, int64_t tokens) {
+  const int from = __ldg(offsets + b), to = min(max(0, __ldg(offsets + b + 1)), (int)tokens);
+  return from < 0 ? 0 : max(0, to - from);
+}
 
 // The blocks that queries at positions first .. last of a sequence of `len` tokens see: the first
 // `sink_blocks` ones, then those from `from` on to `end` (exclusive). count() of them in order.
@@ -118,11 +128,11 @@ struct Span {
   __device__ __forceinline__ int count() const { return sink_blocks + end - from; }
   __device__ __forceinline__ int block(int i) const { return i < sink_blocks ? i : from + i - sink_blocks; }
 };
-__device__ __forceinline__ Span span_of(int first, int last, int window, int sinks) {
+__device__ __forceinline__ Span span_of(int first, int last, int window, int sinks, int cap) {
   const int lo = window > 0 ? max(0, first - window + 1) : 0;  // first position in the window of `first`
   Span s;
-  s.from = lo / kKvBlock;
-  s.end = last < 0 ? s.from : last / kKvBlock + 1;
+  s.from = min(lo / kKvBlock, cap);
+  s.end = last < 0 ? s.from : max(s.from, min(last / kKvBlock + 1, cap));
   s.sink_blocks = min((sinks + kKvBlock - 1) / kKvBlock, s.from);
   return s;
 }
@@ -138,6 +148,7 @@ struct AttnArgs {
   int64_t tokens;      // rows of q
   int batch, heads, group;
   int window, sinks;
+  int cap;  // blocks of a table row
   float scale_log2;
   void* out;
   int out_type;

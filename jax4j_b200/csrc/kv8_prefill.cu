@@ -353,19 +353,23 @@ __device__ __forceinline__ void warp_arrive(uint64_t* bar, int lane) {
 // Items of a sequence, before its kv heads.
 template <int LOG2>
 __device__ __forceinline__ int items_of(const AttnArgs& a, int b) {
-  const int64_t rows = (int64_t)max(0, __ldg(a.offsets + b + 1) - __ldg(a.offsets + b)) * a.group;
+  const int64_t rows = (int64_t)kv8_rows(a.offsets, b, a.tokens) * a.group;
   return (int)((rows + (1 << LOG2) - 1) >> LOG2);
 }
 // Item number f of the call, for a warp: all last items of the sequences, then all last but one, ...
+// `limit`: items that sequences of separate rows have at most; there are no more than 2^25, kv heads
+// apart, so a lane's sum that reaches kSumMost is past every f.
+constexpr unsigned kSumMost = 1u << 26;
 template <int LOG2>
-__device__ __forceinline__ void find_item(const AttnArgs& a, int64_t f, int lane, Item& it) {
+__device__ __forceinline__ void find_item(const AttnArgs& a, int64_t f, int64_t limit, int lane, Item& it) {
   it.seq = -1;
+  if (f >= limit) return;
   const int64_t m = kv8_quotient(f, a.c.kv_heads);
   // of the first 32 sequences, which are mostly all
-  const int own = lane < a.batch ? items_of<LOG2>(a, lane) : 0, own_len = lane < a.batch ? __ldg(a.lengths + lane) : 0;
+  const int own = lane < a.batch ? items_of<LOG2>(a, lane) : 0, own_len = lane < a.batch ? kv8_length(a.lengths, lane) : 0;
   auto items_up_to = [&](int most) -> int64_t {            // sum over the sequences of min(items, most)
     unsigned n = (unsigned)min(most, own);
-    for (int b = lane + 32; b < a.batch; b += 32) n += (unsigned)min(most, items_of<LOG2>(a, b));
+    for (int b = lane + 32; b < a.batch; b += 32) n = min(n + (unsigned)min(most, items_of<LOG2>(a, b)), kSumMost);
     return __reduce_add_sync(0xffffffffu, n);
   };
   if (m >= items_up_to(0x7fffffff)) return;
@@ -382,8 +386,8 @@ __device__ __forceinline__ void find_item(const AttnArgs& a, int64_t f, int lane
       hi = mid;
   }
   int64_t left = m - items_up_to(lo);  // this many sequences of more than lo items come before
-  int b = 0;
-  for (int base = 0;; base += 32) {
+  int b = -1;
+  for (int base = 0; base < a.batch; base += 32) {
     const uint32_t has = __ballot_sync(0xffffffffu, (base == 0 ? own : base + lane < a.batch ? items_of<LOG2>(a, base + lane) : 0) > lo);
     if (left >= __popc(has)) {
       left -= __popc(has);
@@ -392,17 +396,18 @@ __device__ __forceinline__ void find_item(const AttnArgs& a, int64_t f, int lane
     b = base + __fns(has, 0, (int)left + 1);
     break;
   }
+  if (b < 0) return;
   it.seq = b;
   it.head = (int)(f - m * a.c.kv_heads);
   it.row0 = __ldg(a.offsets + b);
-  const int n = __ldg(a.offsets + b + 1) - it.row0;
-  it.len = b < 32 ? __shfl_sync(0xffffffffu, own_len, b) : __ldg(a.lengths + b);
+  const int n = kv8_rows(a.offsets, b, a.tokens);
+  it.len = b < 32 ? __shfl_sync(0xffffffffu, own_len, b) : kv8_length(a.lengths, b);
   it.pos0 = it.len - n;  // negative: the first queries are before the cache and see nothing
   it.first_row = (items_of<LOG2>(a, b) - 1 - lo) << LOG2;
   it.rows = (int)min((int64_t)1 << LOG2, (int64_t)n * a.group - it.first_row);
   auto span_of_tile = [&](int i, int tiles) {  // of tiles i .. i + tiles - 1
     const int from = it.first_row + i * kRows, to = it.first_row + min(it.rows, (i + tiles) * kRows) - 1;
-    return span_of(max(0, it.pos0 + from / a.group), min(it.len - 1, it.pos0 + to / a.group), a.window, a.sinks);
+    return span_of(max(0, it.pos0 + from / a.group), min(it.len - 1, it.pos0 + to / a.group), a.window, a.sinks, a.cap);
   };
   it.span = span_of_tile(0, 2);
 #pragma unroll
@@ -541,7 +546,7 @@ constexpr int kItemReaders = 13;  // warps
 
 // SINGLE: items of one tile of rows.
 template <int D, int TYPE, bool SINGLE>
-__global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const AttnArgs a) {
+__global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const AttnArgs a, int64_t limit) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = aligned_smem(smem_raw);
   uint8_t* sq = smem;                    // [2 tiles]
@@ -623,7 +628,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const AttnArgs
       const int gr = it.first_row + i * kRows + r, tok = gr / a.group, gh = it.head * a.group + gr % a.group;
       const bool valid = i * kRows + r < it.rows && it.row0 + tok >= 0 && it.row0 + tok < a.tokens;
       const int64_t out_row = valid ? ((int64_t)(it.row0 + tok) * a.heads + gh) * D : -1;
-      const int qp = valid ? it.pos0 + tok : -1;
+      const int qp = valid ? max(-1, it.pos0 + tok) : -1;
       const View view = {a.window > 0 ? max(0, qp - a.window + 1) : 0, qp, a.sinks};
       // every valid row of the tile sees the positions [most_lo, least]
       const int least = it.pos0 + (it.first_row + i * kRows) / a.group;
@@ -984,7 +989,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const AttnArgs
       bool more = true;
       for (uint32_t r = 0; more && ok; ++r) {
         Item it;
-        find_item<SINGLE ? 7 : 8>(a, (int64_t)r * gridDim.x + (r & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x), lane, it);
+        find_item<SINGLE ? 7 : 8>(a, (int64_t)r * gridDim.x + (r & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x), limit, lane, it);
         if (r >= kItems) ok = __all_sync(0xffffffffu, ok && kv8_wait(&item_empty[r % kItems], (r / kItems - 1) & 1));
         if (lane == 0) {
           items[r % kItems] = it;
@@ -1013,7 +1018,7 @@ int launch_prefill_kernel(const AttnArgs& a, int64_t items, int dev, cudaStream_
     J4B_CUDA(cudaFuncSetAttribute(kv8_prefill_kernel<D, TYPE, SINGLE>, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<D>::kBytes), "cudaFuncSetAttribute");
     done[dev] = true;
   }
-  kv8_prefill_kernel<D, TYPE, SINGLE><<<(unsigned)std::min<int64_t>(items, device_ctx(dev)->sm_count), kThreads, Smem<D>::kBytes, stream>>>(a);
+  kv8_prefill_kernel<D, TYPE, SINGLE><<<(unsigned)std::min<int64_t>(items, device_ctx(dev)->sm_count), kThreads, Smem<D>::kBytes, stream>>>(a, items);
   J4B_CHECK_LAUNCH("kv8_prefill_kernel");
   return J4B_OK;
 }

@@ -689,3 +689,62 @@ def test_decode_in_shares_does_not_feel_loud_values_it_does_not_see(dim, up, alo
     for b in range(0, len(lengths), 8):
         want = pool.reference(q[b:b + 1].double().cpu().numpy(), b, lengths[b] - 1, window, sinks)[0]
         assert normwise(got[b], want) <= DECODE_BAR, b
+
+
+WILD = [2 ** 31 - 1, 2 ** 31 - 70, 2 ** 30 + 5, -1, -2 ** 31]
+
+
+@pytest.mark.parametrize("window,sinks", [(0, 0), (50, 7)])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_decode_lengths_past_what_a_table_holds(dim, window, sinks):
+    """Any length ends at once: past the table's last page there is nothing to walk over."""
+    rng = np.random.default_rng(61)
+    lengths, heads = [90, 64, 128, 33, 96], 4
+    pool = Pool(rng, lengths, 2, 32, dim)
+    pool.table[2:] = -1  # what a wild length sees: the pages of the first, whole, and none of its own
+    pool.table[2] = pool.table[1]
+    full = int((pool.table[1] >= 0).sum()) * 32
+    q = torch.from_numpy(rng.standard_normal((5, heads, dim)).astype(np.float32)).cuda()
+    for wild in WILD:
+        n = [90, 64, wild, wild, 0]
+        for width in (pool.table.shape[1], 40):  # by a CTA each, and shared out
+            table = torch.full((5, width), -1, dtype=torch.int32, device="cuda")
+            table[:, :pool.table.shape[1]] = ints(pool.table)
+            got = pool.cache.attention_decode(q, table, ints(n), window=window, sinks=sinks).double().cpu().numpy()
+            for b in (0, 1):
+                assert normwise(got[b], pool.reference(q[b:b + 1].double().cpu().numpy(), b, n[b] - 1, window, sinks)[0]) <= DECODE_BAR
+            assert not got[3:].any()
+            if wild < 0:
+                assert not got[2].any()
+            else:  # the sinks, if there is a window: that one lies far past the table
+                pool.lengths[2] = sinks if window else full
+                assert normwise(got[2], pool.reference(q[2:3].double().cpu().numpy(), 2, pool.lengths[2] - 1, 0, 0)[0]) <= DECODE_BAR
+
+
+@pytest.mark.parametrize("heads,kv", [(4, 2), (32, 32)])
+def test_prefill_and_append_of_wild_lengths_and_offsets(heads, kv):
+    """Sequences whose arrays make sense keep their results next to ones whose arrays do not, whose
+    rows lie apart from theirs."""
+    from jax4j_b200.kv8 import rope_table
+    rng = np.random.default_rng(62)
+    dim, page = 64, 32
+    pool = Pool(rng, [70, 300, 60, 60], kv, page, dim, room=64)
+    q = torch.from_numpy(rng.standard_normal((200, heads, dim)).astype(np.float32)).cuda()
+    rope = rope_table(400, dim, device="cuda")
+    qkv = torch.from_numpy(rng.standard_normal((200, (heads + 2 * kv) * dim)).astype(np.float32)).cuda()
+    qh = q.double().cpu().numpy()
+    ref = [pool.reference(qh[:70], 0, 0, 0, 0), pool.reference(qh[70:150], 1, 220, 0, 0)]
+    codes = [t.clone() for t in (pool.cache.k.view(torch.uint8), pool.cache.v.view(torch.uint8))]
+    for wild in WILD:
+        for offsets in ([0, 70, 150, wild, -3], [0, 70, 150, 2 ** 31 - 1, -2 ** 31], [0, 70, 150, 200, 10 ** 9]):
+            got = pool.cache.attention_prefill(q, ints(offsets), ints(pool.table), ints([70, 300, wild, wild])).double().cpu().numpy()
+            for rows, want in zip((slice(0, 70), slice(70, 150)), ref):
+                assert normwise(got[rows], want) <= PREFILL_BAR
+            starts = [70, 300, wild, wild]
+            out = pool.cache.append(qkv, rope, ints(pool.table), ints(starts), heads, offsets=ints(offsets))
+            alone = pool.cache.append(qkv, rope, ints(pool.table[:2]), ints(starts[:2]), heads, offsets=ints(offsets[:3]))
+            assert torch.equal(out[:150], alone[:150])
+            for b in (2, 3):  # nothing was written to their pages
+                for t, before in zip((pool.cache.k, pool.cache.v), codes):
+                    pages = torch.from_numpy(pool.table[b][pool.table[b] >= 0]).cuda()
+                    assert torch.equal(t.view(torch.uint8)[0, pages], before[0, pages])
