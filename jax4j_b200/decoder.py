@@ -245,10 +245,9 @@ class DecoderBlock:
         self._paged(x, pages, tokens)
         starts, lengths, offsets = pages.extend(counts) if layer == 0 else pages.step
         qkv = be.quant_gemm(w.wqkv, self.rmsnorm(x, w.g_attn), precision)
-        q = pages.cache.append(qkv.tensor.view(tokens, -1), self._rope_table(pages), pages.table, starts, w.heads, offsets, layer,
-                               q_dtype=torch.bfloat16)
+        q = pages.cache.append(qkv.tensor.view(tokens, -1), self._rope_table(pages), pages.table, starts, w.heads, offsets, layer)
         del qkv
-        attn = pages.cache.attention_prefill(q, offsets, pages.table, lengths, window, sinks, layer=layer, out_dtype=torch.float32)
+        attn = pages.cache.attention_prefill(q, offsets, pages.table, lengths, window, sinks, layer=layer)
         h = self._sum_ranks(self._add_residual(be.quant_gemm(w.wo, be.wrap(attn.view(tokens, -1)), precision), x))
         gu = be.quant_gemm(w.wgu, self.rmsnorm(h, w.g_ffn), precision)
         return self._sum_ranks(self._add_residual(be.quant_gemm(w.wd, self.swiglu(gu), precision), h))

@@ -748,3 +748,45 @@ def test_prefill_and_append_of_wild_lengths_and_offsets(heads, kv):
                 for t, before in zip((pool.cache.k, pool.cache.v), codes):
                     pages = torch.from_numpy(pool.table[b][pool.table[b] >= 0]).cuda()
                     assert torch.equal(t.view(torch.uint8)[0, pages], before[0, pages])
+
+
+@pytest.mark.parametrize("spans,heads,kv,dim", [([(0, 300), (200, 40)], 4, 2, 64), ([(0, 300), (200, 40)], 8, 2, 128), ([(0, 700)], 32, 32, 128), ([(0, 1)] * 3, 2, 1, 64)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_prefill_keeps_eleven_bits(spans, heads, kv, dim, dtype):
+    """What the operands' 11 bits leave, in the mean: a probability is off by some 0.41 2^-11 of itself,
+    and where queries come as f32, a score by 0.41 2^-11 of its rms S (each product of its sum by
+    as much of itself, signs at random). With values of random signs the result is then off by
+    0.41 2^-11 sqrt(1 + S^2) of its rms; the bar is 2.4 times that. Queries or probabilities of 8
+    bits would be 8 times off."""
+    rng = np.random.default_rng(71 + dim)
+    pool, offsets, q = prefill_inputs(rng, spans, heads, kv, dim, 32, dtype)
+    pool.ks *= 2.0 ** np.round(1 - np.log2(np.sqrt((pool.k ** 2).mean((-1, -2))).reshape(*pool.ks.shape[:2], 1) * pool.ks))  # S about 2
+    pool.vs[:] = 2.0 ** -8
+    pool.cache.k_scale[0], pool.cache.v_scale[0] = torch.from_numpy(pool.ks).float(), torch.from_numpy(pool.vs).float()
+    got = pool.cache.attention_prefill(q, ints(offsets), ints(pool.table), ints(pool.lengths), out_dtype=torch.float32).double().cpu().numpy()
+    qh = q.double().cpu().numpy()
+    kh = pool.k * np.repeat(pool.ks, 16, axis=2)[..., None]
+    rms = float(np.sqrt((kh ** 2).mean() * (qh ** 2).mean())) if dtype is torch.float32 else 0.0
+    assert rms < 4
+    off, of = 0.0, 0.0
+    for b, (past, n) in enumerate(spans):
+        want = pool.reference(qh[offsets[b]:offsets[b + 1]], b, past, 0, 0)
+        off += ((got[offsets[b]:offsets[b + 1]] - want) ** 2).sum()
+        of += (want ** 2).sum()
+    assert np.sqrt(off / of) <= 2.0 ** -11 * np.sqrt(1 + rms ** 2)
+
+
+def test_decoder_block_gives_prefill_the_queries_as_append_rotated_them(backend, monkeypatch):
+    """f32, which the kernel rounds to 11 bits: no type in between that holds fewer."""
+    from jax4j_b200.decoder import DecoderBlock, DecoderWeights
+    from jax4j_b200.kv8 import Kv8Cache, PageTable
+    from jax4j_b200.prng import PrngKey
+    cache = Kv8Cache(8, 2, 32, 128)
+    pages, made, used = PageTable(cache, 2, 100), [], []
+    append, attention = cache.append, cache.attention_prefill
+    monkeypatch.setattr(cache, "append", lambda *a, **k: made.append(append(*a, **k)) or made[-1])
+    monkeypatch.setattr(cache, "attention_prefill", lambda q, *a, **k: used.append(q) or attention(q, *a, **k))
+    block = DecoderBlock(backend, DecoderWeights.random(backend, 256, 2, 512, PrngKey.of(3)))
+    x = np.random.default_rng(1).standard_normal((50, 256)).astype(np.float32)
+    block.prefill_paged(backend.upload(x, x.shape), pages, [20, 30])
+    assert used[0] is made[0] and used[0].dtype == torch.float32
