@@ -204,8 +204,9 @@ class Kv8Cache:
 class PageTable:
     """The host's bookkeeping of a `Kv8Cache`: `slots` sequences of up to `max_tokens` tokens, each a list
     of pages in token order. Full pages of a fork are shared (counted), its partly filled last page
-    is copied. The device sees it through `table` (int32 [slots, pages of a sequence], -1: none)
-    and the arrays that `extend` returns."""
+    is copied. The device sees it through `table` (int32 [slots, pages of a sequence], -1: none),
+    one tensor, which a read of the attribute and `extend` bring up to date on the current stream, and
+    the arrays that `extend` returns."""
 
     def __init__(self, cache: Kv8Cache, slots: int, max_tokens: int):
         if slots <= 0 or max_tokens <= 0:
@@ -216,7 +217,7 @@ class PageTable:
         self.lengths = [0] * slots
         self.refs = [0] * cache.pages
         self._free = list(range(cache.pages))  # a heap: the lowest page first, so what is in use stays low
-        self.table = torch.full((slots, self.width), -1, dtype=torch.int32, device=cache.device)
+        self._table = torch.full((slots, self.width), -1, dtype=torch.int32, device=cache.device)
         self._dirty = False
         self.step = None  # what the last extend returned, for a model's other layers
 
@@ -274,8 +275,13 @@ class PageTable:
     def _upload(self) -> None:
         if self._dirty:
             rows = [p + [-1] * (self.width - len(p)) for p in self.pages]
-            self.table.copy_(torch.tensor(rows, dtype=torch.int32))
+            self._table.copy_(torch.tensor(rows, dtype=torch.int32))
             self._dirty = False
+
+    @property
+    def table(self) -> torch.Tensor:
+        self._upload()
+        return self._table
 
     def release(self, slot: int) -> None:
         """Ends a slot's sequence: its pages that no other shares are free again."""

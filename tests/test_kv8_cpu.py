@@ -204,3 +204,25 @@ def test_decode_calls_of_two_threads_never_share_a_workspace(monkeypatch):
     for t in threads:
         t.join()
     assert not clashes
+
+
+def test_page_table_on_the_device_follows_every_change():
+    """Read as a user reads it, right after a call: nothing else brings it up to date."""
+    from jax4j_b200.kv8 import PageTable
+    t = PageTable(FakeCache(20, 16), 3, 200)
+
+    def check():
+        assert t.table.tolist() == [p + [-1] * (t.width - len(p)) for p in t.pages]
+    check()
+    t.extend([150, 30, 0])
+    check()
+    at = t.table.data_ptr()
+    t.fork(1, [2])
+    check()
+    assert t.trim(40, 20) == 4
+    check()
+    t.release(1)
+    check()
+    assert t.compact() > 0
+    check()
+    assert t.table.data_ptr() == at

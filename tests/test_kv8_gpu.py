@@ -790,3 +790,20 @@ def test_decoder_block_gives_prefill_the_queries_as_append_rotated_them(backend,
     x = np.random.default_rng(1).standard_normal((50, 256)).astype(np.float32)
     block.prefill_paged(backend.upload(x, x.shape), pages, [20, 30])
     assert used[0] is made[0] and used[0].dtype == torch.float32
+
+
+def test_a_fork_reads_as_its_parent_at_once():
+    from jax4j_b200.kv8 import Kv8Cache, PageTable, rope_table
+    torch.manual_seed(5)
+    cache = Kv8Cache(12, 2, 16, 64)
+    pages = PageTable(cache, 3, 100)
+    starts, lengths, offsets = pages.extend([40, 0, 20])
+    cache.append(torch.randn(60, 8 * 64, device="cuda"), rope_table(100, 64, device="cuda"), pages.table, starts, 4, offsets)
+    pages.fork(0, [1])
+    q = torch.randn(1, 4, 64, device="cuda").expand(3, 4, 64).contiguous()
+    out = cache.attention_decode(q, pages.table, ints(pages.lengths))
+    assert torch.equal(out[0], out[1]) and out[0].any()
+    pages.release(0)
+    assert pages.compact() > 0
+    again = cache.attention_decode(q, pages.table, ints(pages.lengths))
+    assert torch.equal(again[1], out[1]) and torch.equal(again[2], out[2]) and not again[0].any()
