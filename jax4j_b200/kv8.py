@@ -315,14 +315,19 @@ class PageTable:
         rest = self.lengths[parent] % self.cache.page
         shared, last = (self.pages[parent][:-1], self.pages[parent][-1]) if rest else (self.pages[parent], -1)
         fresh = self._take(len(children)) if last >= 0 else []
+        if fresh:
+            try:
+                self.cache.copy_pages([last] * len(children), fresh, [rest] * len(children))
+            except BaseException:
+                for p in fresh:
+                    self._drop(p)
+                raise
         for i, c in enumerate(children):
             for p in shared:
                 if p >= 0:
                     self.refs[p] += 1
             self.pages[c] = list(shared) + ([fresh[i]] if last >= 0 else [])
             self.lengths[c] = self.lengths[parent]
-        if fresh:
-            self.cache.copy_pages([last] * len(children), fresh, [rest] * len(children))
         self._dirty = True
 
     def compact(self) -> int:

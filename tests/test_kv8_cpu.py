@@ -226,3 +226,20 @@ def test_page_table_on_the_device_follows_every_change():
     assert t.compact() > 0
     check()
     assert t.table.data_ptr() == at
+
+
+def test_page_table_fork_gives_its_pages_back_if_the_copy_fails():
+    from jax4j_b200.kv8 import PageTable
+    t = PageTable(FakeCache(8, 16), 3, 64)
+    t.extend([20, 0, 0])
+
+    def fail(*args):
+        raise RuntimeError("no copy")
+    copy, t.cache.copy_pages = t.cache.copy_pages, fail
+    with pytest.raises(RuntimeError, match="no copy"):
+        t.fork(0, [1, 2])
+    _consistent(t)
+    assert t.free_pages == 6 and t.lengths == [20, 0, 0]
+    t.cache.copy_pages = copy
+    t.fork(0, [1, 2])
+    _consistent(t)
