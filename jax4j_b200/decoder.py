@@ -211,14 +211,24 @@ class DecoderBlock:
             self._rope = rope_table(positions, HEAD_DIM, self.theta, pages.cache.device)
         return self._rope
 
-    def _paged(self, x: DeviceBuffer, pages: PageTable, tokens: int) -> None:
-        cache = pages.cache
+    def _paged(self, x: DeviceBuffer, pages: PageTable, counts: list, window: int, sinks: int, layer: int) -> tuple:
+        """Checks a paged call, all of it before the sequences change, and makes room for its tokens."""
+        cache, tokens = pages.cache, sum(counts)
         if cache.head_dim != HEAD_DIM or cache.kv_heads != self.w.heads:
             raise ValueError("paged cache does not match the head count or the head size")
+        if not 0 <= layer < cache.layers:
+            raise ValueError(f"layer {layer} outside [0, {cache.layers})")
+        if window < 0 or sinks < 0:
+            raise ValueError("window and sinks must not be negative")
         if tokens <= 0:
             raise ValueError("no new tokens")
         if x.shape[0] != tokens:
             raise ValueError(f"x has {x.shape[0]} rows for {tokens} new tokens")
+        if layer == 0:
+            return pages.extend(counts)
+        if pages.counts != list(counts):
+            raise ValueError(f"layer {layer} must follow layer 0 of the same step")
+        return pages.step
 
     def decode_paged(self, x: DeviceBuffer, pages: PageTable, window: int = 0, sinks: int = 0, layer: int = 0) -> DeviceBuffer:
         """One token for each slot of `pages`, x [slots, d] -> [slots, d]: its key and value join the
@@ -226,8 +236,7 @@ class DecoderBlock:
         the first `sinks`). Layer 0 makes the room for a step's tokens,
         a model's other layers take it as it is."""
         be, w = self.be, self.w
-        self._paged(x, pages, pages.slots)
-        starts, lengths, _ = pages.extend([1] * pages.slots) if layer == 0 else pages.step
+        starts, lengths, _ = self._paged(x, pages, [1] * pages.slots, window, sinks, layer)
         qkv = be.quant_matvec(w.wqkv, self.rmsnorm(x, w.g_attn))
         q = pages.cache.append(qkv.tensor.view(pages.slots, -1), self._rope_table(pages), pages.table, starts, w.heads, layer=layer)
         attn = pages.cache.attention_decode(q, pages.table, lengths, window, sinks, layer=layer)
@@ -242,8 +251,7 @@ class DecoderBlock:
         `precision`; layers as in decode_paged."""
         be, w = self.be, self.w
         tokens = sum(counts)
-        self._paged(x, pages, tokens)
-        starts, lengths, offsets = pages.extend(counts) if layer == 0 else pages.step
+        starts, lengths, offsets = self._paged(x, pages, counts, window, sinks, layer)
         qkv = be.quant_gemm(w.wqkv, self.rmsnorm(x, w.g_attn), precision)
         q = pages.cache.append(qkv.tensor.view(tokens, -1), self._rope_table(pages), pages.table, starts, w.heads, offsets, layer)
         del qkv

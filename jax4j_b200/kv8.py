@@ -219,7 +219,7 @@ class PageTable:
         self._free = list(range(cache.pages))  # a heap: the lowest page first, so what is in use stays low
         self._table = torch.full((slots, self.width), -1, dtype=torch.int32, device=cache.device)
         self._dirty = False
-        self.step = None  # what the last extend returned, for a model's other layers
+        self.step = self.counts = None  # what the last extend returned and was given, for a model's other layers
 
     def _slot(self, slot: int) -> int:
         if not 0 <= slot < self.slots:
@@ -270,6 +270,7 @@ class PageTable:
             offsets.append(offsets[-1] + n)
         packed = torch.tensor(starts + self.lengths + offsets, dtype=torch.int32).to(self.cache.device)
         self.step = packed[:self.slots], packed[self.slots:2 * self.slots], packed[2 * self.slots:]
+        self.counts = list(counts)
         return self.step
 
     def _upload(self) -> None:
@@ -288,6 +289,7 @@ class PageTable:
         for p in self.pages[self._slot(slot)]:
             self._drop(p)
         self.pages[slot], self.lengths[slot], self._dirty = [], 0, True
+        self.step = self.counts = None
 
     def trim(self, window: int, sinks: int = 0) -> int:
         """Frees the pages that no later query sees under a window with sinks; returns how many."""
@@ -329,6 +331,7 @@ class PageTable:
             self.pages[c] = list(shared) + ([fresh[i]] if last >= 0 else [])
             self.lengths[c] = self.lengths[parent]
         self._dirty = True
+        self.step = self.counts = None
 
     def compact(self) -> int:
         """Moves pages so that the ones in use are the lowest (a pool that can then be cut, or saved

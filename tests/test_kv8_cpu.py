@@ -228,6 +228,35 @@ def test_page_table_on_the_device_follows_every_change():
     assert t.table.data_ptr() == at
 
 
+def test_decoder_block_refuses_before_it_changes_the_sequences():
+    from types import SimpleNamespace
+    from jax4j_b200.decoder import DecoderBlock
+    from jax4j_b200.kv8 import PageTable
+    block = DecoderBlock(None, SimpleNamespace(world=1, rank=0, heads=2))
+    cache = FakeCache(9, 16)
+    cache.kv_heads, cache.head_dim, cache.layers = 2, 128, 2
+    t = PageTable(cache, 2, 64)
+    x = [SimpleNamespace(shape=(n, 256)) for n in range(8)]
+
+    def unchanged(match, call, *args, **kw):
+        before = ([list(p) for p in t.pages], list(t.lengths), t.free_pages, t.counts)
+        with pytest.raises(ValueError, match=match):
+            call(*args, **kw)
+        assert before == (t.pages, t.lengths, t.free_pages, t.counts)
+    unchanged("must follow layer 0", block.decode_paged, x[2], t, layer=1)  # no step yet
+    t.extend([3, 2])
+    unchanged("window and sinks", block.decode_paged, x[2], t, window=-1)
+    unchanged("window and sinks", block.prefill_paged, x[2], t, [1, 1], sinks=-1)
+    unchanged("layer 2 outside", block.decode_paged, x[2], t, layer=2)
+    unchanged("layer -1 outside", block.prefill_paged, x[2], t, [1, 1], layer=-1)
+    unchanged("rows for 2", block.decode_paged, x[3], t)
+    unchanged("must follow layer 0", block.decode_paged, x[2], t, layer=1)  # the last step was a prefill
+    unchanged("must follow layer 0", block.prefill_paged, x[5], t, [2, 3], layer=1)
+    t.extend([1, 1])
+    t.release(0)  # its step is over
+    unchanged("must follow layer 0", block.decode_paged, x[2], t, layer=1)
+
+
 def test_page_table_fork_gives_its_pages_back_if_the_copy_fails():
     from jax4j_b200.kv8 import PageTable
     t = PageTable(FakeCache(8, 16), 3, 64)
