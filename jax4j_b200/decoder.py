@@ -211,7 +211,7 @@ class DecoderBlock:
             self._rope = rope_table(positions, HEAD_DIM, self.theta, pages.cache.device)
         return self._rope
 
-    def _paged(self, x: DeviceBuffer, pages: PageTable, counts: list, window: int, sinks: int, layer: int) -> tuple:
+    def _paged(self, x: DeviceBuffer, pages: PageTable, counts: list, window: int, sinks: int, layer: int, rows: int) -> None:
         """Checks a paged call, all of it before the sequences change, and makes room for its tokens."""
         cache, tokens = pages.cache, sum(counts)
         if cache.head_dim != HEAD_DIM or cache.kv_heads != self.w.heads:
@@ -222,21 +222,26 @@ class DecoderBlock:
             raise ValueError("window and sinks must not be negative")
         if tokens <= 0:
             raise ValueError("no new tokens")
-        if x.shape[0] != tokens:
-            raise ValueError(f"x has {x.shape[0]} rows for {tokens} new tokens")
+        if x.shape[0] != rows:
+            raise ValueError(f"x has {x.shape[0]} rows for {rows} {'new tokens' if rows == tokens else 'slots'}")
         if layer == 0:
-            return pages.extend(counts)
-        if pages.counts != list(counts):
+            pages.extend(counts)
+        elif pages.counts != list(counts):
             raise ValueError(f"layer {layer} must follow layer 0 of the same step")
-        return pages.step
 
-    def decode_paged(self, x: DeviceBuffer, pages: PageTable, window: int = 0, sinks: int = 0, layer: int = 0) -> DeviceBuffer:
+    def decode_paged(self, x: DeviceBuffer, pages: PageTable, window: int = 0, sinks: int = 0, layer: int = 0,
+                     active: list | None = None) -> DeviceBuffer:
         """One token for each slot of `pages`, x [slots, d] -> [slots, d]: its key and value join the
         slot's sequence, and attention covers that (with window > 0, the last `window` tokens and
-        the first `sinks`). Layer 0 makes the room for a step's tokens,
-        a model's other layers take it as it is."""
+        the first `sinks`). `active`, a truth value for each slot, names the slots that have a token
+        (default: all); the others keep their sequences as they are, and their rows of the result mean
+        nothing. Layer 0 makes the room for a step's tokens, a model's other layers take it as it is."""
         be, w = self.be, self.w
-        starts, lengths, _ = self._paged(x, pages, [1] * pages.slots, window, sinks, layer)
+        if active is not None and len(active) != pages.slots:
+            raise ValueError(f"active has {len(active)} entries for {pages.slots} slots")
+        counts = [1] * pages.slots if active is None else [1 if a else 0 for a in active]
+        self._paged(x, pages, counts, window, sinks, layer, pages.slots)
+        starts, lengths = pages.rows
         qkv = be.quant_matvec(w.wqkv, self.rmsnorm(x, w.g_attn))
         q = pages.cache.append(qkv.tensor.view(pages.slots, -1), self._rope_table(pages), pages.table, starts, w.heads, layer=layer)
         attn = pages.cache.attention_decode(q, pages.table, lengths, window, sinks, layer=layer)
@@ -251,7 +256,8 @@ class DecoderBlock:
         `precision`; layers as in decode_paged."""
         be, w = self.be, self.w
         tokens = sum(counts)
-        starts, lengths, offsets = self._paged(x, pages, counts, window, sinks, layer)
+        self._paged(x, pages, counts, window, sinks, layer, tokens)
+        starts, lengths, offsets = pages.step
         qkv = be.quant_gemm(w.wqkv, self.rmsnorm(x, w.g_attn), precision)
         q = pages.cache.append(qkv.tensor.view(tokens, -1), self._rope_table(pages), pages.table, starts, w.heads, offsets, layer)
         del qkv

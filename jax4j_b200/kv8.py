@@ -219,7 +219,9 @@ class PageTable:
         self._free = list(range(cache.pages))  # a heap: the lowest page first, so what is in use stays low
         self._table = torch.full((slots, self.width), -1, dtype=torch.int32, device=cache.device)
         self._dirty = False
-        self.step = self.counts = None  # what the last extend returned and was given, for a model's other layers
+        # of the last extend, for a model's other layers: what it returned, (starts, lengths) of decode's
+        # rows, one a slot, and what it was given
+        self.step = self.rows = self.counts = None
 
     def _slot(self, slot: int) -> int:
         if not 0 <= slot < self.slots:
@@ -268,9 +270,12 @@ class PageTable:
         offsets = [0]
         for n in counts:
             offsets.append(offsets[-1] + n)
-        packed = torch.tensor(starts + self.lengths + offsets, dtype=torch.int32).to(self.cache.device)
-        self.step = packed[:self.slots], packed[self.slots:2 * self.slots], packed[2 * self.slots:]
-        self.counts = list(counts)
+        # for a row each of decode: slots without a new token start nowhere and see nothing
+        busy = [(m, n) if k else (-1, 0) for m, n, k in zip(starts, self.lengths, counts)]
+        rows = [m for m, _ in busy] + [n for _, n in busy]
+        packed = torch.tensor(starts + self.lengths + rows + offsets, dtype=torch.int32).to(self.cache.device)
+        starts, lengths, *rows, offsets = packed.split([self.slots] * 4 + [self.slots + 1])
+        self.step, self.rows, self.counts = (starts, lengths, offsets), tuple(rows), list(counts)
         return self.step
 
     def _upload(self) -> None:
@@ -289,7 +294,7 @@ class PageTable:
         for p in self.pages[self._slot(slot)]:
             self._drop(p)
         self.pages[slot], self.lengths[slot], self._dirty = [], 0, True
-        self.step = self.counts = None
+        self.step = self.rows = self.counts = None
 
     def trim(self, window: int, sinks: int = 0) -> int:
         """Frees the pages that no later query sees under a window with sinks; returns how many."""
@@ -331,7 +336,7 @@ class PageTable:
             self.pages[c] = list(shared) + ([fresh[i]] if last >= 0 else [])
             self.lengths[c] = self.lengths[parent]
         self._dirty = True
-        self.step = self.counts = None
+        self.step = self.rows = self.counts = None
 
     def compact(self) -> int:
         """Moves pages so that the ones in use are the lowest (a pool that can then be cut, or saved

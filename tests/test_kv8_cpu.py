@@ -272,3 +272,12 @@ def test_page_table_fork_gives_its_pages_back_if_the_copy_fails():
     t.cache.copy_pages = copy
     t.fork(0, [1, 2])
     _consistent(t)
+
+
+def test_page_table_rows_of_slots_without_a_token_start_nowhere():
+    from jax4j_b200.kv8 import PageTable
+    t = PageTable(FakeCache(8, 16), 3, 64)
+    t.extend([20, 3, 0])
+    starts, lengths, offsets = t.extend([1, 0, 1])
+    assert (starts.tolist(), lengths.tolist(), offsets.tolist()) == ([20, 3, 0], [21, 3, 1], [0, 1, 1, 2])
+    assert [r.tolist() for r in t.rows] == [[20, -1, 0], [21, 0, 1]]

@@ -807,3 +807,29 @@ def test_a_fork_reads_as_its_parent_at_once():
     assert pages.compact() > 0
     again = cache.attention_decode(q, pages.table, ints(pages.lengths))
     assert torch.equal(again[1], out[1]) and torch.equal(again[2], out[2]) and not again[0].any()
+
+
+def test_decoder_block_decodes_only_active_slots(backend):
+    """Idle slots take no pages and keep their sequences; the active ones get what they would get by
+    themselves."""
+    from jax4j_b200.decoder import DecoderBlock, DecoderWeights
+    from jax4j_b200.kv8 import Kv8Cache, PageTable
+    from jax4j_b200.prng import PrngKey
+    block = DecoderBlock(backend, DecoderWeights.random(backend, 256, 2, 512, PrngKey.of(3)))
+    rng = np.random.default_rng(81)
+    prompt, steps = rng.standard_normal((50, 256)).astype(np.float32), rng.standard_normal((20, 4, 256)).astype(np.float32)
+    outs = []
+    for slots, counts, active in ((4, [20, 30, 0, 0], [True, False, False, True]), (2, [20, 0], None)):
+        pages = PageTable(Kv8Cache(8, 2, 16, 128), slots, 64)
+        x = prompt[:sum(counts)]
+        block.prefill_paged(backend.upload(x, x.shape), pages, counts)
+        for step in steps:
+            x = step if active else step[[0, 3]]
+            out = backend.download(block.decode_paged(backend.upload(x, x.shape), pages, active=active))
+        outs.append(out)
+        if active:
+            assert pages.lengths == [40, 30, 0, 20] and [len(p) for p in pages.pages] == [3, 2, 0, 2]
+            pages.fork(0, [2])  # an idle slot is still without a sequence
+    assert normwise(outs[0][[0, 3]], outs[1].astype(np.float64)) <= 1e-4
+    with pytest.raises(ValueError, match="3 entries for 4 slots"):
+        block.decode_paged(backend.upload(steps[0], (4, 256)), PageTable(Kv8Cache(8, 2, 16, 128), 4, 64), active=[1, 1, 1])
