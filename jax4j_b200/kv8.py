@@ -36,7 +36,7 @@ def rope_table(positions: int, head_dim: int, theta: float = 10000.0, device=Non
 
 def _rows(t: torch.Tensor, what: str) -> int:
     """Row stride of a tensor [rows, heads, dim] (or [rows, width]) whose rows are dense."""
-    if t.is_contiguous():
+    if t.is_contiguous() and t.shape[0] > 1:  # the stride of a row alone may be anything
         return t.stride(0)
     inner = 1
     for size, stride in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):

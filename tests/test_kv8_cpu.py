@@ -281,3 +281,16 @@ def test_page_table_rows_of_slots_without_a_token_start_nowhere():
     starts, lengths, offsets = t.extend([1, 0, 1])
     assert (starts.tolist(), lengths.tolist(), offsets.tolist()) == ([20, 3, 0], [21, 3, 1], [0, 1, 1, 2])
     assert [r.tolist() for r in t.rows] == [[20, -1, 0], [21, 0, 1]]
+
+
+def test_row_stride_of_one_row_is_its_width():
+    """PyTorch calls a tensor of one row contiguous whatever that dimension's stride is."""
+    from jax4j_b200.kv8 import _rows
+    assert _rows(torch.zeros(6, 1, 64).transpose(0, 1), "q") == 6 * 64
+    assert _rows(torch.zeros(1, 6, 64).expand(1, 6, 64), "q") == 6 * 64
+    assert _rows(torch.zeros(256, 1).t(), "qkv") == 256
+    assert _rows(torch.zeros(0, 6, 64), "q") == 6 * 64
+    assert _rows(torch.zeros(5, 9, 64)[:, :6], "q") == 9 * 64
+    assert _rows(torch.zeros(5, 9, 64)[:1, :6], "q") == 6 * 64
+    with pytest.raises(ValueError, match="dense within a row"):
+        _rows(torch.zeros(6, 2, 64).transpose(0, 1), "q")

@@ -833,3 +833,14 @@ def test_decoder_block_decodes_only_active_slots(backend):
     assert normwise(outs[0][[0, 3]], outs[1].astype(np.float64)) <= 1e-4
     with pytest.raises(ValueError, match="3 entries for 4 slots"):
         block.decode_paged(backend.upload(steps[0], (4, 256)), PageTable(Kv8Cache(8, 2, 16, 128), 4, 64), active=[1, 1, 1])
+
+
+def test_one_row_of_any_stride():
+    rng = np.random.default_rng(91)
+    pool = Pool(rng, [50], 2, 32, 64)
+    q = torch.from_numpy(rng.standard_normal((1, 6, 64)).astype(np.float32)).cuda()
+    odd = q[0].unsqueeze(1).transpose(0, 1)
+    assert odd.stride(0) == 64 and odd.is_contiguous()
+    table, n = ints(pool.table), ints([50])
+    assert torch.equal(pool.cache.attention_decode(odd, table, n), pool.cache.attention_decode(q, table, n))
+    assert torch.equal(pool.cache.attention_prefill(odd, ints([0, 1]), table, n), pool.cache.attention_prefill(q, ints([0, 1]), table, n))
