@@ -104,10 +104,11 @@ struct Warp {
     for (int i = 0; i < D / 16; ++i)
       most = fmaxf(most, fmaxf(fmaxf(fabsf(f.x[i].x), fabsf(f.x[i].y)), fmaxf(fabsf(f.x[i].z), fabsf(f.x[i].w))));
     most = quad_max(most);
-    // the power of two below `most`, biased; queries of tiny, infinite or no magnitude stay as they are
+    // the power of two below `most`, biased, whose e - 11 and 254 - (e - 11) are exponents of normal
+    // numbers; queries of tiny, infinite or no magnitude stay as they are
     const int e = (int)(__float_as_uint(most) >> 23);
-    const float down = e < 24 || e > 240 ? 1.f : __uint_as_float((uint32_t)(e - 11) << 23);
-    const float up = e < 24 || e > 240 ? 1.f : __uint_as_float((uint32_t)(254 - (e - 11)) << 23);
+    const float down = e < 24 || e > 254 ? 1.f : __uint_as_float((uint32_t)(e - 11) << 23);
+    const float up = e < 24 || e > 254 ? 1.f : __uint_as_float((uint32_t)(254 - (e - 11)) << 23);
     factor = scale_log2 * down;
 #pragma unroll
     for (int i = 0; i < D / 16; ++i) {

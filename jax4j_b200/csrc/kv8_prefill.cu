@@ -512,7 +512,7 @@ __device__ __forceinline__ void bring_queries(const AttnArgs& a, const Item& it,
 #pragma unroll
       for (int o = 1; o < 8; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
       const int e = (int)(__float_as_uint(most) >> 23);
-      const bool plain = e < 24 || e > 240;
+      const bool plain = e < 24 || e > 254;
       float up = plain ? 1.f : __uint_as_float((uint32_t)(254 - (e - 11)) << 23);
       if (a.scale_log2 < 0.f) up = -up;  // maxima are taken before the factor
       if ((lane & 7) == 0) factors[qr] = (uint8_t)(plain ? 127 : e - 11);

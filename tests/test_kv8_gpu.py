@@ -844,3 +844,20 @@ def test_one_row_of_any_stride():
     table, n = ints(pool.table), ints([50])
     assert torch.equal(pool.cache.attention_decode(odd, table, n), pool.cache.attention_decode(q, table, n))
     assert torch.equal(pool.cache.attention_prefill(odd, ints([0, 1]), table, n), pool.cache.attention_prefill(q, ints([0, 1]), table, n))
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_queries_near_the_end_of_f32(dim):
+    """Queries of 2^116 against keys of as little (scores of an rms of 2): as exact as any."""
+    rng = np.random.default_rng(95)
+    pool = Pool(rng, [90], 2, 32, dim)
+    pool.ks *= 2.0 ** np.round(1 - 114 - np.log2(np.sqrt((pool.k ** 2).mean((-1, -2))).reshape(*pool.ks.shape[:2], 1) * pool.ks))
+    pool.cache.k_scale[0] = torch.from_numpy(pool.ks).float()
+    q = (rng.standard_normal((90, 4, dim)) * 2.0 ** 114).astype(np.float32)
+    assert np.isfinite(q).all() and np.abs(q).max() > 2.0 ** 115
+    qd = torch.from_numpy(q).cuda()
+    table, n = ints(pool.table), ints([90])
+    got = pool.cache.attention_decode(qd[-1:], table, n).double().cpu().numpy()
+    assert normwise(got[0], pool.reference(q[-1:], 0, 89, 0, 0)[0]) <= DECODE_BAR
+    got = pool.cache.attention_prefill(qd, ints([0, 90]), table, n).double().cpu().numpy()
+    assert normwise(got, pool.reference(q, 0, 0, 0, 0)) <= PREFILL_BAR
