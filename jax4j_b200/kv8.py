@@ -16,6 +16,7 @@ from __future__ import annotations
 import ctypes
 import heapq
 import threading
+from array import array
 
 import torch
 
@@ -197,8 +198,11 @@ class Kv8Cache:
         n = len(src)
         if len(dst) != n or (tokens is not None and len(tokens) != n):
             raise ValueError("src, dst and tokens must have one entry per move")
-        ints = ctypes.c_int32 * n
-        call("j4b_kv8_copy_pages", self._ref, n, ints(*src), ints(*dst), None if tokens is None else ints(*tokens), self._stream())
+        try:  # ctypes would take what 32 bits hold of a number
+            lists = [None if x is None else (ctypes.c_int32 * n).from_buffer(array("i", x)) for x in (src, dst, tokens)]
+        except OverflowError:
+            raise ValueError("pages and tokens must be numbers of 32 bits") from None
+        call("j4b_kv8_copy_pages", self._ref, n, *lists, self._stream())
 
 
 class PageTable:

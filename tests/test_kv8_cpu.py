@@ -294,3 +294,20 @@ def test_row_stride_of_one_row_is_its_width():
     assert _rows(torch.zeros(5, 9, 64)[:1, :6], "q") == 6 * 64
     with pytest.raises(ValueError, match="dense within a row"):
         _rows(torch.zeros(6, 2, 64).transpose(0, 1), "q")
+
+
+def test_copy_pages_refuses_numbers_that_32_bits_do_not_hold(monkeypatch):
+    """2^32 is not page 0."""
+    from jax4j_b200 import kv8
+    calls = []
+    monkeypatch.setattr(kv8, "call", lambda name, ref, n, src, dst, tokens, stream: calls.append((list(src), list(dst), tokens and list(tokens))))
+    monkeypatch.setattr(kv8.Kv8Cache, "_stream", lambda self: 7)
+    codes = torch.zeros(1, 3, 2, 32, 64, dtype=torch.uint8).view(torch.float8_e4m3fn)
+    cache = kv8.Kv8Cache.wrap(codes, codes, torch.zeros(1, 3, 2, 2), torch.zeros(1, 3, 2, 2))
+    for src, dst, tokens in (([2 ** 32], [1], None), ([0], [2 ** 32 + 1], None), ([0], [1], [2 ** 32 + 16]), ([-2 ** 31 - 1], [1], None)):
+        with pytest.raises(ValueError, match="32 bits"):
+            cache.copy_pages(src, dst, tokens)
+    cache.copy_pages([0, 1], [2, 3], [5, 32])
+    cache.copy_pages([0], [np.int64(2)])
+    cache.copy_pages([], [])
+    assert calls == [([0, 1], [2, 3], [5, 32]), ([0], [2], None), ([], [], None)]
