@@ -342,7 +342,8 @@ int j4b_kv8_attention_decode(const j4b_kv8_cache* cache, int64_t layer, j4b_buf 
 /* Causal attention of ragged chunks: sequence b's queries are the rows [offsets[b], offsets[b + 1])
  * of q [tokens, heads, head_dim] (rows q_stride elements apart), its last tokens: query i of n is
  * at position lengths[b] - n + i. Window, sinks and empty rows as above. Tensor-core products of
- * f16 operands with f32 softmax and accumulation (the rel 1e-2 tensor-core bar). */
+ * f16 operands with f32 softmax and accumulation (the rel 1e-2 tensor-core bar; the tensor cores' sums round
+ * toward zero, which over more than some 4 million tokens is more than that). */
 int j4b_kv8_attention_prefill(const j4b_kv8_cache* cache, int64_t layer, j4b_buf q, int q_type, int64_t q_stride,
                               int64_t tokens, int64_t heads, j4b_buf offsets, j4b_buf table, int64_t table_stride,
                               int64_t table_width, j4b_buf lengths, int64_t batch, int64_t window, int64_t sinks,

@@ -166,8 +166,8 @@ __device__ __forceinline__ uint8_t* aligned_smem(uint8_t* raw) {  // the swizzle
 
 // Waits for an mbarrier's phase, bounded as mbar_wait_timed's waits are, but the clock is read once
 // in 64 polls: the read takes long enough to make a waiter late where tiles are handed on every
-// microsecond.
-__device__ __forceinline__ bool kv8_wait(uint64_t* bar, uint32_t parity) {
+// microsecond. `more`: nanoseconds above the common bound.
+__device__ __forceinline__ bool kv8_wait(uint64_t* bar, uint32_t parity, uint64_t more = 0) {
   const uint32_t at = (uint32_t)__cvta_generic_to_shared(bar);
   if (mbar_try_wait_parity(at, parity)) return true;
   uint64_t t0 = 0;
@@ -178,7 +178,7 @@ __device__ __forceinline__ bool kv8_wait(uint64_t* bar, uint32_t parity) {
     const uint64_t now = global_ns();
     if (t0 == 0)
       t0 = now;
-    else if (now - t0 > kWaitNs)
+    else if (now - t0 > kWaitNs + more)
       return false;
   }
 }

@@ -590,6 +590,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const AttnArgs
   tc_fence_after();
   const uint32_t tmem = tmem_slot;  // S0, S1 at columns 0, 128 (P over them); O0, O1 at 256, 384
   bool ok = true;
+  // The finder of items, and warps that have no part in one, wait while another walks over all its key
+  // tiles: 2.3 us each, so 0.3 s for 2^24 tokens. Their bound is 8 times that above the common one.
+  const uint64_t walk = (uint64_t)a.cap * (8 * 2300 / kTileBlocks);
   // An item of one tile has the other's columns, too: its scores, and the barriers s_full and p_ready,
   // alternate between the two, and a key tile's are there before the last one's softmax ends (5 turns
   // of up to 77 tokens on up to 1000: 27.0 -> 24.5 us).
@@ -599,7 +602,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const AttnArgs
   auto next_item = [&]() -> const Item* {
     __syncwarp();
     if (nth > 0 && lane == 0) bar_arrive(&item_empty[(nth - 1) % kItems]);
-    ok = __all_sync(0xffffffffu, ok && kv8_wait(&item_full[nth % kItems], nth / kItems & 1));  // the warp stays together
+    ok = __all_sync(0xffffffffu, ok && kv8_wait(&item_full[nth % kItems], nth / kItems & 1, walk));  // the warp stays together
     const Item* it = &items[nth % kItems];
     ++nth;
     return ok && it->seq >= 0 ? it : nullptr;
@@ -990,7 +993,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const AttnArgs
       for (uint32_t r = 0; more && ok; ++r) {
         Item it;
         find_item<SINGLE ? 7 : 8>(a, (int64_t)r * gridDim.x + (r & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x), limit, lane, it);
-        if (r >= kItems) ok = __all_sync(0xffffffffu, ok && kv8_wait(&item_empty[r % kItems], (r / kItems - 1) & 1));
+        if (r >= kItems) ok = __all_sync(0xffffffffu, ok && kv8_wait(&item_empty[r % kItems], (r / kItems - 1) & 1, walk));
         if (lane == 0) {
           items[r % kItems] = it;
           bar_arrive(&item_full[r % kItems]);

@@ -861,3 +861,38 @@ def test_queries_near_the_end_of_f32(dim):
     assert normwise(got[0], pool.reference(q[-1:], 0, 89, 0, 0)[0]) <= DECODE_BAR
     got = pool.cache.attention_prefill(qd, ints([0, 90]), table, n).double().cpu().numpy()
     assert normwise(got, pool.reference(q, 0, 0, 0, 0)) <= PREFILL_BAR
+
+
+def repeated_pages(rng, heads, dim, page, width, n):
+    """A sequence whose table names two pages over and over, and n queries at its end."""
+    pool = Pool(rng, [2 * page], heads, page, dim, spare=0)
+    quiet_keys(pool)
+    q = torch.from_numpy(rng.standard_normal((n, heads, dim)).astype(np.float32)).cuda().to(torch.bfloat16)
+    return pool, q, ints(np.array(pool.table[0])[np.arange(width) % 2][None]), width * page
+
+
+def test_prefill_waits_as_long_as_an_item_takes():
+    """Over 2^24 tokens an item (256 rows) takes 0.3 s, longer than most waits may: the ones for a whole
+    item go by the length. Its rows are what they are in a call of few items, where none waits."""
+    heads, n = 16, 7680  # four items for some SMs, which is as many as are found ahead
+    pool, q, table, length = repeated_pages(np.random.default_rng(97), heads, 64, 4096, 4096, n)
+    got = pool.cache.attention_prefill(q, ints([0, n]), table, ints([length]))
+    for i in (0, 3000, n - 1):
+        one = pool.cache.attention_prefill(q[i:i + 1], ints([0, 1]), table, ints([length - n + i + 1]))  # reports a wait that gave up
+        assert torch.equal(got[i], one[0]), i
+
+
+def test_prefill_over_a_million_tokens():
+    """The softmax is one over the two pages' tokens, each as often as it is seen. 2^16 additions to the
+    tensor cores' f32, rounded toward zero, lose up to 2^-24 of the sum each in the mean: 4e-3, and the
+    operands' bits 1e-3."""
+    from oracle.kv8 import values
+    heads, dim, page, n = 4, 128, 4096, 300
+    pool, q, table, length = repeated_pages(np.random.default_rng(98), heads, dim, page, 256, n)
+    got = pool.cache.attention_prefill(q, ints([0, n]), table, ints([length]), out_dtype=torch.float32).double().cpu().numpy()
+    k, v = (values(c, s)[pool.table[0]].transpose(1, 0, 2, 3).reshape(heads, 2 * page, dim) for c, s in ((pool.k, pool.ks), (pool.v, pool.vs)))
+    for i in (0, 130, 255, n - 1):
+        seen = length - n + i + 1
+        count = seen // (2 * page) + (np.arange(2 * page) < seen % (2 * page))
+        w = count * np.exp(np.einsum("hkd,hd->hk", k, q[i].double().cpu().numpy()) * dim ** -0.5)
+        assert normwise(got[i], np.einsum("hk,hkd->hd", w / w.sum(-1, keepdims=True), v)) <= PREFILL_BAR, i
