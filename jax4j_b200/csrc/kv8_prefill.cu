@@ -219,8 +219,21 @@ __device__ __forceinline__ bool holds_values(const AttnArgs& a, int seq, int hea
 // it sees, `before` or here. What it does not see must not count, or a loud value among it would
 // shift the row's probabilities out of f16. A block seen in part has kPartRoom, and beyond that
 // counts only if one of its seen values is not zero (next to a token that much louder, few are
-// anything else). Runs where a tile's scales exceed a row's reference, so seldom.
-__device__ __forceinline__ int seen_exponent(const AttnArgs& a, const Item& it, const TileInfo& info, const View& view, int before, int dim) {
+// anything else). Runs where a tile's largest, `top`, exceeds a row's reference, so seldom; where its
+// scales are alike, and they mostly are, any block stands for all (window 8001: 202 us by blocks).
+// `near`: the tile's first position.
+constexpr int kAlike = 6;
+__device__ __forceinline__ int seen_exponent(const AttnArgs& a, const Item& it, const TileInfo& info, const View& view, int before, int top,
+                                             int near, int dim) {
+  int low = top, far = 0;
+#pragma unroll 2
+  for (int k = 0; k < kTileBlocks; ++k) {
+    if (info.pos[k] == kNowhere) continue;
+    low = min(low, info.ev[k]);
+    far = max(far, info.pos[k] + kKvBlock);
+  }
+  if ((view.lo >= far || view.qp < near) && view.sinks <= near) return before;  // it sees none
+  if (top - low <= kAlike) return max(before, top);
   int most = before, part = before;
 #pragma unroll 1
   for (int k = 0; k < kTileBlocks; ++k) {
@@ -665,7 +678,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const AttnArgs
         };
         const bool begin = j == j0;
         if (__any_sync(0xffffffffu, ev > eref)) {
-          const int now = all ? max(ev, eref) : seen_exponent(a, it, info, view, eref, D);
+          const int now = all ? max(ev, eref) : seen_exponent(a, it, info, view, eref, ev, near, D);
           if (!begin && __any_sync(0xffffffffu, now > eref)) {
             settle();
             rescale<false>(o_at, D, exp2_ftz((float)(eref - now)));

@@ -896,3 +896,19 @@ def test_prefill_over_a_million_tokens():
         count = seen // (2 * page) + (np.arange(2 * page) < seen % (2 * page))
         w = count * np.exp(np.einsum("hkd,hd->hk", k, q[i].double().cpu().numpy()) * dim ** -0.5)
         assert normwise(got[i], np.einsum("hk,hkd->hd", w / w.sum(-1, keepdims=True), v)) <= PREFILL_BAR, i
+
+
+@pytest.mark.parametrize("heads,kv,window,sinks", [(2, 2, 20, 0), (2, 2, 20, 5), (32, 32, 20, 0), (32, 32, 20, 5), (8, 2, 150, 0), (4, 4, 0, 0)])
+def test_prefill_rows_do_not_feel_key_tiles_that_are_loud_throughout(heads, kv, window, sinks):
+    """As above, where all blocks of a key tile are as loud and some rows see none of them."""
+    rng = np.random.default_rng(heads + window + sinks)
+    n, dim = 460, 64
+    pool, offsets, q = prefill_inputs(rng, [(0, n)], heads, kv, dim, 32, torch.float32)
+    quiet_keys(pool)
+    for at in range(64, 208, 16):
+        hide_loud_values(pool, 0, at, 30, False)
+    got = pool.cache.attention_prefill(q, ints(offsets), ints(pool.table), ints(pool.lengths), window=window, sinks=sinks).double().cpu().numpy()
+    qh = q.double().cpu().numpy()
+    for i in np.unique(np.concatenate([np.arange(0, n, 29), np.arange(55, 72), np.arange(200, 232), np.arange(340, 364)])):
+        want = pool.reference(qh[i:i + 1], 0, i, window, sinks)[0]
+        assert normwise(got[i], want) <= PREFILL_BAR, i
