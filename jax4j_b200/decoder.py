@@ -39,7 +39,7 @@ import torch
 
 from ._lib import call
 from .backend import B200Backend, DeviceBuffer, QuantBuffer
-from .kv8 import PageTable, rope_table
+from .kv8 import PageTable
 from .prng import PrngKey
 
 Q4_0 = 2
@@ -135,7 +135,6 @@ class DecoderBlock:
         """`group`: the torch.distributed process group of the ranks sharing the block (default:
         the world group) when the weights are sharded."""
         self.be, self.w, self.eps, self.theta, self.group = backend, weights, eps, theta, group
-        self._rope = None
 
     def _sum_ranks(self, partial: DeviceBuffer) -> DeviceBuffer:
         if self.w.world > 1:
@@ -206,10 +205,7 @@ class DecoderBlock:
         return self._sum_ranks(self._add_residual(be.quant_gemm(w.wd, self.swiglu(gu), precision), h))
 
     def _rope_table(self, pages: PageTable) -> torch.Tensor:
-        positions = pages.width * pages.cache.page
-        if self._rope is None or self._rope.shape[0] < positions:
-            self._rope = rope_table(positions, HEAD_DIM, self.theta, pages.cache.device)
-        return self._rope
+        return pages.rope(self.theta)
 
     def _paged(self, x: DeviceBuffer, pages: PageTable, counts: list, window: int, sinks: int, layer: int, rows: int) -> None:
         """Checks a paged call, all of it before the sequences change, and makes room for its tokens."""

@@ -223,6 +223,7 @@ class PageTable:
         self._free = list(range(cache.pages))  # a heap: the lowest page first, so what is in use stays low
         self._table = torch.full((slots, self.width), -1, dtype=torch.int32, device=cache.device)
         self._dirty = False
+        self._ropes = {}  # theta -> table
         # of the last extend, for a model's other layers: what it returned, (starts, lengths) of decode's
         # rows, one a slot, and what it was given
         self.step = self.rows = self.counts = None
@@ -292,6 +293,12 @@ class PageTable:
     def table(self) -> torch.Tensor:
         self._upload()
         return self._table
+
+    def rope(self, theta: float = 10000.0) -> torch.Tensor:
+        """The `rope_table` of all positions that a slot can have, made once for all layers."""
+        if theta not in self._ropes:
+            self._ropes[theta] = rope_table(self.width * self.cache.page, self.cache.head_dim, theta, self.cache.device)
+        return self._ropes[theta]
 
     def release(self, slot: int) -> None:
         """Ends a slot's sequence: its pages that no other shares are free again."""

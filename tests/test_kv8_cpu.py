@@ -311,3 +311,17 @@ def test_copy_pages_refuses_numbers_that_32_bits_do_not_hold(monkeypatch):
     cache.copy_pages([0], [np.int64(2)])
     cache.copy_pages([], [])
     assert calls == [([0, 1], [2, 3], [5, 32]), ([0], [2], None), ([], [], None)]
+
+
+def test_blocks_of_a_model_share_one_rope_table():
+    from types import SimpleNamespace
+    from jax4j_b200.decoder import DecoderBlock
+    from jax4j_b200.kv8 import PageTable, rope_table
+    cache = FakeCache(9, 16)
+    cache.head_dim = 128
+    t = PageTable(cache, 2, 70)
+    blocks = [DecoderBlock(None, SimpleNamespace(), theta=theta) for theta in (10000.0, 10000.0, 500.0)]
+    tables = [b._rope_table(t) for b in blocks]
+    assert tables[0] is tables[1] and tables[0] is blocks[0]._rope_table(t)
+    for b, got in zip(blocks, tables):
+        assert torch.equal(got, rope_table(80, 128, b.theta))
