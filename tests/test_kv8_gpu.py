@@ -912,3 +912,78 @@ def test_prefill_rows_do_not_feel_key_tiles_that_are_loud_throughout(heads, kv, 
     for i in np.unique(np.concatenate([np.arange(0, n, 29), np.arange(55, 72), np.arange(200, 232), np.arange(340, 364)])):
         want = pool.reference(qh[i:i + 1], 0, i, window, sinks)[0]
         assert normwise(got[i], want) <= PREFILL_BAR, i
+
+
+def nan_scales_of_what_nobody_holds(pool):
+    for t in (pool.cache.k_scale, pool.cache.v_scale):
+        held = torch.zeros(t.shape[1], t.shape[3], dtype=torch.bool)
+        for b, n in enumerate(pool.lengths):
+            for blk in range(-(-n // 16)):
+                held[int(pool.table[b, blk * 16 // pool.page]), blk * 16 % pool.page // 16] = True
+        t[pool.layer][~held[:, None, :].expand(-1, t.shape[2], -1).cuda()] = float("nan")
+
+
+def many_lengths(rng, n, most):
+    """n lengths up to `most`, every fifth sequence (and the first and the last) empty."""
+    return [0 if i % 5 == 0 or i == n - 1 else int(x) for i, x in enumerate(rng.integers(1, most + 1, n))]
+
+
+@pytest.mark.parametrize("n,most,width,window,sinks", [(200, 60, 0, 0, 0), (200, 300, 0, 0, 0), (131, 700, 40, 90, 3), (500, 40, 0, 0, 0)])
+def test_decode_of_many_sequences(n, most, width, window, sinks):
+    """More sequences than a CTA's threads, whose search for a share then gives a thread several."""
+    rng = np.random.default_rng(n + most)
+    lengths = many_lengths(rng, n, most)
+    pool = Pool(rng, lengths, 2, 32, 64)
+    nan_scales_of_what_nobody_holds(pool)
+    table = torch.full((n, max(width, pool.table.shape[1])), -1, dtype=torch.int32, device="cuda")
+    table[:, :pool.table.shape[1]] = ints(pool.table)
+    q = torch.from_numpy(rng.standard_normal((n, 4, 64)).astype(np.float32)).cuda()
+    got = pool.cache.attention_decode(q, table, ints(lengths), window=window, sinks=sinks).double().cpu().numpy()
+    qh = q.double().cpu().numpy()
+    assert np.isfinite(got).all() and not got[np.array(lengths) == 0].any()
+    for b in range(n):
+        if lengths[b]:
+            assert normwise(got[b], pool.reference(qh[b:b + 1], b, lengths[b] - 1, window, sinks)[0]) <= DECODE_BAR, b
+
+
+@pytest.mark.parametrize("n,heads,kv,window,sinks", [(40, 2, 1, 0, 0), (70, 8, 4, 0, 0), (70, 8, 4, 50, 7), (33, 32, 16, 0, 0)])
+def test_prefill_of_many_sequences(n, heads, kv, window, sinks):
+    """More sequences than a warp's lanes, past which the search for an item reads them again."""
+    rng = np.random.default_rng(n + heads + window)
+    new, past = many_lengths(rng, n, 150), many_lengths(rng, n, 100)[::-1]
+    pool, offsets, q = prefill_inputs(rng, list(zip(past, new)), heads, kv, 64, 32, torch.float32)
+    nan_scales_of_what_nobody_holds(pool)
+    got = pool.cache.attention_prefill(q, ints(offsets), ints(pool.table), ints(pool.lengths), window=window, sinks=sinks).double().cpu().numpy()
+    qh = q.double().cpu().numpy()
+    assert np.isfinite(got).all()
+    for b in range(n):
+        for i in sorted({0, new[b] // 2, new[b] - 1} if new[b] else ()):
+            row = int(offsets[b]) + i
+            assert normwise(got[row], pool.reference(qh[row:row + 1], b, past[b] + i, window, sinks)[0]) <= PREFILL_BAR, (b, i)
+
+
+@pytest.mark.parametrize("one", [False, True])
+def test_append_of_many_sequences(one):
+    from jax4j_b200.kv8 import rope_table
+    from oracle import kv8 as O
+    rng = np.random.default_rng(200 + one)
+    n, heads, kv, dim, page = 200, 2, 1, 64, 32
+    starts = many_lengths(rng, n, 40)
+    new = [1] * n if one else many_lengths(rng, n, 25)[::-1]
+    pool = Pool(rng, starts, kv, page, dim, room=25)
+    nan_scales_of_what_nobody_holds(pool)
+    pool.ks, pool.vs = (t[0].double().cpu().numpy() for t in (pool.cache.k_scale, pool.cache.v_scale))
+    offsets = np.cumsum([0] + new)
+    qkv = rng.standard_normal((offsets[-1], (heads + 2 * kv) * dim)).astype(np.float32)
+    rope = rope_table(70, dim, device="cuda")
+    q = pool.cache.append(torch.from_numpy(qkv).cuda(), rope, ints(pool.table), ints(starts), heads, offsets=None if one else ints(offsets))
+    cs, x = rope.cpu().numpy(), qkv.reshape(-1, heads + 2 * kv, dim)
+    k, ks, v, vs = pool.codes[0].copy(), pool.ks.copy(), pool.codes[1].copy(), pool.vs.copy()
+    for b, (start, m) in enumerate(zip(starts, new)):
+        rows = slice(offsets[b], offsets[b + 1])
+        rot = np.stack([O.rope(x[offsets[b] + i, :heads + kv], cs[start + i]) for i in range(m)]) if m else np.empty((0, heads + kv, dim), np.float32)
+        assert np.array_equal(q[rows].cpu().numpy(), rot[:, :heads]), b
+        O.append(k, ks, rot[:, heads:].astype(np.float64), pool.table[b], start)
+        O.append(v, vs, x[rows, heads + kv:].astype(np.float64), pool.table[b], start)
+    for got, want in ((pool.cache.k_scale, ks), (pool.cache.v_scale, vs), (pool.cache.k, k), (pool.cache.v, v)):
+        assert np.array_equal(got[0].double().cpu().numpy(), want, equal_nan=True)
