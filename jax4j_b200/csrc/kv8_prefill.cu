@@ -554,6 +554,19 @@ __device__ __forceinline__ void prefetch_queries(const AttnArgs& a, const Item& 
   }
 }
 
+// The output of an item whose rows see nothing.
+template <int D>
+__device__ __forceinline__ void put_zeros(const AttnArgs& a, const Item& it, int lane) {
+  const int size = a.out_type == J4B_F32 ? 4 : 2;
+#pragma unroll 1
+  for (int r = 0; r < it.rows; ++r) {
+    const int g = it.first_row + r, row = it.row0 + g / a.group;
+    if (row < 0 || row >= a.tokens || lane * 16 >= D * size) continue;
+    char* out = static_cast<char*>(a.out) + ((int64_t)row * a.heads + it.head * a.group + g % a.group) * (D * size);
+    *reinterpret_cast<uint4*>(out + lane * 16) = make_uint4(0, 0, 0, 0);
+  }
+}
+
 constexpr int kItems = 4;         // found ahead
 constexpr int kItemReaders = 13;  // warps
 
@@ -1002,17 +1015,27 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const AttnArgs
       }
     } else if (warp == 13) {
       // ---- items ----
+      // Ones whose rows see nothing go no further. Every other item has a key tile, so the page warps,
+      // which look one tile ahead before they turn the last one, never wait for more than the next
+      // item (past a run of empty ones they would wait for the very item that waits for them).
+      uint32_t found = 0;
       bool more = true;
       for (uint32_t r = 0; more && ok; ++r) {
         Item it;
         find_item<SINGLE ? 7 : 8>(a, (int64_t)r * gridDim.x + (r & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x), limit, lane, it);
-        if (r >= kItems) ok = __all_sync(0xffffffffu, ok && kv8_wait(&item_empty[r % kItems], (r / kItems - 1) & 1, walk));
-        if (lane == 0) {
-          items[r % kItems] = it;
-          bar_arrive(&item_full[r % kItems]);
-        }
-        __syncwarp();
         more = it.seq >= 0;
+        if (more && it.tiles() == 0) {
+          put_zeros<D>(a, it, lane);
+          continue;
+        }
+        const uint32_t slot = found % kItems;
+        if (found >= kItems) ok = __all_sync(0xffffffffu, ok && kv8_wait(&item_empty[slot], (found / kItems - 1) & 1, walk));
+        if (lane == 0) {
+          items[slot] = it;
+          bar_arrive(&item_full[slot]);
+        }
+        ++found;
+        __syncwarp();
         prefetch_queries<D, TYPE>(a, it, lane);  // a CTA's numbers rise
       }
     }

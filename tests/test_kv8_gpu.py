@@ -987,3 +987,28 @@ def test_append_of_many_sequences(one):
         O.append(v, vs, x[rows, heads + kv:].astype(np.float64), pool.table[b], start)
     for got, want in ((pool.cache.k_scale, ks), (pool.cache.v_scale, vs), (pool.cache.k, k), (pool.cache.v, v)):
         assert np.array_equal(got[0].double().cpu().numpy(), want, equal_nan=True)
+
+
+@pytest.mark.parametrize("kv,group,dim", [(16, 7, 128), (16, 1, 64), (2, 2, 64)])
+def test_prefill_past_runs_of_queries_that_see_nothing(kv, group, dim):
+    """Sequences whose queries all lie before their cache (no length, or fewer tokens than queries) give
+    zeros, and however many of them a CTA gets one after the other, the ones between are computed."""
+    rng = np.random.default_rng(kv + group)
+    spans = []  # (tokens, queries)
+    for i in range(60):
+        spans.append((int(rng.integers(1, 150)), int(rng.integers(1, 40))) if i % 11 == 0 or i > 56 else (0, int(rng.integers(1, 4))))
+    pool = Pool(rng, [n for n, _ in spans], kv, 32, dim)
+    offsets = np.cumsum([0] + [n for _, n in spans])
+    q = torch.from_numpy(rng.standard_normal((offsets[-1], kv * group, dim)).astype(np.float32)).cuda()
+    out = torch.full_like(q, 7.0)
+    for window in (0, 2):
+        got = pool.cache.attention_prefill(q, ints(offsets), ints(pool.table), ints(pool.lengths), window=window, out=out).double().cpu().numpy()
+        qh = q.double().cpu().numpy()
+        for b, (m, n) in enumerate(spans):
+            rows, before = slice(offsets[b], offsets[b + 1]), max(0, n - m)
+            assert not got[rows][:before].any(), b
+            if m:
+                assert normwise(got[rows][before:], pool.reference(qh[rows][before:], b, max(0, m - n), window, 0)) <= PREFILL_BAR, b
+    none = pool.cache.attention_prefill(q, ints(offsets), ints(pool.table), ints([0] * 60), out=out)  # also reports a wait that gave up
+    assert not none.any()
+    pool.cache.attention_prefill(q[:1], ints([0, 1]), ints(pool.table[:1]), ints(pool.lengths[:1]))
