@@ -304,7 +304,7 @@ int j4b_swiglu(j4b_buf gate_up, int64_t rows, int64_t width, j4b_buf out, j4b_st
  * table_stride apart); an entry outside [0, pages) is unmapped: its tokens are neither written nor
  * seen. Lengths, starts and offsets are int32 arrays on the device, so a call can be captured in a
  * graph and replayed while they change; a call like it has to have run on the device before (the first
- * of its types and sizes sets its kernel up). They are not checked, but lead nowhere: a negative length
+ * of its types and sizes sets its kernel up). These arrays are not checked, but lead nowhere: a negative length
  * is 0, one past the table's pages sees what these hold, a sequence with a negative start or offset
  * has no rows, and rows past `tokens` are not there. Rows of q, q_out and out that no sequence has
  * are left as they are. heads is a multiple of kv_heads (grouped heads: query head
@@ -333,7 +333,11 @@ int j4b_kv8_append(const j4b_kv8_cache* cache, int64_t layer, j4b_buf qkv, int64
  * the first `sinks` tokens; window 0: all. A query that sees no key (length 0, unmapped pages) gives
  * zeros. f32-accurate (queries and probabilities enter the tensor cores as two f16 terms).
  * workspace: j4b_kv8_decode_workspace bytes of device memory, 16-byte aligned, used by this call
- * alone until it has run. */
+ * alone until it has run: a call may be two launches, between which none of another thread's calls
+ * with the same workspace may come.
+ * Every wait inside the two attention kernels is bounded. Should one give up, the call's output is
+ * not valid, and the process's next attention call, on whichever cache or device, does nothing but
+ * return J4B_ETIMEOUT. */
 int j4b_kv8_decode_workspace(const j4b_kv8_cache* cache, int64_t heads, int64_t batch, int64_t* bytes);
 int j4b_kv8_attention_decode(const j4b_kv8_cache* cache, int64_t layer, j4b_buf q, int q_type, int64_t q_stride,
                              int64_t heads, j4b_buf table, int64_t table_stride, int64_t table_width, j4b_buf lengths,
@@ -342,8 +346,10 @@ int j4b_kv8_attention_decode(const j4b_kv8_cache* cache, int64_t layer, j4b_buf 
 /* Causal attention of ragged chunks: sequence b's queries are the rows [offsets[b], offsets[b + 1])
  * of q [tokens, heads, head_dim] (rows q_stride elements apart), its last tokens: query i of n is
  * at position lengths[b] - n + i. Window, sinks and empty rows as above. Tensor-core products of
- * f16 operands with f32 softmax and accumulation (the rel 1e-2 tensor-core bar; the tensor cores' sums round
- * toward zero, which over more than some 4 million tokens is more than that). */
+ * f16 operands with f32 softmax and accumulation (the rel 1e-2 tensor-core bar). Probabilities are
+ * weighed by their block's value scale over the largest that the query sees, so those of a block
+ * 2^18 or more quieter than another it sees keep fewer bits. The tensor cores' sums round toward
+ * zero, which over more than some 4 million tokens is more than the bar. */
 int j4b_kv8_attention_prefill(const j4b_kv8_cache* cache, int64_t layer, j4b_buf q, int q_type, int64_t q_stride,
                               int64_t tokens, int64_t heads, j4b_buf offsets, j4b_buf table, int64_t table_stride,
                               int64_t table_width, j4b_buf lengths, int64_t batch, int64_t window, int64_t sinks,

@@ -349,15 +349,16 @@ struct Copies {
 // in one share is finished there; one cut by a share's end leaves an unnormalised part (running
 // maximum, sum, 8 x D) in the workspace for kv8_join_kernel.
 //
-// Bound by HBM once the rows are long and D = 128: 64 x 2049 tokens of 32 heads in 180 us, 5.98 TB/s of
-// the 6.55 that a copy reaches; 2 x 131071 of 8 heads 92 us. With D = 64 the ~290 warp instructions of
-// a block (its scores cost as many at any D) bound it: window 4096 of 32 sequences, 41 us against 21
-// of traffic. What the short ones cost is latency, so a warp never lets its copies run dry: it looks
+// Bound by HBM once the rows are long and D = 128: 64 x 2049 tokens of 32 heads in 185 us, 5.83 TB/s of
+// the 6.55 that a copy reaches; 2 x 131071 of 8 heads 93 us. With D = 64 a pair of blocks has half the
+// bytes and nearly all the ~560 warp instructions (its scores cost as many at any D), each step a
+// chain that four warps of a scheduler do not hide (issue 0.53 a cycle, fixed waits the largest stall):
+// window 4096 of 32 sequences, 40 us against 21 of traffic. What the short ones cost is latency, so a warp never lets its copies run dry: it looks
 // up the next 32 blocks, of its next segment too, while it works on these, and fetches the first
 // pair's keys of the next segment before it merges. At the start the pages and the queries are asked
 // for together, and codes before scales (1 x 517 tokens 11.0 -> 10.4 us, ragged batch 61.8 -> 60.0).
 constexpr int kDecWarps = 4;
-// CTAs of an SM: D = 128 fills the registers at 3; with D = 64 (bound by instructions) 4 fit, too:
+// CTAs of an SM: D = 128 fills the registers at 3; with D = 64 (bound by its instructions' chain) 4 fit, too:
 // 32 x window 4096, 40/8 heads of 64: 3 43.2 us, 4 41.0, 5 (spilling) 44.6.
 constexpr int dec_ctas(int dim) { return dim == 64 ? 4 : 3; }
 constexpr int kDecHeads = 8;

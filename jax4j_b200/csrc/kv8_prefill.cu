@@ -9,15 +9,15 @@
 //   P_i = 2^(S_i - m + w)  by the tile's 128 softmax threads, one a row             -> TMEM, over S_i
 //   O_i += P_i V    (P from TMEM, V f16 codes in shared memory, dims contiguous)    -> TMEM
 // Scales never touch the operands: a block's key scale multiplies its scores, and its value scale,
-// over the largest seen, is the w of its probabilities (both powers of two). The running maximum m
+// over the largest that the row sees, is the w of its probabilities (both powers of two). The running maximum m
 // moves only when f16 would not hold a row's probabilities, so O is seldom rescaled.
 //
 // Warps: 0-3 and 4-7 queries, softmax and output of tile 0 and 1; 8-11 bring pages: each thread loads
 // 16-code pieces of the next tile while it turns this one's into the swizzled f16 operands; 12 issues
 // the MMAs; 13 finds the next item. S of one tile is computed while the other's softmax runs.
 //
-// Measured: 8 x 2048 causal, 32 heads of 128: 390 us, 705 TFLOP/s (a bf16 product of matrices reaches
-// 1672); 8001 tokens under a window of 1024, 32/8 heads: 198 us. A step of 128 keys takes 2.3 us, of
+// Measured: 8 x 2048 causal, 32 heads of 128: 392 us, 701 TFLOP/s (a bf16 product of matrices reaches
+// 1672); 8001 tokens under a window of 1024, 32/8 heads: 200 us. A step of 128 keys takes 2.3 us, of
 // which the tensor cores work 0.6: it is a chain of softmax (1.6, its warps waiting on one another's
 // issue slots, MUFU a third busy) and MMAs (0.7 from the last probability to the next scores). What
 // shortened it most was fewer instructions in the softmax and page warps, which share 4 schedulers.

@@ -8,8 +8,8 @@ first tokens that stay visible. `PageTable` is the host's bookkeeping for it: wh
 sequence has, shared pages of forks, freed pages, compaction.
 
 Launches go to PyTorch's current stream of the cache's device; outputs come from its allocator on
-that stream, and the decode workspace is kept, one per stream. The reference has no KV cache; the functions are stated in
-include/jax4j_b200.h.
+that stream, and the decode workspace is kept, one per stream; threads may share a cache and a
+stream. The reference has no KV cache; the functions are stated in include/jax4j_b200.h.
 """
 from __future__ import annotations
 
@@ -206,8 +206,8 @@ class Kv8Cache:
 
 
 class PageTable:
-    """The host's bookkeeping of a `Kv8Cache`: `slots` sequences of up to `max_tokens` tokens, each a list
-    of pages in token order. Full pages of a fork are shared (counted), its partly filled last page
+    """The host's bookkeeping of a `Kv8Cache`: `slots` sequences of up to `max_tokens` tokens (counted from
+    their first one, under a window too), each a list of pages in token order. Full pages of a fork are shared (counted), its partly filled last page
     is copied. The device sees it through `table` (int32 [slots, pages of a sequence], -1: none),
     one tensor, which a read of the attribute and `extend` bring up to date on the current stream, and
     the arrays that `extend` returns."""
