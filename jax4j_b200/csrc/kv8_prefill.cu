@@ -220,20 +220,25 @@ __device__ __forceinline__ bool holds_values(const AttnArgs& a, int seq, int hea
 // shift the row's probabilities out of f16. A block seen in part has kPartRoom, and beyond that
 // counts only if one of its seen values is not zero (next to a token that much louder, few are
 // anything else). Runs where a tile's largest, `top`, exceeds a row's reference, so seldom; where its
-// scales are alike, and they mostly are, any block stands for all (window 8001: 202 us by blocks).
+// scales are alike, and they mostly are, one block seen whole stands for all, or a small rise does no
+// harm (window 8001: 0.7 % more by blocks).
 // `near`: the tile's first position.
 constexpr int kAlike = 6;
 __device__ __forceinline__ int seen_exponent(const AttnArgs& a, const Item& it, const TileInfo& info, const View& view, int before, int top,
                                              int near, int dim) {
-  int low = top, far = 0;
+  int low = top, far = 0, there = 0;
 #pragma unroll 2
   for (int k = 0; k < kTileBlocks; ++k) {
     if (info.pos[k] == kNowhere) continue;
     low = min(low, info.ev[k]);
     far = max(far, info.pos[k] + kKvBlock);
+    there += kKvBlock;
   }
   if ((view.lo >= far || view.qp < near) && view.sinks <= near) return before;  // it sees none
-  if (top - low <= kAlike) return max(before, top);
+  // 31 positions in a row, or those of a block of sinks, hold a whole block
+  const bool whole = (far - near == there && min(view.qp + 1, far) - max(view.lo, near) >= 2 * kKvBlock - 1) ||
+                     (min(view.qp + 1, view.sinks) - near >= kKvBlock);
+  if (top - low <= kAlike && (whole || top - before <= kAlike)) return max(before, top);
   int most = before, part = before;
 #pragma unroll 1
   for (int k = 0; k < kTileBlocks; ++k) {

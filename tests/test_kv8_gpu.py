@@ -1012,3 +1012,27 @@ def test_prefill_past_runs_of_queries_that_see_nothing(kv, group, dim):
     none = pool.cache.attention_prefill(q, ints(offsets), ints(pool.table), ints([0] * 60), out=out)  # also reports a wait that gave up
     assert not none.any()
     pool.cache.attention_prefill(q[:1], ints([0, 1]), ints(pool.table[:1]), ints(pool.lengths[:1]))
+
+
+@pytest.mark.parametrize("heads,kv,window,sinks", [(2, 2, 0, 0), (8, 2, 0, 0), (32, 32, 0, 0), (2, 2, 100, 0), (32, 32, 100, 0), (8, 2, 100, 16), (8, 2, 100, 3), (32, 32, 100, 20)])
+@pytest.mark.parametrize("at", [16, 128, 144, 256])
+def test_prefill_rows_at_the_edge_of_a_loud_key_tile(heads, kv, window, sinks, at):
+    """Rows that see of a key tile, loud throughout, only its first tokens or (under the window) its last
+    ones, whose own values the loud ones in their blocks left as zeros."""
+    rng = np.random.default_rng(heads + window + sinks + at)
+    n, dim = 500, 64
+    pool, offsets, q = prefill_inputs(rng, [(0, n)], heads, kv, dim, 32, torch.float32)
+    quiet_keys(pool)
+    pool.vs[:] = 2.0 ** -5
+    pool.cache.v_scale[0] = 2.0 ** -5
+    for blk in range(at, at + 128, 16):
+        hide_loud_values(pool, 0, blk, 30, False)
+    for lo, hi in ((at, at + 7), (at + 128 - 5, at + 128)):
+        pg = int(pool.table[0, lo // 32])
+        pool.v[pg, :, lo % 32:lo % 32 + hi - lo] = 0
+        pool.cache.v[0, pg].view(torch.uint8).copy_(to_f8(pool.v[pg]).view(torch.uint8))
+    got = pool.cache.attention_prefill(q, ints(offsets), ints(pool.table), ints(pool.lengths), window=window, sinks=sinks).double().cpu().numpy()
+    qh = q.double().cpu().numpy()
+    for i in list(range(at - 3, at + 12)) + (list(range(at + 118 + window, min(n, at + 132 + window)))  if window else []) + [n - 1]:
+        want = pool.reference(qh[i:i + 1], 0, i, window, sinks)[0]
+        assert normwise(got[i], want) <= PREFILL_BAR, i
