@@ -14,7 +14,8 @@
 //
 // Warps: 0-3 and 4-7 queries, softmax and output of tile 0 and 1; 8-11 bring pages: each thread loads
 // 16-code pieces of the next tile while it turns this one's into the swizzled f16 operands; 12 issues
-// the MMAs; 13 finds the next item. S of one tile is computed while the other's softmax runs.
+// the MMAs; 13 finds the next item, and writes the output of those that see nothing. S of one tile is
+// computed while the other's softmax runs.
 //
 // Measured: 8 x 2048 causal, 32 heads of 128: 392 us, 701 TFLOP/s (a bf16 product of matrices reaches
 // 1672); 8001 tokens under a window of 1024, 32/8 heads: 200 us. A step of 128 keys takes 2.3 us, of
